@@ -49,6 +49,8 @@ hipError_t fx_cmap_resident(uint32_t lds_bytes, uint32_t* wide, uint32_t* narrow
 uint32_t fx_cmap_lds_bytes(const FxCmapLaunch& hl);
 uint32_t fx_cmap_chunk_rows();
 #include "fx_attn.h"
+#include "fx_kv.h"
+hipError_t fx_launch_kv_attention(const FxKvAttnArgs& a, int held, int type, int64_t grid, int64_t join_grid, hipStream_t stream);
 #include "fx_lstm_sched.h"
 int fx_launch_lstm_stack(const FxLstmArgs& a, int L, uint32_t* words_ctl, uint32_t* die_ctl, hipStream_t stream);
 int fx_lstm_ask(int form);
@@ -1637,6 +1639,160 @@ int fx_attention_steps(const float* x, const float* k, const float* v, const flo
   g_launches.fetch_add(1, std::memory_order_relaxed);
   g_spec_launches.fetch_add(1, std::memory_order_relaxed);
   return FX_OK;
+}
+
+// ---- paged 8-bit key / value cache (fx_kv.hip, fx_kv_attn.h) ----
+
+namespace {
+int log_page_of(int page_size) { return page_size >= 16 && page_size <= 256 && (page_size & (page_size - 1)) == 0 ? __builtin_ctz((unsigned)page_size) : -1; }
+bool kv_dtype(int dtype) { return dtype == FX_DT_F32 || dtype == FX_DT_F16 || dtype == FX_DT_BF16; }
+// the cache's checks; `at`: the entry point's name
+int kv_cache_of(const char* at, const fx_kv_cache* c, FxKvCache& out) {
+  const std::string op(at);
+  if (!c) return fail(FX_E_INVALID, op + ": null cache");
+  if (c->held != FX_KV_E4M3 && c->held != FX_KV_INT8) return fail(FX_E_UNSUPPORTED, op + ": codes must be FX_KV_E4M3 or FX_KV_INT8");
+  if (log_page_of(c->page_size) < 0) return fail(FX_E_UNSUPPORTED, op + ": page_size must be 16, 32, 64, 128 or 256 (got " + std::to_string(c->page_size) + ")");
+  if (c->depth < 16 || c->depth > FX_KV_MAX_DEPTH || c->depth % 16 != 0)
+    return fail(FX_E_UNSUPPORTED, op + ": depth must be a multiple of 16 up to " + std::to_string(FX_KV_MAX_DEPTH) + " (got " + std::to_string(c->depth) + ")");
+  if (c->pages < 1 || c->heads < 1) return fail(FX_E_INVALID, op + ": a cache has at least one page and one head");
+  if (c->heads > 65536) return fail(FX_E_LIMIT, op + ": more than 65536 heads");
+  if (!c->k || !c->v || !c->k_scale || !c->v_scale) return fail(FX_E_INVALID, op + ": null argument");
+  const int64_t bytes = (int64_t)c->heads * c->page_size * c->depth;
+  if ((((uintptr_t)c->k | (uintptr_t)c->v) & 15u) != 0 || c->k_page_stride % 16 != 0 || c->v_page_stride % 16 != 0)
+    return fail(FX_E_INVALID, op + ": keys and values must be 16-byte aligned, and so their pages");
+  if (c->pages > 1 && (c->k_page_stride < bytes || c->v_page_stride < bytes || c->k_scale_page_stride < c->heads || c->v_scale_page_stride < c->heads))
+    return fail(FX_E_INVALID, op + ": pages overlap");
+  out = FxKvCache{(uint8_t*)c->k, (uint8_t*)c->v, c->k_scale, c->v_scale, c->k_page_stride, c->v_page_stride, c->k_scale_page_stride,
+                  c->v_scale_page_stride, c->pages, c->heads, c->depth, log_page_of(c->page_size)};
+  return FX_OK;
+}
+int kv_rows_of(const char* at, const FxKvCache& c, const fx_kv_rows* r, FxKvRows& out) {
+  const std::string op(at);
+  if (!r) return fail(FX_E_INVALID, op + ": null rows");
+  if (!kv_dtype(r->dtype)) return fail(FX_E_UNSUPPORTED, op + ": rows must be float32, float16 or bfloat16");
+  if (r->tokens < 0) return fail(FX_E_INVALID, op + ": negative size");
+  if (r->tokens > 0 && (!r->k || !r->v || !r->slots)) return fail(FX_E_INVALID, op + ": null argument");
+  if (r->tokens >= 1 << 30 || (int64_t)r->tokens * c.heads >= int64_t{1} << 32) return fail(FX_E_LIMIT, op + ": more rows than a launch holds");
+  out = FxKvRows{r->k, r->v, r->k_token_stride, r->k_head_stride, r->v_token_stride, r->v_head_stride, r->slots, r->tokens, r->dtype};
+  return FX_OK;
+}
+int kv_launched(int n) {
+  g_launches.fetch_add(n, std::memory_order_relaxed);
+  g_spec_launches.fetch_add(n, std::memory_order_relaxed);
+  return FX_OK;
+}
+// what a call of fx_kv_attention may be cut into
+struct KvShape {
+  bool shared;          // requests may be long enough to be cut
+  int64_t items, grid;  // tiles of rows of all heads, at most; workgroups
+};
+KvShape kv_shape(const FxKvCache& c, const fx_kv_attention_desc& d) {
+  KvShape s;
+  const int64_t group = d.q_heads / c.heads;
+  s.shared = ((int64_t)d.columns << c.log_page) > 4 * FX_KV_STEP;
+  const int64_t all = (int64_t)d.tokens * group / FX_KV_ROWS + std::min(d.requests, d.tokens);
+  const int64_t each = d.max_new > 0 ? d.requests * ((d.max_new * group + FX_KV_ROWS - 1) / FX_KV_ROWS) : all;
+  s.items = c.heads * std::min(all, each);
+  s.grid = std::min<int64_t>(std::max<int64_t>(s.items + (s.shared ? FX_KV_TARGET : 0), 1), 1 << 20);   // (a workgroup takes several where they are more)
+  return s;
+}
+size_t kv_round(size_t n) { return (n + 255) / 256 * 256; }
+}  // namespace
+
+int fx_kv_plan(const fx_kv_plan_desc* desc, void* stream) {
+  if (!desc) return fail(FX_E_INVALID, "fx_kv_plan: null descriptor");
+  const fx_kv_plan_desc& d = *desc;
+  if (log_page_of(d.page_size) < 0) return fail(FX_E_UNSUPPORTED, "fx_kv_plan: page_size must be 16, 32, 64, 128 or 256 (got " + std::to_string(d.page_size) + ")");
+  if (d.requests < 0 || d.columns < 0 || d.n_free < 0 || d.tokens < 0) return fail(FX_E_INVALID, "fx_kv_plan: negative size");
+  if (d.tokens >= 1 << 30 || d.requests >= 1 << 30 || ((int64_t)d.columns << log_page_of(d.page_size)) > int64_t{1} << 30)
+    return fail(FX_E_LIMIT, "fx_kv_plan: 2^30 tokens or requests, or more than 2^30 tokens of one request");
+  if (!d.starts || !d.taken || (d.requests > 0 && (!d.past || !d.added || !d.lens)) || (d.requests > 0 && d.columns > 0 && !d.table) ||
+      (d.n_free > 0 && !d.free_pages) || (d.tokens > 0 && (!d.slots || !d.positions)))
+    return fail(FX_E_INVALID, "fx_kv_plan: null argument");
+  if (d.requests > 1 && d.table_stride < d.columns) return fail(FX_E_INVALID, "fx_kv_plan: rows of the table overlap");
+  const FxKvPlanArgs a{d.past, d.added, d.free_pages, d.free_start, d.table, d.slots, d.positions, d.starts, d.lens, d.taken,
+                       d.table_stride, d.requests, d.columns, d.n_free, log_page_of(d.page_size), d.tokens};
+  HIP_OK(fx_launch_kv_plan(a, (hipStream_t)stream));
+  return kv_launched(1);
+}
+
+int fx_kv_store(const fx_kv_cache* cache, const fx_kv_rows* rows, void* stream) {
+  FxKvCache c;
+  FxKvRows r;
+  if (int rc = kv_cache_of("fx_kv_store", cache, c)) return rc;
+  if (int rc = kv_rows_of("fx_kv_store", c, rows, r)) return rc;
+  if (r.tokens == 0) return FX_OK;
+  HIP_OK(fx_launch_kv_store(c, r, cache->held, (hipStream_t)stream));
+  return kv_launched(1);
+}
+
+int fx_kv_read(const fx_kv_cache* cache, const fx_kv_rows* rows, void* stream) {
+  FxKvCache c;
+  FxKvRows r;
+  if (int rc = kv_cache_of("fx_kv_read", cache, c)) return rc;
+  if (int rc = kv_rows_of("fx_kv_read", c, rows, r)) return rc;
+  if (r.tokens == 0) return FX_OK;
+  HIP_OK(fx_launch_kv_read(c, r, cache->held, (hipStream_t)stream));
+  return kv_launched(1);
+}
+
+size_t fx_kv_attention_workspace_bytes(const fx_kv_cache* cache, const fx_kv_attention_desc* desc) {
+  FxKvCache c;
+  if (!desc || kv_cache_of("fx_kv_attention", cache, c) != FX_OK) return 0;
+  const size_t parts = 2 * FX_KV_TARGET * FX_KV_ROWS;
+  return 256 + kv_round(FX_KV_TARGET * sizeof(FxKvItem)) + kv_round(parts * 2 * sizeof(float)) + kv_round(parts * (size_t)c.depth * sizeof(float));
+}
+
+int fx_kv_attention(const fx_kv_cache* cache, const fx_kv_attention_desc* desc, void* stream) {
+  static const char at[] = "fx_kv_attention";
+  FxKvCache c;
+  if (int rc = kv_cache_of(at, cache, c)) return rc;
+  if (!desc) return fail(FX_E_INVALID, "fx_kv_attention: null descriptor");
+  const fx_kv_attention_desc& d = *desc;
+  if (!kv_dtype(d.dtype)) return fail(FX_E_UNSUPPORTED, "fx_kv_attention: queries must be float32, float16 or bfloat16");
+  if (d.tokens < 0 || d.requests < 0 || d.columns < 0 || d.window < 0 || d.max_new < 0) return fail(FX_E_INVALID, "fx_kv_attention: negative size");
+  if (d.q_heads < 1 || d.q_heads % c.heads != 0)
+    return fail(FX_E_INVALID, "fx_kv_attention: the query heads must be a multiple of the cache's heads (got " + std::to_string(d.q_heads) + " of " + std::to_string(c.heads) + ")");
+  if (!(d.scale > 0.0f) || !(d.scale <= std::numeric_limits<float>::max())) return fail(FX_E_INVALID, "fx_kv_attention: scale must be positive and finite");
+  if (d.tokens == 0) return FX_OK;
+  if (!d.q || !d.out || !d.lse || !d.starts || (d.requests > 0 && !d.lens) || (d.requests > 0 && d.columns > 0 && !d.table))
+    return fail(FX_E_INVALID, "fx_kv_attention: null argument");
+  if (((uintptr_t)d.out & 15u) != 0) return fail(FX_E_INVALID, "fx_kv_attention: out must be 16-byte aligned");
+  if (((int64_t)d.columns << c.log_page) > int64_t{1} << 30 || (int64_t)d.tokens * d.q_heads >= int64_t{1} << 31 || d.requests >= 1 << 30 ||
+      ((int64_t)d.tokens * d.q_heads / FX_KV_ROWS + (int64_t)std::min(d.requests, d.tokens) * c.heads) >= int64_t{1} << 30)
+    return fail(FX_E_LIMIT, "fx_kv_attention: more than 2^30 tokens of one request, or 2^31 rows of all heads");
+  if (!d.workspace || ((uintptr_t)d.workspace & 255u) != 0 || d.workspace_bytes < fx_kv_attention_workspace_bytes(cache, desc))
+    return fail(FX_E_INVALID, "fx_kv_attention: workspace must be 256-byte aligned and hold fx_kv_attention_workspace_bytes()");
+  const KvShape s = kv_shape(c, d);
+  FxKvAttnArgs a;
+  memset(&a, 0, sizeof a);
+  a.c = c;
+  a.q = d.q;
+  a.out = d.out;
+  a.lse = d.lse;
+  a.table = d.table;
+  a.lens = d.lens;
+  a.starts = d.starts;
+  a.q_token = d.q_token_stride;
+  a.q_head = d.q_head_stride;
+  a.out_token = (int64_t)d.q_heads * c.depth;
+  a.table_stride = d.table_stride;
+  a.tokens = d.tokens;
+  a.requests = d.requests;
+  a.columns = d.columns;
+  a.q_heads = d.q_heads;
+  a.group = d.q_heads / c.heads;
+  a.window = d.window >= (d.columns << c.log_page) ? 0 : d.window;   // (none so far back: all tokens)
+  a.scale = d.scale * 1.44269504088896341f;
+  a.fill = d.clear_rest;
+  char* w = (char*)d.workspace;
+  a.n_items = (int32_t*)w;
+  a.items = (FxKvItem*)(w += 256);
+  a.part_ml = (float*)(w += kv_round(FX_KV_TARGET * sizeof(FxKvItem)));
+  a.part_acc = (float*)(w += kv_round((size_t)2 * FX_KV_TARGET * FX_KV_ROWS * 2 * sizeof(float)));
+  const int type = d.dtype == FX_DT_BF16 ? 0 : d.dtype == FX_DT_F16 ? 1 : 2;
+  HIP_OK(fx_launch_kv_attention(a, cache->held, type, s.grid, s.shared ? 2048 : 0, (hipStream_t)stream));
+  return kv_launched(s.shared ? 2 : 1);
 }
 
 // ---- detection tail (fx_nms.hip) ----

@@ -1,0 +1,58 @@
+// The paged 8-bit key / value cache: arguments of its kernels (fx_kv.hip, fx_kv_attn.h).
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "../../../include/fxhip.h"
+#include "fx_kv_split.h"
+
+// A cache as the kernels see it.  Keys [pages][heads][page][depth]; values [pages][heads][page / 16][depth][16]: the
+// second product of attention contracts over tokens, and a lane's operand is 8 or 16 of them side by side.
+struct FxKvCache {
+  uint8_t *k, *v;
+  float *k_scale, *v_scale;               // [pages][heads], rows scale_stride apart
+  int64_t k_stride, v_stride;             // bytes from page to page
+  int64_t ks_stride, vs_stride;           // floats from page to page
+  int32_t pages, heads, depth, log_page;  // (page: 16 to 256 tokens, a power of two)
+};
+
+struct FxKvPlanArgs {
+  const int32_t *past, *added, *free_pages, *free_start;
+  int32_t* table;
+  int64_t* slots;
+  int32_t *positions, *starts, *lens, *taken;
+  int64_t table_stride;
+  int32_t requests, columns, n_free, log_page, tokens;
+};
+
+// rows of keys and values outside the cache: [tokens][heads][depth], a depth contiguous
+struct FxKvRows {
+  void *k, *v;
+  int64_t k_token, k_head, v_token, v_head;  // elements
+  const int64_t* slots;
+  int32_t tokens, dtype;
+};
+
+hipError_t fx_launch_kv_plan(const FxKvPlanArgs& a, hipStream_t stream);
+hipError_t fx_launch_kv_store(const FxKvCache& c, const FxKvRows& r, int held, hipStream_t stream);
+hipError_t fx_launch_kv_read(const FxKvCache& c, const FxKvRows& r, int held, hipStream_t stream);
+
+#define FX_KV_ROWS 16      // rows (tokens of a request times query heads of a key head) of a tile that a wave takes
+struct FxKvItem {   // rows whose cached tokens several workgroups shared
+  int32_t request, head, tile, first, parts;
+};
+struct FxKvAttnArgs {
+  FxKvCache c;
+  const void* q;
+  void* out;
+  float* lse;
+  const int32_t *table, *lens, *starts;
+  int64_t q_token, q_head, out_token, table_stride;   // elements (out and lse: contiguous rows of all heads)
+  int32_t tokens, requests, columns, q_heads, group, window;
+  float scale;                                        // times log2(e)
+  float* part_acc;                                    // [parts][rows of a tile][depth]
+  float* part_ml;                                     // [parts][rows of a tile][2]
+  FxKvItem* items;
+  int32_t* n_items;
+  int32_t fill;                                       // rows of no request are cleared
+};

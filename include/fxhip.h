@@ -496,6 +496,117 @@ int fx_attention_steps(const float* x, const float* k, const float* v, const flo
                        const float* wo, float* k_out, float* v_out, float* x_out, int batch, int heads, int depth, int rows,
                        int start, int steps, float scale, float k_add, float v_add, void* stream);
 
+/* ---- a paged key / value cache held in 8 bits ----
+ * What fx_attention_steps keeps in two fp32 tensors of one length (functs/benchmark/simpleops/attention/attention.py:38-58),
+ * for many requests of any length: pages of `page_size` tokens that requests share, a table of pages for each
+ * request, keys and values in 8 bits with a scale for each page and head.
+ *   fx_kv_plan       where the tokens of a step go: pages, slots, positions, offsets, from the requests' lengths
+ *   fx_kv_store      writes keys and values
+ *   fx_kv_read       gives them back as numbers
+ *   fx_kv_attention  attention over them: single tokens, a few, or whole prompts behind what is cached
+ * Everything that changes from step to step (lengths, tables, slots) is read on the device: a captured call serves any lengths
+ * that fit its tensors.  Indices are checked there: pages and slots outside the cache are passed over.
+ *
+ * A cache: k [pages][heads][page_size][depth] and v [pages][heads][page_size / 16][depth][16] codes of one byte, k_scale and
+ * v_scale [pages][heads]; a number is its code times the scale of its page and head.  Codes are e4m3 (FX_KV_E4M3, the form with
+ * no infinities) or int8 (FX_KV_INT8).  A scale is a power of two, the least 2^e with max |x| <= 448 * 2^e (e4m3) or
+ * 127 * 2^e (int8), e in [-100, 119] or [-100, 121]; a number becomes the nearest code (ties to even), infinities the largest one,
+ * NaN e4m3's NaN or int8's 0 (neither counts for the scale).
+ * page_size is 16, 32, 64, 128 or 256, depth a multiple of 16 up to 256.  k and v: 16-byte aligned, the distances from page to page
+ * (bytes; scales: floats) free otherwise, k's and v's multiples of 16. */
+#define FX_KV_E4M3 0
+#define FX_KV_INT8 1
+#define FX_KV_MAX_DEPTH 256
+typedef struct fx_kv_cache {
+  void* k;
+  void* v;
+  float* k_scale;
+  float* v_scale;
+  int64_t k_page_stride;       /* bytes */
+  int64_t v_page_stride;
+  int64_t k_scale_page_stride; /* floats */
+  int64_t v_scale_page_stride;
+  int32_t pages, heads, page_size, depth;
+  int32_t held; /* FX_KV_E4M3, FX_KV_INT8 */
+  int32_t reserved;
+} fx_kv_cache;
+
+/* Request b has past[b] cached tokens and gets added[b] more, whose rows lie one request behind the other in arrays of `tokens`
+ * rows.  A request is granted when past and added are not negative, past + added fits its row of the table
+ * (columns * page_size), its rows fit `tokens`, and the free pages that are left for it (those of all requests
+ * before it taken) are enough, or it needs none.
+ *   starts[b]     first row of request b (at most `tokens`); starts[requests]: behind the last
+ *   lens[b]       past + added if granted, else 0
+ *   positions[t]  past + j for row j of a granted request, else -1 (rows behind the last request: -1)
+ *   slots[t]      page * page_size + position % page_size, else -1
+ *   table[b]      new pages are entered behind those of the past; nothing else is written
+ *   taken[0]      how many of free_pages were given out, from free_pages[free_start[0]] on (free_start null: 0)
+ * All arrays are int32 on the device, slots int64; free_pages [n_free]; table rows table_stride apart.  One launch. */
+typedef struct fx_kv_plan_desc {
+  const int32_t* past;
+  const int32_t* added;
+  const int32_t* free_pages;
+  const int32_t* free_start;
+  int32_t* table;
+  int64_t table_stride;
+  int64_t* slots;
+  int32_t* positions;
+  int32_t* starts;
+  int32_t* lens;
+  int32_t* taken;
+  int32_t requests, columns, n_free, page_size, tokens;
+  int32_t reserved;
+} fx_kv_plan_desc;
+int fx_kv_plan(const fx_kv_plan_desc* desc, void* stream);
+
+/* Rows outside the cache: k and v [tokens][heads][depth], a depth contiguous, strides in elements; slots int64 [tokens] */
+typedef struct fx_kv_rows {
+  void* k;
+  void* v;
+  int64_t k_token_stride, k_head_stride, v_token_stride, v_head_stride;
+  const int64_t* slots;
+  int32_t tokens;
+  int32_t dtype; /* FX_DT_F32, FX_DT_F16, FX_DT_BF16 */
+} fx_kv_rows;
+/* Neighbours in `slots` that lie in one page are written together.  Where the first of them is the first of its page, the page
+ * starts anew: its scale is that of these rows.  Otherwise the page keeps its scale or takes the larger one of these rows, and its
+ * tokens before the first of them are rounded again to it; those behind are left as they were.  The rows of one page must be neighbours
+ * (as fx_kv_plan lays them): two groups of rows for one page leave what either wrote.  Slots outside the cache are passed over. */
+int fx_kv_store(const fx_kv_cache* cache, const fx_kv_rows* rows, void* stream);
+/* The numbers at `slots`, in any order, rounded once to dtype; zeros for slots outside the cache. */
+int fx_kv_read(const fx_kv_cache* cache, const fx_kv_rows* rows, void* stream);
+
+/* Rows starts[b] to starts[b + 1] of q are the last ones of request b's lens[b] tokens: of n rows, row i has position
+ * p = lens[b] - n + i and sees the tokens j <= p (window > 0: and j > p - window) whose page is in the cache.
+ *   out = sum_j softmax_j(scale * q . k_j) v_j        lse = log sum_j exp(scale * q . k_j)   (fp32)
+ * A row that sees nothing gets zeros and -infinity.  Query head h reads head h / (q_heads / heads).  What lies in the cache where
+ * a row does not see it has no influence, NaN included.
+ * q [tokens][q_heads][depth], a depth contiguous; out [tokens][q_heads][depth] and lse [tokens][q_heads] contiguous.  Rows of no
+ * request are left as they were, or get zeros and -infinity (clear_rest).  max_new: how many rows the longest request
+ * has, at most, as far as the caller knows (0: unknown); it decides on forms, not on results.  scale is positive and finite.
+ * workspace: fx_kv_attention_workspace_bytes() of device memory for each call under way, 256-byte aligned; nothing is expected in it. */
+typedef struct fx_kv_attention_desc {
+  const void* q;
+  void* out;
+  float* lse;
+  int64_t q_token_stride, q_head_stride; /* elements */
+  const int32_t* table;                  /* [requests][columns], rows table_stride apart */
+  int64_t table_stride;
+  const int32_t* lens;   /* [requests] */
+  const int32_t* starts; /* [requests + 1] */
+  int32_t tokens, requests, columns, q_heads;
+  int32_t dtype; /* of q and out: FX_DT_F32, FX_DT_F16, FX_DT_BF16 */
+  int32_t window;
+  int32_t max_new;
+  int32_t clear_rest;
+  float scale;
+  int32_t reserved;
+  void* workspace;
+  size_t workspace_bytes;
+} fx_kv_attention_desc;
+size_t fx_kv_attention_workspace_bytes(const fx_kv_cache* cache, const fx_kv_attention_desc* desc);
+int fx_kv_attention(const fx_kv_cache* cache, const fx_kv_attention_desc* desc, void* stream);
+
 /* ---- detection tail: score threshold + sort + class-aware greedy NMS + top-k, one launch ----
  * The step behind row compaction in the reference's detection programs, which it runs as ATen /
  * torchvision kernels with host synchronisations in between:
