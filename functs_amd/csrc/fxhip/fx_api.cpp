@@ -50,7 +50,6 @@ uint32_t fx_cmap_lds_bytes(const FxCmapLaunch& hl);
 uint32_t fx_cmap_chunk_rows();
 #include "fx_attn.h"
 #include "fx_kv.h"
-hipError_t fx_launch_kv_attention(const FxKvAttnArgs& a, int held, int type, int64_t grid, int64_t join_grid, hipStream_t stream);
 #include "fx_lstm_sched.h"
 int fx_launch_lstm_stack(const FxLstmArgs& a, int L, uint32_t* words_ctl, uint32_t* die_ctl, hipStream_t stream);
 int fx_lstm_ask(int form);
@@ -1681,20 +1680,26 @@ int kv_launched(int n) {
   g_spec_launches.fetch_add(n, std::memory_order_relaxed);
   return FX_OK;
 }
-// what a call of fx_kv_attention may be cut into
-struct KvShape {
-  bool shared;          // requests may be long enough to be cut
-  int64_t items, grid;  // tiles of rows of all heads, at most; workgroups
-};
-KvShape kv_shape(const FxKvCache& c, const fx_kv_attention_desc& d) {
-  KvShape s;
-  const int64_t group = d.q_heads / c.heads;
-  s.shared = ((int64_t)d.columns << c.log_page) > 4 * FX_KV_STEP;
-  const int64_t all = (int64_t)d.tokens * group / FX_KV_ROWS + std::min(d.requests, d.tokens);
-  const int64_t each = d.max_new > 0 ? d.requests * ((d.max_new * group + FX_KV_ROWS - 1) / FX_KV_ROWS) : all;
-  s.items = c.heads * std::min(all, each);
-  s.grid = std::min<int64_t>(std::max<int64_t>(s.items + (s.shared ? FX_KV_TARGET : 0), 1), 1 << 20);   // (a workgroup takes several where they are more)
-  return s;
+// Which kernels a call of fx_kv_attention needs, and how many workgroups: what the host knows are sizes, not lengths.
+// One request has one kernel; of several some may have few rows and some many, which max_new can rule out.
+FxKvLaunch kv_launch(const FxKvCache& c, const fx_kv_attention_desc& d) {
+  FxKvLaunch l;
+  memset(&l, 0, sizeof l);
+  l.held = 0;
+  l.type = d.dtype == FX_DT_BF16 ? 0 : d.dtype == FX_DT_F16 ? 1 : 2;
+  l.shared = ((int64_t)d.columns << c.log_page) > 4 * FX_KV_STEP;
+  const int64_t group = d.q_heads / c.heads, some = std::min(d.requests, d.tokens);
+  const int64_t longest = (d.max_new > 0 ? std::min(d.max_new, d.tokens) : d.tokens) * group;   // rows of one request
+  const int64_t all = (int64_t)d.tokens * group;
+  const bool many = longest > FX_KV_FEW, few = !many || d.requests != 1;
+  // (at least 1: requests or rows may be none; at most 2^20: a workgroup takes several units where there are more)
+  auto grid = [&](int tile, int64_t longest) {
+    const int64_t items = c.heads * std::min(all / tile + some, some * ((longest + tile - 1) / tile));
+    return std::min<int64_t>(std::max<int64_t>(items + (l.shared ? FX_KV_TARGET : 0), 1), 1 << 20);
+  };
+  if (many) l.tiles_grid = grid(FX_KV_TILE, longest);
+  if (few) l.rows_grid = grid(FX_KV_ROWS, many ? FX_KV_FEW : longest);
+  return l;
 }
 size_t kv_round(size_t n) { return (n + 255) / 256 * 256; }
 }  // namespace
@@ -1739,8 +1744,10 @@ int fx_kv_read(const fx_kv_cache* cache, const fx_kv_rows* rows, void* stream) {
 size_t fx_kv_attention_workspace_bytes(const fx_kv_cache* cache, const fx_kv_attention_desc* desc) {
   FxKvCache c;
   if (!desc || kv_cache_of("fx_kv_attention", cache, c) != FX_OK) return 0;
-  const size_t parts = 2 * FX_KV_TARGET * FX_KV_ROWS;
-  return 256 + kv_round(FX_KV_TARGET * sizeof(FxKvItem)) + kv_round(parts * 2 * sizeof(float)) + kv_round(parts * (size_t)c.depth * sizeof(float));
+  // (one after the other, the kernels of a call use the same memory)
+  const size_t parts = (size_t)2 * FX_KV_TARGET * (kv_launch(c, *desc).tiles_grid > 0 ? FX_KV_TILE : FX_KV_ROWS);
+  const size_t offsets = kv_round(((size_t)std::max(desc->requests, 0) * 2 + 3) * sizeof(int32_t));   // (fx_kv_offsets)
+  return 256 + offsets + kv_round(FX_KV_TARGET * sizeof(FxKvItem)) + kv_round(parts * 2 * sizeof(float)) + kv_round(parts * (size_t)c.depth * sizeof(float));
 }
 
 int fx_kv_attention(const fx_kv_cache* cache, const fx_kv_attention_desc* desc, void* stream) {
@@ -1759,11 +1766,12 @@ int fx_kv_attention(const fx_kv_cache* cache, const fx_kv_attention_desc* desc, 
     return fail(FX_E_INVALID, "fx_kv_attention: null argument");
   if (((uintptr_t)d.out & 15u) != 0) return fail(FX_E_INVALID, "fx_kv_attention: out must be 16-byte aligned");
   if (((int64_t)d.columns << c.log_page) > int64_t{1} << 30 || (int64_t)d.tokens * d.q_heads >= int64_t{1} << 31 || d.requests >= 1 << 30 ||
-      ((int64_t)d.tokens * d.q_heads / FX_KV_ROWS + (int64_t)std::min(d.requests, d.tokens) * c.heads) >= int64_t{1} << 30)
+      (int64_t)std::min(d.requests, d.tokens) * c.heads >= int64_t{1} << 30)
     return fail(FX_E_LIMIT, "fx_kv_attention: more than 2^30 tokens of one request, or 2^31 rows of all heads");
   if (!d.workspace || ((uintptr_t)d.workspace & 255u) != 0 || d.workspace_bytes < fx_kv_attention_workspace_bytes(cache, desc))
     return fail(FX_E_INVALID, "fx_kv_attention: workspace must be 256-byte aligned and hold fx_kv_attention_workspace_bytes()");
-  const KvShape s = kv_shape(c, d);
+  FxKvLaunch l = kv_launch(c, d);
+  l.held = cache->held;
   FxKvAttnArgs a;
   memset(&a, 0, sizeof a);
   a.c = c;
@@ -1785,14 +1793,16 @@ int fx_kv_attention(const fx_kv_cache* cache, const fx_kv_attention_desc* desc, 
   a.window = d.window >= (d.columns << c.log_page) ? 0 : d.window;   // (none so far back: all tokens)
   a.scale = d.scale * 1.44269504088896341f;
   a.fill = d.clear_rest;
+  const int64_t q_size = d.dtype == FX_DT_F32 ? 4 : 2;
+  a.q_vec = ((uintptr_t)d.q & 15u) == 0 && d.q_token_stride * q_size % 16 == 0 && d.q_head_stride * q_size % 16 == 0;
   char* w = (char*)d.workspace;
   a.n_items = (int32_t*)w;
-  a.items = (FxKvItem*)(w += 256);
+  a.offsets = (int32_t*)(w += 256);
+  a.items = (FxKvItem*)(w += kv_round(((size_t)d.requests * 2 + 3) * sizeof(int32_t)));
   a.part_ml = (float*)(w += kv_round(FX_KV_TARGET * sizeof(FxKvItem)));
-  a.part_acc = (float*)(w += kv_round((size_t)2 * FX_KV_TARGET * FX_KV_ROWS * 2 * sizeof(float)));
-  const int type = d.dtype == FX_DT_BF16 ? 0 : d.dtype == FX_DT_F16 ? 1 : 2;
-  HIP_OK(fx_launch_kv_attention(a, cache->held, type, s.grid, s.shared ? 2048 : 0, (hipStream_t)stream));
-  return kv_launched(s.shared ? 2 : 1);
+  a.part_acc = (float*)(w += kv_round((size_t)2 * FX_KV_TARGET * (l.tiles_grid > 0 ? FX_KV_TILE : FX_KV_ROWS) * 2 * sizeof(float)));
+  HIP_OK(fx_launch_kv_attention(a, l, (hipStream_t)stream));
+  return kv_launched(((l.rows_grid > 0) + (l.tiles_grid > 0)) * (l.shared ? 2 : 1));   // (fx_kv_offsets aside)
 }
 
 // ---- detection tail (fx_nms.hip) ----

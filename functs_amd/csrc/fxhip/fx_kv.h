@@ -37,7 +37,9 @@ hipError_t fx_launch_kv_plan(const FxKvPlanArgs& a, hipStream_t stream);
 hipError_t fx_launch_kv_store(const FxKvCache& c, const FxKvRows& r, int held, hipStream_t stream);
 hipError_t fx_launch_kv_read(const FxKvCache& c, const FxKvRows& r, int held, hipStream_t stream);
 
-#define FX_KV_ROWS 16      // rows (tokens of a request times query heads of a key head) of a tile that a wave takes
+#define FX_KV_ROWS 16   // rows (tokens of a request times query heads of a key head) of a tile of fx_kv_rows
+#define FX_KV_TILE 128  // rows of a tile of fx_kv_tiles
+#define FX_KV_FEW 48    // requests of more rows are fx_kv_tiles' where a call may have both
 struct FxKvItem {   // rows whose cached tokens several workgroups shared
   int32_t request, head, tile, first, parts;
 };
@@ -54,5 +56,14 @@ struct FxKvAttnArgs {
   float* part_ml;                                     // [parts][rows of a tile][2]
   FxKvItem* items;
   int32_t* n_items;
+  int32_t* offsets;                                   // of more than 256 requests: see fx_kv_offsets
   int32_t fill;                                       // rows of no request are cleared
+  int32_t q_vec;                                      // rows of queries are 16-byte aligned
+  int64_t rows_above, rows_upto;                      // requests that this kernel takes: by rows of all query heads of a key head
 };
+struct FxKvLaunch {
+  int held, type;                   // FX_KV_E4M3, FX_KV_INT8; 0 bf16, 1 fp16, 2 fp32
+  bool shared;                      // items may be shared by workgroups
+  int64_t rows_grid, tiles_grid;    // workgroups of fx_kv_rows and fx_kv_tiles (0: not needed)
+};
+hipError_t fx_launch_kv_attention(const FxKvAttnArgs& a, const FxKvLaunch& l, hipStream_t stream);

@@ -52,6 +52,8 @@ __device__ __forceinline__ Frag eight(unsigned lo, unsigned hi) {
   f.u[3] = two<HELD, F16, true>(hi);
   return f;
 }
+// the bytes of a word that are e4m3's NaN: 0x80 in each
+__device__ __forceinline__ unsigned nan_codes(unsigned w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
 template <bool F16>
 __device__ __forceinline__ fx_f32x4 mfma16(const Frag& a, const Frag& b, fx_f32x4 c) {
   if constexpr (F16) return __builtin_amdgcn_mfma_f32_16x16x32_f16(a.h, b.h, c, 0, 0, 0);
@@ -84,75 +86,140 @@ struct Unit {
   FxKvRequest r;
   int request, head, tile, split, splits, part, item;
 };
-__device__ __forceinline__ FxKvRequest request_at(const FxKvAttnArgs& a, int b, int tile_rows) {
-  if (b >= a.requests) return FxKvRequest{0, 0, 0, 0, 0};
-  return fx_kv_request(a.starts[b], a.starts[b + 1], a.lens[b], a.tokens, a.columns << a.c.log_page, a.group, a.window, tile_rows);
+// (a request whose rows are the other kernel's has no tiles here)
+__device__ __forceinline__ FxKvRequest request_of(const FxKvAttnArgs& a, int start, int end, int len, int tile_rows) {
+  FxKvRequest r = fx_kv_request(start, end, len, a.tokens, a.columns << a.c.log_page, a.group, a.window, tile_rows);
+  if ((int64_t)r.rows * a.group <= a.rows_above || (int64_t)r.rows * a.group > a.rows_upto) r.tiles = 0;
+  return r;
 }
-template <int THREADS>
-__device__ __forceinline__ int64_t sum_before(int64_t v, int64_t* scratch, int64_t* total) {
-  const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6;
-  int64_t s = v;
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int dpp_add(int v) { return v + __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xf, false); }
+// sum over the lanes up to this one
+__device__ __forceinline__ int sum_upto(int v) {
+  v = dpp_add<0x111, 0xf>(v);   // row_shr: 1, 2, 4, 8
+  v = dpp_add<0x112, 0xf>(v);
+  v = dpp_add<0x114, 0xf>(v);
+  v = dpp_add<0x118, 0xf>(v);
+  v = dpp_add<0x142, 0xa>(v);   // row_bcast: 15, 31
+  return dpp_add<0x143, 0xc>(v);
+}
+// 43-bit numbers of the lanes, added up in two parts; one that is larger (no call has so many steps) counts as endless: nothing is cut then
+__device__ __forceinline__ int64_t wave_total(int64_t v) {
+  const bool endless = v >= int64_t{1} << 43;
+  const int low = sum_upto((int)(v & 0xfffff)), high = sum_upto(endless ? 0 : (int)(v >> 20));
+  const int64_t all = ((int64_t)__builtin_amdgcn_readlane(high, 63) << 20) + __builtin_amdgcn_readlane(low, 63);
+  return __any(endless) ? int64_t{1} << 60 : all;
+}
+__device__ __forceinline__ int64_t all_steps(const FxKvAttnArgs& a, int64_t steps) {   // of all heads
+  return steps >= int64_t{1} << 60 ? steps : steps * a.c.heads;
+}
+
+// Unit u of the call, or false behind the last one: every wave finds it by itself, in scalar registers, without a barrier.  Up
+// to kScanned requests are added up here, a lane four of them at most; of more, fx_kv_offsets has left the sums.
+// SORTED: of up to 64 requests those of more steps come first, so that what is left at the end of a call is short.
+constexpr int kScanned = 256, kScanPer = kScanned / 64;
+constexpr int kRowLeast = 4, kTileLeast = 8;   // chunks are multiples of so many steps (fx_kv_rows: of one for each wave)
+template <bool SORTED>
+__device__ __forceinline__ bool unit_at(const FxKvAttnArgs& a, int tile_rows, int least, int u, Unit& x, int* shared_items) {
+  const int lane = (int)threadIdx.x & 63;
+  int chunk, rest, parts;   // rest: the unit's number in its request; parts: items << 16 | parts before the request
+  if (a.requests <= kScanned) {
+    const int per = (a.requests + 63) >> 6;
+    int start[kScanPer], end[kScanPer], len[kScanPer], tiles[kScanPer], steps[kScanPer];
+    int64_t work = 0;
 #pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const int64_t o = (int64_t)__shfl_up((unsigned long long)s, (unsigned)d, 64);
-    if (lane >= d) s += o;
-  }
-  if (lane == 63) scratch[wave] = s;
-  __syncthreads();
-  int64_t before = 0, all = 0;
-#pragma unroll
-  for (int w = 0; w < THREADS / 64; ++w) {
-    if (w < wave) before += scratch[w];
-    all += scratch[w];
-  }
-  __syncthreads();
-  *total = all;
-  return before + s - v;
-}
-template <int THREADS>
-__device__ int chunk_of(const FxKvAttnArgs& a, int tile_rows, int least, int64_t* scratch) {
-  int64_t work = 0, all = 0;
-  for (int b0 = 0; b0 < a.requests; b0 += THREADS) {
-    const FxKvRequest r = request_at(a, b0 + (int)threadIdx.x, tile_rows);
-    work += (int64_t)r.tiles * r.steps;
-  }
-  sum_before<THREADS>(work, scratch, &all);
-  return fx_kv_chunk(all * a.c.heads, least);
-}
-// Unit u of the call, or false behind the last one; *shared_items: how many items several workgroups share
-template <int THREADS>
-__device__ bool unit_at(const FxKvAttnArgs& a, int tile_rows, int chunk, int u, Unit& out, Unit* s_unit, int64_t* scratch, int* shared_items) {
-  int64_t carry_units = 0, carry_parts = 0;   // carry_parts: items << 32 | parts
-  if (threadIdx.x == 0) s_unit->r.rows = 0;
-  for (int b0 = 0; b0 < a.requests; b0 += THREADS) {
-    const int b = b0 + (int)threadIdx.x;
-    const FxKvRequest r = request_at(a, b, tile_rows);
-    const int splits = fx_kv_parts(r.steps, chunk);
-    const int64_t items = (int64_t)r.tiles * a.c.heads, units = items * splits;
-    int64_t all_units, all_parts;
-    const int64_t before = carry_units + sum_before<THREADS>(units, scratch, &all_units);
-    const int64_t parts = carry_parts + sum_before<THREADS>(splits > 1 ? (items << 32) + units : 0, scratch, &all_parts);
-    if (u >= before && u < before + units) {
-      const int i = (int)(u - before), item = i / splits;
-      Unit x;
-      x.r = r;
-      x.request = b;
-      x.head = item % a.c.heads;
-      x.tile = item / a.c.heads;
-      x.split = i - item * splits;
-      x.splits = splits;
-      x.part = (int)(parts & 0xffffffff) + item * splits;
-      x.item = (int)(parts >> 32) + item;
-      *s_unit = x;
+    for (int j = 0; j < kScanPer; ++j) {
+      start[j] = end[j] = len[j] = tiles[j] = steps[j] = 0;
+      if (j < per) {
+        const int b = lane * per + j, c = min(b, a.requests - 1);
+        start[j] = a.starts[c];
+        end[j] = b < a.requests ? a.starts[c + 1] : start[j];
+        len[j] = a.lens[c];
+      }
     }
-    carry_units += all_units;
-    carry_parts += all_parts;
+#pragma unroll
+    for (int j = 0; j < kScanPer; ++j)
+      if (j < per) {
+        const FxKvRequest r = request_of(a, start[j], end[j], len[j], tile_rows);
+        tiles[j] = r.tiles;
+        steps[j] = r.steps;
+        work += (int64_t)r.tiles * r.steps;
+      }
+    chunk = fx_kv_chunk(all_steps(a, wave_total(work)), least);
+    int units[kScanPer], cut[kScanPer], mine = 0, cuts = 0;
+#pragma unroll
+    for (int j = 0; j < kScanPer; ++j) {
+      units[j] = cut[j] = 0;
+      if (j < per) {
+        const int splits = fx_kv_parts(steps[j], chunk), items = tiles[j] * a.c.heads;
+        units[j] = items * splits;
+        cut[j] = splits > 1 ? (items << 16) + units[j] : 0;
+        mine += units[j];
+        cuts += cut[j];
+      }
+    }
+    const int upto_cuts = sum_upto(cuts);
+    int before;
+    if (SORTED && per <= 1) {
+      before = 0;
+      for (int c = 0; c < a.requests; ++c) {
+        const int n = __builtin_amdgcn_readlane(steps[0], c), add = __builtin_amdgcn_readlane(mine, c);
+        if (n > steps[0] || (n == steps[0] && c < lane)) before += add;
+      }
+    } else {
+      before = sum_upto(mine) - mine;
+    }
+    *shared_items = (unsigned)__builtin_amdgcn_readlane(upto_cuts, 63) >> 16;
+    const unsigned long long owner = __ballot(u >= before && u < before + mine);
+    if (owner == 0) return false;
+    const int L = __builtin_ctzll(owner);
+    int at = u - before, cut_before = upto_cuts - cuts, which = 0;
+#pragma unroll
+    for (int j = 0; j + 1 < kScanPer; ++j)
+      if (which == j && at >= units[j]) {
+        at -= units[j];
+        cut_before += cut[j];
+        which = j + 1;
+      }
+    int s = start[0], e = end[0], n = len[0];
+#pragma unroll
+    for (int j = 1; j < kScanPer; ++j)
+      if (which == j) {
+        s = start[j];
+        e = end[j];
+        n = len[j];
+      }
+    x.request = L * per + __builtin_amdgcn_readlane(which, L);
+    x.r = request_of(a, __builtin_amdgcn_readlane(s, L), __builtin_amdgcn_readlane(e, L), __builtin_amdgcn_readlane(n, L), tile_rows);
+    rest = __builtin_amdgcn_readlane(at, L);
+    parts = __builtin_amdgcn_readlane(cut_before, L);
+  } else {
+    const int32_t* units = a.offsets + 2;   // [requests + 1], then [requests] of parts
+    chunk = a.offsets[0];
+    *shared_items = a.offsets[1];
+    int lo = 0, hi = a.requests;
+    if (u >= units[hi]) return false;
+    while (hi - lo > 1) {
+      const int step = (hi - lo + 63) >> 6, at = min(lo + lane * step, hi);
+      const int last = 63 - __builtin_clzll(__ballot(at < hi && units[at] <= u));   // (lane 0 always)
+      lo += last * step;
+      hi = min(lo + step, hi);
+    }
+    x.request = __builtin_amdgcn_readfirstlane(lo);
+    rest = u - __builtin_amdgcn_readfirstlane(units[lo]);
+    parts = __builtin_amdgcn_readfirstlane(units[a.requests + 1 + lo]);
+    x.r = request_of(a, __builtin_amdgcn_readfirstlane(a.starts[lo]), __builtin_amdgcn_readfirstlane(a.starts[lo + 1]), __builtin_amdgcn_readfirstlane(a.lens[lo]), tile_rows);
   }
-  __syncthreads();
-  out = *s_unit;
-  *shared_items = (int)(carry_parts >> 32);
-  return out.r.rows > 0;
+  x.splits = fx_kv_parts(x.r.steps, chunk);
+  const int item = rest / x.splits;
+  x.split = rest - item * x.splits;
+  x.tile = item / a.c.heads;
+  x.head = item - x.tile * a.c.heads;
+  x.part = (parts & 0xffff) + item * x.splits;
+  x.item = (int)((unsigned)parts >> 16) + item;
+  return true;
 }
+static_assert(2 * FX_KV_TARGET < 1 << 15 && FX_KV_TARGET < 1 << 15, "parts and items in 16 bits each");
 
 template <class T>
 __device__ __forceinline__ void store4(T* p, const float* x) {
@@ -166,6 +233,34 @@ template <int TQ> struct TypeOf;
 template <> struct TypeOf<kBf16> { typedef __bf16 type; };
 template <> struct TypeOf<kF16> { typedef _Float16 type; };
 template <> struct TypeOf<kF32> { typedef float type; };
+
+// Eight numbers of a row of queries at depth d as operands (zeros where `in` is false: what is loaded then is the row's first ones)
+template <int TQ, int NQ, class T>
+__device__ __forceinline__ void load_query(Frag* const (&f)[NQ], const T* src, int d, bool in, bool vec) {
+  const T* p = src + (in ? d : 0);
+  union { uint4 u[sizeof(T) / 2]; T e[8]; } w;
+  if (vec) {
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) w.u[i] = ((const uint4*)p)[i];
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) w.e[e] = p[e];
+  }
+  if constexpr (TQ == kF32) {
+    float v[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = in ? w.e[e] : 0.0f;
+    Frag s[NQ];
+    split8<NQ>(s, v);
+#pragma unroll
+    for (int k = 0; k < NQ; ++k) *f[k] = s[k];
+  } else {
+    f[0]->u[0] = in ? w.u[0].x : 0u;
+    f[0]->u[1] = in ? w.u[0].y : 0u;
+    f[0]->u[2] = in ? w.u[0].z : 0u;
+    f[0]->u[3] = in ? w.u[0].w : 0u;
+  }
+}
 
 // Rows of no request: zeros, and nothing under the logarithm
 template <class T>
@@ -190,20 +285,16 @@ __global__ __launch_bounds__(256) void fx_kv_rows(const FxKvAttnArgs a) {
   constexpr bool F16 = TQ == kF16;
   __shared__ __align__(16) float s_acc[W][FX_KV_ROWS][LD];
   __shared__ float s_ml[W][FX_KV_ROWS][2];
-  __shared__ int64_t s_scan[W];
-  __shared__ Unit s_unit;
   const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6;
   const int col = lane & 15, kg = lane >> 4;
   const int D = EXACT ? DP : a.c.depth, G = a.group, lp = a.c.log_page, pm = (1 << lp) - 1;
-  if (a.fill) fill_rest<T>(a);
-  const int chunk = chunk_of<256>(a, FX_KV_ROWS, W, s_scan);
   for (int u = (int)blockIdx.x;; u += (int)gridDim.x) {
     Unit x;
-    int shared_items;
-    if (u != (int)blockIdx.x) __syncthreads();
-    const bool live = unit_at<256>(a, FX_KV_ROWS, chunk, u, x, &s_unit, s_scan, &shared_items);
+    int shared_items = 0;
+    const bool live = unit_at<false>(a, FX_KV_ROWS, kRowLeast, u, x, &shared_items);
     if (u == 0 && threadIdx.x == 0) *a.n_items = shared_items;
-    if (!live) return;
+    if (!live) break;
+    if (u != (int)blockIdx.x) __syncthreads();   // (LDS is free again)
     // rows
     const int r0 = x.tile * FX_KV_ROWS, row = r0 + col;
     const bool valid = row < x.r.rows * G;
@@ -219,21 +310,10 @@ __global__ __launch_bounds__(256) void fx_kv_rows(const FxKvAttnArgs a) {
 #pragma unroll
       for (int c = 0; c < 2 * C; ++c) {
         const int d = (c >> 1) * 64 + kg * 16 + (c & 1) * 8;
-        const bool in = valid && d < D;
-        if constexpr (TQ == kF32) {
-          float v[8];
+        Frag* f[NQ];
 #pragma unroll
-          for (int e = 0; e < 8; ++e) v[e] = in ? src[d + e] : 0.0f;
-          Frag f[NQ];
-          split8<NQ>(f, v);
-#pragma unroll
-          for (int k = 0; k < NQ; ++k) q[k][c] = f[k];
-        } else {
-          T v[8];
-#pragma unroll
-          for (int e = 0; e < 8; ++e) v[e] = in ? src[d + e] : (T)0.0f;
-          q[0][c] = *(const Frag*)v;
-        }
+        for (int k = 0; k < NQ; ++k) f[k] = &q[k][c];
+        load_query<TQ, NQ, T>(f, src, d, valid && d < D, a.q_vec != 0);
       }
     }
     fx_f32x4 acc[DT];
@@ -245,6 +325,10 @@ __global__ __launch_bounds__(256) void fx_kv_rows(const FxKvAttnArgs a) {
     const int64_t head_at = (int64_t)x.head * (pm + 1) * D;
     auto page_of = [&](int token) { return fx_kv_page(table[min(token >> lp, a.columns - 1)], a.c.pages); };   // -1: none
     uint4 kr[4][C];
+    // a lane beyond the depth takes its row's first numbers again: its queries there are 0
+    int k_at[C];
+#pragma unroll
+    for (int c = 0; c < C; ++c) k_at[c] = c * 64 + kg * 16 < D ? c * 64 : -kg * 16;
     auto load_keys = [&](int step, int page) {
       const int at = (step * FX_KV_STEP + k_group) & pm;
       const uint8_t* p = a.c.k + (int64_t)page * a.c.k_stride + head_at + (int64_t)(at + k_row) * D + kg * 16;
@@ -252,8 +336,7 @@ __global__ __launch_bounds__(256) void fx_kv_rows(const FxKvAttnArgs a) {
       for (int r = 0; r < 4; ++r)
 #pragma unroll
         for (int c = 0; c < C; ++c)
-          if (EXACT || c * 64 + kg * 16 < D) kr[r][c] = *(const uint4*)(p + r * 4 * D + c * 64);
-          else kr[r][c] = make_uint4(0, 0, 0, 0);
+          kr[r][c] = *(const uint4*)(p + r * 4 * D + (EXACT ? c * 64 : k_at[c]));
     };
         int step = from + wave, pk = 0, pv = 0;
     if (step < to) {
@@ -321,7 +404,7 @@ __global__ __launch_bounds__(256) void fx_kv_rows(const FxKvAttnArgs a) {
 #pragma unroll
             for (int w = 0; w < 4; ++w) {
               v[w] &= keep[w];
-              if constexpr (HELD == 0) nans |= ((v[w] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
+              if constexpr (HELD == 0) nans |= nan_codes(v[w]);
             }
           }
         if constexpr (HELD == 0) {
@@ -344,7 +427,7 @@ __global__ __launch_bounds__(256) void fx_kv_rows(const FxKvAttnArgs a) {
                 unsigned is[4];
 #pragma unroll
                 for (int w = 0; w < 4; ++w) {
-                  const unsigned n = (((v[w] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) >> 7;
+                  const unsigned n = nan_codes(v[w]) >> 7;
                   is[w] = n * 0x38u;   // e4m3's 1
                   v[w] &= ~(n * 0xffu);
                 }
@@ -451,49 +534,414 @@ __global__ __launch_bounds__(256) void fx_kv_rows(const FxKvAttnArgs a) {
     if (x.splits > 1 && x.split == 0 && threadIdx.x == 0)
       a.items[x.item] = FxKvItem{x.request, x.head, x.tile, x.part, x.splits};
   }
+  if (a.fill) fill_rest<T>(a);
 }
 
-// What several workgroups found for the same rows, added up in their order.  A workgroup takes a row of an item, a wave the
-// depths of it.
+// ---- 128 rows a tile: prompts ----
+// Bound: the vector units, which turn scores into weights, beside the matrix cores.  Four waves take 32 rows each and share the
+// cached tokens, 64 a step: each wave turns a quarter of the step's codes into 16-bit floats and leaves them in LDS for all four,
+// in one of two buffers while the other one is computed with.  32 x 32 products; as above the scores stay where the second
+// product reads them: row 8 g + 4 h + j of K's operand is token 16 h + 4 g + j, so a lane holds the 16 tokens of one group.
+// In LDS a key's row of 16-byte pieces is permuted by its token (key_piece), which spreads the 32 rows of an operand over the banks; values
+// lie as [group][8 tokens of it][depth][8 tokens].
+typedef float fx_f32x16 __attribute__((ext_vector_type(16)));
+template <bool F16>
+__device__ __forceinline__ fx_f32x16 mfma32(const Frag& a, const Frag& b, fx_f32x16 c) {
+  if constexpr (F16) return __builtin_amdgcn_mfma_f32_32x32x16_f16(a.h, b.h, c, 0, 0, 0);
+  else return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.b, b.b, c, 0, 0, 0);
+}
+template <int DP>
+__device__ __forceinline__ int key_piece(int token, int piece) {   // where 8 numbers of a key lie in its row
+  constexpr int kMask = DP / 8 - 1 < 15 ? DP / 8 - 1 : 15;
+  return piece ^ (((token & 3) | ((token >> 2) & 4) | ((token << 1) & 8)) & kMask);
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {   // (fmaxf quiets what the matrix cores give it, an instruction for each)
+  float r;
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+  return r;
+}
+
+// N operands from LDS, four at a time, each four on their way while the four before are used: read(i) gives operand i, use(i, operand)
+// takes it.  (Left to itself the compiler reads each one right before its product, to save registers.)
+template <int N, class Read, class Use>
+__device__ __forceinline__ void piped(Read read, Use use) {
+  Frag f[2][4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) f[0][e] = read(e);
+#pragma unroll
+  for (int b = 0; b < N / 4; ++b) {
+    __builtin_amdgcn_sched_barrier(0);
+    if (b + 1 < N / 4)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) f[(b + 1) & 1][e] = read((b + 1) * 4 + e);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) use(b * 4 + e, f[b & 1][e]);
+  }
+}
+
+template <int HELD, int TQ, int DP, bool EXACT>
+__global__ __launch_bounds__(256, DP <= 128 && TQ != kF32 ? 2 : 1) void fx_kv_tiles(const FxKvAttnArgs a) {
+  typedef typename TypeOf<TQ>::type T;
+  constexpr int W = 4, NQ = TQ == kF32 ? 3 : 1, NP = TQ == kF32 ? 3 : TQ == kF16 ? 2 : 1, C = DP / 16, DT = DP / 32;
+  constexpr int kBlocks = DP / 64;   // KB of a step's keys that a wave takes, and as many of its values
+  constexpr int kTile = FX_KV_STEP * DP * 2;
+  constexpr bool F16 = TQ == kF16;
+  __shared__ __align__(16) uint8_t s_kv[2][2][kTile];
+  __shared__ int s_nan;   // e4m3: there were NaN among the values
+  const int lane = (int)threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int col = lane & 31, half = lane >> 5;
+  const int D = EXACT ? DP : a.c.depth, G = a.group, lp = a.c.log_page, pm = (1 << lp) - 1;
+  for (int u = (int)blockIdx.x;; u += (int)gridDim.x) {
+    Unit x;
+    int shared_items = 0;
+    const bool live = unit_at<true>(a, FX_KV_TILE, kTileLeast, u, x, &shared_items);
+    if (u == 0 && threadIdx.x == 0) *a.n_items = shared_items;
+    if (!live) break;
+    __syncthreads();   // (LDS is free again)
+    if (threadIdx.x == 0) s_nan = 0;
+    __syncthreads();
+    x.tile = x.r.tiles - 1 - x.tile;   // (the last rows see most: they begin first)
+    const int r0 = x.tile * FX_KV_TILE, w0 = r0 + wave * 32, row = w0 + col, n_rows = x.r.rows * G;
+    const bool valid = row < n_rows;
+    const int i = valid ? row / G : 0, g = valid ? row - i * G : 0;
+    const int hi_row = valid ? x.r.len - x.r.rows + i + 1 : 0;
+    const int lo_row = a.window > 0 ? max(hi_row - a.window, 0) : 0;
+    const FxKvSpan span = fx_kv_span(x.r, G, a.window, r0, FX_KV_TILE, x.split, x.splits);
+    FxKvSpan mine = fx_kv_span(x.r, G, a.window, min(w0, n_rows - 1), 32, 0, 1);   // of this wave's rows
+    if (w0 >= n_rows) mine.high = 0;
+    const int from = span.from, to = span.to;
+    Frag q[NQ][C];
+    {
+      const T* src = (const T*)a.q + (int64_t)(x.r.start + i) * a.q_token + (int64_t)(x.head * G + g) * a.q_head;
+#pragma unroll
+      for (int c = 0; c < C; ++c) {
+        const int d = c * 16 + half * 8;
+        Frag* f[NQ];
+#pragma unroll
+        for (int k = 0; k < NQ; ++k) f[k] = &q[k][c];
+        load_query<TQ, NQ, T>(f, src, d, valid && d < D, a.q_vec != 0);
+      }
+    }
+    fx_f32x16 acc[DT];
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) acc[d][e] = 0.0f;
+    float m = -kInf, l = 0.0f;
+    const int32_t* table = a.table + (int64_t)x.request * a.table_stride;
+    const int64_t head_at = (int64_t)x.head * (pm + 1) * D;
+    // the entry for group `lane & 3` of a step, as it is: looked at when it is used, a step later
+    auto entries_of = [&](int step) { return table[min((step * FX_KV_STEP + (lane & 3) * 16) >> lp, a.columns - 1)]; };
+    // A step's codes on their way: block k * W + wave of 1 KB is 64 bytes of depth for the 16 tokens of a group
+    uint4 kraw[kBlocks], vraw[kBlocks];
+    constexpr int kPieces = DP / 16, kRows = 1024 / DP;
+    auto load_step = [&](int step, int pages) {
+#pragma unroll
+      for (int k = 0; k < kBlocks; ++k) {
+        const int block = k * W + wave, group = block / kBlocks, part = block % kBlocks;
+        const int page = max(__builtin_amdgcn_readlane(pages, group), 0);
+        const int at = (step * FX_KV_STEP + group * 16) & pm;
+        const int token = part * kRows + lane / kPieces;   // of its group
+        int piece = lane % kPieces, d = part * 64 + lane;
+        if (!EXACT) {   // (queries beyond the depth are 0, results there are dropped)
+          piece = piece * 16 < D ? piece : 0;
+          d = min(d, D - 1);
+        }
+        kraw[k] = *(const uint4*)(a.c.k + (int64_t)page * a.c.k_stride + head_at + (int64_t)(at + token) * D + piece * 16);
+        vraw[k] = *(const uint4*)(a.c.v + (int64_t)page * a.c.v_stride + head_at + (int64_t)at * D + d * 16);
+      }
+    };
+    auto write_step = [&](int buffer) {
+      uint8_t* kt = s_kv[buffer][0];
+      uint8_t* vt = s_kv[buffer][1];
+      if constexpr (HELD == 0) {
+        unsigned nans = 0;
+#pragma unroll
+        for (int k = 0; k < kBlocks; ++k) nans |= nan_codes(vraw[k].x) | nan_codes(vraw[k].y) | nan_codes(vraw[k].z) | nan_codes(vraw[k].w);
+        if (__any(nans != 0)) {
+          if (lane == 0) s_nan = 1;
+#pragma unroll
+          for (int k = 0; k < kBlocks; ++k) {
+            unsigned* u = (unsigned*)&vraw[k];
+#pragma unroll
+            for (int w = 0; w < 4; ++w) u[w] &= ~((nan_codes(u[w]) >> 7) * 0xffu);
+          }
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < kBlocks; ++k) {
+        const int block = k * W + wave, group = block / kBlocks, part = block % kBlocks;
+        const int token = group * 16 + part * kRows + lane / kPieces, piece = lane % kPieces;
+        *(Frag*)(kt + token * DP * 2 + key_piece<DP>(token, piece * 2) * 16) = eight<HELD, F16>(kraw[k].x, kraw[k].y);
+        *(Frag*)(kt + token * DP * 2 + key_piece<DP>(token, piece * 2 + 1) * 16) = eight<HELD, F16>(kraw[k].z, kraw[k].w);
+        uint8_t* v = vt + (group * 2 * DP + part * 64 + lane) * 16;
+        *(Frag*)v = eight<HELD, false>(vraw[k].x, vraw[k].y);
+        *(Frag*)(v + DP * 16) = eight<HELD, false>(vraw[k].z, vraw[k].w);
+      }
+    };
+    int pg[2] = {0, 0};             // pages of the lane's two groups of a step (-1: none), and their scales
+    float ks[2], vs[2];
+    auto scales_of = [&](int pages) {
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        pg[t] = __shfl(pages, t * 2 + half, 64);
+        ks[t] = a.c.k_scale[(int64_t)max(pg[t], 0) * a.c.ks_stride + x.head];
+        vs[t] = a.c.v_scale[(int64_t)max(pg[t], 0) * a.c.vs_stride + x.head];
+      }
+    };
+    // What is under way: codes of step + 1 in registers, entries of step + 2, scales of `step`
+    int pages1 = 0, entries2 = 0;
+    if (from < to) {
+      const int pages0 = fx_kv_page(entries_of(from), a.c.pages);
+      load_step(from, pages0);
+      scales_of(pages0);
+      if (from + 1 < to) pages1 = fx_kv_page(entries_of(from + 1), a.c.pages);
+      write_step(0);
+      if (from + 1 < to) load_step(from + 1, pages1);
+      if (from + 2 < to) entries2 = entries_of(from + 2);
+    }
+    for (int step = from; step < to; ++step) {
+      const int base = step * FX_KV_STEP, buffer = (step - from) & 1;
+      const uint8_t* kt = s_kv[buffer][0];
+      const uint8_t* vt = s_kv[buffer][1];
+      const int p0 = pg[0], p1 = pg[1];
+      float cs[2] = {ks[0] * a.scale, ks[1] * a.scale}, cv[2] = {vs[0], vs[1]};
+      __syncthreads();   // this step's numbers are there, and everyone is done with the other buffer
+      if (step + 1 < to) {
+        write_step(buffer ^ 1);
+        const int pages2 = fx_kv_page(entries2, a.c.pages);
+        if (step + 2 < to) load_step(step + 2, pages2);
+        scales_of(pages1);
+        pages1 = pages2;
+        if (step + 3 < to) entries2 = entries_of(step + 3);
+      }
+      __builtin_amdgcn_sched_barrier(0);   // (here and below: what is loaded early stays in registers that are not there)
+      if (base >= mine.high || base + FX_KV_STEP <= mine.low) continue;   // (none of this wave's rows sees it)
+      float s[2][16];
+      int krow = ((col >> 2) & 1) * 16 + (col >> 3) * 4 + (col & 3);
+      int kpiece = key_piece<DP>(krow, half) * 16;
+      krow *= DP * 2;
+      asm volatile("" : "+v"(krow), "+v"(kpiece));   // (16 addresses that are not worth a register each)
+      fx_f32x16 r[2];
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) r[t][e] = 0.0f;
+      piped<2 * C>([&](int n) { return *(const Frag*)(kt + n / C * 32 * DP * 2 + krow + (kpiece ^ (n % C * 32))); },
+                   [&](int n, const Frag& kf) {
+#pragma unroll
+                     for (int k = NQ - 1; k >= 0; --k) r[n / C] = mfma32<F16>(kf, q[k][n % C], r[n / C]);
+                   });
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) s[t][e] = r[t][e];
+      const bool inside = base >= mine.all_low && base + FX_KV_STEP <= mine.all_high && __all(p0 >= 0 && p1 >= 0);
+      if (!inside) {
+        int hi_row_ = hi_row, lo_row_ = lo_row;
+        asm volatile("" : "+v"(hi_row_), "+v"(lo_row_));   // (compared here, not ahead of the branch)
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          const int t0 = base + (t * 2 + half) * 16;
+          const bool ok = (t ? p1 : p0) >= 0;
+          if (!ok || mine.high <= t0) cs[t] = cv[t] = 1.0f;   // (what lies there may be anything)
+          const int h = ok ? hi_row_ - t0 : 0, b = lo_row_ - t0;
+#pragma unroll
+          for (int e = 0; e < 16; ++e) s[t][e] = e < h && e >= b ? s[t][e] : -kInf;
+        }
+      }
+      float top[2];
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        top[t] = max3(s[t][0], s[t][1], s[t][2]);
+#pragma unroll
+        for (int e = 3; e < 15; e += 2) top[t] = max3(top[t], s[t][e], s[t][e + 1]);
+        top[t] = fmaxf(top[t], s[t][15]) * cs[t];
+      }
+      float up = fmaxf(top[0], top[1]);
+      if (__any(up > m + 8.0f || (m == -kInf && up > -kInf))) {
+        up = fmaxf(up, __shfl_xor(up, 32, 64));
+        const float to_m = fmaxf(m, up);
+        const float by = to_m == -kInf ? 1.0f : __builtin_amdgcn_exp2f(m - to_m);
+        m = to_m;
+        l *= by;
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) acc[d][e] *= by;
+      }
+      const float sub = m == -kInf ? 0.0f : m;
+      // weights times the values' scale, a power of two: part of the exponent, and taken out of their sum again
+      Frag p[2][2][NP];
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const float off = __builtin_amdgcn_logf(cv[t]) - sub;
+        float sum[2] = {0.0f, 0.0f};
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          s[t][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][e], cs[t], off));
+          sum[e & 1] += s[t][e];
+        }
+        l = __builtin_fmaf(sum[0] + sum[1], 1.0f / cv[t], l);
+        split8<NP>(p[t][0], s[t]);
+        split8<NP>(p[t][1], s[t] + 8);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      piped<4 * DT>([&](int n) { return *(const Frag*)(vt + (((n / 2 % 2 * 2 + half) * 2 + n % 2) * DP + n / 4 * 32 + col) * 16); },
+                    [&](int n, const Frag& v) {
+#pragma unroll
+                      for (int k = NP - 1; k >= 0; --k) acc[n / 4] = mfma32<false>(v, p[n / 2 % 2][n % 2][k], acc[n / 4]);
+                    });
+    }
+    if constexpr (HELD == 0) {
+      // Values that are NaN were left out of LDS, because 0 * NaN would reach the rows that do not see their tokens: the
+      // rows that do get their NaN here, from the cache itself.
+      __syncthreads();
+      if (__builtin_amdgcn_readfirstlane(s_nan)) {
+        for (int step = from; step < to; ++step)
+          for (int t = 0; t < 2; ++t) {
+            const int t0 = step * FX_KV_STEP + (t * 2 + half) * 16;
+            const int page = fx_kv_page(table[min(t0 >> lp, a.columns - 1)], a.c.pages), hi = page >= 0 ? hi_row - t0 : 0, lo = lo_row - t0;
+            Frag sees[2];
+#pragma unroll
+            for (int w = 0; w < 8; ++w)
+              sees[w >> 2].u[w & 3] = (2 * w < hi && 2 * w >= lo ? 0x3f80u : 0u) | (2 * w + 1 < hi && 2 * w + 1 >= lo ? 0x3f800000u : 0u);
+            const uint8_t* v = a.c.v + (int64_t)max(page, 0) * a.c.v_stride + head_at + (int64_t)((t0 & pm) >> 4) * 16 * D;
+#pragma unroll
+            for (int d = 0; d < DT; ++d) {
+              uint4 is = *(const uint4*)(v + min(d * 32 + col, D - 1) * 16);
+              unsigned* u = (unsigned*)&is;
+#pragma unroll
+              for (int w = 0; w < 4; ++w) u[w] = (nan_codes(u[w]) >> 7) * 0x38u;   // e4m3's 1
+              fx_f32x16 r;
+#pragma unroll
+              for (int e = 0; e < 16; ++e) r[e] = 0.0f;
+              r = mfma32<false>(eight<0, false>(is.x, is.y), sees[0], r);
+              r = mfma32<false>(eight<0, false>(is.z, is.w), sees[1], r);
+#pragma unroll
+              for (int e = 0; e < 16; ++e)
+                if (r[e] > 0.0f) acc[d][e] = __builtin_nanf("");
+            }
+          }
+      }
+    }
+    l += __shfl_xor(l, 32, 64);
+    if (valid) {
+      const int64_t t = x.r.start + i;
+      const int h = x.head * G + g;
+      const float per = l == 0.0f ? 0.0f : 1.0f / l;
+      const int64_t at = (int64_t)(x.part + x.split) * FX_KV_TILE + wave * 32 + col;
+#pragma unroll
+      for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int depth = d * 32 + e * 8 + half * 4;
+          if (!EXACT && depth >= D) continue;
+          float o[4];
+          if (x.splits == 1) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) o[k] = acc[d][e * 4 + k] * per;
+            store4((T*)a.out + t * a.out_token + (int64_t)h * D + depth, o);
+          } else {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) o[k] = acc[d][e * 4 + k];
+            store4(a.part_acc + at * D + depth, o);
+          }
+        }
+      if (half == 0) {
+        if (x.splits == 1) {
+          a.lse[t * a.q_heads + h] = l == 0.0f ? -kInf : (m + __builtin_amdgcn_logf(l)) * kLn2;
+        } else {
+          a.part_ml[at * 2] = m;
+          a.part_ml[at * 2 + 1] = l;
+        }
+      }
+    }
+    if (x.splits > 1 && x.split == 0 && threadIdx.x == 0)
+      a.items[x.item] = FxKvItem{x.request, x.head, x.tile, x.part, x.splits};
+  }
+  if (a.fill) fill_rest<T>(a);
+}
+
+// What several workgroups found for the same rows, added up.  A workgroup takes a row of an item: 16 bytes of the result a
+// lane, the parts in turn over the groups of lanes that are left, whose sums meet in LDS in a fixed order.
 template <class T>
 __global__ __launch_bounds__(256) void fx_kv_join(const FxKvAttnArgs a, int tile_rows) {
+  __shared__ float s_m[64], s_l[64];
+  __shared__ __align__(16) float s_o[256 * 4];
   const int items = *a.n_items;
-  const int D = a.c.depth, G = a.group, d = (int)threadIdx.x;
+  const int D = a.c.depth, G = a.group, lanes = D / 4, groups = 256 / lanes;
+  const int group = (int)threadIdx.x / lanes, d = ((int)threadIdx.x - group * lanes) * 4;
   for (int64_t w = blockIdx.x; w < (int64_t)items * tile_rows; w += gridDim.x) {
     const FxKvItem it = a.items[w / tile_rows];
     const int c = (int)(w % tile_rows), row = it.tile * tile_rows + c;
     const int s = min(max(a.starts[it.request], 0), a.tokens), e = min(max(a.starts[it.request + 1], 0), a.tokens);
     if (row >= (e - s) * G) continue;
-    float top = -kInf;
-    for (int p = 0; p < it.parts; ++p) top = fmaxf(top, a.part_ml[((int64_t)(it.first + p) * tile_rows + c) * 2]);
-    float sum = 0.0f, o = 0.0f;
-    for (int p = 0; p < it.parts; ++p) {
-      const int64_t at = (int64_t)(it.first + p) * tile_rows + c;
-      const float m = a.part_ml[at * 2], f = m == -kInf ? 0.0f : __builtin_amdgcn_exp2f(m - top);
-      sum = __builtin_fmaf(a.part_ml[at * 2 + 1], f, sum);
-      if (d < D) o = __builtin_fmaf(a.part_acc[at * D + d], f, o);
+    float m = -kInf, l = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (group < groups) {
+#pragma unroll 4
+      for (int p = group; p < it.parts; p += groups) {
+        const int64_t at = (int64_t)(it.first + p) * tile_rows + c;
+        const float2 ml = *(const float2*)(a.part_ml + at * 2);
+        const float4 v = *(const float4*)(a.part_acc + at * D + d);
+        const float now = fmaxf(m, ml.x), f = m == -kInf ? 0.0f : __builtin_amdgcn_exp2f(m - now),
+                    g = ml.x == -kInf ? 0.0f : __builtin_amdgcn_exp2f(ml.x - now);
+        m = now;
+        l = __builtin_fmaf(l, f, ml.y * g);
+        o[0] = __builtin_fmaf(o[0], f, v.x * g);
+        o[1] = __builtin_fmaf(o[1], f, v.y * g);
+        o[2] = __builtin_fmaf(o[2], f, v.z * g);
+        o[3] = __builtin_fmaf(o[3], f, v.w * g);
+      }
+      if (d == 0) {
+        s_m[group] = m;
+        s_l[group] = l;
+      }
+      *(float4*)&s_o[(group * lanes) * 4 + d] = make_float4(o[0], o[1], o[2], o[3]);
     }
-    const int64_t t = s + row / G;
-    const int h = it.head * G + row % G;
-    if (d < D) ((T*)a.out)[t * a.out_token + (int64_t)h * D + d] = (T)(sum == 0.0f ? 0.0f : o / sum);
-    if (d == 0) a.lse[t * a.q_heads + h] = sum == 0.0f ? -kInf : (top + __builtin_amdgcn_logf(sum)) * kLn2;
+    __syncthreads();
+    if (group == 0) {
+      float top = -kInf, sum = 0.0f;
+      for (int k = 0; k < groups; ++k) top = fmaxf(top, s_m[k]);
+      o[0] = o[1] = o[2] = o[3] = 0.0f;
+      for (int k = 0; k < groups; ++k) {
+        const float f = s_m[k] == -kInf ? 0.0f : __builtin_amdgcn_exp2f(s_m[k] - top);
+        sum = __builtin_fmaf(s_l[k], f, sum);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o[j] = __builtin_fmaf(s_o[(k * lanes) * 4 + d + j], f, o[j]);
+      }
+      const int64_t t = s + row / G;
+      const int h = it.head * G + row % G;
+      const float per = sum == 0.0f ? 0.0f : 1.0f / sum;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) o[j] *= per;
+      store4((T*)a.out + t * a.out_token + (int64_t)h * D + d, o);
+      if (d == 0) a.lse[t * a.q_heads + h] = sum == 0.0f ? -kInf : (top + __builtin_amdgcn_logf(sum)) * kLn2;
+    }
+    __syncthreads();
   }
 }
 
+struct Kernels {
+  const void *rows, *tiles;
+};
 template <int HELD, int TQ>
-const void* rows_kernel(int depth) {
-  if (depth == 64) return (const void*)fx_kv_rows<HELD, TQ, 64, true>;
-  if (depth == 128) return (const void*)fx_kv_rows<HELD, TQ, 128, true>;
-  if (depth == 256) return (const void*)fx_kv_rows<HELD, TQ, 256, true>;
-  if (depth < 128) return (const void*)fx_kv_rows<HELD, TQ, 128, false>;
-  return (const void*)fx_kv_rows<HELD, TQ, 256, false>;
+Kernels kernels_of(int depth) {
+#define FX_KV_PAIR(DP, EXACT) Kernels{(const void*)fx_kv_rows<HELD, TQ, DP, EXACT>, (const void*)fx_kv_tiles<HELD, TQ, DP, EXACT>}
+  if (depth == 64) return FX_KV_PAIR(64, true);
+  if (depth == 128) return FX_KV_PAIR(128, true);
+  if (depth == 256) return FX_KV_PAIR(256, true);
+  if (depth < 128) return FX_KV_PAIR(128, false);
+  return FX_KV_PAIR(256, false);
+#undef FX_KV_PAIR
 }
 template <int HELD>
-const void* rows_kernel(int type, int depth) {
-  return type == kBf16 ? rows_kernel<HELD, kBf16>(depth) : type == kF16 ? rows_kernel<HELD, kF16>(depth) : rows_kernel<HELD, kF32>(depth);
+Kernels kernels_of(int type, int depth) {
+  return type == kBf16 ? kernels_of<HELD, kBf16>(depth) : type == kF16 ? kernels_of<HELD, kF16>(depth) : kernels_of<HELD, kF32>(depth);
 }
 }  // namespace fxkv
 
-const void* fx_kv_rows_kernel_e4m3(int type, int depth);
-const void* fx_kv_rows_kernel_int8(int type, int depth);
-hipError_t fx_launch_kv_attention(const FxKvAttnArgs& a, int held, int type, int64_t grid, int64_t join_grid, hipStream_t stream);
+fxkv::Kernels fx_kv_kernels_e4m3(int type, int depth);
+fxkv::Kernels fx_kv_kernels_int8(int type, int depth);

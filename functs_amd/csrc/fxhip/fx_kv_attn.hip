@@ -1,0 +1,106 @@
+// Attention over the paged 8-bit cache: launches.
+#include "fx_kv_attn.h"
+
+namespace fxkv {
+// The sums of unit_at for more requests than a wave adds up: one workgroup
+__global__ __launch_bounds__(1024) void fx_kv_offsets(const FxKvAttnArgs a, int tile_rows, int least) {
+  constexpr int W = 16;
+  __shared__ int64_t s_work[W];
+  __shared__ int s_units[W], s_cuts[W];
+  const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6;
+  int64_t work = 0;
+  for (int b = (int)threadIdx.x; b < a.requests; b += 1024) {
+    const FxKvRequest r = request_of(a, a.starts[b], a.starts[b + 1], a.lens[b], tile_rows);
+    work += (int64_t)r.tiles * r.steps;
+  }
+  work = wave_total(work);
+  if (lane == 0) s_work[wave] = work;
+  __syncthreads();
+  work = 0;
+  bool endless = false;
+  for (int w = 0; w < W; ++w) {
+    endless |= s_work[w] >= int64_t{1} << 60;
+    work += s_work[w];
+  }
+  const int chunk = fx_kv_chunk(all_steps(a, endless ? int64_t{1} << 60 : work), least);
+  int32_t* units_to = a.offsets + 2;
+  int units = 0, cuts = 0;   // of the rounds before
+  for (int b0 = 0; b0 < a.requests; b0 += 1024) {
+    const int b = b0 + (int)threadIdx.x;
+    int mine = 0, cut = 0;
+    if (b < a.requests) {
+      const FxKvRequest r = request_of(a, a.starts[b], a.starts[b + 1], a.lens[b], tile_rows);
+      const int splits = fx_kv_parts(r.steps, chunk), items = r.tiles * a.c.heads;
+      mine = items * splits;
+      cut = splits > 1 ? (items << 16) + mine : 0;
+    }
+    const int u = sum_upto(mine), c = sum_upto(cut);
+    __syncthreads();
+    if (lane == 63) {
+      s_units[wave] = u;
+      s_cuts[wave] = c;
+    }
+    __syncthreads();
+    int before_u = units + u - mine, before_c = cuts + c - cut;
+    for (int w = 0; w < W; ++w) {
+      if (w < wave) {
+        before_u += s_units[w];
+        before_c += s_cuts[w];
+      }
+      units += s_units[w];
+      cuts += s_cuts[w];
+    }
+    if (b < a.requests) {
+      units_to[b] = before_u;
+      units_to[a.requests + 1 + b] = before_c;
+    }
+  }
+  if (threadIdx.x == 0) {
+    units_to[a.requests] = units;
+    a.offsets[0] = chunk;
+    a.offsets[1] = (int)((unsigned)cuts >> 16);
+  }
+}
+}  // namespace fxkv
+
+namespace {
+template <class... A>
+hipError_t launch(const void* kernel, int64_t grid, hipStream_t stream, A... args) {
+  void* kargs[sizeof...(A)] = {(void*)&args...};
+  return hipLaunchKernel(kernel, dim3((unsigned)grid), dim3(256), kargs, 0, stream);
+}
+hipError_t offsets(const FxKvAttnArgs& a, int tile_rows, int least, hipStream_t stream) {
+  if (a.requests <= fxkv::kScanned) return hipSuccess;
+  FxKvAttnArgs args = a;
+  void* kargs[3] = {(void*)&args, (void*)&tile_rows, (void*)&least};
+  return hipLaunchKernel((const void*)fxkv::fx_kv_offsets, dim3(1), dim3(1024), kargs, 0, stream);
+}
+hipError_t join(const FxKvAttnArgs& a, int type, int tile_rows, hipStream_t stream) {
+  const void* kernel = type == fxkv::kBf16 ? (const void*)fxkv::fx_kv_join<__bf16>
+                       : type == fxkv::kF16 ? (const void*)fxkv::fx_kv_join<_Float16>
+                                            : (const void*)fxkv::fx_kv_join<float>;
+  return launch(kernel, 2048, stream, a, tile_rows);
+}
+}  // namespace
+
+hipError_t fx_launch_kv_attention(const FxKvAttnArgs& a, const FxKvLaunch& l, hipStream_t stream) {
+  const fxkv::Kernels k = l.held == 0 ? fx_kv_kernels_e4m3(l.type, a.c.depth) : fx_kv_kernels_int8(l.type, a.c.depth);
+  hipError_t e = hipSuccess;
+  FxKvAttnArgs args = a;
+  if (l.tiles_grid > 0) {
+    args.rows_above = l.rows_grid > 0 ? FX_KV_FEW : 0;
+    args.rows_upto = int64_t{1} << 31;
+    if ((e = offsets(args, FX_KV_TILE, fxkv::kTileLeast, stream)) != hipSuccess) return e;
+    if ((e = launch(k.tiles, l.tiles_grid, stream, args)) != hipSuccess) return e;
+    if (l.shared && (e = join(args, l.type, FX_KV_TILE, stream)) != hipSuccess) return e;
+    args.fill = 0;
+  }
+  if (l.rows_grid > 0) {
+    args.rows_above = 0;
+    args.rows_upto = l.tiles_grid > 0 ? FX_KV_FEW : int64_t{1} << 31;
+    if ((e = offsets(args, FX_KV_ROWS, fxkv::kRowLeast, stream)) != hipSuccess) return e;
+    if ((e = launch(k.rows, l.rows_grid, stream, args)) != hipSuccess) return e;
+    if (l.shared && (e = join(args, l.type, FX_KV_ROWS, stream)) != hipSuccess) return e;
+  }
+  return e;
+}

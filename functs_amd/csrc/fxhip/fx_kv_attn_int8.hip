@@ -1,4 +1,4 @@
 // Attention over int8 caches.
 #include "fx_kv_attn.h"
 
-const void* fx_kv_rows_kernel_int8(int type, int depth) { return fxkv::rows_kernel<1>(type, depth); }
+fxkv::Kernels fx_kv_kernels_int8(int type, int depth) { return fxkv::kernels_of<1>(type, depth); }
