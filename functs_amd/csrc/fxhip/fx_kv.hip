@@ -158,30 +158,71 @@ __global__ __launch_bounds__(kThreads) void fx_kv_plan_kernel(const FxKvPlanArgs
 // ---- fx_kv_store ----
 // Bound: HBM (2 or 4 bytes read and 1 written for each number); single tokens: latency.
 // A run is the neighbours in `slots` that lie in one page; a wave takes the keys or the values of one head of a
-// run, so a page's scale and codes have one writer and nothing is locked.  Two passes over the run's numbers,
-// the second from the caches: their largest magnitude gives the scale, then codes.  The old tokens of a page whose scale
-// grows are rounded again to the new one.
+// run, so a page's scale and codes have one writer and nothing is locked.  The run's numbers are read, their largest magnitude
+// gives the scale, then they become codes; of more than a few tokens they are read a second time, from the caches (keeping all of a
+// page in registers left two waves a SIMD and a quarter of the bandwidth).  Keys: 8 numbers of a token a lane.  Values: 2
+// columns of a group of 16 tokens a lane, which are 32 neighbouring bytes of the cache.
+// Magnitudes are compared as the integers that their bits are.  Where the largest one is finite and below the largest scale, no number
+// needs to be held to the range of the codes or looked at for NaN (PLAIN).
 constexpr int kStoreWaves = kThreads / 64;
+typedef unsigned short fx_u16x2 __attribute__((ext_vector_type(2)));
 
-template <class T>
-__device__ __forceinline__ void load8(float (&x)[8], const T* p, bool vec) {
+// 2 and 8 numbers as they are loaded; the magnitudes' bits (16-bit types: two to a word)
+template <class T> struct Pack {   // 16 bits
+  typedef unsigned two;
+  typedef uint4 eight;
+  static __device__ __forceinline__ unsigned larger(unsigned m, unsigned w) {
+    return __builtin_bit_cast(unsigned, __builtin_elementwise_max(__builtin_bit_cast(fx_u16x2, m), __builtin_bit_cast(fx_u16x2, w & 0x7fff7fffu)));
+  }
+  static __device__ __forceinline__ unsigned see(unsigned m, two w) { return larger(m, w); }
+  static __device__ __forceinline__ unsigned see(unsigned m, const eight& w) { return larger(larger(larger(larger(m, w.x), w.y), w.z), w.w); }
+  static __device__ __forceinline__ float value(unsigned m) {   // of the larger half; infinity or NaN where there is one
+    const unsigned short u = (unsigned short)max(m & 0xffffu, m >> 16);
+    return (float)__builtin_bit_cast(T, u);
+  }
+};
+template <> struct Pack<float> {
+  typedef uint2 two;
+  typedef struct { uint4 a, b; } eight;
+  static __device__ __forceinline__ unsigned larger(unsigned m, unsigned w) { return max(m, w & 0x7fffffffu); }
+  static __device__ __forceinline__ unsigned see(unsigned m, const two& w) { return larger(larger(m, w.x), w.y); }
+  static __device__ __forceinline__ unsigned see(unsigned m, const eight& w) {
+    m = larger(larger(larger(larger(m, w.a.x), w.a.y), w.a.z), w.a.w);
+    return larger(larger(larger(larger(m, w.b.x), w.b.y), w.b.z), w.b.w);
+  }
+  static __device__ __forceinline__ float value(unsigned m) { return __uint_as_float(m); }
+};
+template <class T, int N, class P>
+__device__ __forceinline__ P load_numbers(const T* p, bool vec) {
+  union { P u; T e[N]; } w;
   if (vec) {
-    if constexpr (sizeof(T) == 2) {
-      union { uint4 u; T e[8]; } w;
-      w.u = *(const uint4*)p;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = (float)w.e[i];
-    } else {
-      union { uint4 u[2]; T e[8]; } w;
-      w.u[0] = *(const uint4*)p;
-      w.u[1] = *(const uint4*)(p + 4);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = (float)w.e[i];
-    }
+    w.u = *(const P*)p;
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = (float)p[i];
+    for (int i = 0; i < N; ++i) w.e[i] = p[i];
   }
+  return w.u;
+}
+template <class T, int N, class P>
+__device__ __forceinline__ void floats(float (&x)[N], const P& p) {
+  union { P u; T e[N]; } w;
+  w.u = p;
+#pragma unroll
+  for (int i = 0; i < N; ++i) x[i] = (float)w.e[i];
+}
+// the largest of a wave's words, each half by itself where HALVES
+template <bool HALVES>
+__device__ __forceinline__ unsigned wave_largest(unsigned m) {
+  auto larger = [](unsigned a, unsigned b) {
+    return HALVES ? __builtin_bit_cast(unsigned, __builtin_elementwise_max(__builtin_bit_cast(fx_u16x2, a), __builtin_bit_cast(fx_u16x2, b))) : max(a, b);
+  };
+  m = larger(m, (unsigned)__builtin_amdgcn_update_dpp(0, (int)m, 0x111, 0xf, 0xf, false));   // row_shr: 1, 2, 4, 8
+  m = larger(m, (unsigned)__builtin_amdgcn_update_dpp(0, (int)m, 0x112, 0xf, 0xf, false));
+  m = larger(m, (unsigned)__builtin_amdgcn_update_dpp(0, (int)m, 0x114, 0xf, 0xf, false));
+  m = larger(m, (unsigned)__builtin_amdgcn_update_dpp(0, (int)m, 0x118, 0xf, 0xf, false));
+  m = larger(m, (unsigned)__builtin_amdgcn_update_dpp(0, (int)m, 0x142, 0xa, 0xf, false));   // row_bcast: 15, 31
+  m = larger(m, (unsigned)__builtin_amdgcn_update_dpp(0, (int)m, 0x143, 0xc, 0xf, false));
+  return (unsigned)__builtin_amdgcn_readlane((int)m, 63);
 }
 __device__ __forceinline__ float finite_abs(float x) {
   const float m = __builtin_fabsf(x);
@@ -191,6 +232,25 @@ __device__ __forceinline__ float wave_max64(float v) {
 #pragma unroll
   for (int d = 1; d < 64; d <<= 1) v = fmaxf(v, __shfl_xor(v, d, 64));
   return v;
+}
+// codes of x * inv
+template <int HELD, bool PLAIN>
+__device__ __forceinline__ unsigned codes4(const float* x, float inv) {
+  float y[4];
+  if constexpr (PLAIN && HELD == 1) {   // the sum with 1.5 * 2^23 rounds to whole numbers: its last byte is the code
+#pragma unroll
+    for (int i = 0; i < 4; ++i) y[i] = __builtin_fmaf(x[i], inv, 12582912.0f);
+    return __builtin_amdgcn_perm(__float_as_uint(y[1]), __float_as_uint(y[0]), 0x0c0c0400u) |
+           __builtin_amdgcn_perm(__float_as_uint(y[3]), __float_as_uint(y[2]), 0x04000c0cu);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) y[i] = x[i] * inv;
+    if constexpr (PLAIN) {
+      const int w = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], 0, false);
+      return (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], w, true);
+    }
+    return encode4<HELD>(y);
+  }
 }
 
 // 16 codes under a scale `ratio` times as large, those before `n` of them
@@ -211,176 +271,351 @@ __device__ __forceinline__ uint4 again16(uint4 w, float ratio, int n) {
   return w;
 }
 
+__device__ __forceinline__ int64_t lane_of(int64_t v, int lane) {   // in scalar registers
+  return ((int64_t)__builtin_amdgcn_readlane((int)(v >> 32), lane) << 32) | (unsigned)__builtin_amdgcn_readlane((int)v, lane);
+}
+// One run: rows [0, n) of `rows` go to offsets o0 on of a page (straight), or to those that `slots` says
+template <int HELD, class T, bool VALUES>
+struct StoreRun {
+  typedef typename Pack<T>::eight P8;
+  typedef typename Pack<T>::two P2;
+  const T* rows;
+  int64_t stride;
+  int n, o0, D, lane;
+  uint8_t* codes;
+  bool vec;
+  // lane -> (row of an iteration, eight of its depth), or (group of an iteration, pair of columns)
+  int width, abreast, sub, at, blocks, g0, count, iterations;
+
+  __device__ __forceinline__ void shape() {
+    width = VALUES ? D >> 1 : D >> 3;
+    abreast = width >= 64 ? 1 : 64 / width;
+    sub = lane / width;
+    at = lane - sub * width;
+    blocks = width > 64 ? (width + 63) >> 6 : 1;   // (values of depth above 128)
+    g0 = o0 >> 4;
+    count = VALUES ? ((o0 + n + 15) >> 4) - g0 : n;
+    iterations = (count + abreast - 1) / abreast * blocks;
+  }
+  // rows beyond the run: its last or first one again, which is in the maximum anyway and not written
+  __device__ __forceinline__ P8 load_eight(int k) const {
+    const T* p = rows + at * 8;
+    if ((k + 1) * abreast <= n) return load_numbers<T, 8, P8>(p + (int64_t)(k * abreast) * stride + (int64_t)sub * stride, vec);
+    return load_numbers<T, 8, P8>(p + (int64_t)min(k * abreast + sub, n - 1) * stride, vec);
+  }
+  __device__ __forceinline__ int group_of(int k) const { return blocks > 1 ? k / blocks : k * abreast + sub; }
+  __device__ __forceinline__ int pair_of(int k) const { return blocks > 1 ? at + (k % blocks) * 64 : at; }
+  __device__ __forceinline__ bool whole(int k) const {   // all rows of the iteration's groups are in the run
+    const int g = blocks > 1 ? k / blocks : k * abreast;
+    return (g0 + g) * 16 >= o0 && (g0 + g + abreast) * 16 <= o0 + n;
+  }
+  __device__ __forceinline__ void load_column(P2 (&c)[16], int k) const {
+    const int first = (g0 + group_of(k)) * 16 - o0;
+    const T* p = rows + min(pair_of(k), width - 1) * 2;
+    if (whole(k)) {
+      p += (int64_t)first * stride;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) c[e] = load_numbers<T, 2, P2>(p + e * stride, vec);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) c[e] = load_numbers<T, 2, P2>(p + (int64_t)min(max(first + e, 0), n - 1) * stride, vec);
+    }
+  }
+  template <bool PLAIN>
+  __device__ __forceinline__ void write_eight(int k, const P8& p, float inv) const {
+    const int j = k * abreast + sub;
+    if (j >= n) return;
+    float x[8];
+    floats<T, 8>(x, p);
+    *(uint2*)(codes + (o0 + j) * D + at * 8) = make_uint2(codes4<HELD, PLAIN>(x, inv), codes4<HELD, PLAIN>(x + 4, inv));
+  }
+  template <bool PLAIN>
+  __device__ __forceinline__ void write_column(int k, const P2 (&c)[16], float inv, float ratio) const {
+    const int g = group_of(k), pair = pair_of(k);
+    if (g >= count || pair >= width) return;
+    uint4* to = (uint4*)(codes + ((g0 + g) * D + pair * 2) * 16);
+    uint4 u[2];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      float x[4], y[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        float z[2];
+        floats<T, 2>(z, c[q * 4 + e]);
+        x[e] = z[0];
+        y[e] = z[1];
+      }
+      ((unsigned*)&u[0])[q] = codes4<HELD, PLAIN>(x, inv);
+      ((unsigned*)&u[1])[q] = codes4<HELD, PLAIN>(y, inv);
+    }
+    if (!whole(k)) {
+      const int low = o0 - (g0 + g) * 16, high = low + n;   // tokens of the group that are written: [low, high)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        uint4 was = to[h];
+        if (ratio != 1.0f && low > 0) was = again16<HELD>(was, ratio, low);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int up = min(max(high - 4 * q, 0), 4), down = min(max(low - 4 * q, 0), 4);
+          const unsigned fresh = (up == 4 ? ~0u : (1u << (8 * up)) - 1) & ~(down == 4 ? ~0u : (1u << (8 * down)) - 1);
+          ((unsigned*)&u[h])[q] = (((unsigned*)&u[h])[q] & fresh) | (((unsigned*)&was)[q] & ~fresh);
+        }
+      }
+    }
+    to[0] = u[0];
+    to[1] = u[1];
+  }
+  static constexpr int kKept = VALUES ? 1 : 4;   // iterations whose numbers stay in registers: more of them cost waves
+  template <bool PLAIN>
+  __device__ __forceinline__ void write(const P8 (&kept8)[VALUES ? 1 : kKept], const P2 (&kept2)[16], bool keep, float inv, float ratio) const {
+    if (keep) {
+      if constexpr (VALUES) {
+        write_column<PLAIN>(0, kept2, inv, ratio);
+      } else {
+#pragma unroll
+        for (int k = 0; k < kKept; ++k)
+          if (k < iterations) write_eight<PLAIN>(k, kept8[k], inv);
+      }
+      return;
+    }
+#pragma unroll 2
+    for (int k = 0; k < iterations; ++k) {
+      if constexpr (VALUES) {
+        P2 c[16];
+        load_column(c, k);
+        write_column<PLAIN>(k, c, inv, ratio);
+      } else {
+        write_eight<PLAIN>(k, load_eight(k), inv);
+      }
+    }
+  }
+
+  __device__ __forceinline__ void run(bool straight, const int64_t* slots, int page_mask, float* scale_at) {
+    lane = (int)threadIdx.x & 63;
+    shape();
+    const float old = o0 > 0 ? *scale_at : 0.0f;
+    P8 kept8[VALUES ? 1 : kKept];
+    P2 kept2[16];
+    const bool keep = iterations <= kKept, used = sub < abreast;
+    unsigned m = 0;
+    if (straight && used) {
+      if (keep) {
+        if constexpr (VALUES) {
+          load_column(kept2, 0);
+#pragma unroll
+          for (int e = 0; e < 16; ++e) m = Pack<T>::see(m, kept2[e]);
+        } else {
+#pragma unroll
+          for (int k = 0; k < kKept; ++k)
+            if (k < iterations) kept8[k] = load_eight(k);
+#pragma unroll
+          for (int k = 0; k < kKept; ++k)
+            if (k < iterations) m = Pack<T>::see(m, kept8[k]);
+        }
+      } else {
+#pragma unroll 2
+        for (int k = 0; k < iterations; ++k) {
+          if constexpr (VALUES) {
+            P2 c[16];
+            load_column(c, k);
+#pragma unroll
+            for (int e = 0; e < 16; ++e) m = Pack<T>::see(m, c[e]);
+          } else {
+            m = Pack<T>::see(m, load_eight(k));
+          }
+        }
+      }
+    }
+    float top = Pack<T>::value(wave_largest<sizeof(T) == 2>(m));
+    constexpr float kMost = HELD == 0 ? 448.0f * 0x1p119f : 127.0f * 0x1p121f;
+    const bool plain = straight && top <= kMost;
+    if (!plain) {   // infinities or NaN (or slots in any order): the largest finite one
+      float t = 0.0f;
+      for (int j = 0; j < n; ++j)
+        for (int d = lane; d < D; d += 64) t = fmaxf(t, finite_abs((float)rows[(int64_t)j * stride + d]));
+      top = wave_max64(t);
+    }
+    float scale = scale_of<HELD>(top);
+    float ratio = 1.0f;   // of the page's scale before to the one from now on
+    if (o0 > 0) {
+      if (old > scale && old <= 3.402823466e38f) scale = old;
+      else if (old > 0.0f && old < scale) ratio = old / scale;
+    }
+    if (lane == 0) *scale_at = scale;
+    if (ratio != 1.0f) {
+      // what the page holds below o0; the group in which o0 lies, if it is written below, is done there
+      const int words = VALUES ? (straight ? g0 : (o0 + 15) >> 4) * D : (o0 * D) >> 4;
+      for (int i = lane; i < words; i += 64) {
+        uint4* w = (uint4*)codes + i;
+        *w = again16<HELD>(*w, ratio, VALUES ? o0 - (i / D) * 16 : 16);
+      }
+    }
+    const float inv = 1.0f / scale;   // (a power of two: exact)
+    if (straight) {
+      if (!used) return;
+      if (plain) write<true>(kept8, kept2, keep, inv, ratio);
+      else write<false>(kept8, kept2, keep, inv, ratio);
+      return;
+    }
+    // slots in any order: token by token, so that of two rows for one slot the later one stays
+    __threadfence_block();   // (the words above and the bytes below come from different lanes)
+    for (int j = 0; j < n; ++j) {
+      const int o = (int)(slots[j] & page_mask);
+      for (int d = lane; d < D; d += 64) {
+        const float x[4] = {(float)rows[(int64_t)j * stride + d] * inv, 0.0f, 0.0f, 0.0f};
+        const uint8_t code = (uint8_t)encode4<HELD>(x);
+        if (VALUES) codes[((o >> 4) * D + d) * 16 + (o & 15)] = code;
+        else codes[o * D + d] = code;
+      }
+    }
+  }
+};
+
 template <int HELD, class T>
-__global__ __launch_bounds__(kThreads) void fx_kv_store_kernel(const FxKvCache c, const FxKvRows r, int per_wave, int n_chunks, int vec) {
+__global__ __launch_bounds__(kThreads, 4) void fx_kv_store_kernel(const FxKvCache c, const FxKvRows r, int per_wave, int n_chunks, int vec) {
   const int lane = (int)threadIdx.x & 63;
-  const int64_t w = (int64_t)blockIdx.x * kStoreWaves + ((int)threadIdx.x >> 6);
-  const int half = (int)(w % 2), head = (int)((w / 2) % c.heads);
-  const int64_t chunk = w / 2 / c.heads;
+  const int64_t w = (int64_t)blockIdx.x * kStoreWaves + __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const unsigned chunk_head = (unsigned)(w >> 1);   // (below 2^32: checked on the host)
+  const int half = (int)(w & 1), chunk = (int)(chunk_head / (unsigned)c.heads), head = (int)(chunk_head - (unsigned)chunk * (unsigned)c.heads);
   if (chunk >= n_chunks) return;
-  const int D = c.depth, page = 1 << c.log_page, cpt = D >> 3;   // (8 numbers a lane and load)
+  const int D = c.depth, page = 1 << c.log_page;
   const int64_t n_slots = (int64_t)c.pages << c.log_page;
-  const T* src = (const T*)(half ? r.v : r.k) + (int64_t)head * (half ? r.v_head : r.k_head);
-  const int64_t stride = half ? r.v_token : r.k_token;
-  const int t0 = (int)chunk * per_wave, t1 = min(r.tokens, t0 + per_wave);
-  auto page_of = [&](int t) -> int64_t {   // -1: nowhere
-    const int64_t s = r.slots[t];
-    return s >= 0 && s < n_slots ? s >> c.log_page : -1;
+  const int t0 = chunk * per_wave, t1 = min(r.tokens, t0 + per_wave);
+  // lane i: the slot of token t0 - 1 + i, which a run that begins in the chunk needs (the first 64 - per_wave of it, at least)
+  auto slot_of = [&](int t) -> int64_t {
+    const int64_t s = t >= 0 && t < r.tokens ? r.slots[min(max(t, 0), r.tokens - 1)] : -1;
+    return s >= 0 && s < n_slots ? s : -1;
   };
+  const int64_t mine = slot_of(t0 - 1 + lane);
   for (int t = t0; t < t1; ++t) {
-    const int64_t p = page_of(t);
-    if (p < 0 || (t > 0 && page_of(t - 1) == p)) continue;   // (uniform: every lane reads the same slots)
+    const int at = t - t0 + 1;
+    const int64_t s0 = lane_of(mine, at), s1 = lane_of(mine, at - 1);
+    const int64_t p = s0 >> c.log_page;   // -1: nowhere
+    if (s0 < 0 || (s1 >= 0 && s1 >> c.log_page == p)) continue;
     // the run's length, and whether its slots rise by one
     int n = 0;
     bool straight = true;
-    const int64_t s0 = r.slots[t];
+    int64_t seen = mine;
+    int first = at;   // the lane of the run's next token
     for (;;) {
-      const int u = t + n + lane;
-      const bool mine = u < r.tokens && page_of(u) == p;
-      const unsigned long long same = __ballot(mine), rising = __ballot(mine && r.slots[u] == s0 + n + lane);
-      const int more = ~same == 0 ? 64 : __builtin_ctzll(~same);
+      const bool here = lane >= first && seen >= 0 && seen >> c.log_page == p;
+      const unsigned long long same = __ballot(here) >> first, rising = __ballot(here && seen == s0 + n + lane - first) >> first;
+      const int most = 64 - first, more = ~same == 0 ? 64 : min(__builtin_ctzll(~same), most);
       const unsigned long long part = more == 64 ? ~0ull : (1ull << more) - 1;
       straight = straight && (rising & part) == part;
       n += more;
-      if (more < 64) break;
+      if (more < most) break;
+      first = 0;
+      seen = slot_of(t + n + lane);
     }
     const int o0 = (int)(s0 & (page - 1));
-    uint8_t* codes = (half ? c.v + p * c.v_stride : c.k + p * c.k_stride) + (int64_t)head * page * D;
-    float* scales = half ? c.v_scale + p * c.vs_stride + head : c.k_scale + p * c.ks_stride + head;
-    const T* rows = src + (int64_t)t * stride;
-    // the scale
-    float top = 0.0f;
-    const int64_t n8 = (int64_t)n * cpt;
-    for (int64_t i = lane; i < n8; i += 64) {
-      const int64_t j = i / cpt;
-      float x[8];
-      load8(x, rows + j * stride + (i - j * cpt) * 8, vec);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) top = fmaxf(top, finite_abs(x[e]));
-    }
-    float scale = scale_of<HELD>(wave_max64(top));
-    if (o0 > 0) {
-      const float old = *scales;
-      if (old > scale && old <= 3.402823466e38f) {
-        scale = old;
-      } else if (old < scale && old > 0.0f) {
-        // what the page holds below o0: as many whole columns of 16 as there are, the last one in part
-        const float ratio = old / scale;
-        const int words = half ? ((o0 + 15) >> 4) * D : (o0 * D) >> 4;
-        for (int i = lane; i < words; i += 64) {
-          uint4* at = (uint4*)codes + i;
-          *at = again16<HELD>(*at, ratio, half ? o0 - (i / D) * 16 : 16);
-        }
-      }
-    }
-    if (lane == 0) *scales = scale;
-    const float inv = 1.0f / scale;   // (a power of two: exact)
-    if (straight && !half) {
-      for (int64_t i = lane; i < n8; i += 64) {
-        const int64_t j = i / cpt;
-        float x[8];
-        load8(x, rows + j * stride + (i - j * cpt) * 8, vec);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] *= inv;
-        uint2 u;
-        u.x = encode4<HELD>(x);
-        u.y = encode4<HELD>(x + 4);
-        *(uint2*)(codes + (int64_t)(o0 + j) * D + (i - j * cpt) * 8) = u;
-      }
-      continue;
-    }
-    // values, or slots in any order: whole groups of 16 tokens that lie as in the cache, the others token by token (in order,
-    // so that of two rows for one slot the later one stays)
-    for (int i = 0; i < n;) {
-      const int o = (int)(r.slots[t + i] & (page - 1));
-      if (half && straight && (o & 15) == 0 && n - i >= 16) {
-        for (int d = lane; d < D; d += 64) {
-          unsigned u[4];
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            float x[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) x[e] = (float)rows[(int64_t)(i + 4 * q + e) * stride + d] * inv;
-            u[q] = encode4<HELD>(x);
-          }
-          *(uint4*)(codes + (int64_t)(o >> 4) * 16 * D + (int64_t)d * 16) = make_uint4(u[0], u[1], u[2], u[3]);
-        }
-        i += 16;
-        continue;
-      }
-      for (int d = lane; d < D; d += 64) {
-        const float x[4] = {(float)rows[(int64_t)i * stride + d] * inv, 0.0f, 0.0f, 0.0f};
-        const uint8_t code = (uint8_t)encode4<HELD>(x);
-        if (half) codes[(int64_t)(o >> 4) * 16 * D + (int64_t)d * 16 + (o & 15)] = code;
-        else codes[(int64_t)o * D + d] = code;
-      }
-      ++i;
+    const int64_t in_page = (int64_t)head * page * D;
+    if (half == 0) {
+      StoreRun<HELD, T, false> run;
+      run.rows = (const T*)r.k + (int64_t)t * r.k_token + (int64_t)head * r.k_head;
+      run.stride = r.k_token;
+      run.n = n, run.o0 = o0, run.D = D, run.vec = vec != 0;
+      run.codes = c.k + p * c.k_stride + in_page;
+      run.run(straight, r.slots + t, page - 1, c.k_scale + p * c.ks_stride + head);
+    } else {
+      StoreRun<HELD, T, true> run;
+      run.rows = (const T*)r.v + (int64_t)t * r.v_token + (int64_t)head * r.v_head;
+      run.stride = r.v_token;
+      run.n = n, run.o0 = o0, run.D = D, run.vec = vec != 0;
+      run.codes = c.v + p * c.v_stride + in_page;
+      run.run(straight, r.slots + t, page - 1, c.v_scale + p * c.vs_stride + head);
     }
   }
 }
 
 // ---- fx_kv_read ----
-// Bound: HBM (1 byte read and 2 or 4 written for each number).  A wave takes the keys or the values of one head for
-// up to 16 entries of `slots`; values by the group of 16 tokens that neighbours share, a lane a column.
+// Bound: HBM (1 byte read and 2 or 4 written for each number).  A wave takes the keys or the values of one head for up
+// to 16 entries of `slots`.  Keys: 16 numbers of a token a lane.  Values: 2 columns of the group of 16 tokens that neighbours share.
 template <int HELD, class T>
-__global__ __launch_bounds__(kThreads) void fx_kv_read_kernel(const FxKvCache c, const FxKvRows r, int per_wave, int n_chunks) {
+__global__ __launch_bounds__(kThreads) void fx_kv_read_kernel(const FxKvCache c, const FxKvRows r, int per_wave, int n_chunks, int vec) {
   const int lane = (int)threadIdx.x & 63;
-  const int64_t w = (int64_t)blockIdx.x * kStoreWaves + ((int)threadIdx.x >> 6);
-  const int half = (int)(w % 2), head = (int)((w / 2) % c.heads);
-  const int64_t chunk = w / 2 / c.heads;
+  const int64_t w = (int64_t)blockIdx.x * kStoreWaves + __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const unsigned chunk_head = (unsigned)(w >> 1);
+  const int half = (int)(w & 1), chunk = (int)(chunk_head / (unsigned)c.heads), head = (int)(chunk_head - (unsigned)chunk * (unsigned)c.heads);
   if (chunk >= n_chunks) return;
   const int D = c.depth, page = 1 << c.log_page;
-  const int64_t n_slots = (int64_t)c.pages << c.log_page;
-  T* dst = (T*)(half ? r.v : r.k) + (int64_t)head * (half ? r.v_head : r.k_head);
-  const int64_t stride = half ? r.v_token : r.k_token;
-  const int t0 = (int)chunk * per_wave, t1 = min(r.tokens, t0 + per_wave);
-  for (int t = t0; t < t1;) {
-    const int64_t s = r.slots[t];
-    T* row = dst + (int64_t)t * stride;
-    if (s < 0 || s >= n_slots) {
-      for (int d = lane; d < D; d += 64) row[d] = (T)0.0f;
-      ++t;
-      continue;
-    }
-    const int64_t p = s >> c.log_page;
-    const int o = (int)(s & (page - 1));
-    const float scale = half ? c.v_scale[p * c.vs_stride + head] : c.k_scale[p * c.ks_stride + head];
-    if (!half) {
-      const uint8_t* codes = c.k + p * c.k_stride + ((int64_t)head * page + o) * D;
-      for (int d = lane * 4; d < D; d += 256) {
-        float x[4];
-        decode4<HELD>(x, *(const unsigned*)(codes + d));
-#pragma unroll
-        for (int e = 0; e < 4; ++e) row[d + e] = (T)(x[e] * scale);
-      }
-      ++t;
-      continue;
-    }
-    int n = 1;
-    while (t + n < t1 && (o & 15) + n < 16 && r.slots[t + n] == s + n) ++n;
-    const uint8_t* codes = c.v + p * c.v_stride + (int64_t)head * page * D + (int64_t)(o >> 4) * 16 * D;
-    for (int d = lane; d < D; d += 64) {
-      const uint4 u = *(const uint4*)(codes + (int64_t)d * 16);
-      const unsigned word[4] = {u.x, u.y, u.z, u.w};
+  const int64_t n_slots = (int64_t)c.pages << c.log_page, in_page = (int64_t)head * page * D;
+  const int t0 = chunk * per_wave, n = min(r.tokens - t0, per_wave);
+  int64_t mine = r.slots[t0 + min(lane, n - 1)];   // lane i: of token t0 + i
+  if (mine < 0 || mine >= n_slots) mine = -1;
+  if (half == 0) {
+    const int width = D >> 4, abreast = 64 / width, sub = lane / width, at = lane - sub * width;
+    T* dst = (T*)r.k + (int64_t)t0 * r.k_token + (int64_t)head * r.k_head + at * 16;
+    for (int j0 = 0; j0 < n; j0 += abreast) {
+      const int j = j0 + sub;
+      const int64_t s = __shfl(mine, min(j, 63), 64);
+      if (sub >= abreast || j >= n) continue;
+      const int64_t p = s < 0 ? 0 : s >> c.log_page;
+      const float scale = s < 0 ? 0.0f : c.k_scale[p * c.ks_stride + head];
+      uint4 u = *(const uint4*)(c.k + p * c.k_stride + in_page + (s < 0 ? 0 : s & (page - 1)) * D + at * 16);
+      if (s < 0) u = make_uint4(0, 0, 0, 0);
+      union { T e[16]; uint4 u[sizeof(T)]; } y;
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
         float x[4];
-        decode4<HELD>(x, word[q]);
+        decode4<HELD>(x, ((const unsigned*)&u)[q]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) y.e[q * 4 + e] = (T)(x[e] * scale);
+      }
+      T* to = dst + (int64_t)j * r.k_token;
+      if (vec) {
+#pragma unroll
+        for (int q = 0; q < (int)sizeof(T); ++q) ((uint4*)to)[q] = y.u[q];
+      } else {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) to[e] = y.e[e];
+      }
+    }
+    return;
+  }
+  T* dst = (T*)r.v + (int64_t)t0 * r.v_token + (int64_t)head * r.v_head;
+  for (int j = 0; j < n;) {
+    const int64_t slot = lane_of(mine, j);
+    // neighbours of the same group of 16 whose slots rise by one
+    const unsigned long long rising = __ballot(lane >= j && lane < n && mine == slot + (lane - j)) >> j;
+    const int o = (int)(slot & 15);
+    const int m = slot < 0 ? 1 : min(min(~rising == 0 ? 64 : __builtin_ctzll(~rising), 16 - o), n - j);
+    const int64_t p = slot < 0 ? 0 : slot >> c.log_page;
+    const float scale = slot < 0 ? 0.0f : c.v_scale[p * c.vs_stride + head];
+    const uint8_t* codes = c.v + p * c.v_stride + in_page + (slot < 0 ? 0 : (slot & (page - 1)) >> 4) * 16 * D;
+    for (int pair = lane; pair < D >> 1; pair += 64) {
+      uint4 u[2] = {((const uint4*)codes)[pair * 2], ((const uint4*)codes)[pair * 2 + 1]};
+      if (slot < 0) u[0] = u[1] = make_uint4(0, 0, 0, 0);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        float x[4], y[4];
+        decode4<HELD>(x, ((const unsigned*)&u[0])[q]);
+        decode4<HELD>(y, ((const unsigned*)&u[1])[q]);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const int j = 4 * q + e - (o & 15);
-          if (j >= 0 && j < n) row[(int64_t)j * stride + d] = (T)(x[e] * scale);
+          const int k = 4 * q + e - o;   // of the neighbours
+          if (k < 0 || k >= m) continue;
+          T* to = dst + (int64_t)(j + k) * r.v_token + pair * 2;
+          union { T e[2]; typename Pack<T>::two u; } z;
+          z.e[0] = (T)(x[e] * scale);
+          z.e[1] = (T)(y[e] * scale);
+          if (vec) {
+            *(typename Pack<T>::two*)to = z.u;
+          } else {
+            to[0] = z.e[0];
+            to[1] = z.e[1];
+          }
         }
       }
     }
-    t += n;
+    j += m;
   }
 }
 
-// tokens a wave takes: as many as leave some 8 192 waves (32 a CU), 16 at most
-int tokens_a_wave(const FxKvCache& c, const FxKvRows& r) {
-  int64_t per = (int64_t)r.tokens * c.heads * 2 / 8192;
-  return (int)(per < 1 ? 1 : per > 16 ? 16 : per);
+// tokens a wave takes: as many as leave some 8 192 waves (32 a CU), `most` at most
+int tokens_a_wave(const FxKvCache& c, const FxKvRows& r, int most) {
+  const int64_t per = (int64_t)r.tokens * c.heads * 2 / 8192;
+  return (int)(per < 1 ? 1 : per > most ? most : per);
 }
 bool aligned16(const void* p, int64_t a, int64_t b, size_t size) {
   return ((uintptr_t)p & 15u) == 0 && a * (int64_t)size % 16 == 0 && b * (int64_t)size % 16 == 0;
@@ -399,7 +634,7 @@ hipError_t fx_launch_kv_store(const FxKvCache& c, const FxKvRows& r, int held, h
       {(const void*)fx_kv_store_kernel<0, float>, (const void*)fx_kv_store_kernel<0, _Float16>, (const void*)fx_kv_store_kernel<0, __bf16>},
       {(const void*)fx_kv_store_kernel<1, float>, (const void*)fx_kv_store_kernel<1, _Float16>, (const void*)fx_kv_store_kernel<1, __bf16>}};
   const size_t size = r.dtype == FX_DT_F32 ? 4 : 2;
-  int per = tokens_a_wave(c, r), chunks = (r.tokens + per - 1) / per;
+  int per = tokens_a_wave(c, r, 32), chunks = (r.tokens + per - 1) / per;
   int vec = aligned16(r.k, r.k_token, r.k_head, size) && aligned16(r.v, r.v_token, r.v_head, size);
   FxKvCache cache = c;
   FxKvRows rows = r;
@@ -413,10 +648,12 @@ hipError_t fx_launch_kv_read(const FxKvCache& c, const FxKvRows& r, int held, hi
   static const void* const kernels[2][3] = {
       {(const void*)fx_kv_read_kernel<0, float>, (const void*)fx_kv_read_kernel<0, _Float16>, (const void*)fx_kv_read_kernel<0, __bf16>},
       {(const void*)fx_kv_read_kernel<1, float>, (const void*)fx_kv_read_kernel<1, _Float16>, (const void*)fx_kv_read_kernel<1, __bf16>}};
-  int per = tokens_a_wave(c, r), chunks = (r.tokens + per - 1) / per;
+  const size_t size = r.dtype == FX_DT_F32 ? 4 : 2;
+  int per = tokens_a_wave(c, r, 16), chunks = (r.tokens + per - 1) / per;
+  int vec = aligned16(r.k, r.k_token, r.k_head, size) && aligned16(r.v, r.v_token, r.v_head, size);
   FxKvCache cache = c;
   FxKvRows rows = r;
-  void* kargs[4] = {(void*)&cache, (void*)&rows, (void*)&per, (void*)&chunks};
+  void* kargs[5] = {(void*)&cache, (void*)&rows, (void*)&per, (void*)&chunks, (void*)&vec};
   const int64_t waves = (int64_t)chunks * c.heads * 2;
   return hipLaunchKernel(kernels[held][r.dtype == FX_DT_F32 ? 0 : r.dtype == FX_DT_F16 ? 1 : 2],
                          dim3((unsigned)((waves + kStoreWaves - 1) / kStoreWaves)), dim3(kThreads), kargs, 0, stream);

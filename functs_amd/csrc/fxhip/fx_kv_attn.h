@@ -23,6 +23,7 @@ typedef float fx_f32x4 __attribute__((ext_vector_type(4)));
 
 namespace fxkv {
 constexpr float kInf = __builtin_inff(), kLn2 = 0.693147180559945309f;
+constexpr float kTiny = 1.17549435e-38f;   // in place of scales of 0 (memory that nobody has written): -inf and 0 stay what they are under it
 enum { kBf16 = 0, kF16 = 1, kF32 = 2 };   // types of queries and results
 
 union Frag {   // eight 16-bit numbers of an operand
@@ -115,84 +116,59 @@ __device__ __forceinline__ int64_t all_steps(const FxKvAttnArgs& a, int64_t step
 }
 
 // Unit u of the call, or false behind the last one: every wave finds it by itself, in scalar registers, without a barrier.  Up
-// to kScanned requests are added up here, a lane four of them at most; of more, fx_kv_offsets has left the sums.
+// to kScanned requests are added up here, a lane one of 64 a round; of more, fx_kv_offsets has left the sums.
 // SORTED: of up to 64 requests those of more steps come first, so that what is left at the end of a call is short.
-constexpr int kScanned = 256, kScanPer = kScanned / 64;
+constexpr int kScanned = 256;
 constexpr int kRowLeast = 4, kTileLeast = 8;   // chunks are multiples of so many steps (fx_kv_rows: of one for each wave)
 template <bool SORTED>
 __device__ __forceinline__ bool unit_at(const FxKvAttnArgs& a, int tile_rows, int least, int u, Unit& x, int* shared_items) {
   const int lane = (int)threadIdx.x & 63;
   int chunk, rest, parts;   // rest: the unit's number in its request; parts: items << 16 | parts before the request
   if (a.requests <= kScanned) {
-    const int per = (a.requests + 63) >> 6;
-    int start[kScanPer], end[kScanPer], len[kScanPer], tiles[kScanPer], steps[kScanPer];
+    FxKvRequest r;
+    auto load = [&](int b0) {   // (all three loads at once, whatever the lane)
+      const int b = b0 + lane, c = max(min(b, a.requests - 1), 0);
+      const int start = a.starts[c], end = a.starts[c + (a.requests > 0 ? 1 : 0)], len = a.requests > 0 ? a.lens[c] : 0;
+      r = request_of(a, start, b < a.requests ? end : start, len, tile_rows);
+    };
     int64_t work = 0;
-#pragma unroll
-    for (int j = 0; j < kScanPer; ++j) {
-      start[j] = end[j] = len[j] = tiles[j] = steps[j] = 0;
-      if (j < per) {
-        const int b = lane * per + j, c = min(b, a.requests - 1);
-        start[j] = a.starts[c];
-        end[j] = b < a.requests ? a.starts[c + 1] : start[j];
-        len[j] = a.lens[c];
-      }
+    for (int b0 = 0; b0 < a.requests; b0 += 64) {
+      load(b0);
+      work += (int64_t)r.tiles * r.steps;
     }
-#pragma unroll
-    for (int j = 0; j < kScanPer; ++j)
-      if (j < per) {
-        const FxKvRequest r = request_of(a, start[j], end[j], len[j], tile_rows);
-        tiles[j] = r.tiles;
-        steps[j] = r.steps;
-        work += (int64_t)r.tiles * r.steps;
-      }
     chunk = fx_kv_chunk(all_steps(a, wave_total(work)), least);
-    int units[kScanPer], cut[kScanPer], mine = 0, cuts = 0;
-#pragma unroll
-    for (int j = 0; j < kScanPer; ++j) {
-      units[j] = cut[j] = 0;
-      if (j < per) {
-        const int splits = fx_kv_parts(steps[j], chunk), items = tiles[j] * a.c.heads;
-        units[j] = items * splits;
-        cut[j] = splits > 1 ? (items << 16) + units[j] : 0;
-        mine += units[j];
-        cuts += cut[j];
+    int units_before = 0, cuts_before = 0;   // of the rounds before
+    bool found = false;
+    for (int b0 = 0; b0 < a.requests; b0 += 64) {
+      if (a.requests > 64) load(b0);
+      const int splits = fx_kv_parts(r.steps, chunk), items = r.tiles * a.c.heads, mine = items * splits, cut = splits > 1 ? (items << 16) + mine : 0;
+      const int upto = sum_upto(mine), cuts = sum_upto(cut);
+      int before = units_before + upto - mine;
+      if (SORTED && a.requests <= 64) {
+        before = 0;
+        for (int c = 0; c < a.requests; ++c) {
+          const int n = __builtin_amdgcn_readlane(r.steps, c), add = __builtin_amdgcn_readlane(mine, c);
+          if (n > r.steps || (n == r.steps && c < lane)) before += add;
+        }
       }
+      const unsigned long long owner = __ballot(u >= before && u < before + mine);
+      if (owner != 0) {
+        const int L = __builtin_ctzll(owner);
+        x.request = b0 + L;
+        x.r.start = __builtin_amdgcn_readlane(r.start, L);
+        x.r.rows = __builtin_amdgcn_readlane(r.rows, L);
+        x.r.len = __builtin_amdgcn_readlane(r.len, L);
+        x.r.tiles = __builtin_amdgcn_readlane(r.tiles, L);
+        x.r.steps = __builtin_amdgcn_readlane(r.steps, L);
+        rest = u - __builtin_amdgcn_readlane(before, L);
+        parts = cuts_before + __builtin_amdgcn_readlane(cuts - cut, L);
+        found = true;
+      }
+      units_before += __builtin_amdgcn_readlane(upto, 63);
+      cuts_before += __builtin_amdgcn_readlane(cuts, 63);
     }
-    const int upto_cuts = sum_upto(cuts);
-    int before;
-    if (SORTED && per <= 1) {
-      before = 0;
-      for (int c = 0; c < a.requests; ++c) {
-        const int n = __builtin_amdgcn_readlane(steps[0], c), add = __builtin_amdgcn_readlane(mine, c);
-        if (n > steps[0] || (n == steps[0] && c < lane)) before += add;
-      }
-    } else {
-      before = sum_upto(mine) - mine;
-    }
-    *shared_items = (unsigned)__builtin_amdgcn_readlane(upto_cuts, 63) >> 16;
-    const unsigned long long owner = __ballot(u >= before && u < before + mine);
-    if (owner == 0) return false;
-    const int L = __builtin_ctzll(owner);
-    int at = u - before, cut_before = upto_cuts - cuts, which = 0;
-#pragma unroll
-    for (int j = 0; j + 1 < kScanPer; ++j)
-      if (which == j && at >= units[j]) {
-        at -= units[j];
-        cut_before += cut[j];
-        which = j + 1;
-      }
-    int s = start[0], e = end[0], n = len[0];
-#pragma unroll
-    for (int j = 1; j < kScanPer; ++j)
-      if (which == j) {
-        s = start[j];
-        e = end[j];
-        n = len[j];
-      }
-    x.request = L * per + __builtin_amdgcn_readlane(which, L);
-    x.r = request_of(a, __builtin_amdgcn_readlane(s, L), __builtin_amdgcn_readlane(e, L), __builtin_amdgcn_readlane(n, L), tile_rows);
-    rest = __builtin_amdgcn_readlane(at, L);
-    parts = __builtin_amdgcn_readlane(cut_before, L);
+    *shared_items = (unsigned)cuts_before >> 16;
+    if (!found) return false;
   } else {
     const int32_t* units = a.offsets + 2;   // [requests + 1], then [requests] of parts
     chunk = a.offsets[0];
@@ -274,18 +250,24 @@ __device__ __forceinline__ void fill_rest(const FxKvAttnArgs& a) {
   }
 }
 
+__device__ __forceinline__ float max3(float a, float b, float c) {   // (fmaxf quiets what the matrix cores give it, an instruction for each)
+  float r;
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+  return r;
+}
+
 // ---- 16 rows a tile: single tokens and few rows ----
 // Bound: HBM, each key and value is read once by one wave, straight into the registers of its operand; 64 tokens a
 // step, the four waves of a workgroup in turn.  The loads of the next step's keys are under way during the softmax and the second
 // product, those of the values during the first.
 template <int HELD, int TQ, int DP, bool EXACT>
-__global__ __launch_bounds__(256) void fx_kv_rows(const FxKvAttnArgs a) {
+__global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void fx_kv_rows(const FxKvAttnArgs a) {
   typedef typename TypeOf<TQ>::type T;
   constexpr int W = 4, NQ = TQ == kF32 ? 3 : 1, NP = TQ == kF32 ? 3 : 2, C = DP / 64, DT = DP / 16, LD = DP + 4;
   constexpr bool F16 = TQ == kF16;
   __shared__ __align__(16) float s_acc[W][FX_KV_ROWS][LD];
   __shared__ float s_ml[W][FX_KV_ROWS][2];
-  const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6;
+  const int lane = (int)threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int col = lane & 15, kg = lane >> 4;
   const int D = EXACT ? DP : a.c.depth, G = a.group, lp = a.c.log_page, pm = (1 << lp) - 1;
   for (int u = (int)blockIdx.x;; u += (int)gridDim.x) {
@@ -320,10 +302,11 @@ __global__ __launch_bounds__(256) void fx_kv_rows(const FxKvAttnArgs a) {
 #pragma unroll
     for (int d = 0; d < DT; ++d) acc[d] = fx_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     float m = -kInf, l = 0.0f;
+    bool nans = false;   // a step had values that are NaN and rows that do not see all its tokens
     const int32_t* table = a.table + (int64_t)x.request * a.table_stride;
     const int k_group = (col >> 2) * 16, k_row = col & 3;
     const int64_t head_at = (int64_t)x.head * (pm + 1) * D;
-    auto page_of = [&](int token) { return fx_kv_page(table[min(token >> lp, a.columns - 1)], a.c.pages); };   // -1: none
+    auto entry_of = [&](int token) { return table[min(token >> lp, a.columns - 1)]; };   // as it is: looked at when it is used, a step later
     uint4 kr[4][C];
     // a lane beyond the depth takes its row's first numbers again: its queries there are 0
     int k_at[C];
@@ -338,11 +321,15 @@ __global__ __launch_bounds__(256) void fx_kv_rows(const FxKvAttnArgs a) {
         for (int c = 0; c < C; ++c)
           kr[r][c] = *(const uint4*)(p + r * 4 * D + (EXACT ? c * 64 : k_at[c]));
     };
-        int step = from + wave, pk = 0, pv = 0;
+        // entries of the step after this one, and the page of this one's values
+    int step = from + wave, entry = 0, next_k = 0, next_v = 0, pv = 0;
     if (step < to) {
-      pk = page_of(step * FX_KV_STEP + k_group);
-      pv = page_of(step * FX_KV_STEP + kg * 16);
-      load_keys(step, max(pk, 0));
+      entry = entry_of(step * FX_KV_STEP + k_group);
+      const int ev = entry_of(step * FX_KV_STEP + kg * 16);
+      next_k = entry_of((step + W) * FX_KV_STEP + k_group);
+      next_v = entry_of((step + W) * FX_KV_STEP + kg * 16);
+      load_keys(step, max(fx_kv_page(entry, a.c.pages), 0));
+      pv = fx_kv_page(ev, a.c.pages);
     }
     for (; step < to; step += W) {
       const int base = step * FX_KV_STEP;
@@ -353,14 +340,16 @@ __global__ __launch_bounds__(256) void fx_kv_rows(const FxKvAttnArgs a) {
       {
         const uint8_t* p = a.c.v + (int64_t)page * a.c.v_stride + head_at + (int64_t)(((base + kg * 16) & pm) >> 4) * 16 * D + col * 16;
 #pragma unroll
-        for (int d = 0; d < DT; ++d)
-          if (EXACT || d * 16 < D) vr[d] = *(const uint4*)(p + d * 256);
+        for (int d = 0; d < DT; ++d) vr[d] = *(const uint4*)(p + (EXACT ? d * 256 : min(d * 16, D - 16) * 16));   // (beyond the depth: not used)
       }
+      // (the last step loads its own keys once more: with a load that may not happen the compiler waits for the values and the next
+      // keys together)
       const bool more = step + W < to;
-      if (more) {
-        pk = page_of(base + W * FX_KV_STEP + k_group);
-        pv = page_of(base + W * FX_KV_STEP + kg * 16);
-      }
+      const int pk = max(fx_kv_page(more ? next_k : entry, a.c.pages), 0);
+      pv = fx_kv_page(next_v, a.c.pages);
+      entry = next_k;
+      next_k = entry_of(base + 2 * W * FX_KV_STEP + k_group);
+      next_v = entry_of(base + 2 * W * FX_KV_STEP + kg * 16);
       // scores
       float s[16];
 #pragma unroll
@@ -378,74 +367,38 @@ __global__ __launch_bounds__(256) void fx_kv_rows(const FxKvAttnArgs a) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) s[r * 4 + e] = t[e];
       }
-      if (more) load_keys(step + W, max(pk, 0));
-      float cs = ks * a.scale, vscale = vs;
+      load_keys(more ? step + W : step, pk);
+      float cs = fmaxf(ks * a.scale, kTiny), vscale = fmaxf(vs, kTiny);
       const bool inside = base >= span.all_low && base + FX_KV_STEP <= span.all_high && __all(ok);
       if (!inside) {
+        int hi_row_ = hi_row, lo_row_ = lo_row;
+        asm volatile("" : "+v"(hi_row_), "+v"(lo_row_));   // (compared here, not ahead of the branch)
         const int t0 = base + kg * 16;
-        const int n_any = ok ? min(max(span.high - t0, 0), 16) : 0;   // tokens of this group that some row may see
-        if (n_any == 0) cs = vscale = 1.0f;                      // (what lies there may be anything)
-        const int h = ok ? hi_row - t0 : 0, b = lo_row - t0;
+        if (!ok || span.high <= t0) cs = vscale = 1.0f;   // (what lies there may be anything)
+        const int h = ok ? hi_row_ - t0 : 0, b = lo_row_ - t0;
 #pragma unroll
         for (int e = 0; e < 16; ++e) s[e] = e < h && e >= b ? s[e] : -kInf;
-        const int skip = min(max(span.low - t0, 0), 16);
-        unsigned keep[4];
+        if constexpr (HELD == 0) {
+          // a value that is NaN would reach the rows that do not see its token, as 0 * NaN: see below
+          unsigned any = 0;
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {   // bytes of tokens that some row may see
-          const int up = min(max(n_any - 4 * w, 0), 4), down = min(max(skip - 4 * w, 0), 4);
-          const unsigned upper = up == 4 ? ~0u : (1u << (8 * up)) - 1, lower = down == 4 ? ~0u : (1u << (8 * down)) - 1;
-          keep[w] = upper & ~lower;
-        }
-        unsigned nans = 0;
-#pragma unroll
-        for (int d = 0; d < DT; ++d)
-          if (EXACT || d * 16 < D) {
+          for (int d = 0; d < DT; ++d) {
             unsigned* v = (unsigned*)&vr[d];
 #pragma unroll
             for (int w = 0; w < 4; ++w) {
-              v[w] &= keep[w];
-              if constexpr (HELD == 0) nans |= nan_codes(v[w]);
+              const unsigned n = nan_codes(v[w]);
+              any |= n;
+              v[w] &= ~((n >> 7) * 0xffu);
             }
           }
-        if constexpr (HELD == 0) {
-          // A value that is NaN must not reach the rows that do not see its token, and 0 * NaN would: such codes
-          // are taken out, and the rows that see them get their NaN here.
-          if (__any(nans != 0)) {
-            Frag sees[2];
-            float y[16];
-#pragma unroll
-            for (int e = 0; e < 16; ++e) y[e] = e < h && e >= b ? 1.0f : 0.0f;
-            Frag one[1];
-            split8<1>(one, y);
-            sees[0] = one[0];
-            split8<1>(one, y + 8);
-            sees[1] = one[0];
-#pragma unroll
-            for (int d = 0; d < DT; ++d)
-              if (EXACT || d * 16 < D) {
-                unsigned* v = (unsigned*)&vr[d];
-                unsigned is[4];
-#pragma unroll
-                for (int w = 0; w < 4; ++w) {
-                  const unsigned n = nan_codes(v[w]) >> 7;
-                  is[w] = n * 0x38u;   // e4m3's 1
-                  v[w] &= ~(n * 0xffu);
-                }
-                fx_f32x4 t = {0.0f, 0.0f, 0.0f, 0.0f};
-                t = mfma16<false>(eight<0, false>(is[0], is[1]), sees[0], t);
-                t = mfma16<false>(eight<0, false>(is[2], is[3]), sees[1], t);
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                  if (t[e] > 0.0f) acc[d][e] = __builtin_nanf("");
-              }
-          }
+          nans = nans || __any(any != 0);
         }
       }
       // running maximum: raised only where a score is 8 or more above it (weights stay below 2^8)
-      float top = s[0];
+      float top = max3(s[0], s[1], s[2]);
 #pragma unroll
-      for (int e = 1; e < 16; ++e) top = fmaxf(top, s[e]);
-      top *= cs;
+      for (int e = 3; e < 15; e += 2) top = max3(top, s[e], s[e + 1]);
+      top = fmaxf(top, s[15]) * cs;
       if (__any(top > m + 8.0f || (m == -kInf && top > -kInf))) {
         top = fmaxf(top, __shfl_xor(top, 16, 64));
         top = fmaxf(top, __shfl_xor(top, 32, 64));
@@ -459,14 +412,16 @@ __global__ __launch_bounds__(256) void fx_kv_rows(const FxKvAttnArgs a) {
           for (int e = 0; e < 4; ++e) acc[d][e] *= by;
       }
       const float sub = m == -kInf ? 0.0f : m;
+      // weights times the values' scale, a power of two: part of the exponent, and taken out of their sum again
       Frag p[2][NP];
-      float w[16];
+      float w[16], sum[2] = {0.0f, 0.0f};
+      const float off = __builtin_amdgcn_logf(vscale) - sub;
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
-        w[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e], cs, -sub));
-        l += w[e];
-        w[e] *= vscale;
+        w[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e], cs, off));
+        sum[e & 1] += w[e];
       }
+      l = __builtin_fmaf(sum[0] + sum[1], __builtin_amdgcn_rcpf(vscale), l);
       split8<NP>(p[0], w);
       split8<NP>(p[1], w + 8);
 #pragma unroll
@@ -479,6 +434,31 @@ __global__ __launch_bounds__(256) void fx_kv_rows(const FxKvAttnArgs a) {
             acc[d] = mfma16<false>(v1, p[1][k], acc[d]);
           }
         }
+    }
+    if constexpr (HELD == 0) {
+      if (nans) {   // the rows that see a NaN get it here: in which column of the values, by a product of ones
+        for (int again = from + wave; again < to; again += W) {
+          const int t0 = again * FX_KV_STEP + kg * 16, page = fx_kv_page(entry_of(t0), a.c.pages), h = page >= 0 ? hi_row - t0 : 0, b = lo_row - t0;
+          Frag sees[2];
+#pragma unroll
+          for (int k = 0; k < 8; ++k)
+            sees[k >> 2].u[k & 3] = (2 * k < h && 2 * k >= b ? 0x3f80u : 0u) | (2 * k + 1 < h && 2 * k + 1 >= b ? 0x3f800000u : 0u);
+          const uint8_t* v = a.c.v + (int64_t)max(page, 0) * a.c.v_stride + head_at + (int64_t)((t0 & pm) >> 4) * 16 * D;
+#pragma unroll
+          for (int d = 0; d < DT; ++d) {
+            uint4 is = *(const uint4*)(v + min(d * 16 + col, D - 1) * 16);
+            unsigned* k = (unsigned*)&is;
+#pragma unroll
+            for (int w = 0; w < 4; ++w) k[w] = (nan_codes(k[w]) >> 7) * 0x38u;   // e4m3's 1
+            fx_f32x4 n = {0.0f, 0.0f, 0.0f, 0.0f};
+            n = mfma16<false>(eight<0, false>(is.x, is.y), sees[0], n);
+            n = mfma16<false>(eight<0, false>(is.z, is.w), sees[1], n);
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (n[e] > 0.0f) acc[d][e] = __builtin_nanf("");
+          }
+        }
+      }
     }
     // the four waves' results into one
     l += __shfl_xor(l, 16, 64);
@@ -554,11 +534,6 @@ template <int DP>
 __device__ __forceinline__ int key_piece(int token, int piece) {   // where 8 numbers of a key lie in its row
   constexpr int kMask = DP / 8 - 1 < 15 ? DP / 8 - 1 : 15;
   return piece ^ (((token & 3) | ((token >> 2) & 4) | ((token << 1) & 8)) & kMask);
-}
-__device__ __forceinline__ float max3(float a, float b, float c) {   // (fmaxf quiets what the matrix cores give it, an instruction for each)
-  float r;
-  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
-  return r;
 }
 
 // N operands from LDS, four at a time, each four on their way while the four before are used: read(i) gives operand i, use(i, operand)
@@ -706,7 +681,7 @@ __global__ __launch_bounds__(256, DP <= 128 && TQ != kF32 ? 2 : 1) void fx_kv_ti
       const uint8_t* kt = s_kv[buffer][0];
       const uint8_t* vt = s_kv[buffer][1];
       const int p0 = pg[0], p1 = pg[1];
-      float cs[2] = {ks[0] * a.scale, ks[1] * a.scale}, cv[2] = {vs[0], vs[1]};
+      float cs[2] = {fmaxf(ks[0] * a.scale, kTiny), fmaxf(ks[1] * a.scale, kTiny)}, cv[2] = {fmaxf(vs[0], kTiny), fmaxf(vs[1], kTiny)};
       __syncthreads();   // this step's numbers are there, and everyone is done with the other buffer
       if (step + 1 < to) {
         write_step(buffer ^ 1);
@@ -784,7 +759,7 @@ __global__ __launch_bounds__(256, DP <= 128 && TQ != kF32 ? 2 : 1) void fx_kv_ti
           s[t][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][e], cs[t], off));
           sum[e & 1] += s[t][e];
         }
-        l = __builtin_fmaf(sum[0] + sum[1], 1.0f / cv[t], l);
+        l = __builtin_fmaf(sum[0] + sum[1], __builtin_amdgcn_rcpf(cv[t]), l);
         split8<NP>(p[t][0], s[t]);
         split8<NP>(p[t][1], s[t] + 8);
       }

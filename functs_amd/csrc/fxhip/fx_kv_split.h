@@ -15,7 +15,7 @@
 #endif
 
 #define FX_KV_STEP 64    // cached tokens of a step of a wave
-#define FX_KV_TARGET 512 // parts that a call's work is cut into, about
+#define FX_KV_TARGET 256 // parts that a call's work is cut into, about
 
 struct FxKvRequest {
   int start, rows, len, tiles, steps;   // steps: of all its rows together
