@@ -69,7 +69,13 @@ fx_kv_cache cacheOf(const char* op, const Tensor& k, const Tensor& v, const Tens
   for (const Tensor* s : {&ks, &vs})
     TORCH_CHECK(s->scalar_type() == at::kFloat && s->dim() == 2 && s->size(0) == N && s->size(1) == H && (H == 1 || s->stride(1) == 1), op,
                 ": scales must be float32 [pages, heads], heads side by side, got ", s->scalar_type(), " ", s->sizes());
-  TORCH_CHECK(N == 0 || (k.select(0, 0).is_contiguous() && v.select(0, 0).is_contiguous()), op, ": a page of the cache must be contiguous");
+  const auto packed = [](const Tensor& t) {   // (sizes of 1 have any stride)
+    int64_t step = 1;
+    for (int64_t d = t.dim() - 1; d > 0; step *= t.size(d--))
+      if (t.size(d) != 1 && t.stride(d) != step) return false;
+    return true;
+  };
+  TORCH_CHECK(packed(k) && packed(v), op, ": a page of the cache must be contiguous");
   fx_kv_cache c;
   memset(&c, 0, sizeof c);
   c.k = k.data_ptr();
@@ -248,6 +254,7 @@ void attend(const Tensor& q_, const Tensor& k_cache, const Tensor& v_cache, cons
   // (scratch memory of this call alone, from the allocator of the current stream: calls on other streams and captured
   // graphs have their own)
   const size_t bytes = fx_kv_attention_workspace_bytes(&c, &d);
+  TORCH_CHECK(bytes > 0 || d.tokens == 0, "fxhip: ", fx_last_error(), " (", op, ")");
   const Tensor ws = at::empty({(int64_t)std::max<size_t>(bytes, 256)}, at::TensorOptions().dtype(at::kByte).device(dev));
   d.workspace = ws.data_ptr();
   d.workspace_bytes = (size_t)ws.numel();

@@ -508,6 +508,9 @@ def test_long_caches_are_shared_by_workgroups(kind):
     check_attention([(9000, 1)], INT8, kind, 16, 1, 1, 128, seed=10)
     check_attention([(5000, 40), (33, 2), (3000, 90)], E4M3, kind, 64, 1, 3, 64, seed=11)
     check_attention([(4100, 131)], INT8, kind, 32, 2, 1, 128, seed=12, window=2500)
+    check_attention([(5000, 1), (64, 1), (3001, 2), (0, 1)], E4M3, kind, 128, 4, 4, 128, seed=13)
+    check_attention([(4000, 3)], INT8, kind, 64, 5, 7, 80, seed=14, window=3300)
+    check_attention([(1500, 1), (900, 1)], E4M3, kind, 64, 8, 1, 256, seed=15)
 
 
 @pytest.mark.gpu
@@ -573,6 +576,18 @@ def test_what_a_row_does_not_see_has_no_influence(n, window):
     got, l = cache.attention(*args)
     assert bool(torch.isnan(got[n - 2:, :G]).all()) and bool(torch.isnan(l[n - 2:, :G]).all())
     assert torch.equal(got[:n - 2], out[:n - 2]) and torch.equal(l[:n - 2], lse[:n - 2])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [1, 70])
+def test_memory_that_nobody_has_written(n):
+    """A cache of zeros, its scales too, as a warm-up may have it: results are finite, and next to nothing."""
+    c = KvCache(*[torch.zeros_like(t.view(torch.uint8) if t.element_size() == 1 else t) for t in (lambda c: (c.k, c.v, c.k_scale, c.v_scale))(KvCache.empty(4, 2, 32, 64))])
+    c.k, c.v = c.k.view(E4M3), c.v.view(E4M3)
+    out, lse = c.attention(torch.randn(n, 4, 64).cuda(), i32([[0, 1, 2, 3]]), i32([100]), i32([0, n]))
+    assert float(out.abs().max()) < 1e-30
+    seen = torch.arange(100 - n + 1, 101).double()[:, None].expand(n, 4)
+    assert bool(((lse.cpu().double() - seen.log()).abs() < 1e-5).all())
 
 
 @pytest.mark.gpu
@@ -755,12 +770,13 @@ def test_a_captured_step_serves_other_lengths():
 
 
 @pytest.mark.gpu
-def test_two_streams_at_once():
+@pytest.mark.parametrize("heads", [2, 4])
+def test_two_streams_at_once(heads):
     """Calls on two streams, and two captured graphs that run side by side, keep their results apart (each has its own scratch memory)."""
-    cache = filled(300, 2, 64, 64, E4M3, 4)
+    cache = filled(300, heads, 64, 64, E4M3, 4)
     table, lens, starts = requests([(9000, 1), (5000, 1)], 64, 300, 1)
     table, lens, starts = i32(table), i32(lens), i32(starts)
-    qs = [torch.randn(2, 8, 64, generator=torch.Generator().manual_seed(i)).cuda() for i in range(2)]
+    qs = [torch.randn(2, heads * 4, 64, generator=torch.Generator().manual_seed(i)).cuda() for i in range(2)]
     want = [cache.attention(q, table, lens, starts)[0] for q in qs]
     torch.cuda.synchronize()
     streams, graphs, outs = [torch.cuda.Stream() for _ in qs], [], []
@@ -784,10 +800,11 @@ def test_two_streams_at_once():
 
 
 @pytest.mark.gpu
-def test_results_do_not_change_from_call_to_call():
-    cache = filled(200, 2, 64, 128, E4M3, 4)
+@pytest.mark.parametrize("heads", [2, 8])
+def test_results_do_not_change_from_call_to_call(heads):
+    cache = filled(200, heads, 64, 128, E4M3, 4)
     table, lens, starts = requests([(9000, 1), (500, 3), (64, 1)], 64, 200, 1)
-    q = torch.randn(5, 8, 128).half().cuda()
+    q = torch.randn(5, heads * 4, 128).half().cuda()
     first = cache.attention(q, i32(table), i32(lens), i32(starts))
     for _ in range(10):
         again = cache.attention(q, i32(table), i32(lens), i32(starts))
