@@ -1661,8 +1661,12 @@ int kv_cache_of(const char* at, const fx_kv_cache* c, FxKvCache& out) {
     return fail(FX_E_INVALID, op + ": keys and values must be 16-byte aligned, and so their pages");
   if (c->pages > 1 && (c->k_page_stride < bytes || c->v_page_stride < bytes || c->k_scale_page_stride < c->heads || c->v_scale_page_stride < c->heads))
     return fail(FX_E_INVALID, op + ": pages overlap");
-  out = FxKvCache{(uint8_t*)c->k, (uint8_t*)c->v, c->k_scale, c->v_scale, c->k_page_stride, c->v_page_stride, c->k_scale_page_stride,
-                  c->v_scale_page_stride, c->pages, c->heads, c->depth, log_page_of(c->page_size)};
+  // (distances are 32 bits in the kernels, which multiply them by page numbers in 64)
+  if (bytes >= int64_t{1} << 31 || (c->pages > 1 && (c->k_page_stride >= int64_t{1} << 32 || c->v_page_stride >= int64_t{1} << 32 ||
+                                                     c->k_scale_page_stride >= int64_t{1} << 30 || c->v_scale_page_stride >= int64_t{1} << 30)))
+    return fail(FX_E_LIMIT, op + ": pages of 2 GiB and more, or 4 GiB and more apart");
+  out = FxKvCache{(uint8_t*)c->k, (uint8_t*)c->v, c->k_scale, c->v_scale, (uint32_t)c->k_page_stride, (uint32_t)c->v_page_stride,
+                  (uint32_t)c->k_scale_page_stride, (uint32_t)c->v_scale_page_stride, c->pages, c->heads, c->depth, log_page_of(c->page_size)};
   return FX_OK;
 }
 int kv_rows_of(const char* at, const FxKvCache& c, const fx_kv_rows* r, FxKvRows& out) {
@@ -1745,7 +1749,7 @@ size_t fx_kv_attention_workspace_bytes(const fx_kv_cache* cache, const fx_kv_att
   FxKvCache c;
   if (!desc || kv_cache_of("fx_kv_attention", cache, c) != FX_OK) return 0;
   // (one after the other, the kernels of a call use the same memory)
-  const size_t parts = (size_t)2 * FX_KV_TARGET * (kv_launch(c, *desc).tiles_grid > 0 ? FX_KV_TILE : FX_KV_ROWS);
+  const size_t parts = (size_t)2 * FX_KV_TARGET * (kv_launch(c, *desc).tiles_grid > 0 ? FX_KV_TILE_MOST : FX_KV_ROWS);
   const size_t offsets = kv_round(((size_t)std::max(desc->requests, 0) * 2 + 3) * sizeof(int32_t));   // (fx_kv_offsets)
   return 256 + offsets + kv_round(FX_KV_TARGET * sizeof(FxKvItem)) + kv_round(parts * 2 * sizeof(float)) + kv_round(parts * (size_t)c.depth * sizeof(float));
 }
@@ -1800,7 +1804,7 @@ int fx_kv_attention(const fx_kv_cache* cache, const fx_kv_attention_desc* desc, 
   a.offsets = (int32_t*)(w += 256);
   a.items = (FxKvItem*)(w += kv_round(((size_t)d.requests * 2 + 3) * sizeof(int32_t)));
   a.part_ml = (float*)(w += kv_round(FX_KV_TARGET * sizeof(FxKvItem)));
-  a.part_acc = (float*)(w += kv_round((size_t)2 * FX_KV_TARGET * (l.tiles_grid > 0 ? FX_KV_TILE : FX_KV_ROWS) * 2 * sizeof(float)));
+  a.part_acc = (float*)(w += kv_round((size_t)2 * FX_KV_TARGET * (l.tiles_grid > 0 ? FX_KV_TILE_MOST : FX_KV_ROWS) * 2 * sizeof(float)));
   HIP_OK(fx_launch_kv_attention(a, l, (hipStream_t)stream));
   return kv_launched(((l.rows_grid > 0) + (l.tiles_grid > 0)) * (l.shared ? 2 : 1));   // (fx_kv_offsets aside)
 }

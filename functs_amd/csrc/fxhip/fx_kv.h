@@ -11,8 +11,8 @@
 struct FxKvCache {
   uint8_t *k, *v;
   float *k_scale, *v_scale;               // [pages][heads], rows scale_stride apart
-  int64_t k_stride, v_stride;             // bytes from page to page
-  int64_t ks_stride, vs_stride;           // floats from page to page
+  uint32_t k_stride, v_stride;            // bytes from page to page
+  uint32_t ks_stride, vs_stride;          // floats from page to page
   int32_t pages, heads, depth, log_page;  // (page: 16 to 256 tokens, a power of two)
 };
 
@@ -38,7 +38,8 @@ hipError_t fx_launch_kv_store(const FxKvCache& c, const FxKvRows& r, int held, h
 hipError_t fx_launch_kv_read(const FxKvCache& c, const FxKvRows& r, int held, hipStream_t stream);
 
 #define FX_KV_ROWS 16   // rows (tokens of a request times query heads of a key head) of a tile of fx_kv_rows
-#define FX_KV_TILE 128  // rows of a tile of fx_kv_tiles
+#define FX_KV_TILE 128  // rows of a tile of fx_kv_tiles, at least
+#define FX_KV_TILE_MOST 256
 #define FX_KV_FEW 48    // requests of more rows are fx_kv_tiles' where a call may have both
 struct FxKvItem {   // rows whose cached tokens several workgroups shared
   int32_t request, head, tile, first, parts;

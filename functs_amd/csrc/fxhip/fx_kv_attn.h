@@ -12,6 +12,8 @@
 //   queries  bf16, f16: as they are;  fp32: three bf16 (24 bits)
 //   weights  bf16, f16 results: two bf16 (16 bits);  fp32 results: three
 #pragma once
+#include <type_traits>
+
 #include "fx_kv.h"
 #include "fx_kv_device.h"
 
@@ -22,6 +24,7 @@ typedef _Float16 fx_f16x2 __attribute__((ext_vector_type(2)));
 typedef float fx_f32x4 __attribute__((ext_vector_type(4)));
 
 namespace fxkv {
+typedef const __attribute__((address_space(4))) FxKvAttnArgs KernelArgs;   // where a kernel's arguments are
 constexpr float kInf = __builtin_inff(), kLn2 = 0.693147180559945309f;
 constexpr float kTiny = 1.17549435e-38f;   // in place of scales of 0 (memory that nobody has written): -inf and 0 stay what they are under it
 enum { kBf16 = 0, kF16 = 1, kF32 = 2 };   // types of queries and results
@@ -186,14 +189,22 @@ __device__ __forceinline__ bool unit_at(const FxKvAttnArgs& a, int tile_rows, in
     parts = __builtin_amdgcn_readfirstlane(units[a.requests + 1 + lo]);
     x.r = request_of(a, __builtin_amdgcn_readfirstlane(a.starts[lo]), __builtin_amdgcn_readfirstlane(a.starts[lo + 1]), __builtin_amdgcn_readfirstlane(a.lens[lo]), tile_rows);
   }
-  x.splits = fx_kv_parts(x.r.steps, chunk);
-  const int item = rest / x.splits;
+  // (the compiler does not know them as the same in all lanes)
+  auto scalar = [](int v) { return __builtin_amdgcn_readfirstlane(v); };
+  x.request = scalar(x.request), rest = scalar(rest), parts = scalar(parts), chunk = scalar(chunk);
+  x.r = FxKvRequest{scalar(x.r.start), scalar(x.r.rows), scalar(x.r.len), scalar(x.r.tiles), scalar(x.r.steps)};
+  x.splits = scalar(fx_kv_parts(x.r.steps, chunk));
+  const int item = scalar(rest / x.splits);
   x.split = rest - item * x.splits;
-  x.tile = item / a.c.heads;
+  x.tile = scalar(item / a.c.heads);
   x.head = item - x.tile * a.c.heads;
   x.part = (parts & 0xffff) + item * x.splits;
   x.item = (int)((unsigned)parts >> 16) + item;
   return true;
+}
+__device__ __forceinline__ FxKvSpan scalars(const FxKvSpan& s) {
+  return FxKvSpan{__builtin_amdgcn_readfirstlane(s.low),      __builtin_amdgcn_readfirstlane(s.high), __builtin_amdgcn_readfirstlane(s.all_low),
+                  __builtin_amdgcn_readfirstlane(s.all_high), __builtin_amdgcn_readfirstlane(s.from), __builtin_amdgcn_readfirstlane(s.to)};
 }
 static_assert(2 * FX_KV_TARGET < 1 << 15 && FX_KV_TARGET < 1 << 15, "parts and items in 16 bits each");
 
@@ -250,11 +261,8 @@ __device__ __forceinline__ void fill_rest(const FxKvAttnArgs& a) {
   }
 }
 
-__device__ __forceinline__ float max3(float a, float b, float c) {   // (fmaxf quiets what the matrix cores give it, an instruction for each)
-  float r;
-  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
-  return r;
-}
+// the larger one; a NaN loses (fmaxf does the same and quiets what the matrix cores give it, an instruction for each)
+__device__ __forceinline__ float larger(float a, float b) { return __builtin_amdgcn_fmed3f(a, b, __builtin_inff()); }
 
 // ---- 16 rows a tile: single tokens and few rows ----
 // Bound: HBM, each key and value is read once by one wave, straight into the registers of its operand; 64 tokens a
@@ -283,7 +291,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void fx_kv_rows(const FxKvA
     const int i = valid ? row / G : 0, g = valid ? row - i * G : 0;
     const int hi_row = valid ? x.r.len - x.r.rows + i + 1 : 0;                             // tokens [lo_row, hi_row)
     const int lo_row = a.window > 0 ? max(hi_row - a.window, 0) : 0;
-    const FxKvSpan span = fx_kv_span(x.r, G, a.window, r0, FX_KV_ROWS, x.split, x.splits);
+    const FxKvSpan span = scalars(fx_kv_span(x.r, G, a.window, r0, FX_KV_ROWS, x.split, x.splits));
     const int from = span.from, to = span.to;
     // queries: lane kg holds depths 64 c + 16 kg ... + 15 of its row
     Frag q[NQ][2 * C];
@@ -395,10 +403,10 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void fx_kv_rows(const FxKvA
         }
       }
       // running maximum: raised only where a score is 8 or more above it (weights stay below 2^8)
-      float top = max3(s[0], s[1], s[2]);
+      float top = larger(s[0], s[1]);
 #pragma unroll
-      for (int e = 3; e < 15; e += 2) top = max3(top, s[e], s[e + 1]);
-      top = fmaxf(top, s[15]) * cs;
+      for (int e = 2; e < 16; ++e) top = larger(top, s[e]);
+      top *= cs;
       if (__any(top > m + 8.0f || (m == -kInf && top > -kInf))) {
         top = fmaxf(top, __shfl_xor(top, 16, 64));
         top = fmaxf(top, __shfl_xor(top, 32, 64));
@@ -517,11 +525,15 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void fx_kv_rows(const FxKvA
   if (a.fill) fill_rest<T>(a);
 }
 
-// ---- 128 rows a tile: prompts ----
-// Bound: the vector units, which turn scores into weights, beside the matrix cores.  Four waves take 32 rows each and share the
-// cached tokens, 64 a step: each wave turns a quarter of the step's codes into 16-bit floats and leaves them in LDS for all four,
-// in one of two buffers while the other one is computed with.  32 x 32 products; as above the scores stay where the second
-// product reads them: row 8 g + 4 h + j of K's operand is token 16 h + 4 g + j, so a lane holds the 16 tokens of one group.
+// ---- 32 rows a wave: prompts ----
+// Bound: the matrix cores and the vector units, which turn scores into weights, side by side.  The waves of a workgroup take 32 rows
+// each and share the cached tokens, 64 a step: together they turn a step's codes into 16-bit floats and leave them in LDS.  32 x 32
+// products; as above the scores stay where the second product reads them: row 8 g + 4 h + j of K's operand is token
+// 16 h + 4 g + j, so a lane holds the 16 tokens of one group.
+// Two groups of four waves, one of each on every SIMD, half a step apart: while one is at its products (those of the
+// step before with the values, then the next scores) the other one makes its weights and its share of the operands, and a barrier
+// changes them over.  Without it both were at the same thing most of the time: MEASURE.  Where a wave's registers are more than half
+// of a SIMD's (fp32 queries, depths above 128) there is one group, which does one after the other.
 // In LDS a key's row of 16-byte pieces is permuted by its token (key_piece), which spreads the 32 rows of an operand over the banks; values
 // lie as [group][8 tokens of it][depth][8 tokens].
 typedef float fx_f32x16 __attribute__((ext_vector_type(16)));
@@ -535,14 +547,15 @@ __device__ __forceinline__ int key_piece(int token, int piece) {   // where 8 nu
   constexpr int kMask = DP / 8 - 1 < 15 ? DP / 8 - 1 : 15;
   return piece ^ (((token & 3) | ((token >> 2) & 4) | ((token << 1) & 8)) & kMask);
 }
-
 // N operands from LDS, four at a time, each four on their way while the four before are used: read(i) gives operand i, use(i, operand)
-// takes it.  (Left to itself the compiler reads each one right before its product, to save registers.)
-template <int N, class Read, class Use>
-__device__ __forceinline__ void piped(Read read, Use use) {
+// takes it; meanwhile() comes while the first four are awaited.  (Left to itself the compiler reads each one right before its product, to save registers.)
+template <int N, class Read, class Use, class Meanwhile>
+__device__ __forceinline__ void piped(Read read, Use use, Meanwhile meanwhile) {
   Frag f[2][4];
 #pragma unroll
   for (int e = 0; e < 4; ++e) f[0][e] = read(e);
+  __builtin_amdgcn_sched_barrier(0);
+  meanwhile();
 #pragma unroll
   for (int b = 0; b < N / 4; ++b) {
     __builtin_amdgcn_sched_barrier(0);
@@ -554,38 +567,42 @@ __device__ __forceinline__ void piped(Read read, Use use) {
     for (int e = 0; e < 4; ++e) use(b * 4 + e, f[b & 1][e]);
   }
 }
+constexpr int tile_waves(int type, int dp) { return dp <= 128 && type != kF32 ? 8 : 4; }
+constexpr int tile_rows(int type, int dp) { return 32 * tile_waves(type, dp); }
 
 template <int HELD, int TQ, int DP, bool EXACT>
-__global__ __launch_bounds__(256, DP <= 128 && TQ != kF32 ? 2 : 1) void fx_kv_tiles(const FxKvAttnArgs a) {
+__global__ __launch_bounds__(64 * tile_waves(TQ, DP), tile_waves(TQ, DP) / 4) void fx_kv_tiles(const FxKvAttnArgs a) {
   typedef typename TypeOf<TQ>::type T;
-  constexpr int W = 4, NQ = TQ == kF32 ? 3 : 1, NP = TQ == kF32 ? 3 : TQ == kF16 ? 2 : 1, C = DP / 16, DT = DP / 32;
-  constexpr int kBlocks = DP / 64;   // KB of a step's keys that a wave takes, and as many of its values
+  constexpr int W = tile_waves(TQ, DP), kGroups = W / 4, kRows = 32 * W;
+  constexpr int NQ = TQ == kF32 ? 3 : 1, NP = TQ == kF32 ? 3 : TQ == kF16 ? 2 : 1, C = DP / 16, DT = DP / 32;
+  constexpr int kShare = DP / 8 / W;   // KB of a step's keys and values that a wave takes
   constexpr int kTile = FX_KV_STEP * DP * 2;
   constexpr bool F16 = TQ == kF16;
-  __shared__ __align__(16) uint8_t s_kv[2][2][kTile];
+  __shared__ __align__(16) uint8_t s_k[2][kTile], s_v[2][kTile];
   __shared__ int s_nan;   // e4m3: there were NaN among the values
   const int lane = (int)threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int late = kGroups == 2 ? wave >> 2 : 0;   // the group that is half a step behind
   const int col = lane & 31, half = lane >> 5;
   const int D = EXACT ? DP : a.c.depth, G = a.group, lp = a.c.log_page, pm = (1 << lp) - 1;
   for (int u = (int)blockIdx.x;; u += (int)gridDim.x) {
     Unit x;
     int shared_items = 0;
-    const bool live = unit_at<true>(a, FX_KV_TILE, kTileLeast, u, x, &shared_items);
+    const bool live = unit_at<true>(a, kRows, kTileLeast, u, x, &shared_items);
     if (u == 0 && threadIdx.x == 0) *a.n_items = shared_items;
     if (!live) break;
     __syncthreads();   // (LDS is free again)
     if (threadIdx.x == 0) s_nan = 0;
     __syncthreads();
     x.tile = x.r.tiles - 1 - x.tile;   // (the last rows see most: they begin first)
-    const int r0 = x.tile * FX_KV_TILE, w0 = r0 + wave * 32, row = w0 + col, n_rows = x.r.rows * G;
+    const int r0 = x.tile * kRows, w0 = r0 + wave * 32, row = w0 + col, n_rows = x.r.rows * G;
     const bool valid = row < n_rows;
     const int i = valid ? row / G : 0, g = valid ? row - i * G : 0;
     const int hi_row = valid ? x.r.len - x.r.rows + i + 1 : 0;
     const int lo_row = a.window > 0 ? max(hi_row - a.window, 0) : 0;
-    const FxKvSpan span = fx_kv_span(x.r, G, a.window, r0, FX_KV_TILE, x.split, x.splits);
-    FxKvSpan mine = fx_kv_span(x.r, G, a.window, min(w0, n_rows - 1), 32, 0, 1);   // of this wave's rows
+    const FxKvSpan span = scalars(fx_kv_span(x.r, G, a.window, r0, kRows, x.split, x.splits));
+    FxKvSpan mine = scalars(fx_kv_span(x.r, G, a.window, min(w0, n_rows - 1), 32, 0, 1));   // of this wave's rows
     if (w0 >= n_rows) mine.high = 0;
-    const int from = span.from, to = span.to;
+    const int from = span.from, n = span.to - span.from;
     Frag q[NQ][C];
     {
       const T* src = (const T*)a.q + (int64_t)(x.r.start + i) * a.q_token + (int64_t)(x.head * G + g) * a.q_head;
@@ -605,209 +622,259 @@ __global__ __launch_bounds__(256, DP <= 128 && TQ != kF32 ? 2 : 1) void fx_kv_ti
       for (int e = 0; e < 16; ++e) acc[d][e] = 0.0f;
     float m = -kInf, l = 0.0f;
     const int32_t* table = a.table + (int64_t)x.request * a.table_stride;
-    const int64_t head_at = (int64_t)x.head * (pm + 1) * D;
-    // the entry for group `lane & 3` of a step, as it is: looked at when it is used, a step later
-    auto entries_of = [&](int step) { return table[min((step * FX_KV_STEP + (lane & 3) * 16) >> lp, a.columns - 1)]; };
-    // A step's codes on their way: block k * W + wave of 1 KB is 64 bytes of depth for the 16 tokens of a group
-    uint4 kraw[kBlocks], vraw[kBlocks];
-    constexpr int kPieces = DP / 16, kRows = 1024 / DP;
-    auto load_step = [&](int step, int pages) {
+    const uint32_t head_at = (uint32_t)x.head * (uint32_t)(pm + 1) * (uint32_t)D;
+    // A lane's two groups of a step are `half` and 2 + half.  Their entries are taken as they are, and looked at when they are used, a step later
+    auto entry_of = [&](int s, int which) { return table[min(((from + s) * FX_KV_STEP + which * 32 + half * 16) >> lp, a.columns - 1)]; };
+    // A wave's share: blocks of 1 KB, first of the keys, then of the values; block b is 64 bytes of depth for the 16 tokens of a group
+    constexpr int kHalf = DP / 16, kPieces = DP / 16, kRowsOf = 1024 / DP, kParts = DP / 64;
+    uint4 raw[kShare];
+    auto is_keys = [&](int k) { return kShare >= 2 ? k < kShare / 2 : wave < W / 2; };
+    auto block_of = [&](int k) { return (k * W + wave) % kHalf; };
+    uint32_t key_at[kShare], to_at[kShare][2];   // of a lane: bytes from its group's first key or value, and in LDS
 #pragma unroll
-      for (int k = 0; k < kBlocks; ++k) {
-        const int block = k * W + wave, group = block / kBlocks, part = block % kBlocks;
-        const int page = max(__builtin_amdgcn_readlane(pages, group), 0);
-        const int at = (step * FX_KV_STEP + group * 16) & pm;
-        const int token = part * kRows + lane / kPieces;   // of its group
-        int piece = lane % kPieces, d = part * 64 + lane;
-        if (!EXACT) {   // (queries beyond the depth are 0, results there are dropped)
-          piece = piece * 16 < D ? piece : 0;
-          d = min(d, D - 1);
-        }
-        kraw[k] = *(const uint4*)(a.c.k + (int64_t)page * a.c.k_stride + head_at + (int64_t)(at + token) * D + piece * 16);
-        vraw[k] = *(const uint4*)(a.c.v + (int64_t)page * a.c.v_stride + head_at + (int64_t)at * D + d * 16);
+    for (int k = 0; k < kShare; ++k) {
+      const int group = block_of(k) / kParts, part = block_of(k) % kParts;
+      if (is_keys(k)) {
+        const int token = part * kRowsOf + lane / kPieces, piece = lane % kPieces, row_at = (group * 16 + token) * DP * 2;
+        key_at[k] = token * D + (EXACT || piece * 16 < D ? piece : 0) * 16;   // (queries beyond the depth are 0)
+        to_at[k][0] = row_at + key_piece<DP>(group * 16 + token, piece * 2) * 16;
+        to_at[k][1] = row_at + key_piece<DP>(group * 16 + token, piece * 2 + 1) * 16;
+      } else {
+        key_at[k] = (EXACT ? part * 64 + lane : min(part * 64 + lane, D - 1)) * 16;
+        to_at[k][0] = (group * 2 * DP + part * 64 + lane) * 16;
+        to_at[k][1] = to_at[k][0] + DP * 16;
+      }
+    }
+    // Round r: the keys of step r + 1 and the values of step r, on their way in registers and then to LDS.  (Steps behind the last one
+    // are the table's last entries again, and are not used.)
+    auto load_round = [&](int r, const int (&key_pages)[2], const int (&value_pages)[2]) {
+#pragma unroll
+      for (int k = 0; k < kShare; ++k) {
+        const int group = block_of(k) / kParts, lane_of = (group & 1) * 32;
+        const bool keys = is_keys(k);
+        const int first = __builtin_amdgcn_readlane(keys ? key_pages[0] : value_pages[0], lane_of), second = __builtin_amdgcn_readlane(keys ? key_pages[1] : value_pages[1], lane_of);
+        const uint32_t page = (uint32_t)max(group < 2 ? first : second, 0);
+        const uint32_t at = (uint32_t)(((from + r + (keys ? 1 : 0)) * FX_KV_STEP + group * 16) & pm);
+        const uint8_t* base = (keys ? a.c.k : a.c.v) + ((uint64_t)page * (keys ? a.c.k_stride : a.c.v_stride) + (head_at + at * (uint32_t)D));
+        raw[k] = *(const uint4*)(base + key_at[k]);
       }
     };
-    auto write_step = [&](int buffer) {
-      uint8_t* kt = s_kv[buffer][0];
-      uint8_t* vt = s_kv[buffer][1];
-      if constexpr (HELD == 0) {
-        unsigned nans = 0;
+    auto write_round = [&](int r) {
 #pragma unroll
-        for (int k = 0; k < kBlocks; ++k) nans |= nan_codes(vraw[k].x) | nan_codes(vraw[k].y) | nan_codes(vraw[k].z) | nan_codes(vraw[k].w);
-        if (__any(nans != 0)) {
-          if (lane == 0) s_nan = 1;
+      for (int k = 0; k < kShare; ++k) {
+        if (is_keys(k)) {
+          uint8_t* to = s_k[(r + 1) & 1];
+          *(Frag*)(to + to_at[k][0]) = eight<HELD, F16>(raw[k].x, raw[k].y);
+          *(Frag*)(to + to_at[k][1]) = eight<HELD, F16>(raw[k].z, raw[k].w);
+        } else if (r >= 0) {
+          if constexpr (HELD == 0) {
+            if (__any((nan_codes(raw[k].x) | nan_codes(raw[k].y) | nan_codes(raw[k].z) | nan_codes(raw[k].w)) != 0)) {   // (see below)
+              if (lane == 0) s_nan = 1;
+              unsigned* w = (unsigned*)&raw[k];
 #pragma unroll
-          for (int k = 0; k < kBlocks; ++k) {
-            unsigned* u = (unsigned*)&vraw[k];
-#pragma unroll
-            for (int w = 0; w < 4; ++w) u[w] &= ~((nan_codes(u[w]) >> 7) * 0xffu);
+              for (int e = 0; e < 4; ++e) w[e] &= ~((nan_codes(w[e]) >> 7) * 0xffu);
+            }
           }
+          uint8_t* to = s_v[r & 1];
+          *(Frag*)(to + to_at[k][0]) = eight<HELD, false>(raw[k].x, raw[k].y);
+          *(Frag*)(to + to_at[k][1]) = eight<HELD, false>(raw[k].z, raw[k].w);
         }
       }
-#pragma unroll
-      for (int k = 0; k < kBlocks; ++k) {
-        const int block = k * W + wave, group = block / kBlocks, part = block % kBlocks;
-        const int token = group * 16 + part * kRows + lane / kPieces, piece = lane % kPieces;
-        *(Frag*)(kt + token * DP * 2 + key_piece<DP>(token, piece * 2) * 16) = eight<HELD, F16>(kraw[k].x, kraw[k].y);
-        *(Frag*)(kt + token * DP * 2 + key_piece<DP>(token, piece * 2 + 1) * 16) = eight<HELD, F16>(kraw[k].z, kraw[k].w);
-        uint8_t* v = vt + (group * 2 * DP + part * 64 + lane) * 16;
-        *(Frag*)v = eight<HELD, false>(vraw[k].x, vraw[k].y);
-        *(Frag*)(v + DP * 16) = eight<HELD, false>(vraw[k].z, vraw[k].w);
-      }
     };
-    int pg[2] = {0, 0};             // pages of the lane's two groups of a step (-1: none), and their scales
-    float ks[2], vs[2];
-    auto scales_of = [&](int pages) {
+    int pg[2] = {-1, -1};           // pages of the lane's two groups of a step (-1: none), and their scales
+    float ks[2] = {1.0f, 1.0f}, vs[2] = {1.0f, 1.0f};
+    const float *k_scales = a.c.k_scale + x.head, *v_scales = a.c.v_scale + x.head;
+    auto scales_of = [&](const int (&pages)[2]) {
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
-        pg[t] = __shfl(pages, t * 2 + half, 64);
-        ks[t] = a.c.k_scale[(int64_t)max(pg[t], 0) * a.c.ks_stride + x.head];
-        vs[t] = a.c.v_scale[(int64_t)max(pg[t], 0) * a.c.vs_stride + x.head];
+        pg[t] = pages[t];
+        const uint32_t page = (uint32_t)max(pages[t], 0);
+        ks[t] = *(const float*)((const char*)k_scales + (uint64_t)page * (a.c.ks_stride * 4));
+        vs[t] = *(const float*)((const char*)v_scales + (uint64_t)page * (a.c.vs_stride * 4));
       }
     };
-    // What is under way: codes of step + 1 in registers, entries of step + 2, scales of `step`
-    int pages1 = 0, entries2 = 0;
-    if (from < to) {
-      const int pages0 = fx_kv_page(entries_of(from), a.c.pages);
-      load_step(from, pages0);
-      scales_of(pages0);
-      if (from + 1 < to) pages1 = fx_kv_page(entries_of(from + 1), a.c.pages);
-      write_step(0);
-      if (from + 1 < to) load_step(from + 1, pages1);
-      if (from + 2 < to) entries2 = entries_of(from + 2);
-    }
-    for (int step = from; step < to; ++step) {
-      const int base = step * FX_KV_STEP, buffer = (step - from) & 1;
-      const uint8_t* kt = s_kv[buffer][0];
-      const uint8_t* vt = s_kv[buffer][1];
-      const int p0 = pg[0], p1 = pg[1];
-      float cs[2] = {fmaxf(ks[0] * a.scale, kTiny), fmaxf(ks[1] * a.scale, kTiny)}, cv[2] = {fmaxf(vs[0], kTiny), fmaxf(vs[1], kTiny)};
-      __syncthreads();   // this step's numbers are there, and everyone is done with the other buffer
-      if (step + 1 < to) {
-        write_step(buffer ^ 1);
-        const int pages2 = fx_kv_page(entries2, a.c.pages);
-        if (step + 2 < to) load_step(step + 2, pages2);
-        scales_of(pages1);
-        pages1 = pages2;
-        if (step + 3 < to) entries2 = entries_of(step + 3);
+    // pages of steps s and s + 1, and entries of step s + 2, of the products of step s
+    int pages0[2] = {-1, -1}, pages1[2] = {-1, -1}, entries2[2] = {-1, -1};
+    if (n > 0) {
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        pages0[t] = fx_kv_page(entry_of(0, t), a.c.pages);
+        pages1[t] = fx_kv_page(entry_of(1, t), a.c.pages);
+        entries2[t] = entry_of(2, t);
       }
-      __builtin_amdgcn_sched_barrier(0);   // (here and below: what is loaded early stays in registers that are not there)
-      if (base >= mine.high || base + FX_KV_STEP <= mine.low) continue;   // (none of this wave's rows sees it)
-      float s[2][16];
-      int krow = ((col >> 2) & 1) * 16 + (col >> 3) * 4 + (col & 3);
-      int kpiece = key_piece<DP>(krow, half) * 16;
-      krow *= DP * 2;
-      asm volatile("" : "+v"(krow), "+v"(kpiece));   // (16 addresses that are not worth a register each)
-      fx_f32x16 r[2];
+      load_round(-1, pages0, pages0);
+      write_round(-1);
+      if (late) load_round(0, pages1, pages0);
+    }
+    __syncthreads();
+    fx_f32x16 r[2];     // scores of a step
+    Frag p[2][2][NP];   // its weights
 #pragma unroll
-      for (int t = 0; t < 2; ++t)
+    for (int t = 0; t < 2; ++t)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) r[t][e] = 0.0f;
-      piped<2 * C>([&](int n) { return *(const Frag*)(kt + n / C * 32 * DP * 2 + krow + (kpiece ^ (n % C * 32))); },
-                   [&](int n, const Frag& kf) {
+      for (int e = 0; e < 16; ++e) r[t][e] = 0.0f;
 #pragma unroll
-                     for (int k = NQ - 1; k >= 0; --k) r[n / C] = mfma32<F16>(kf, q[k][n % C], r[n / C]);
-                   });
-      __builtin_amdgcn_sched_barrier(0);
+    for (int t = 0; t < 4; ++t)
 #pragma unroll
-      for (int t = 0; t < 2; ++t)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) s[t][e] = r[t][e];
-      const bool inside = base >= mine.all_low && base + FX_KV_STEP <= mine.all_high && __all(p0 >= 0 && p1 >= 0);
-      if (!inside) {
-        int hi_row_ = hi_row, lo_row_ = lo_row;
-        asm volatile("" : "+v"(hi_row_), "+v"(lo_row_));   // (compared here, not ahead of the branch)
+      for (int k = 0; k < NP; ++k) p[t >> 1][t & 1][k].u[0] = p[t >> 1][t & 1][k].u[1] = p[t >> 1][t & 1][k].u[2] = p[t >> 1][t & 1][k].u[3] = 0;
+    auto sees = [&](int s) { return (from + s) * FX_KV_STEP < mine.high && (from + s + 1) * FX_KV_STEP > mine.low; };   // a row of this wave does
+    // The weights of step s - 1 with its values, and the scores of step s.  While its first operands are awaited the next round and the
+    // scales of step s are sent for: round s, which this group writes with the weights of step s, and of the late group round s + 1.
+    auto products = [&](int s, auto is_late) {
+      auto send = [&]() {
+        const int pages2[2] = {fx_kv_page(entries2[0], a.c.pages), fx_kv_page(entries2[1], a.c.pages)};
+        if constexpr (is_late) load_round(s + 1, pages2, pages1);
+        else load_round(s, pages1, pages0);
+        scales_of(pages0);
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
-          const int t0 = base + (t * 2 + half) * 16;
-          const bool ok = (t ? p1 : p0) >= 0;
-          if (!ok || mine.high <= t0) cs[t] = cv[t] = 1.0f;   // (what lies there may be anything)
-          const int h = ok ? hi_row_ - t0 : 0, b = lo_row_ - t0;
-#pragma unroll
-          for (int e = 0; e < 16; ++e) s[t][e] = e < h && e >= b ? s[t][e] : -kInf;
+          pages0[t] = pages1[t];
+          pages1[t] = pages2[t];
+          entries2[t] = entry_of(s + 3, t);
         }
+      };
+      if (s > 0 && sees(s - 1)) {
+        const uint8_t* vt = s_v[(s - 1) & 1];
+        piped<4 * DT>([&](int k) { return *(const Frag*)(vt + (((k / DT / 2 * 2 + half) * 2 + k / DT % 2) * DP + k % DT * 32 + col) * 16); },
+                      [&](int k, const Frag& v) {
+#pragma unroll
+                        for (int e = NP - 1; e >= 0; --e) acc[k % DT] = mfma32<false>(v, p[k / DT / 2][k / DT % 2][e], acc[k % DT]);
+                      }, send);
+        __builtin_amdgcn_sched_barrier(0);
+      } else {
+        send();
       }
-      float top[2];
+      if (s < n && sees(s)) {
+        const uint8_t* kt = s_k[s & 1];
+        int krow = ((col >> 2) & 1) * 16 + (col >> 3) * 4 + (col & 3);
+        int kpiece = key_piece<DP>(krow, half) * 16;
+        krow *= DP * 2;
+        asm volatile("" : "+v"(krow), "+v"(kpiece));   // (16 addresses that are not worth a register each)
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        top[t] = max3(s[t][0], s[t][1], s[t][2]);
+        for (int t = 0; t < 2; ++t)
 #pragma unroll
-        for (int e = 3; e < 15; e += 2) top[t] = max3(top[t], s[t][e], s[t][e + 1]);
-        top[t] = fmaxf(top[t], s[t][15]) * cs[t];
+          for (int e = 0; e < 16; ++e) r[t][e] = 0.0f;
+        piped<2 * C>([&](int k) { return *(const Frag*)(kt + k % 2 * 32 * DP * 2 + krow + (kpiece ^ (k / 2 * 32))); },
+                     [&](int k, const Frag& kf) {
+#pragma unroll
+                       for (int e = NQ - 1; e >= 0; --e) r[k % 2] = mfma32<F16>(kf, q[e][k / 2], r[k % 2]);
+                     }, []() {});
       }
-      float up = fmaxf(top[0], top[1]);
-      if (__any(up > m + 8.0f || (m == -kInf && up > -kInf))) {
-        up = fmaxf(up, __shfl_xor(up, 32, 64));
-        const float to_m = fmaxf(m, up);
-        const float by = to_m == -kInf ? 1.0f : __builtin_amdgcn_exp2f(m - to_m);
-        m = to_m;
-        l *= by;
+    };
+    // the weights of step s, and a share of round `round`
+    auto weights = [&](int s, int round) {
+        const int p0 = pg[0], p1 = pg[1];
+        float cs[2] = {fmaxf(ks[0] * a.scale, kTiny), fmaxf(ks[1] * a.scale, kTiny)}, cv[2] = {fmaxf(vs[0], kTiny), fmaxf(vs[1], kTiny)};
+        if (round < n) write_round(round);
+        __builtin_amdgcn_sched_barrier(0);   // (what is loaded later stays out of registers that are not there)
+        if (s >= 0 && sees(s)) {
+          const int base = (from + s) * FX_KV_STEP;
+          const bool inside = base >= mine.all_low && base + FX_KV_STEP <= mine.all_high && __all(p0 >= 0 && p1 >= 0);
+          if (!inside) {
+            int hi_row_ = hi_row, lo_row_ = lo_row;
+            asm volatile("" : "+v"(hi_row_), "+v"(lo_row_));   // (compared here, not ahead of the branch)
 #pragma unroll
-        for (int d = 0; d < DT; ++d)
+            for (int t = 0; t < 2; ++t) {
+              const int t0 = base + (t * 2 + half) * 16;
+              const bool ok = (t ? p1 : p0) >= 0;
+              if (!ok || mine.high <= t0) cs[t] = cv[t] = 1.0f;   // (what lies there may be anything)
+              const int h = ok ? hi_row_ - t0 : 0, b = lo_row_ - t0;
 #pragma unroll
-          for (int e = 0; e < 16; ++e) acc[d][e] *= by;
-      }
-      const float sub = m == -kInf ? 0.0f : m;
-      // weights times the values' scale, a power of two: part of the exponent, and taken out of their sum again
-      Frag p[2][2][NP];
+              for (int e = 0; e < 16; ++e) r[t][e] = e < h && e >= b ? r[t][e] : -kInf;
+            }
+          }
+          float top[2];
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        const float off = __builtin_amdgcn_logf(cv[t]) - sub;
-        float sum[2] = {0.0f, 0.0f};
+          for (int t = 0; t < 2; ++t) {
+            top[t] = larger(r[t][0], r[t][1]);
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          s[t][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][e], cs[t], off));
-          sum[e & 1] += s[t][e];
+            for (int e = 2; e < 16; ++e) top[t] = larger(top[t], r[t][e]);
+            top[t] *= cs[t];
+          }
+          float up = fmaxf(top[0], top[1]);
+          if (__any(up > m + 8.0f || (m == -kInf && up > -kInf))) {
+            up = fmaxf(up, __shfl_xor(up, 32, 64));
+            const float to_m = fmaxf(m, up);
+            const float by = to_m == -kInf ? 1.0f : __builtin_amdgcn_exp2f(m - to_m);
+            m = to_m;
+            l *= by;
+#pragma unroll
+            for (int d = 0; d < DT; ++d)
+#pragma unroll
+              for (int e = 0; e < 16; ++e) acc[d][e] *= by;
+          }
+          const float sub = m == -kInf ? 0.0f : m;
+          // weights times the values' scale, a power of two: part of the exponent, and taken out of their sum again
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            const float off = __builtin_amdgcn_logf(cv[t]) - sub;
+            float w[16], sum[2] = {0.0f, 0.0f};
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+              w[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(r[t][e], cs[t], off));
+              sum[e & 1] += w[e];
+            }
+            l = __builtin_fmaf(sum[0] + sum[1], __builtin_amdgcn_rcpf(cv[t]), l);
+            split8<NP>(p[t][0], w);
+            split8<NP>(p[t][1], w + 8);
+          }
         }
-        l = __builtin_fmaf(sum[0] + sum[1], __builtin_amdgcn_rcpf(cv[t]), l);
-        split8<NP>(p[t][0], s[t]);
-        split8<NP>(p[t][1], s[t] + 8);
+    };
+    if (!late) {
+      for (int s = 0; s <= n; ++s) {
+        products(s, std::false_type());
+        __syncthreads();
+        if (s < n) weights(s, s);
+        __syncthreads();
       }
-      __builtin_amdgcn_sched_barrier(0);
-      piped<4 * DT>([&](int n) { return *(const Frag*)(vt + (((n / 2 % 2 * 2 + half) * 2 + n % 2) * DP + n / 4 * 32 + col) * 16); },
-                    [&](int n, const Frag& v) {
-#pragma unroll
-                      for (int k = NP - 1; k >= 0; --k) acc[n / 4] = mfma32<false>(v, p[n / 2 % 2][n % 2][k], acc[n / 4]);
-                    });
+    } else {
+      for (int s = 0; s <= n; ++s) {
+        weights(s - 1, s);
+        __syncthreads();
+        products(s, std::true_type());
+        __syncthreads();
+      }
     }
     if constexpr (HELD == 0) {
       // Values that are NaN were left out of LDS, because 0 * NaN would reach the rows that do not see their tokens: the
       // rows that do get their NaN here, from the cache itself.
-      __syncthreads();
       if (__builtin_amdgcn_readfirstlane(s_nan)) {
-        for (int step = from; step < to; ++step)
+        for (int s = 0; s < n; ++s)
           for (int t = 0; t < 2; ++t) {
-            const int t0 = step * FX_KV_STEP + (t * 2 + half) * 16;
+            const int t0 = (from + s) * FX_KV_STEP + (t * 2 + half) * 16;
             const int page = fx_kv_page(table[min(t0 >> lp, a.columns - 1)], a.c.pages), hi = page >= 0 ? hi_row - t0 : 0, lo = lo_row - t0;
-            Frag sees[2];
+            Frag see[2];
 #pragma unroll
             for (int w = 0; w < 8; ++w)
-              sees[w >> 2].u[w & 3] = (2 * w < hi && 2 * w >= lo ? 0x3f80u : 0u) | (2 * w + 1 < hi && 2 * w + 1 >= lo ? 0x3f800000u : 0u);
+              see[w >> 2].u[w & 3] = (2 * w < hi && 2 * w >= lo ? 0x3f80u : 0u) | (2 * w + 1 < hi && 2 * w + 1 >= lo ? 0x3f800000u : 0u);
             const uint8_t* v = a.c.v + (int64_t)max(page, 0) * a.c.v_stride + head_at + (int64_t)((t0 & pm) >> 4) * 16 * D;
 #pragma unroll
             for (int d = 0; d < DT; ++d) {
               uint4 is = *(const uint4*)(v + min(d * 32 + col, D - 1) * 16);
-              unsigned* u = (unsigned*)&is;
+              unsigned* w = (unsigned*)&is;
 #pragma unroll
-              for (int w = 0; w < 4; ++w) u[w] = (nan_codes(u[w]) >> 7) * 0x38u;   // e4m3's 1
-              fx_f32x16 r;
+              for (int e = 0; e < 4; ++e) w[e] = (nan_codes(w[e]) >> 7) * 0x38u;   // e4m3's 1
+              fx_f32x16 y;
 #pragma unroll
-              for (int e = 0; e < 16; ++e) r[e] = 0.0f;
-              r = mfma32<false>(eight<0, false>(is.x, is.y), sees[0], r);
-              r = mfma32<false>(eight<0, false>(is.z, is.w), sees[1], r);
+              for (int e = 0; e < 16; ++e) y[e] = 0.0f;
+              y = mfma32<false>(eight<0, false>(is.x, is.y), see[0], y);
+              y = mfma32<false>(eight<0, false>(is.z, is.w), see[1], y);
 #pragma unroll
               for (int e = 0; e < 16; ++e)
-                if (r[e] > 0.0f) acc[d][e] = __builtin_nanf("");
+                if (y[e] > 0.0f) acc[d][e] = __builtin_nanf("");
             }
           }
       }
     }
+    // (read again from memory rather than kept in scalar registers all along)
+    const KernelArgs* z = (const KernelArgs*)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(z));
     l += __shfl_xor(l, 32, 64);
     if (valid) {
       const int64_t t = x.r.start + i;
       const int h = x.head * G + g;
       const float per = l == 0.0f ? 0.0f : 1.0f / l;
-      const int64_t at = (int64_t)(x.part + x.split) * FX_KV_TILE + wave * 32 + col;
+      const int64_t at = (int64_t)(x.part + x.split) * kRows + wave * 32 + col;
 #pragma unroll
       for (int d = 0; d < DT; ++d)
 #pragma unroll
@@ -818,24 +885,24 @@ __global__ __launch_bounds__(256, DP <= 128 && TQ != kF32 ? 2 : 1) void fx_kv_ti
           if (x.splits == 1) {
 #pragma unroll
             for (int k = 0; k < 4; ++k) o[k] = acc[d][e * 4 + k] * per;
-            store4((T*)a.out + t * a.out_token + (int64_t)h * D + depth, o);
+            store4((T*)z->out + t * z->out_token + (int64_t)h * D + depth, o);
           } else {
 #pragma unroll
             for (int k = 0; k < 4; ++k) o[k] = acc[d][e * 4 + k];
-            store4(a.part_acc + at * D + depth, o);
+            store4(z->part_acc + at * D + depth, o);
           }
         }
       if (half == 0) {
         if (x.splits == 1) {
-          a.lse[t * a.q_heads + h] = l == 0.0f ? -kInf : (m + __builtin_amdgcn_logf(l)) * kLn2;
+          z->lse[t * z->q_heads + h] = l == 0.0f ? -kInf : (m + __builtin_amdgcn_logf(l)) * kLn2;
         } else {
-          a.part_ml[at * 2] = m;
-          a.part_ml[at * 2 + 1] = l;
+          z->part_ml[at * 2] = m;
+          z->part_ml[at * 2 + 1] = l;
         }
       }
     }
     if (x.splits > 1 && x.split == 0 && threadIdx.x == 0)
-      a.items[x.item] = FxKvItem{x.request, x.head, x.tile, x.part, x.splits};
+      z->items[x.item] = FxKvItem{x.request, x.head, x.tile, x.part, x.splits};
   }
   if (a.fill) fill_rest<T>(a);
 }
@@ -901,10 +968,11 @@ __global__ __launch_bounds__(256) void fx_kv_join(const FxKvAttnArgs a, int tile
 
 struct Kernels {
   const void *rows, *tiles;
+  int tile_rows;   // of `tiles`; twice as many threads
 };
 template <int HELD, int TQ>
 Kernels kernels_of(int depth) {
-#define FX_KV_PAIR(DP, EXACT) Kernels{(const void*)fx_kv_rows<HELD, TQ, DP, EXACT>, (const void*)fx_kv_tiles<HELD, TQ, DP, EXACT>}
+#define FX_KV_PAIR(DP, EXACT) Kernels{(const void*)fx_kv_rows<HELD, TQ, DP, EXACT>, (const void*)fx_kv_tiles<HELD, TQ, DP, EXACT>, tile_rows(TQ, DP)}
   if (depth == 64) return FX_KV_PAIR(64, true);
   if (depth == 128) return FX_KV_PAIR(128, true);
   if (depth == 256) return FX_KV_PAIR(256, true);

@@ -65,9 +65,9 @@ __global__ __launch_bounds__(1024) void fx_kv_offsets(const FxKvAttnArgs a, int 
 
 namespace {
 template <class... A>
-hipError_t launch(const void* kernel, int64_t grid, hipStream_t stream, A... args) {
+hipError_t launch(const void* kernel, int64_t grid, int threads, hipStream_t stream, A... args) {
   void* kargs[sizeof...(A)] = {(void*)&args...};
-  return hipLaunchKernel(kernel, dim3((unsigned)grid), dim3(256), kargs, 0, stream);
+  return hipLaunchKernel(kernel, dim3((unsigned)grid), dim3((unsigned)threads), kargs, 0, stream);
 }
 hipError_t offsets(const FxKvAttnArgs& a, int tile_rows, int least, hipStream_t stream) {
   if (a.requests <= fxkv::kScanned) return hipSuccess;
@@ -79,7 +79,7 @@ hipError_t join(const FxKvAttnArgs& a, int type, int tile_rows, hipStream_t stre
   const void* kernel = type == fxkv::kBf16 ? (const void*)fxkv::fx_kv_join<__bf16>
                        : type == fxkv::kF16 ? (const void*)fxkv::fx_kv_join<_Float16>
                                             : (const void*)fxkv::fx_kv_join<float>;
-  return launch(kernel, 2048, stream, a, tile_rows);
+  return launch(kernel, 2048, 256, stream, a, tile_rows);
 }
 }  // namespace
 
@@ -90,16 +90,16 @@ hipError_t fx_launch_kv_attention(const FxKvAttnArgs& a, const FxKvLaunch& l, hi
   if (l.tiles_grid > 0) {
     args.rows_above = l.rows_grid > 0 ? FX_KV_FEW : 0;
     args.rows_upto = int64_t{1} << 31;
-    if ((e = offsets(args, FX_KV_TILE, fxkv::kTileLeast, stream)) != hipSuccess) return e;
-    if ((e = launch(k.tiles, l.tiles_grid, stream, args)) != hipSuccess) return e;
-    if (l.shared && (e = join(args, l.type, FX_KV_TILE, stream)) != hipSuccess) return e;
+    if ((e = offsets(args, k.tile_rows, fxkv::kTileLeast, stream)) != hipSuccess) return e;
+    if ((e = launch(k.tiles, l.tiles_grid, 2 * k.tile_rows, stream, args)) != hipSuccess) return e;
+    if (l.shared && (e = join(args, l.type, k.tile_rows, stream)) != hipSuccess) return e;
     args.fill = 0;
   }
   if (l.rows_grid > 0) {
     args.rows_above = 0;
     args.rows_upto = l.tiles_grid > 0 ? FX_KV_FEW : int64_t{1} << 31;
     if ((e = offsets(args, FX_KV_ROWS, fxkv::kRowLeast, stream)) != hipSuccess) return e;
-    if ((e = launch(k.rows, l.rows_grid, stream, args)) != hipSuccess) return e;
+    if ((e = launch(k.rows, l.rows_grid, 256, stream, args)) != hipSuccess) return e;
     if (l.shared && (e = join(args, l.type, FX_KV_ROWS, stream)) != hipSuccess) return e;
   }
   return e;

@@ -187,7 +187,7 @@ def split(tmp_path_factory):
     return ctypes.CDLL(so)
 
 
-@pytest.mark.parametrize("rows,least", [(16, 4), (128, 4), (64, 2)])
+@pytest.mark.parametrize("rows,least", [(16, 4), (128, 4), (64, 2), (256, 8)])
 def test_every_step_is_taken_once_and_the_parts_fit_the_workspace(split, rows, least):
     rng = random.Random(rows)
     for case in range(400):
