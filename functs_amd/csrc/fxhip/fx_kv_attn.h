@@ -10,7 +10,9 @@
 // weights) a lane.  The depth of the first product is contracted in the order in which lanes load 16 bytes each.
 // Codes become bf16 (or f16) exactly; fp32 queries and the weights are sums of two or three such numbers:
 //   queries  bf16, f16: as they are;  fp32: three bf16 (24 bits)
-//   weights  bf16, f16 results: two bf16 (16 bits);  fp32 results: three
+//   weights  fp32 results: three bf16;  f16: two (16 bits);  bf16: two in fx_kv_rows, which waits for memory anyway, one in
+//            fx_kv_tiles: weights of one bf16 are off by half a step each, no more than the result's own rounding is, and
+//            two took 721 us where one took 587 (prompts, before later steps).  Sums of the weights are fp32, of weights as they were
 #pragma once
 #include <type_traits>
 
@@ -532,8 +534,12 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void fx_kv_rows(const FxKvA
 // 16 h + 4 g + j, so a lane holds the 16 tokens of one group.
 // Two groups of four waves, one of each on every SIMD, half a step apart: while one is at its products (those of the
 // step before with the values, then the next scores) the other one makes its weights and its share of the operands, and a barrier
-// changes them over.  Without it both were at the same thing most of the time: MEASURE.  Where a wave's registers are more than half
-// of a SIMD's (fp32 queries, depths above 128) there is one group, which does one after the other.
+// changes them over.  Products go first (their waves' priority): what they wait for is longer.  Where a wave's registers are more than
+// half of a SIMD's (fp32 queries, depths above 128) there is one group, which does one after the other.
+// Measured at 4 requests of 511 to 2 047 rows behind up to 6 001 cached tokens, 32 query heads on 8, depth 128, e4m3, bf16 (0.30
+// TFLOP): 391 us, 770 TFLOP/s, of 1 430 that a large library product reaches here.  Without the second group 438 us, without the
+// priority 397, with a page a lane and group of 16 tokens (below) in place of one a step 421.  A step takes about 2 300 clocks for either
+// half of its work: 1 024 of the matrix cores and their operands' way from LDS (64 reads of 16 bytes a lane), or 1 750 of the vector units.
 // In LDS a key's row of 16-byte pieces is permuted by its token (key_piece), which spreads the 32 rows of an operand over the banks; values
 // lie as [group][8 tokens of it][depth][8 tokens].
 typedef float fx_f32x16 __attribute__((ext_vector_type(16)));
@@ -570,7 +576,9 @@ __device__ __forceinline__ void piped(Read read, Use use, Meanwhile meanwhile) {
 constexpr int tile_waves(int type, int dp) { return dp <= 128 && type != kF32 ? 8 : 4; }
 constexpr int tile_rows(int type, int dp) { return 32 * tile_waves(type, dp); }
 
-template <int HELD, int TQ, int DP, bool EXACT>
+// WIDE: pages of 64 tokens and more, so that a step lies in one page and all about its page is the same in all lanes; smaller pages
+// need a page for each group of 16 tokens, and took 421 us instead of 397 in the call above
+template <int HELD, int TQ, int DP, bool EXACT, bool WIDE>
 __global__ __launch_bounds__(64 * tile_waves(TQ, DP), tile_waves(TQ, DP) / 4) void fx_kv_tiles(const FxKvAttnArgs a) {
   typedef typename TypeOf<TQ>::type T;
   constexpr int W = tile_waves(TQ, DP), kGroups = W / 4, kRows = 32 * W;
@@ -624,7 +632,9 @@ __global__ __launch_bounds__(64 * tile_waves(TQ, DP), tile_waves(TQ, DP) / 4) vo
     const int32_t* table = a.table + (int64_t)x.request * a.table_stride;
     const uint32_t head_at = (uint32_t)x.head * (uint32_t)(pm + 1) * (uint32_t)D;
     // A lane's two groups of a step are `half` and 2 + half.  Their entries are taken as they are, and looked at when they are used, a step later
-    auto entry_of = [&](int s, int which) { return table[min(((from + s) * FX_KV_STEP + which * 32 + half * 16) >> lp, a.columns - 1)]; };
+    constexpr int kP = WIDE ? 1 : 2;   // pages of a lane and step
+    auto entry_of = [&](int s, int which) { return table[min(((from + s) * FX_KV_STEP + (WIDE ? 0 : which * 32 + half * 16)) >> lp, a.columns - 1)]; };
+    auto page_of = [&](int entry) { return fx_kv_page(WIDE ? __builtin_amdgcn_readfirstlane(entry) : entry, a.c.pages); };
     // A wave's share: blocks of 1 KB, first of the keys, then of the values; block b is 64 bytes of depth for the 16 tokens of a group
     constexpr int kHalf = DP / 16, kPieces = DP / 16, kRowsOf = 1024 / DP, kParts = DP / 64;
     uint4 raw[kShare];
@@ -647,13 +657,19 @@ __global__ __launch_bounds__(64 * tile_waves(TQ, DP), tile_waves(TQ, DP) / 4) vo
     }
     // Round r: the keys of step r + 1 and the values of step r, on their way in registers and then to LDS.  (Steps behind the last one
     // are the table's last entries again, and are not used.)
-    auto load_round = [&](int r, const int (&key_pages)[2], const int (&value_pages)[2]) {
+    auto load_round = [&](int r, const int (&key_pages)[kP], const int (&value_pages)[kP]) {
 #pragma unroll
       for (int k = 0; k < kShare; ++k) {
-        const int group = block_of(k) / kParts, lane_of = (group & 1) * 32;
+        const int group = block_of(k) / kParts;
         const bool keys = is_keys(k);
-        const int first = __builtin_amdgcn_readlane(keys ? key_pages[0] : value_pages[0], lane_of), second = __builtin_amdgcn_readlane(keys ? key_pages[1] : value_pages[1], lane_of);
-        const uint32_t page = (uint32_t)max(group < 2 ? first : second, 0);
+        uint32_t page;
+        if constexpr (WIDE) {
+          page = (uint32_t)max(keys ? key_pages[0] : value_pages[0], 0);
+        } else {
+          const int lane_of = (group & 1) * 32, first = __builtin_amdgcn_readlane(keys ? key_pages[0] : value_pages[0], lane_of),
+                    second = __builtin_amdgcn_readlane(keys ? key_pages[1] : value_pages[1], lane_of);
+          page = (uint32_t)max(group < 2 ? first : second, 0);
+        }
         const uint32_t at = (uint32_t)(((from + r + (keys ? 1 : 0)) * FX_KV_STEP + group * 16) & pm);
         const uint8_t* base = (keys ? a.c.k : a.c.v) + ((uint64_t)page * (keys ? a.c.k_stride : a.c.v_stride) + (head_at + at * (uint32_t)D));
         raw[k] = *(const uint4*)(base + key_at[k]);
@@ -681,12 +697,14 @@ __global__ __launch_bounds__(64 * tile_waves(TQ, DP), tile_waves(TQ, DP) / 4) vo
         }
       }
     };
-    int pg[2] = {-1, -1};           // pages of the lane's two groups of a step (-1: none), and their scales
-    float ks[2] = {1.0f, 1.0f}, vs[2] = {1.0f, 1.0f};
-    const float *k_scales = a.c.k_scale + x.head, *v_scales = a.c.v_scale + x.head;
-    auto scales_of = [&](const int (&pages)[2]) {
+    int pg[kP];           // pages of the lane's groups of a step (-1: none), and their scales
+    float ks[kP], vs[kP];
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
+    for (int t = 0; t < kP; ++t) pg[t] = -1, ks[t] = vs[t] = 1.0f;
+    const float *k_scales = a.c.k_scale + x.head, *v_scales = a.c.v_scale + x.head;
+    auto scales_of = [&](const int (&pages)[kP]) {
+#pragma unroll
+      for (int t = 0; t < kP; ++t) {
         pg[t] = pages[t];
         const uint32_t page = (uint32_t)max(pages[t], 0);
         ks[t] = *(const float*)((const char*)k_scales + (uint64_t)page * (a.c.ks_stride * 4));
@@ -694,12 +712,14 @@ __global__ __launch_bounds__(64 * tile_waves(TQ, DP), tile_waves(TQ, DP) / 4) vo
       }
     };
     // pages of steps s and s + 1, and entries of step s + 2, of the products of step s
-    int pages0[2] = {-1, -1}, pages1[2] = {-1, -1}, entries2[2] = {-1, -1};
+    int pages0[kP], pages1[kP], entries2[kP];
+#pragma unroll
+    for (int t = 0; t < kP; ++t) pages0[t] = pages1[t] = entries2[t] = -1;
     if (n > 0) {
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        pages0[t] = fx_kv_page(entry_of(0, t), a.c.pages);
-        pages1[t] = fx_kv_page(entry_of(1, t), a.c.pages);
+      for (int t = 0; t < kP; ++t) {
+        pages0[t] = page_of(entry_of(0, t));
+        pages1[t] = page_of(entry_of(1, t));
         entries2[t] = entry_of(2, t);
       }
       load_round(-1, pages0, pages0);
@@ -722,12 +742,14 @@ __global__ __launch_bounds__(64 * tile_waves(TQ, DP), tile_waves(TQ, DP) / 4) vo
     // scales of step s are sent for: round s, which this group writes with the weights of step s, and of the late group round s + 1.
     auto products = [&](int s, auto is_late) {
       auto send = [&]() {
-        const int pages2[2] = {fx_kv_page(entries2[0], a.c.pages), fx_kv_page(entries2[1], a.c.pages)};
+        int pages2[kP];
+#pragma unroll
+        for (int t = 0; t < kP; ++t) pages2[t] = page_of(entries2[t]);
         if constexpr (is_late) load_round(s + 1, pages2, pages1);
         else load_round(s, pages1, pages0);
         scales_of(pages0);
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
+        for (int t = 0; t < kP; ++t) {
           pages0[t] = pages1[t];
           pages1[t] = pages2[t];
           entries2[t] = entry_of(s + 3, t);
@@ -763,66 +785,73 @@ __global__ __launch_bounds__(64 * tile_waves(TQ, DP), tile_waves(TQ, DP) / 4) vo
     };
     // the weights of step s, and a share of round `round`
     auto weights = [&](int s, int round) {
-        const int p0 = pg[0], p1 = pg[1];
-        float cs[2] = {fmaxf(ks[0] * a.scale, kTiny), fmaxf(ks[1] * a.scale, kTiny)}, cv[2] = {fmaxf(vs[0], kTiny), fmaxf(vs[1], kTiny)};
-        if (round < n) write_round(round);
-        __builtin_amdgcn_sched_barrier(0);   // (what is loaded later stays out of registers that are not there)
-        if (s >= 0 && sees(s)) {
-          const int base = (from + s) * FX_KV_STEP;
-          const bool inside = base >= mine.all_low && base + FX_KV_STEP <= mine.all_high && __all(p0 >= 0 && p1 >= 0);
-          if (!inside) {
-            int hi_row_ = hi_row, lo_row_ = lo_row;
-            asm volatile("" : "+v"(hi_row_), "+v"(lo_row_));   // (compared here, not ahead of the branch)
+      const int p0 = pg[0], p1 = pg[kP - 1];
+      float cs[2], cv[2];
 #pragma unroll
-            for (int t = 0; t < 2; ++t) {
-              const int t0 = base + (t * 2 + half) * 16;
-              const bool ok = (t ? p1 : p0) >= 0;
-              if (!ok || mine.high <= t0) cs[t] = cv[t] = 1.0f;   // (what lies there may be anything)
-              const int h = ok ? hi_row_ - t0 : 0, b = lo_row_ - t0;
-#pragma unroll
-              for (int e = 0; e < 16; ++e) r[t][e] = e < h && e >= b ? r[t][e] : -kInf;
-            }
-          }
-          float top[2];
+      for (int t = 0; t < 2; ++t) {
+        cs[t] = fmaxf(ks[t % kP] * a.scale, kTiny);
+        cv[t] = fmaxf(vs[t % kP], kTiny);
+      }
+      if (round < n) write_round(round);
+      __builtin_amdgcn_sched_barrier(0);   // (what is loaded later stays out of registers that are not there)
+      if (s >= 0 && sees(s)) {
+        const int base = (from + s) * FX_KV_STEP;
+        const bool inside = base >= mine.all_low && base + FX_KV_STEP <= mine.all_high && __all(p0 >= 0 && p1 >= 0);
+        if (!inside) {
+          int hi_row_ = hi_row, lo_row_ = lo_row;
+          asm volatile("" : "+v"(hi_row_), "+v"(lo_row_));   // (compared here, not ahead of the branch)
 #pragma unroll
           for (int t = 0; t < 2; ++t) {
-            top[t] = larger(r[t][0], r[t][1]);
+            const int t0 = base + (t * 2 + half) * 16;
+            const bool ok = (t ? p1 : p0) >= 0;
+            if (!ok || mine.high <= t0) cs[t] = cv[t] = 1.0f;   // (what lies there may be anything)
+            const int h = ok ? hi_row_ - t0 : 0, b = lo_row_ - t0;
 #pragma unroll
-            for (int e = 2; e < 16; ++e) top[t] = larger(top[t], r[t][e]);
-            top[t] *= cs[t];
-          }
-          float up = fmaxf(top[0], top[1]);
-          if (__any(up > m + 8.0f || (m == -kInf && up > -kInf))) {
-            up = fmaxf(up, __shfl_xor(up, 32, 64));
-            const float to_m = fmaxf(m, up);
-            const float by = to_m == -kInf ? 1.0f : __builtin_amdgcn_exp2f(m - to_m);
-            m = to_m;
-            l *= by;
-#pragma unroll
-            for (int d = 0; d < DT; ++d)
-#pragma unroll
-              for (int e = 0; e < 16; ++e) acc[d][e] *= by;
-          }
-          const float sub = m == -kInf ? 0.0f : m;
-          // weights times the values' scale, a power of two: part of the exponent, and taken out of their sum again
-#pragma unroll
-          for (int t = 0; t < 2; ++t) {
-            const float off = __builtin_amdgcn_logf(cv[t]) - sub;
-            float w[16], sum[2] = {0.0f, 0.0f};
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-              w[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(r[t][e], cs[t], off));
-              sum[e & 1] += w[e];
-            }
-            l = __builtin_fmaf(sum[0] + sum[1], __builtin_amdgcn_rcpf(cv[t]), l);
-            split8<NP>(p[t][0], w);
-            split8<NP>(p[t][1], w + 8);
+            for (int e = 0; e < 16; ++e) r[t][e] = e < h && e >= b ? r[t][e] : -kInf;
           }
         }
+        float top[2];
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          top[t] = larger(r[t][0], r[t][1]);
+#pragma unroll
+          for (int e = 2; e < 16; ++e) top[t] = larger(top[t], r[t][e]);
+          top[t] *= cs[t];
+        }
+        float up = fmaxf(top[0], top[1]);
+        if (__any(up > m + 8.0f || (m == -kInf && up > -kInf))) {
+          up = fmaxf(up, __shfl_xor(up, 32, 64));
+          const float to_m = fmaxf(m, up);
+          const float by = to_m == -kInf ? 1.0f : __builtin_amdgcn_exp2f(m - to_m);
+          m = to_m;
+          l *= by;
+#pragma unroll
+          for (int d = 0; d < DT; ++d)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[d][e] *= by;
+        }
+        const float sub = m == -kInf ? 0.0f : m;
+        // weights times the values' scale, a power of two: part of the exponent, and taken out of their sum again
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          const float off = __builtin_amdgcn_logf(cv[t]) - sub;
+          float w[16], sum[2] = {0.0f, 0.0f};
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            w[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(r[t][e], cs[t], off));
+            sum[e & 1] += w[e];
+          }
+          l = __builtin_fmaf(sum[0] + sum[1], __builtin_amdgcn_rcpf(cv[t]), l);
+          split8<NP>(p[t][0], w);
+          split8<NP>(p[t][1], w + 8);
+        }
+      }
     };
     if (!late) {
       for (int s = 0; s <= n; ++s) {
+        __builtin_amdgcn_s_setprio(1);
         products(s, std::false_type());
+        __builtin_amdgcn_s_setprio(0);
         __syncthreads();
         if (s < n) weights(s, s);
         __syncthreads();
@@ -831,7 +860,9 @@ __global__ __launch_bounds__(64 * tile_waves(TQ, DP), tile_waves(TQ, DP) / 4) vo
       for (int s = 0; s <= n; ++s) {
         weights(s - 1, s);
         __syncthreads();
+        __builtin_amdgcn_s_setprio(1);
         products(s, std::true_type());
+        __builtin_amdgcn_s_setprio(0);
         __syncthreads();
       }
     }
@@ -971,8 +1002,9 @@ struct Kernels {
   int tile_rows;   // of `tiles`; twice as many threads
 };
 template <int HELD, int TQ>
-Kernels kernels_of(int depth) {
-#define FX_KV_PAIR(DP, EXACT) Kernels{(const void*)fx_kv_rows<HELD, TQ, DP, EXACT>, (const void*)fx_kv_tiles<HELD, TQ, DP, EXACT>, tile_rows(TQ, DP)}
+Kernels kernels_of(int depth, bool wide) {
+#define FX_KV_PAIR(DP, EXACT) \
+  Kernels{(const void*)fx_kv_rows<HELD, TQ, DP, EXACT>, wide ? (const void*)fx_kv_tiles<HELD, TQ, DP, EXACT, true> : (const void*)fx_kv_tiles<HELD, TQ, DP, EXACT, false>, tile_rows(TQ, DP)}
   if (depth == 64) return FX_KV_PAIR(64, true);
   if (depth == 128) return FX_KV_PAIR(128, true);
   if (depth == 256) return FX_KV_PAIR(256, true);
@@ -981,10 +1013,10 @@ Kernels kernels_of(int depth) {
 #undef FX_KV_PAIR
 }
 template <int HELD>
-Kernels kernels_of(int type, int depth) {
-  return type == kBf16 ? kernels_of<HELD, kBf16>(depth) : type == kF16 ? kernels_of<HELD, kF16>(depth) : kernels_of<HELD, kF32>(depth);
+Kernels kernels_of(int type, int depth, bool wide) {
+  return type == kBf16 ? kernels_of<HELD, kBf16>(depth, wide) : type == kF16 ? kernels_of<HELD, kF16>(depth, wide) : kernels_of<HELD, kF32>(depth, wide);
 }
 }  // namespace fxkv
 
-fxkv::Kernels fx_kv_kernels_e4m3(int type, int depth);
-fxkv::Kernels fx_kv_kernels_int8(int type, int depth);
+fxkv::Kernels fx_kv_kernels_e4m3(int type, int depth, bool wide);
+fxkv::Kernels fx_kv_kernels_int8(int type, int depth, bool wide);

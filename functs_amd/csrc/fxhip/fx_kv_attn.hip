@@ -84,7 +84,8 @@ hipError_t join(const FxKvAttnArgs& a, int type, int tile_rows, hipStream_t stre
 }  // namespace
 
 hipError_t fx_launch_kv_attention(const FxKvAttnArgs& a, const FxKvLaunch& l, hipStream_t stream) {
-  const fxkv::Kernels k = l.held == 0 ? fx_kv_kernels_e4m3(l.type, a.c.depth) : fx_kv_kernels_int8(l.type, a.c.depth);
+  const bool wide = (1 << a.c.log_page) >= FX_KV_STEP;
+  const fxkv::Kernels k = l.held == 0 ? fx_kv_kernels_e4m3(l.type, a.c.depth, wide) : fx_kv_kernels_int8(l.type, a.c.depth, wide);
   hipError_t e = hipSuccess;
   FxKvAttnArgs args = a;
   if (l.tiles_grid > 0) {
