@@ -5,6 +5,8 @@
 // amax <= top * 2^e (top: 448 for e4m3, 127 for int8), -100 <= e <= 119 (e4m3) or 121 (int8), which keeps
 // top * 2^e finite.  Powers of two cost e4m3 no precision, make dividing and multiplying exact (so codes are
 // exactly defined), and a page whose scale grows keeps its e4m3 codes but for underflow.
+#include <algorithm>
+
 #include "fx_kv.h"
 #include "fx_kv_device.h"
 
@@ -157,11 +159,12 @@ __global__ __launch_bounds__(kThreads) void fx_kv_plan_kernel(const FxKvPlanArgs
 
 // ---- fx_kv_store ----
 // Bound: HBM (2 or 4 bytes read and 1 written for each number); single tokens: latency.
-// A run is the neighbours in `slots` that lie in one page; a wave takes the keys or the values of one head of a
-// run, so a page's scale and codes have one writer and nothing is locked.  The run's numbers are read, their largest magnitude
-// gives the scale, then they become codes; of more than a few tokens they are read a second time, from the caches (keeping all of a
-// page in registers left two waves a SIMD and a quarter of the bandwidth).  Keys: 8 numbers of a token a lane.  Values: 2
-// columns of a group of 16 tokens a lane, which are 32 neighbouring bytes of the cache.
+// A run is the neighbours in `slots` that lie in one page; a workgroup takes the keys or the values of one head of the runs that
+// begin in its chunk of tokens, so a page's scale and codes have one writer and nothing is locked.  The run's numbers are read, their
+// largest magnitude gives the scale, then they become codes.  Of a run of more than 16 tokens each of the four waves takes a
+// quarter, which stays in registers between the two (beyond those it is read a second time, from the caches), and the
+// magnitudes meet in LDS; shorter ones, and those in no order, are the waves' in turn.  Keys: 8 numbers of a token a lane.  Values: 2 columns
+// of a group of 16 tokens a lane, which are 32 neighbouring bytes of the cache.
 // Magnitudes are compared as the integers that their bits are.  Where the largest one is finite and below the largest scale, no number
 // needs to be held to the range of the codes or looked at for NaN (PLAIN).
 constexpr int kStoreWaves = kThreads / 64;
@@ -274,7 +277,7 @@ __device__ __forceinline__ uint4 again16(uint4 w, float ratio, int n) {
 __device__ __forceinline__ int64_t lane_of(int64_t v, int lane) {   // in scalar registers
   return ((int64_t)__builtin_amdgcn_readlane((int)(v >> 32), lane) << 32) | (unsigned)__builtin_amdgcn_readlane((int)v, lane);
 }
-// One run: rows [0, n) of `rows` go to offsets o0 on of a page (straight), or to those that `slots` says
+// One run, or a wave's share of it: rows [0, n) of `rows` go to offsets o0 on of a page (straight), or to those that `slots` says
 template <int HELD, class T, bool VALUES>
 struct StoreRun {
   typedef typename Pack<T>::eight P8;
@@ -367,14 +370,14 @@ struct StoreRun {
   }
   static constexpr int kKept = VALUES ? 1 : 4;   // iterations whose numbers stay in registers: more of them cost waves
   template <bool PLAIN>
-  __device__ __forceinline__ void write(const P8 (&kept8)[VALUES ? 1 : kKept], const P2 (&kept2)[16], bool keep, float inv, float ratio) const {
+  __device__ __forceinline__ void write(const P8 (&kept8)[VALUES ? 1 : kKept], const P2 (&kept2)[VALUES ? kKept : 1][16], bool keep, float inv, float ratio) const {
     if (keep) {
-      if constexpr (VALUES) {
-        write_column<PLAIN>(0, kept2, inv, ratio);
-      } else {
 #pragma unroll
-        for (int k = 0; k < kKept; ++k)
-          if (k < iterations) write_eight<PLAIN>(k, kept8[k], inv);
+      for (int k = 0; k < kKept; ++k) {
+        if (k < iterations) {
+          if constexpr (VALUES) write_column<PLAIN>(k, kept2[k], inv, ratio);
+          else write_eight<PLAIN>(k, kept8[k], inv);
+        }
       }
       return;
     }
@@ -390,27 +393,42 @@ struct StoreRun {
     }
   }
 
-  __device__ __forceinline__ void run(bool straight, const int64_t* slots, int page_mask, float* scale_at) {
+  // tops: of a run that the workgroup shares, where its waves' largest magnitudes meet (nullptr: the run is this wave's)
+  __device__ __forceinline__ void run(bool straight, const int64_t* slots, int page_mask, float* scale_at, unsigned* tops) {
     lane = (int)threadIdx.x & 63;
+    const int wave = tops ? __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6) : 0, first = o0;   // (of the run)
+    const float old = first > 0 ? *scale_at : 0.0f;
+    if (tops) {   // a quarter of the groups of 16 tokens
+      const int before = o0 >> 4, groups = ((o0 + n + 15) >> 4) - before, per = (groups + kStoreWaves - 1) / kStoreWaves;
+      const int from = max((before + wave * per) * 16 - o0, 0), to = min((before + (wave + 1) * per) * 16 - o0, n);
+      n = max(to - from, 0);
+      o0 += from;
+      rows += (int64_t)from * stride;
+    }
     shape();
-    const float old = o0 > 0 ? *scale_at : 0.0f;
     P8 kept8[VALUES ? 1 : kKept];
-    P2 kept2[16];
+    P2 kept2[VALUES ? kKept : 1][16];
     const bool keep = iterations <= kKept, used = sub < abreast;
     unsigned m = 0;
     if (straight && used) {
       if (keep) {
-        if constexpr (VALUES) {
-          load_column(kept2, 0);
 #pragma unroll
-          for (int e = 0; e < 16; ++e) m = Pack<T>::see(m, kept2[e]);
-        } else {
+        for (int k = 0; k < kKept; ++k) {
+          if (k < iterations) {
+            if constexpr (VALUES) load_column(kept2[k], k);
+            else kept8[k] = load_eight(k);
+          }
+        }
 #pragma unroll
-          for (int k = 0; k < kKept; ++k)
-            if (k < iterations) kept8[k] = load_eight(k);
+        for (int k = 0; k < kKept; ++k) {
+          if (k < iterations) {
+            if constexpr (VALUES) {
 #pragma unroll
-          for (int k = 0; k < kKept; ++k)
-            if (k < iterations) m = Pack<T>::see(m, kept8[k]);
+              for (int e = 0; e < 16; ++e) m = Pack<T>::see(m, kept2[k][e]);
+            } else {
+              m = Pack<T>::see(m, kept8[k]);
+            }
+          }
         }
       } else {
 #pragma unroll 2
@@ -426,7 +444,15 @@ struct StoreRun {
         }
       }
     }
-    float top = Pack<T>::value(wave_largest<sizeof(T) == 2>(m));
+    m = wave_largest<sizeof(T) == 2>(m);
+    if (tops) {
+      if (lane == 0) tops[wave] = m;
+      __syncthreads();   // (and the scale has been read)
+      m = 0;
+#pragma unroll
+      for (int w = 0; w < kStoreWaves; ++w) m = Pack<T>::larger(m, tops[w]);
+    }
+    float top = Pack<T>::value(m);
     constexpr float kMost = HELD == 0 ? 448.0f * 0x1p119f : 127.0f * 0x1p121f;
     const bool plain = straight && top <= kMost;
     if (!plain) {   // infinities or NaN (or slots in any order): the largest finite one
@@ -434,15 +460,22 @@ struct StoreRun {
       for (int j = 0; j < n; ++j)
         for (int d = lane; d < D; d += 64) t = fmaxf(t, finite_abs((float)rows[(int64_t)j * stride + d]));
       top = wave_max64(t);
+      if (tops) {
+        __syncthreads();
+        if (lane == 0) tops[wave] = __float_as_uint(top);
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < kStoreWaves; ++w) top = fmaxf(top, __uint_as_float(tops[w]));
+      }
     }
     float scale = scale_of<HELD>(top);
     float ratio = 1.0f;   // of the page's scale before to the one from now on
-    if (o0 > 0) {
+    if (first > 0) {
       if (old > scale && old <= 3.402823466e38f) scale = old;
       else if (old > 0.0f && old < scale) ratio = old / scale;
     }
-    if (lane == 0) *scale_at = scale;
-    if (ratio != 1.0f) {
+    if (lane == 0 && wave == 0) *scale_at = scale;
+    if (ratio != 1.0f && wave == 0) {
       // what the page holds below o0; the group in which o0 lies, if it is written below, is done there
       const int words = VALUES ? (straight ? g0 : (o0 + 15) >> 4) * D : (o0 * D) >> 4;
       for (int i = lane; i < words; i += 64) {
@@ -472,26 +505,26 @@ struct StoreRun {
 };
 
 template <int HELD, class T>
-__global__ __launch_bounds__(kThreads, 4) void fx_kv_store_kernel(const FxKvCache c, const FxKvRows r, int per_wave, int n_chunks, int vec) {
-  const int lane = (int)threadIdx.x & 63;
-  const int64_t w = (int64_t)blockIdx.x * kStoreWaves + __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-  const unsigned chunk_head = (unsigned)(w >> 1);   // (below 2^32: checked on the host)
-  const int half = (int)(w & 1), chunk = (int)(chunk_head / (unsigned)c.heads), head = (int)(chunk_head - (unsigned)chunk * (unsigned)c.heads);
-  if (chunk >= n_chunks) return;
+__global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 5 : 4) void fx_kv_store_kernel(const FxKvCache c, const FxKvRows r, int per, int vec) {
+  __shared__ unsigned s_tops[2][kStoreWaves];
+  const int lane = (int)threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const unsigned chunk_head = blockIdx.x >> 1;
+  const int half = (int)(blockIdx.x & 1), chunk = (int)(chunk_head / (unsigned)c.heads), head = (int)(chunk_head - (unsigned)chunk * (unsigned)c.heads);
   const int D = c.depth, page = 1 << c.log_page;
   const int64_t n_slots = (int64_t)c.pages << c.log_page;
-  const int t0 = chunk * per_wave, t1 = min(r.tokens, t0 + per_wave);
-  // lane i: the slot of token t0 - 1 + i, which a run that begins in the chunk needs (the first 64 - per_wave of it, at least)
+  const int t0 = chunk * per, t1 = min(r.tokens, t0 + per);
+  // lane i: the slot of token t0 - 1 + i, which a run that begins in the chunk needs (the first 64 - per of it, at least)
   auto slot_of = [&](int t) -> int64_t {
     const int64_t s = t >= 0 && t < r.tokens ? r.slots[min(max(t, 0), r.tokens - 1)] : -1;
     return s >= 0 && s < n_slots ? s : -1;
   };
   const int64_t mine = slot_of(t0 - 1 + lane);
-  for (int t = t0; t < t1; ++t) {
-    const int at = t - t0 + 1;
-    const int64_t s0 = lane_of(mine, at), s1 = lane_of(mine, at - 1);
-    const int64_t p = s0 >> c.log_page;   // -1: nowhere
-    if (s0 < 0 || (s1 >= 0 && s1 >> c.log_page == p)) continue;
+  int alone = 0, shared = 0;   // runs of one wave, and of all of them, so far
+  const int64_t prior = (int64_t)__shfl_up((unsigned long long)mine, 1u, 64);
+  unsigned long long begins = __ballot(lane > 0 && lane <= t1 - t0 && mine >= 0 && !(prior >= 0 && prior >> c.log_page == mine >> c.log_page));
+  for (; begins != 0; begins &= begins - 1) {
+    const int at = __builtin_ctzll(begins), t = t0 + at - 1;
+    const int64_t s0 = lane_of(mine, at), p = s0 >> c.log_page;
     // the run's length, and whether its slots rise by one
     int n = 0;
     bool straight = true;
@@ -508,6 +541,9 @@ __global__ __launch_bounds__(kThreads, 4) void fx_kv_store_kernel(const FxKvCach
       first = 0;
       seen = slot_of(t + n + lane);
     }
+    const bool together = straight && n > 16;   // (what decides is the same in all waves)
+    if (!together && alone++ % kStoreWaves != wave) continue;
+    unsigned* tops = together ? s_tops[shared++ & 1] : nullptr;
     const int o0 = (int)(s0 & (page - 1));
     const int64_t in_page = (int64_t)head * page * D;
     if (half == 0) {
@@ -516,14 +552,14 @@ __global__ __launch_bounds__(kThreads, 4) void fx_kv_store_kernel(const FxKvCach
       run.stride = r.k_token;
       run.n = n, run.o0 = o0, run.D = D, run.vec = vec != 0;
       run.codes = c.k + p * c.k_stride + in_page;
-      run.run(straight, r.slots + t, page - 1, c.k_scale + p * c.ks_stride + head);
+      run.run(straight, r.slots + t, page - 1, c.k_scale + p * c.ks_stride + head, tops);
     } else {
       StoreRun<HELD, T, true> run;
       run.rows = (const T*)r.v + (int64_t)t * r.v_token + (int64_t)head * r.v_head;
       run.stride = r.v_token;
       run.n = n, run.o0 = o0, run.D = D, run.vec = vec != 0;
       run.codes = c.v + p * c.v_stride + in_page;
-      run.run(straight, r.slots + t, page - 1, c.v_scale + p * c.vs_stride + head);
+      run.run(straight, r.slots + t, page - 1, c.v_scale + p * c.vs_stride + head, tops);
     }
   }
 }
@@ -634,14 +670,14 @@ hipError_t fx_launch_kv_store(const FxKvCache& c, const FxKvRows& r, int held, h
       {(const void*)fx_kv_store_kernel<0, float>, (const void*)fx_kv_store_kernel<0, _Float16>, (const void*)fx_kv_store_kernel<0, __bf16>},
       {(const void*)fx_kv_store_kernel<1, float>, (const void*)fx_kv_store_kernel<1, _Float16>, (const void*)fx_kv_store_kernel<1, __bf16>}};
   const size_t size = r.dtype == FX_DT_F32 ? 4 : 2;
-  int per = tokens_a_wave(c, r, 32), chunks = (r.tokens + per - 1) / per;
+  // (63: a lane each, and one for the token before them)
+  int per = std::max(std::min(tokens_a_wave(c, r, 63) * kStoreWaves, 63), kStoreWaves);
   int vec = aligned16(r.k, r.k_token, r.k_head, size) && aligned16(r.v, r.v_token, r.v_head, size);
   FxKvCache cache = c;
   FxKvRows rows = r;
-  void* kargs[5] = {(void*)&cache, (void*)&rows, (void*)&per, (void*)&chunks, (void*)&vec};
-  const int64_t waves = (int64_t)chunks * c.heads * 2;
-  return hipLaunchKernel(kernels[held][r.dtype == FX_DT_F32 ? 0 : r.dtype == FX_DT_F16 ? 1 : 2],
-                         dim3((unsigned)((waves + kStoreWaves - 1) / kStoreWaves)), dim3(kThreads), kargs, 0, stream);
+  void* kargs[4] = {(void*)&cache, (void*)&rows, (void*)&per, (void*)&vec};
+  const int64_t grid = (int64_t)((r.tokens + per - 1) / per) * c.heads * 2;
+  return hipLaunchKernel(kernels[held][r.dtype == FX_DT_F32 ? 0 : r.dtype == FX_DT_F16 ? 1 : 2], dim3((unsigned)grid), dim3(kThreads), kargs, 0, stream);
 }
 
 hipError_t fx_launch_kv_read(const FxKvCache& c, const FxKvRows& r, int held, hipStream_t stream) {
@@ -649,7 +685,7 @@ hipError_t fx_launch_kv_read(const FxKvCache& c, const FxKvRows& r, int held, hi
       {(const void*)fx_kv_read_kernel<0, float>, (const void*)fx_kv_read_kernel<0, _Float16>, (const void*)fx_kv_read_kernel<0, __bf16>},
       {(const void*)fx_kv_read_kernel<1, float>, (const void*)fx_kv_read_kernel<1, _Float16>, (const void*)fx_kv_read_kernel<1, __bf16>}};
   const size_t size = r.dtype == FX_DT_F32 ? 4 : 2;
-  int per = tokens_a_wave(c, r, 16), chunks = (r.tokens + per - 1) / per;
+  int per = std::max(tokens_a_wave(c, r, 16), 4), chunks = (r.tokens + per - 1) / per;
   int vec = aligned16(r.k, r.k_token, r.k_head, size) && aligned16(r.v, r.v_token, r.v_head, size);
   FxKvCache cache = c;
   FxKvRows rows = r;
