@@ -1701,11 +1701,34 @@ FxKvLaunch kv_launch(const FxKvCache& c, const fx_kv_attention_desc& d) {
     const int64_t items = c.heads * std::min(all / tile + some, some * ((longest + tile - 1) / tile));
     return std::min<int64_t>(std::max<int64_t>(items + (l.shared ? FX_KV_TARGET : 0), 1), 1 << 20);
   };
-  if (many) l.tiles_grid = grid(FX_KV_TILE, longest);
+  const int tile_rows = fx_kv_tile_rows(d.dtype == FX_DT_F32, c.depth);
+  if (many) l.tiles_grid = grid(tile_rows, longest);
   if (few) l.rows_grid = grid(FX_KV_ROWS, many ? FX_KV_FEW : longest);
+  l.tiles_parts.tile_rows = tile_rows;
+  l.rows_parts.tile_rows = FX_KV_ROWS;
   return l;
 }
 size_t kv_round(size_t n) { return (n + 255) / 256 * 256; }
+// Lays the workspace out from `base` on (nullptr: only its size counts)
+size_t kv_workspace(FxKvAttnArgs& a, FxKvLaunch& l, int depth, int requests, char* base) {
+  size_t at = 0;
+  auto take = [&](size_t bytes) {
+    char* p = base ? base + at : nullptr;
+    at += kv_round(bytes);
+    return p;
+  };
+  a.offsets = (int32_t*)take(((size_t)requests * 2 + 3) * sizeof(int32_t));   // (of one kernel after the other)
+  auto parts_of = [&](FxKvParts& p) {
+    const size_t rows = (size_t)2 * FX_KV_TARGET * p.tile_rows;
+    p.n_items = (int32_t*)take(sizeof(int32_t));
+    p.items = (FxKvItem*)take(FX_KV_TARGET * sizeof(FxKvItem));
+    p.ml = (float*)take(rows * 2 * sizeof(float));
+    p.acc = (float*)take(rows * (size_t)depth * sizeof(float));
+  };
+  if (l.tiles_grid > 0) parts_of(l.tiles_parts);
+  if (l.rows_grid > 0) parts_of(l.rows_parts);
+  return at;
+}
 }  // namespace
 
 int fx_kv_plan(const fx_kv_plan_desc* desc, void* stream) {
@@ -1748,10 +1771,9 @@ int fx_kv_read(const fx_kv_cache* cache, const fx_kv_rows* rows, void* stream) {
 size_t fx_kv_attention_workspace_bytes(const fx_kv_cache* cache, const fx_kv_attention_desc* desc) {
   FxKvCache c;
   if (!desc || kv_cache_of("fx_kv_attention", cache, c) != FX_OK) return 0;
-  // (one after the other, the kernels of a call use the same memory)
-  const size_t parts = (size_t)2 * FX_KV_TARGET * (kv_launch(c, *desc).tiles_grid > 0 ? FX_KV_TILE_MOST : FX_KV_ROWS);
-  const size_t offsets = kv_round(((size_t)std::max(desc->requests, 0) * 2 + 3) * sizeof(int32_t));   // (fx_kv_offsets)
-  return 256 + offsets + kv_round(FX_KV_TARGET * sizeof(FxKvItem)) + kv_round(parts * 2 * sizeof(float)) + kv_round(parts * (size_t)c.depth * sizeof(float));
+  FxKvAttnArgs a;
+  FxKvLaunch l = kv_launch(c, *desc);
+  return kv_workspace(a, l, c.depth, std::max(desc->requests, 0), nullptr);
 }
 
 int fx_kv_attention(const fx_kv_cache* cache, const fx_kv_attention_desc* desc, void* stream) {
@@ -1799,14 +1821,9 @@ int fx_kv_attention(const fx_kv_cache* cache, const fx_kv_attention_desc* desc, 
   a.fill = d.clear_rest;
   const int64_t q_size = d.dtype == FX_DT_F32 ? 4 : 2;
   a.q_vec = ((uintptr_t)d.q & 15u) == 0 && d.q_token_stride * q_size % 16 == 0 && d.q_head_stride * q_size % 16 == 0;
-  char* w = (char*)d.workspace;
-  a.n_items = (int32_t*)w;
-  a.offsets = (int32_t*)(w += 256);
-  a.items = (FxKvItem*)(w += kv_round(((size_t)d.requests * 2 + 3) * sizeof(int32_t)));
-  a.part_ml = (float*)(w += kv_round(FX_KV_TARGET * sizeof(FxKvItem)));
-  a.part_acc = (float*)(w += kv_round((size_t)2 * FX_KV_TARGET * (l.tiles_grid > 0 ? FX_KV_TILE_MOST : FX_KV_ROWS) * 2 * sizeof(float)));
+  kv_workspace(a, l, c.depth, d.requests, (char*)d.workspace);
   HIP_OK(fx_launch_kv_attention(a, l, (hipStream_t)stream));
-  return kv_launched(((l.rows_grid > 0) + (l.tiles_grid > 0)) * (l.shared ? 2 : 1));   // (fx_kv_offsets aside)
+  return kv_launched((l.rows_grid > 0) + (l.tiles_grid > 0) + (l.shared ? 1 : 0));   // (fx_kv_offsets aside)
 }
 
 // ---- detection tail (fx_nms.hip) ----

@@ -38,11 +38,21 @@ hipError_t fx_launch_kv_store(const FxKvCache& c, const FxKvRows& r, int held, h
 hipError_t fx_launch_kv_read(const FxKvCache& c, const FxKvRows& r, int held, hipStream_t stream);
 
 #define FX_KV_ROWS 16   // rows (tokens of a request times query heads of a key head) of a tile of fx_kv_rows
-#define FX_KV_TILE 128  // rows of a tile of fx_kv_tiles, at least
-#define FX_KV_TILE_MOST 256
-#define FX_KV_FEW 48    // requests of more rows are fx_kv_tiles' where a call may have both
+// rows of a tile of fx_kv_tiles: 32 for each of 8 waves; of 4 where a wave needs more than half of a SIMD's registers
+FX_KV_HD int fx_kv_tile_rows(bool f32, int depth) { return depth <= 128 && !f32 ? 256 : 128; }
+// Requests of more rows are fx_kv_tiles', the others fx_kv_rows'.  Measured, fx_kv_rows against fx_kv_tiles (us, bf16, e4m3): 16 requests of
+// 2 000 cached tokens, 8 heads of 128: 128 rows 53 / 85, 256 rows 99 / 118; 64 of 500: 96 rows 75 / 83, 128 rows 97 / 86, 256 rows 183 /
+// 121; one of 8 000: 128 rows 23 / 31, 256 rows 35 / 38; depth 80, 4 heads, 16 of 1 000: 125 rows 20 / 54.
+#define FX_KV_FEW 128
 struct FxKvItem {   // rows whose cached tokens several workgroups shared
   int32_t request, head, tile, first, parts;
+};
+struct FxKvParts {
+  float* acc;        // [parts][tile_rows][depth]
+  float* ml;         // [parts][tile_rows][2]: maximum, sum
+  FxKvItem* items;
+  int32_t* n_items;
+  int32_t tile_rows;
 };
 struct FxKvAttnArgs {
   FxKvCache c;
@@ -53,10 +63,7 @@ struct FxKvAttnArgs {
   int64_t q_token, q_head, out_token, table_stride;   // elements (out and lse: contiguous rows of all heads)
   int32_t tokens, requests, columns, q_heads, group, window;
   float scale;                                        // times log2(e)
-  float* part_acc;                                    // [parts][rows of a tile][depth]
-  float* part_ml;                                     // [parts][rows of a tile][2]
-  FxKvItem* items;
-  int32_t* n_items;
+  FxKvParts parts;
   int32_t* offsets;                                   // of more than 256 requests: see fx_kv_offsets
   int32_t fill;                                       // rows of no request are cleared
   int32_t q_vec;                                      // rows of queries are 16-byte aligned
@@ -66,5 +73,6 @@ struct FxKvLaunch {
   int held, type;                   // FX_KV_E4M3, FX_KV_INT8; 0 bf16, 1 fp16, 2 fp32
   bool shared;                      // items may be shared by workgroups
   int64_t rows_grid, tiles_grid;    // workgroups of fx_kv_rows and fx_kv_tiles (0: not needed)
+  FxKvParts rows_parts, tiles_parts;
 };
 hipError_t fx_launch_kv_attention(const FxKvAttnArgs& a, const FxKvLaunch& l, hipStream_t stream);

@@ -124,7 +124,9 @@ __device__ __forceinline__ int64_t all_steps(const FxKvAttnArgs& a, int64_t step
 // to kScanned requests are added up here, a lane one of 64 a round; of more, fx_kv_offsets has left the sums.
 // SORTED: of up to 64 requests those of more steps come first, so that what is left at the end of a call is short.
 constexpr int kScanned = 256;
-constexpr int kRowLeast = 4, kTileLeast = 8;   // chunks are multiples of so many steps (fx_kv_rows: of one for each wave)
+// Chunks are multiples of so many steps: fx_kv_rows, of one for each wave; fx_kv_tiles, so that what a part costs by itself (some 8 us) stays
+// small: 4 requests of 256 rows on 3 000 cached tokens, 12 heads of 64, took 67 us with 4, 68 with 8 and 86 with 2; one of 8 000 37, 39 and 37
+constexpr int kRowLeast = 4, kTileLeast = 4;
 template <bool SORTED>
 __device__ __forceinline__ bool unit_at(const FxKvAttnArgs& a, int tile_rows, int least, int u, Unit& x, int* shared_items) {
   const int lane = (int)threadIdx.x & 63;
@@ -284,7 +286,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void fx_kv_rows(const FxKvA
     Unit x;
     int shared_items = 0;
     const bool live = unit_at<false>(a, FX_KV_ROWS, kRowLeast, u, x, &shared_items);
-    if (u == 0 && threadIdx.x == 0) *a.n_items = shared_items;
+    if (u == 0 && threadIdx.x == 0) *a.parts.n_items = shared_items;
     if (!live) break;
     if (u != (int)blockIdx.x) __syncthreads();   // (LDS is free again)
     // rows
@@ -508,21 +510,21 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void fx_kv_rows(const FxKvA
           for (int e = 0; e < 4; ++e) o[e] *= per;
           store4((T*)a.out + t * a.out_token + (int64_t)h * D + d, o);
         } else {
-          *(float4*)(a.part_acc + ((int64_t)(x.part + x.split) * FX_KV_ROWS + c) * D + d) = make_float4(o[0], o[1], o[2], o[3]);
+          *(float4*)(a.parts.acc + ((int64_t)(x.part + x.split) * FX_KV_ROWS + c) * D + d) = make_float4(o[0], o[1], o[2], o[3]);
         }
       }
       if (part == 0) {
         if (x.splits == 1) {
           a.lse[t * a.q_heads + h] = sum == 0.0f ? -kInf : (top + __builtin_amdgcn_logf(sum)) * kLn2;
         } else {
-          float* ml = a.part_ml + ((int64_t)(x.part + x.split) * FX_KV_ROWS + c) * 2;
+          float* ml = a.parts.ml + ((int64_t)(x.part + x.split) * FX_KV_ROWS + c) * 2;
           ml[0] = top;
           ml[1] = sum;
         }
       }
     }
     if (x.splits > 1 && x.split == 0 && threadIdx.x == 0)
-      a.items[x.item] = FxKvItem{x.request, x.head, x.tile, x.part, x.splits};
+      a.parts.items[x.item] = FxKvItem{x.request, x.head, x.tile, x.part, x.splits};
   }
   if (a.fill) fill_rest<T>(a);
 }
@@ -573,8 +575,7 @@ __device__ __forceinline__ void piped(Read read, Use use, Meanwhile meanwhile) {
     for (int e = 0; e < 4; ++e) use(b * 4 + e, f[b & 1][e]);
   }
 }
-constexpr int tile_waves(int type, int dp) { return dp <= 128 && type != kF32 ? 8 : 4; }
-constexpr int tile_rows(int type, int dp) { return 32 * tile_waves(type, dp); }
+constexpr int tile_waves(int type, int dp) { return dp <= 128 && type != kF32 ? 8 : 4; }   // (fx_kv_tile_rows)
 
 // WIDE: pages of 64 tokens and more, so that a step lies in one page and all about its page is the same in all lanes; smaller pages
 // need a page for each group of 16 tokens, and took 421 us instead of 397 in the call above
@@ -596,7 +597,7 @@ __global__ __launch_bounds__(64 * tile_waves(TQ, DP), tile_waves(TQ, DP) / 4) vo
     Unit x;
     int shared_items = 0;
     const bool live = unit_at<true>(a, kRows, kTileLeast, u, x, &shared_items);
-    if (u == 0 && threadIdx.x == 0) *a.n_items = shared_items;
+    if (u == 0 && threadIdx.x == 0) *a.parts.n_items = shared_items;
     if (!live) break;
     __syncthreads();   // (LDS is free again)
     if (threadIdx.x == 0) s_nan = 0;
@@ -920,36 +921,38 @@ __global__ __launch_bounds__(64 * tile_waves(TQ, DP), tile_waves(TQ, DP) / 4) vo
           } else {
 #pragma unroll
             for (int k = 0; k < 4; ++k) o[k] = acc[d][e * 4 + k];
-            store4(z->part_acc + at * D + depth, o);
+            store4(z->parts.acc + at * D + depth, o);
           }
         }
       if (half == 0) {
         if (x.splits == 1) {
           z->lse[t * z->q_heads + h] = l == 0.0f ? -kInf : (m + __builtin_amdgcn_logf(l)) * kLn2;
         } else {
-          z->part_ml[at * 2] = m;
-          z->part_ml[at * 2 + 1] = l;
+          z->parts.ml[at * 2] = m;
+          z->parts.ml[at * 2 + 1] = l;
         }
       }
     }
     if (x.splits > 1 && x.split == 0 && threadIdx.x == 0)
-      z->items[x.item] = FxKvItem{x.request, x.head, x.tile, x.part, x.splits};
+      z->parts.items[x.item] = FxKvItem{x.request, x.head, x.tile, x.part, x.splits};
   }
   if (a.fill) fill_rest<T>(a);
 }
 
-// What several workgroups found for the same rows, added up.  A workgroup takes a row of an item: 16 bytes of the result a
+// What several workgroups found for the same rows, added up, of fx_kv_tiles and fx_kv_rows in one launch.  A workgroup takes a row of an item: 16 bytes of the result a
 // lane, the parts in turn over the groups of lanes that are left, whose sums meet in LDS in a fixed order.
 template <class T>
-__global__ __launch_bounds__(256) void fx_kv_join(const FxKvAttnArgs a, int tile_rows) {
+__global__ __launch_bounds__(256) void fx_kv_join(const FxKvAttnArgs a, const FxKvParts tiles, const FxKvParts rows) {
   __shared__ float s_m[64], s_l[64];
   __shared__ __align__(16) float s_o[256 * 4];
-  const int items = *a.n_items;
+  const int64_t of_tiles = tiles.n_items ? (int64_t)*tiles.n_items * tiles.tile_rows : 0, all = of_tiles + (rows.n_items ? (int64_t)*rows.n_items * rows.tile_rows : 0);
   const int D = a.c.depth, G = a.group, lanes = D / 4, groups = 256 / lanes;
   const int group = (int)threadIdx.x / lanes, d = ((int)threadIdx.x - group * lanes) * 4;
-  for (int64_t w = blockIdx.x; w < (int64_t)items * tile_rows; w += gridDim.x) {
-    const FxKvItem it = a.items[w / tile_rows];
-    const int c = (int)(w % tile_rows), row = it.tile * tile_rows + c;
+  for (int64_t w = blockIdx.x; w < all; w += gridDim.x) {
+    const FxKvParts& from = w < of_tiles ? tiles : rows;
+    const int tile_rows = from.tile_rows, at_row = (int)(w < of_tiles ? w : w - of_tiles), c = at_row % tile_rows;
+    const FxKvItem it = from.items[at_row / tile_rows];
+    const int row = it.tile * tile_rows + c;
     const int s = min(max(a.starts[it.request], 0), a.tokens), e = min(max(a.starts[it.request + 1], 0), a.tokens);
     if (row >= (e - s) * G) continue;
     float m = -kInf, l = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -957,8 +960,8 @@ __global__ __launch_bounds__(256) void fx_kv_join(const FxKvAttnArgs a, int tile
 #pragma unroll 4
       for (int p = group; p < it.parts; p += groups) {
         const int64_t at = (int64_t)(it.first + p) * tile_rows + c;
-        const float2 ml = *(const float2*)(a.part_ml + at * 2);
-        const float4 v = *(const float4*)(a.part_acc + at * D + d);
+        const float2 ml = *(const float2*)(from.ml + at * 2);
+        const float4 v = *(const float4*)(from.acc + at * D + d);
         const float now = fmaxf(m, ml.x), f = m == -kInf ? 0.0f : __builtin_amdgcn_exp2f(m - now),
                     g = ml.x == -kInf ? 0.0f : __builtin_amdgcn_exp2f(ml.x - now);
         m = now;
@@ -999,12 +1002,11 @@ __global__ __launch_bounds__(256) void fx_kv_join(const FxKvAttnArgs a, int tile
 
 struct Kernels {
   const void *rows, *tiles;
-  int tile_rows;   // of `tiles`; twice as many threads
 };
 template <int HELD, int TQ>
 Kernels kernels_of(int depth, bool wide) {
 #define FX_KV_PAIR(DP, EXACT) \
-  Kernels{(const void*)fx_kv_rows<HELD, TQ, DP, EXACT>, wide ? (const void*)fx_kv_tiles<HELD, TQ, DP, EXACT, true> : (const void*)fx_kv_tiles<HELD, TQ, DP, EXACT, false>, tile_rows(TQ, DP)}
+  Kernels{(const void*)fx_kv_rows<HELD, TQ, DP, EXACT>, wide ? (const void*)fx_kv_tiles<HELD, TQ, DP, EXACT, true> : (const void*)fx_kv_tiles<HELD, TQ, DP, EXACT, false>}
   if (depth == 64) return FX_KV_PAIR(64, true);
   if (depth == 128) return FX_KV_PAIR(128, true);
   if (depth == 256) return FX_KV_PAIR(256, true);

@@ -75,11 +75,12 @@ hipError_t offsets(const FxKvAttnArgs& a, int tile_rows, int least, hipStream_t 
   void* kargs[3] = {(void*)&args, (void*)&tile_rows, (void*)&least};
   return hipLaunchKernel((const void*)fxkv::fx_kv_offsets, dim3(1), dim3(1024), kargs, 0, stream);
 }
-hipError_t join(const FxKvAttnArgs& a, int type, int tile_rows, hipStream_t stream) {
+hipError_t join(const FxKvAttnArgs& a, const FxKvLaunch& l, hipStream_t stream) {
+  const int type = l.type;
   const void* kernel = type == fxkv::kBf16 ? (const void*)fxkv::fx_kv_join<__bf16>
                        : type == fxkv::kF16 ? (const void*)fxkv::fx_kv_join<_Float16>
                                             : (const void*)fxkv::fx_kv_join<float>;
-  return launch(kernel, 2048, 256, stream, a, tile_rows);
+  return launch(kernel, 2048, 256, stream, a, l.tiles_parts, l.rows_parts);
 }
 }  // namespace
 
@@ -91,17 +92,17 @@ hipError_t fx_launch_kv_attention(const FxKvAttnArgs& a, const FxKvLaunch& l, hi
   if (l.tiles_grid > 0) {
     args.rows_above = l.rows_grid > 0 ? FX_KV_FEW : 0;
     args.rows_upto = int64_t{1} << 31;
-    if ((e = offsets(args, k.tile_rows, fxkv::kTileLeast, stream)) != hipSuccess) return e;
-    if ((e = launch(k.tiles, l.tiles_grid, 2 * k.tile_rows, stream, args)) != hipSuccess) return e;
-    if (l.shared && (e = join(args, l.type, k.tile_rows, stream)) != hipSuccess) return e;
+    args.parts = l.tiles_parts;
+    if ((e = offsets(args, l.tiles_parts.tile_rows, fxkv::kTileLeast, stream)) != hipSuccess) return e;
+    if ((e = launch(k.tiles, l.tiles_grid, 2 * l.tiles_parts.tile_rows, stream, args)) != hipSuccess) return e;
     args.fill = 0;
   }
   if (l.rows_grid > 0) {
     args.rows_above = 0;
     args.rows_upto = l.tiles_grid > 0 ? FX_KV_FEW : int64_t{1} << 31;
+    args.parts = l.rows_parts;
     if ((e = offsets(args, FX_KV_ROWS, fxkv::kRowLeast, stream)) != hipSuccess) return e;
     if ((e = launch(k.rows, l.rows_grid, 256, stream, args)) != hipSuccess) return e;
-    if (l.shared && (e = join(args, l.type, FX_KV_ROWS, stream)) != hipSuccess) return e;
   }
-  return e;
+  return l.shared ? join(args, l, stream) : e;
 }
