@@ -616,6 +616,35 @@ def test_what_a_row_does_not_see_has_no_influence(n, window):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("kind", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("P", [16, 64, 256])
+@pytest.mark.parametrize("n", [6, 150])
+def test_nan_that_is_not_seen_and_nan_that_is(kind, P, n):
+    """The same on pages of all kinds: codes behind the last token and before the window are NaN, then one value that some rows see."""
+    H, G, D, L, window = 1, 2, 128, 330, 100
+    pages = -(-L // P)
+    cache = filled(pages + 1, H, P, D, E4M3, 4)
+    order = torch.randperm(pages + 1, generator=torch.Generator().manual_seed(P))[:pages].tolist()
+    q = torch.randn(n, H * G, D, generator=torch.Generator().manual_seed(n)).to(kind).cuda()
+    args = (q, i32([order + [-1]]), i32([L]), i32([0, n]), 0.125, window)
+    out, lse = cache.attention(*args)
+    k8, v8 = cache.k.view(torch.uint8), cache.v.view(torch.uint8)
+
+    def spoil(t, columns=slice(None)):
+        v8[order[t // P], :, t % P // 16, columns, t % 16] = 0x7F
+
+    for t in list(range(max(L - n + 1 - window, 0))) + list(range(L, pages * P)):
+        k8[order[t // P], :, t % P] = 0xFF
+        spoil(t)
+    again, lse2 = cache.attention(*args)
+    assert torch.equal(out, again) and torch.equal(lse, lse2)
+    spoil(L - 3, 77)                                   # seen by the last three rows
+    got, lse2 = cache.attention(*args)
+    assert bool(torch.isnan(got[n - 3:, :, 77]).all()) and int(torch.isnan(got).sum()) == 3 * G and torch.equal(lse, lse2)
+    assert torch.equal(torch.where(torch.isnan(got), 0.0, got), torch.where(torch.isnan(got), 0.0, out))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("n", [1, 70])
 def test_memory_that_nobody_has_written(n):
     """A cache of zeros, its scales too, as a warm-up may have it: results are finite, and next to nothing."""
