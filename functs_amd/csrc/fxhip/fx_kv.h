@@ -64,7 +64,7 @@ struct FxKvAttnArgs {
   int32_t tokens, requests, columns, q_heads, group, window;
   float scale;                                        // times log2(e)
   FxKvParts parts;
-  int32_t* offsets;                                   // of more than 256 requests: see fx_kv_offsets
+  int32_t* offsets;                                   // of more than 64 requests: see fx_kv_offsets
   int32_t fill;                                       // rows of no request are cleared
   int32_t q_vec;                                      // rows of queries are 16-byte aligned
   int64_t rows_above, rows_upto;                      // requests that this kernel takes: by rows of all query heads of a key head

@@ -166,7 +166,7 @@ __global__ __launch_bounds__(kThreads) void fx_kv_plan_kernel(const FxKvPlanArgs
 // magnitudes meet in LDS; shorter ones, and those in no order, are the waves' in turn.  Keys: 8 numbers of a token a lane.  Values: 2 columns
 // of a group of 16 tokens a lane, which are 32 neighbouring bytes of the cache.
 // Measured: 19 000 tokens of 9 prompts, 8 heads of 128, pages of 64, fp16 to int8: 36 us, 3.3 TB/s (a large copy: 5.4); whole runs a wave: 46.
-// 96 single tokens: 5.9 us, most of it the way to slots, rows and codes, one after the other.
+// 96 single tokens: 8 us, most of it the way to slots, rows and codes, one after the other.
 // Magnitudes are compared as the integers that their bits are.  Where the largest one is finite and below the largest scale, no number
 // needs to be held to the range of the codes or looked at for NaN (PLAIN).
 constexpr int kStoreWaves = kThreads / 64;

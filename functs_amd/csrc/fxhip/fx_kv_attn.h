@@ -121,9 +121,11 @@ __device__ __forceinline__ int64_t all_steps(const FxKvAttnArgs& a, int64_t step
 }
 
 // Unit u of the call, or false behind the last one: every wave finds it by itself, in scalar registers, without a barrier.  Up
-// to kScanned requests are added up here, a lane one of 64 a round; of more, fx_kv_offsets has left the sums.
-// SORTED: of up to 64 requests those of more steps come first, so that what is left at the end of a call is short.
-constexpr int kScanned = 256;
+// to kScanned requests are added up here, one a lane; of more, fx_kv_offsets has left the sums (130 requests of 300 tokens took 35 us so,
+// 39 with rounds of 64 here; 250 took 51 and 64, 700 of 100 tokens 86 and 211).
+// SORTED: of up to 64 requests those of more steps come first, so that what is left at the end of a call is short: fx_kv_tiles (prompts
+// 415 us without, 391 with); fx_kv_rows, of many workgroups a CU, took 71 us for 64 requests of up to 4 000 tokens with it and 62 without.
+constexpr int kScanned = 64;
 // Chunks are multiples of so many steps: fx_kv_rows, of one for each wave; fx_kv_tiles, so that what a part costs by itself (some 8 us) stays
 // small: 4 requests of 256 rows on 3 000 cached tokens, 12 heads of 64, took 67 us with 4, 68 with 8 and 86 with 2; one of 8 000 37, 39 and 37
 constexpr int kRowLeast = 4, kTileLeast = 4;
@@ -132,50 +134,33 @@ __device__ __forceinline__ bool unit_at(const FxKvAttnArgs& a, int tile_rows, in
   const int lane = (int)threadIdx.x & 63;
   int chunk, rest, parts;   // rest: the unit's number in its request; parts: items << 16 | parts before the request
   if (a.requests <= kScanned) {
-    FxKvRequest r;
-    auto load = [&](int b0) {   // (all three loads at once, whatever the lane)
-      const int b = b0 + lane, c = max(min(b, a.requests - 1), 0);
-      const int start = a.starts[c], end = a.starts[c + (a.requests > 0 ? 1 : 0)], len = a.requests > 0 ? a.lens[c] : 0;
-      r = request_of(a, start, b < a.requests ? end : start, len, tile_rows);
-    };
-    int64_t work = 0;
-    for (int b0 = 0; b0 < a.requests; b0 += 64) {
-      load(b0);
-      work += (int64_t)r.tiles * r.steps;
-    }
-    chunk = fx_kv_chunk(all_steps(a, wave_total(work)), least);
-    int units_before = 0, cuts_before = 0;   // of the rounds before
-    bool found = false;
-    for (int b0 = 0; b0 < a.requests; b0 += 64) {
-      if (a.requests > 64) load(b0);
-      const int splits = fx_kv_parts(r.steps, chunk), items = r.tiles * a.c.heads, mine = items * splits, cut = splits > 1 ? (items << 16) + mine : 0;
-      const int upto = sum_upto(mine), cuts = sum_upto(cut);
-      int before = units_before + upto - mine;
-      if (SORTED && a.requests <= 64) {
-        before = 0;
-        for (int c = 0; c < a.requests; ++c) {
-          const int n = __builtin_amdgcn_readlane(r.steps, c), add = __builtin_amdgcn_readlane(mine, c);
-          if (n > r.steps || (n == r.steps && c < lane)) before += add;
-        }
+    // (all three loads at once, whatever the lane)
+    const int c = max(min(lane, a.requests - 1), 0), start = a.starts[c], end = a.starts[c + (a.requests > 0 ? 1 : 0)], len = a.requests > 0 ? a.lens[c] : 0;
+    const FxKvRequest r = request_of(a, start, lane < a.requests ? end : start, len, tile_rows);
+    chunk = fx_kv_chunk(all_steps(a, wave_total((int64_t)r.tiles * r.steps)), least);
+    const int splits = fx_kv_parts(r.steps, chunk), items = r.tiles * a.c.heads, mine = items * splits, cut = splits > 1 ? (items << 16) + mine : 0;
+    const int cuts = sum_upto(cut);
+    int before = 0;
+    if constexpr (SORTED) {
+      for (int c = 0; c < a.requests; ++c) {
+        const int n = __builtin_amdgcn_readlane(r.steps, c), add = __builtin_amdgcn_readlane(mine, c);
+        if (n > r.steps || (n == r.steps && c < lane)) before += add;
       }
-      const unsigned long long owner = __ballot(u >= before && u < before + mine);
-      if (owner != 0) {
-        const int L = __builtin_ctzll(owner);
-        x.request = b0 + L;
-        x.r.start = __builtin_amdgcn_readlane(r.start, L);
-        x.r.rows = __builtin_amdgcn_readlane(r.rows, L);
-        x.r.len = __builtin_amdgcn_readlane(r.len, L);
-        x.r.tiles = __builtin_amdgcn_readlane(r.tiles, L);
-        x.r.steps = __builtin_amdgcn_readlane(r.steps, L);
-        rest = u - __builtin_amdgcn_readlane(before, L);
-        parts = cuts_before + __builtin_amdgcn_readlane(cuts - cut, L);
-        found = true;
-      }
-      units_before += __builtin_amdgcn_readlane(upto, 63);
-      cuts_before += __builtin_amdgcn_readlane(cuts, 63);
+    } else {
+      before = sum_upto(mine) - mine;
     }
-    *shared_items = (unsigned)cuts_before >> 16;
-    if (!found) return false;
+    *shared_items = (unsigned)__builtin_amdgcn_readlane(cuts, 63) >> 16;
+    const unsigned long long owner = __ballot(u >= before && u < before + mine);
+    if (owner == 0) return false;
+    const int L = __builtin_ctzll(owner);
+    x.request = L;
+    x.r.start = __builtin_amdgcn_readlane(r.start, L);
+    x.r.rows = __builtin_amdgcn_readlane(r.rows, L);
+    x.r.len = __builtin_amdgcn_readlane(r.len, L);
+    x.r.tiles = __builtin_amdgcn_readlane(r.tiles, L);
+    x.r.steps = __builtin_amdgcn_readlane(r.steps, L);
+    rest = u - __builtin_amdgcn_readlane(before, L);
+    parts = __builtin_amdgcn_readlane(cuts - cut, L);
   } else {
     const int32_t* units = a.offsets + 2;   // [requests + 1], then [requests] of parts
     chunk = a.offsets[0];

@@ -5,6 +5,8 @@
 // request of more steps than a chunk has its items shared by several workgroups.  An item of t steps, more than a
 // chunk of c, gets ceil(t / c) <= 2 t / c parts, so there are fewer than FX_KV_TARGET shared items and at most
 // 2 FX_KV_TARGET parts whatever the lengths: the sizes of the workspace.
+// Measured with 128, 256 and 512: one request of 130 000 tokens 64, 55 and 57 us; 64 of up to 4 000 64, 63 and 72; prompts 390, 391 and
+// 421; 24 requests of a few rows 19, 20 and 23.
 #pragma once
 #include <stdint.h>
 
