@@ -18,6 +18,7 @@ constexpr int kThreads = 256;
 // takes kPlanTokens tokens and adds up the lengths of all requests by itself (kPlanRequests a round).  The
 // request of a token: the workgroup's requests leave their number at their first token, and a maximum over
 // the tokens before spreads it.
+// Measured: 17 requests of one token 5.4 us, 700 requests of 89 000 tokens 7.4, either below the host's work for a call.
 constexpr int kPlanTokens = 1024, kPlanRequests = 1024, kPer = 4;
 static_assert(kPlanTokens == kThreads * kPer && kPlanRequests == kThreads * kPer, "four of each a thread");
 
@@ -569,10 +570,9 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 5 : 4) void fx_kv_store_
 // ---- fx_kv_read ----
 // Bound: HBM (1 byte read and 2 or 4 written for each number).  A wave takes the keys or the values of one head for 4 to 16
 // entries of `slots`.  Keys: 8 numbers of a token a lane, four loads under way.  Values: 4 columns of 8 of the 16 tokens of a
-// group that neighbours share, so that a lane writes 4 numbers side by side.
-// Measured: 25 500 tokens, 8 heads of 128, e4m3 to bf16, caches and results that are in no cache of the chip: 46 us, 3.4 TB/s (a large
-// copy: 5.4).  2 columns of 16 tokens a lane: 43 us, but 816 tokens in runs of 8 take 14.2 us with the step that stores them
-// instead of 15.8.  32 tokens a wave 45 to 47 us, 8 tokens 54.
+// group, so that a lane writes 4 numbers side by side; the group is the wave's in whose entries its first token is.
+// Measured: 25 500 tokens, 8 heads of 128, e4m3 to bf16, caches and results that are in no cache of the chip: 45 us, 3.5 TB/s (a large
+// copy: 5.4), keys alone 18 and values 25.  32 entries a wave 45 to 47 us, 8 entries 54; groups cut where the entries end 46.
 template <int HELD, class T>
 __global__ __launch_bounds__(kThreads) void fx_kv_read_kernel(const FxKvCache c, const FxKvRows r, int per_wave, int n_chunks, int vec) {
   const int lane = (int)threadIdx.x & 63;
@@ -623,13 +623,18 @@ __global__ __launch_bounds__(kThreads) void fx_kv_read_kernel(const FxKvCache c,
     }
     return;
   }
+  // The wave's are the neighbours of one group of 16, their slots rising by one, that begin in its chunk; lane i has token t0 - 1 + i
   T* dst = (T*)r.v + (int64_t)t0 * r.v_token + (int64_t)head * r.v_head;
-  for (int j = 0; j < n;) {
-    const int64_t slot = lane_of(mine, j);
-    // neighbours of the same group of 16 whose slots rise by one
-    const unsigned long long rising = __ballot(lane >= j && lane < n && mine == slot + (lane - j)) >> j;
+  const int token = t0 - 1 + lane;
+  mine = r.slots[min(max(token, 0), r.tokens - 1)];
+  if (token < 0 || token >= r.tokens || mine < 0 || mine >= n_slots) mine = -1;
+  const int64_t prior = (int64_t)__shfl_up((unsigned long long)mine, 1u, 64);
+  const unsigned long long follows = __ballot(lane > 0 && mine >= 0 && prior + 1 == mine && (mine & 15) != 0);
+  for (unsigned long long begins = ~follows & ((2ull << n) - 2); begins != 0; begins &= begins - 1) {
+    const int at = __builtin_ctzll(begins), j = at - 1;
+    const int64_t slot = lane_of(mine, at);
     const int o = (int)(slot & 15);
-    const int m = slot < 0 ? 1 : min(min(~rising == 0 ? 64 : __builtin_ctzll(~rising), 16 - o), n - j);
+    const int m = slot < 0 ? 1 : __builtin_ctzll(~(follows >> at >> 1)) + 1;
     const int64_t p = slot < 0 ? 0 : slot >> c.log_page;
     const float scale = slot < 0 ? 0.0f : c.v_scale[p * c.vs_stride + head];
     const uint8_t* codes = c.v + p * c.v_stride + in_page + (slot < 0 ? 0 : (slot & (page - 1)) >> 4) * 16 * D;
@@ -661,7 +666,6 @@ __global__ __launch_bounds__(kThreads) void fx_kv_read_kernel(const FxKvCache c,
         }
       }
     }
-    j += m;
   }
 }
 

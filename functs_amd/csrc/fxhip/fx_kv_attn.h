@@ -257,6 +257,9 @@ __device__ __forceinline__ float larger(float a, float b) { return __builtin_amd
 // Bound: HBM, each key and value is read once by one wave, straight into the registers of its operand; 64 tokens a
 // step, the four waves of a workgroup in turn.  The loads of the next step's keys are under way during the softmax and the second
 // product, those of the values during the first.
+// Measured (e4m3, depth 128, 8 heads): one request of 130 000 tokens, 8 query heads to each, fp16, 49.5 us, 5.4 TB/s, as a large copy,
+// and 4.6 of fx_kv_join; 64 requests of up to 4 000, 4 query heads, bf16, 58 to 62, 4.3 TB/s: units of unequal length.  A single
+// request of 50 tokens 6.8 us, a chain of launch, lengths, table, codes and join within the workgroup.
 template <int HELD, int TQ, int DP, bool EXACT>
 __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void fx_kv_rows(const FxKvAttnArgs a) {
   typedef typename TypeOf<TQ>::type T;
@@ -523,10 +526,11 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void fx_kv_rows(const FxKvA
 // step before with the values, then the next scores) the other one makes its weights and its share of the operands, and a barrier
 // changes them over.  Products go first (their waves' priority): what they wait for is longer.  Where a wave's registers are more than
 // half of a SIMD's (fp32 queries, depths above 128) there is one group, which does one after the other.
-// Measured at 4 requests of 511 to 2 047 rows behind up to 6 001 cached tokens, 32 query heads on 8, depth 128, e4m3, bf16 (0.30
-// TFLOP): 391 us, 770 TFLOP/s, of 1 430 that a large library product reaches here.  Without the second group 438 us, without the
-// priority 397, with a page a lane and group of 16 tokens (below) in place of one a step 421.  A step takes about 2 300 clocks for either
-// half of its work: 1 024 of the matrix cores and their operands' way from LDS (64 reads of 16 bytes a lane), or 1 750 of the vector units.
+// Measured at 4 requests of 511 to 2 047 rows behind up to 6 001 cached tokens, 32 query heads on 8, depth 128, e4m3, bf16 (0.33
+// TFLOP): 380 us, 875 TFLOP/s, of 1 430 that a large library product reaches here.  Without the second group 438 us (before the next
+// two steps), with a page a lane and group of 16 tokens (below) in place of one a step 421, without the priority 397.  A step takes about
+// 2 300 clocks for either half of its work: 1 024 of the matrix cores and their operands' way from LDS (64 reads of 16 bytes a
+// lane), or 1 750 of the vector units.
 // In LDS a key's row of 16-byte pieces is permuted by its token (key_piece), which spreads the 32 rows of an operand over the banks; values
 // lie as [group][8 tokens of it][depth][8 tokens].
 typedef float fx_f32x16 __attribute__((ext_vector_type(16)));
@@ -924,8 +928,10 @@ __global__ __launch_bounds__(64 * tile_waves(TQ, DP), tile_waves(TQ, DP) / 4) vo
   if (a.fill) fill_rest<T>(a);
 }
 
-// What several workgroups found for the same rows, added up, of fx_kv_tiles and fx_kv_rows in one launch.  A workgroup takes a row of an item: 16 bytes of the result a
-// lane, the parts in turn over the groups of lanes that are left, whose sums meet in LDS in a fixed order.
+// What several workgroups found for the same rows, added up, of fx_kv_tiles and fx_kv_rows in one launch.  A workgroup takes a row of
+// an item: 16 bytes of the result a lane, the parts in turn over the groups of lanes that are left, whose sums meet in LDS in a fixed order.
+// Bound: latency, 4.6 us whatever there is to add up.  (Done by the last workgroup to arrive, at counters, it gained nothing: 54 and 56 us
+// for the long request above.)
 template <class T>
 __global__ __launch_bounds__(256) void fx_kv_join(const FxKvAttnArgs a, const FxKvParts tiles, const FxKvParts rows) {
   __shared__ float s_m[64], s_l[64];
