@@ -61,6 +61,8 @@ fx_kv_cache cacheOf(const char* op, const Tensor& k, const Tensor& v, const Tens
   onGpu(op, v, "v_cache", dev);
   onGpu(op, ks, "k_scale", dev);
   onGpu(op, vs, "v_scale", dev);
+  noGrad(op, ks, "k_scale");
+  noGrad(op, vs, "v_scale");
   TORCH_CHECK(k.scalar_type() == at::kFloat8_e4m3fn || k.scalar_type() == at::kChar, op, ": a cache holds float8_e4m3fn or int8, got ", k.scalar_type());
   TORCH_CHECK(k.dim() == 4, op, ": k_cache must be [pages, heads, page, depth], got ", k.sizes());
   const int64_t N = k.size(0), H = k.size(1), P = k.size(2), D = k.size(3);
@@ -212,7 +214,7 @@ void attend(const Tensor& q_, const Tensor& k_cache, const Tensor& v_cache, cons
   TORCH_CHECK(block_table.scalar_type() == at::kInt && block_table.dim() == 2, op, ": block_table must be int32 [requests, columns], got ",
               block_table.scalar_type(), " ", block_table.sizes());
   const int64_t B = block_table.size(0);
-  TORCH_CHECK(std::isfinite(scale) && scale > 0, op, ": scale must be positive and finite, got ", scale);
+  TORCH_CHECK(scale >= 0x1p-26 && scale <= 32.0, op, ": scale must lie between 2^-26 and 32, got ", scale);
   TORCH_CHECK(window >= 0 && max_new >= 0, op, ": window and max_new must not be negative, got ", window, " and ", max_new);
   const int dtype = dtypeOf(op, q_.scalar_type(), "q");
   c10::DeviceGuard guard(dev);
@@ -222,6 +224,8 @@ void attend(const Tensor& q_, const Tensor& k_cache, const Tensor& v_cache, cons
   if (out_) {
     onGpu(op, *out_, "out", dev);
     onGpu(op, *lse_, "lse", dev);
+    noGrad(op, *out_, "out");
+    noGrad(op, *lse_, "lse");
     TORCH_CHECK(out_->scalar_type() == q.scalar_type() && out_->sizes() == q.sizes() && out_->is_contiguous(), op, ": out must be contiguous, of the type and sizes of q");
     TORCH_CHECK(lse_->scalar_type() == at::kFloat && lse_->dim() == 2 && lse_->size(0) == q.size(0) && lse_->size(1) == q.size(1) && lse_->is_contiguous(), op,
                 ": lse must be contiguous float32 [tokens, heads]");

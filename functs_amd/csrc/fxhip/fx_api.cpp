@@ -1786,7 +1786,8 @@ int fx_kv_attention(const fx_kv_cache* cache, const fx_kv_attention_desc* desc, 
   if (d.tokens < 0 || d.requests < 0 || d.columns < 0 || d.window < 0 || d.max_new < 0) return fail(FX_E_INVALID, "fx_kv_attention: negative size");
   if (d.q_heads < 1 || d.q_heads % c.heads != 0)
     return fail(FX_E_INVALID, "fx_kv_attention: the query heads must be a multiple of the cache's heads (got " + std::to_string(d.q_heads) + " of " + std::to_string(c.heads) + ")");
-  if (!(d.scale > 0.0f) || !(d.scale <= std::numeric_limits<float>::max())) return fail(FX_E_INVALID, "fx_kv_attention: scale must be positive and finite");
+  // (times log2(e) and the scales of pages, 2^-100 to 2^121, it stays a normal number)
+  if (!(d.scale >= 0x1p-26f) || !(d.scale <= 32.0f)) return fail(FX_E_INVALID, "fx_kv_attention: scale must lie between 2^-26 and 32");
   if (d.tokens == 0) return FX_OK;
   if (!d.q || !d.out || !d.lse || !d.starts || (d.requests > 0 && !d.lens) || (d.requests > 0 && d.columns > 0 && !d.table))
     return fail(FX_E_INVALID, "fx_kv_attention: null argument");

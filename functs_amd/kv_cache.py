@@ -86,7 +86,7 @@ class KvCache:
                   max_new: int = 0, out: Optional[Tensor] = None, lse: Optional[Tensor] = None) -> Tuple[Tensor, Tensor]:
         """Rows starts[b] to starts[b + 1] of q [tokens, query heads, depth] are the last tokens of request b's lens[b]; each sees
         the tokens up to its own (the last `window` of them, if not 0).  Returns the weighted values (type of q) and the logarithm of
-        the sum of exponentials (fp32 [tokens, query heads]).  scale: depth ** -0.5 unless given.  max_new: the most rows of one request, if known (1
+        the sum of exponentials (fp32 [tokens, query heads]).  scale: depth ** -0.5 unless given, 2^-26 to 32.  max_new: the most rows of one request, if known (1
         for a decoding step): a matter of speed alone.  With out and lse, rows of no request stay as they are there."""
         if scale is None:
             scale = self.k.size(3) ** -0.5

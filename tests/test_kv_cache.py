@@ -746,6 +746,38 @@ def test_refusals():
         c.attention(q.clone().requires_grad_(), table, lens, starts)
 
 
+@pytest.mark.gpu
+def test_more_refusals():
+    """Scales that would leave the range of normal numbers with a page's, and gradients asked of what is written."""
+    c = filled(4, 2, 16, 64, E4M3, 1)
+    table, lens, starts, slots = i32([[0, 1]]), i32([20]), i32([0, 2]), torch.tensor([3, 4]).cuda()
+    q, k = torch.zeros(2, 4, 64, device="cuda"), torch.zeros(2, 2, 64, device="cuda")
+    grown = KvCache(c.k, c.v, c.k_scale.clone().requires_grad_(), c.v_scale)
+    for call in (lambda: c.attention(q, table, lens, starts, 2.0 ** -27), lambda: c.attention(q, table, lens, starts, 33.0), lambda: grown.attention(q, table, lens, starts),
+                 lambda: grown.store(k, k, slots), lambda: grown.read(slots),
+                 lambda: c.attention(q, table, lens, starts, out=torch.zeros_like(q).requires_grad_(), lse=torch.zeros(2, 4, device="cuda"))):
+        with pytest.raises(RuntimeError):
+            call()
+    with torch.no_grad():
+        grown.store(k, k, slots)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("held,top", [(E4M3, 119), (INT8, 121)])
+@pytest.mark.parametrize("n", [1, 140])
+def test_the_smallest_and_largest_scales(held, top, n):
+    """Pages under the ends of the range of scales, and scale at its own: scores of ordinary size from numbers that are not."""
+    for e, scale, size in ((-100, 2.0 ** -26, 2.0 ** 112), (top, 2.0 ** -20, 2.0 ** -105), (0, 32.0, 2.0 ** -8)):
+        c = filled(6, 1, 64, 64, held, 3)
+        c.k_scale.fill_(2.0 ** e)
+        q = torch.randn(n, 2, 64, generator=torch.Generator().manual_seed(n)) * size
+        table, lens, starts = [[4, 1, 2, 0]], [200], [0, n]
+        out, lse = c.attention(q.cuda(), i32(table), i32(lens), i32(starts), scale)
+        ref, rl, spread, most = PlainCache(c).attention(q, table, lens, starts, scale, 0)
+        bound, lbound = tolerance(torch.float32, ref, rl, spread, most, 200, 64)
+        assert bool(((out.cpu().double() - ref).abs() <= bound).all()) and bool(((lse.cpu().double() - rl).abs() <= lbound).all())
+
+
 # ---- GPU: together ----
 
 def serve(steps, cache, table, free, tokens, seed, layers=1):
