@@ -1695,13 +1695,13 @@ FxKvLaunch kv_launch(const FxKvCache& c, const fx_kv_attention_desc& d) {
   const int64_t group = d.q_heads / c.heads, some = std::min(d.requests, d.tokens);
   const int64_t longest = (d.max_new > 0 ? std::min(d.max_new, d.tokens) : d.tokens) * group;   // rows of one request
   const int64_t all = (int64_t)d.tokens * group;
-  const bool many = longest > FX_KV_FEW, few = !many || d.requests != 1;
+  const bool many = longest > FX_KV_FEW && l.type != 2 && (int64_t)d.tokens * d.q_heads >= FX_KV_MANY, few = !many || d.requests != 1;
   // (at least 1: requests or rows may be none; at most 2^20: a workgroup takes several units where there are more)
   auto grid = [&](int tile, int64_t longest) {
     const int64_t items = c.heads * std::min(all / tile + some, some * ((longest + tile - 1) / tile));
     return std::min<int64_t>(std::max<int64_t>(items + (l.shared ? FX_KV_TARGET : 0), 1), 1 << 20);
   };
-  const int tile_rows = fx_kv_tile_rows(d.dtype == FX_DT_F32, c.depth);
+  const int tile_rows = fx_kv_tile_rows(c.depth);
   if (many) l.tiles_grid = grid(tile_rows, longest);
   if (few) l.rows_grid = grid(FX_KV_ROWS, many ? FX_KV_FEW : longest);
   l.tiles_parts.tile_rows = tile_rows;

@@ -39,11 +39,15 @@ hipError_t fx_launch_kv_read(const FxKvCache& c, const FxKvRows& r, int held, hi
 
 #define FX_KV_ROWS 16   // rows (tokens of a request times query heads of a key head) of a tile of fx_kv_rows
 // rows of a tile of fx_kv_tiles: 32 for each of 8 waves; of 4 where a wave needs more than half of a SIMD's registers
-FX_KV_HD int fx_kv_tile_rows(bool f32, int depth) { return depth <= 128 && !f32 ? 256 : 128; }
-// Requests of more rows are fx_kv_tiles', the others fx_kv_rows'.  Measured, fx_kv_rows against fx_kv_tiles (us, bf16, e4m3): 16 requests of
-// 2 000 cached tokens, 8 heads of 128: 128 rows 53 / 85, 256 rows 99 / 118; 64 of 500: 96 rows 75 / 83, 128 rows 97 / 86, 256 rows 183 /
-// 121; one of 8 000: 128 rows 23 / 31, 256 rows 35 / 38; depth 80, 4 heads, 16 of 1 000: 125 rows 20 / 54.
+FX_KV_HD int fx_kv_tile_rows(int depth) { return depth <= 128 ? 256 : 128; }
+// fx_kv_tiles takes the requests of more than FX_KV_FEW rows of calls of 16-bit queries with at least FX_KV_MANY rows of all heads (192 for
+// each CU: with fewer its large tiles leave CUs idle); all others are fx_kv_rows'.  Measured, fx_kv_rows against fx_kv_tiles (us, e4m3, bf16):
+//   calls     1 request, 32 heads of 128: 32 000 rows 84 / 104, 64 000 rows 188 / 105; 4 requests, 192 000 rows 880 / 414; 12 heads of 64,
+//             96 000 rows 95 / 85, 192 000 rows 204 / 156; depth 256: 16 000 rows 76 / 86, 64 000 rows 447 / 368; depth 80: 32 000 rows 67 / 111
+//   requests  of 100 rows, 51 200 in all 46 / 71; of 128 rows, 65 536 in all 97 / 86, of 400 rows, 102 400 in all 116 / 84
+//   fp32      (three numbers for each query and weight) 64 000 rows 238 / 267, 192 000 rows 1 000 / 1 335, depth 256 517 / 1 002: fx_kv_rows always
 #define FX_KV_FEW 128
+#define FX_KV_MANY 49152
 struct FxKvItem {   // rows whose cached tokens several workgroups shared
   int32_t request, head, tile, first, parts;
 };

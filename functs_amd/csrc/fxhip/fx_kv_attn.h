@@ -518,14 +518,14 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void fx_kv_rows(const FxKvA
 }
 
 // ---- 32 rows a wave: prompts ----
-// Bound: the matrix cores and the vector units, which turn scores into weights, side by side.  The waves of a workgroup take 32 rows
+// Queries of 16 bits.  Bound: the matrix cores and the vector units, which turn scores into weights, side by side.  The waves of a workgroup take 32 rows
 // each and share the cached tokens, 64 a step: together they turn a step's codes into 16-bit floats and leave them in LDS.  32 x 32
 // products; as above the scores stay where the second product reads them: row 8 g + 4 h + j of K's operand is token
 // 16 h + 4 g + j, so a lane holds the 16 tokens of one group.
 // Two groups of four waves, one of each on every SIMD, half a step apart: while one is at its products (those of the
 // step before with the values, then the next scores) the other one makes its weights and its share of the operands, and a barrier
 // changes them over.  Products go first (their waves' priority): what they wait for is longer.  Where a wave's registers are more than
-// half of a SIMD's (fp32 queries, depths above 128) there is one group, which does one after the other.
+// half of a SIMD's (depths above 128) there is one group, which does one after the other.
 // Measured at 4 requests of 511 to 2 047 rows behind up to 6 001 cached tokens, 32 query heads on 8, depth 128, e4m3, bf16 (0.33
 // TFLOP): 380 us, 875 TFLOP/s, of 1 430 that a large library product reaches here.  Without the second group 438 us (before the next
 // two steps), with a page a lane and group of 16 tokens (below) in place of one a step 421, without the priority 397.  A step takes about
@@ -564,15 +564,15 @@ __device__ __forceinline__ void piped(Read read, Use use, Meanwhile meanwhile) {
     for (int e = 0; e < 4; ++e) use(b * 4 + e, f[b & 1][e]);
   }
 }
-constexpr int tile_waves(int type, int dp) { return dp <= 128 && type != kF32 ? 8 : 4; }   // (fx_kv_tile_rows)
+constexpr int tile_waves(int dp) { return dp <= 128 ? 8 : 4; }   // (fx_kv_tile_rows)
 
 // WIDE: pages of 64 tokens and more, so that a step lies in one page and all about its page is the same in all lanes; smaller pages
 // need a page for each group of 16 tokens, and took 421 us instead of 397 in the call above
 template <int HELD, int TQ, int DP, bool EXACT, bool WIDE>
-__global__ __launch_bounds__(64 * tile_waves(TQ, DP), tile_waves(TQ, DP) / 4) void fx_kv_tiles(const FxKvAttnArgs a) {
+__global__ __launch_bounds__(64 * tile_waves(DP), tile_waves(DP) / 4) void fx_kv_tiles(const FxKvAttnArgs a) {
   typedef typename TypeOf<TQ>::type T;
-  constexpr int W = tile_waves(TQ, DP), kGroups = W / 4, kRows = 32 * W;
-  constexpr int NQ = TQ == kF32 ? 3 : 1, NP = TQ == kF32 ? 3 : TQ == kF16 ? 2 : 1, C = DP / 16, DT = DP / 32;
+  constexpr int W = tile_waves(DP), kGroups = W / 4, kRows = 32 * W;
+  constexpr int NP = TQ == kF16 ? 2 : 1, C = DP / 16, DT = DP / 32;
   constexpr int kShare = DP / 8 / W;   // KB of a step's keys and values that a wave takes
   constexpr int kTile = FX_KV_STEP * DP * 2;
   constexpr bool F16 = TQ == kF16;
@@ -601,16 +601,14 @@ __global__ __launch_bounds__(64 * tile_waves(TQ, DP), tile_waves(TQ, DP) / 4) vo
     FxKvSpan mine = scalars(fx_kv_span(x.r, G, a.window, min(w0, n_rows - 1), 32, 0, 1));   // of this wave's rows
     if (w0 >= n_rows) mine.high = 0;
     const int from = span.from, n = span.to - span.from;
-    Frag q[NQ][C];
+    Frag q[C];
     {
       const T* src = (const T*)a.q + (int64_t)(x.r.start + i) * a.q_token + (int64_t)(x.head * G + g) * a.q_head;
 #pragma unroll
       for (int c = 0; c < C; ++c) {
         const int d = c * 16 + half * 8;
-        Frag* f[NQ];
-#pragma unroll
-        for (int k = 0; k < NQ; ++k) f[k] = &q[k][c];
-        load_query<TQ, NQ, T>(f, src, d, valid && d < D, a.q_vec != 0);
+        Frag* f[1] = {&q[c]};
+        load_query<TQ, 1, T>(f, src, d, valid && d < D, a.q_vec != 0);
       }
     }
     fx_f32x16 acc[DT];
@@ -767,10 +765,7 @@ __global__ __launch_bounds__(64 * tile_waves(TQ, DP), tile_waves(TQ, DP) / 4) vo
 #pragma unroll
           for (int e = 0; e < 16; ++e) r[t][e] = 0.0f;
         piped<2 * C>([&](int k) { return *(const Frag*)(kt + k % 2 * 32 * DP * 2 + krow + (kpiece ^ (k / 2 * 32))); },
-                     [&](int k, const Frag& kf) {
-#pragma unroll
-                       for (int e = NQ - 1; e >= 0; --e) r[k % 2] = mfma32<F16>(kf, q[e][k / 2], r[k % 2]);
-                     }, []() {});
+                     [&](int k, const Frag& kf) { r[k % 2] = mfma32<F16>(kf, q[k / 2], r[k % 2]); }, []() {});
       }
     };
     // the weights of step s, and a share of round `round`
@@ -996,14 +991,16 @@ struct Kernels {
 };
 template <int HELD, int TQ>
 Kernels kernels_of(int depth, bool wide) {
-#define FX_KV_PAIR(DP, EXACT) \
-  Kernels{(const void*)fx_kv_rows<HELD, TQ, DP, EXACT>, wide ? (const void*)fx_kv_tiles<HELD, TQ, DP, EXACT, true> : (const void*)fx_kv_tiles<HELD, TQ, DP, EXACT, false>}
+  // (fp32 queries: fx_kv_rows alone)
+#define FX_KV_TILES(DP, EXACT) (wide ? (const void*)fx_kv_tiles<HELD, TQ == kF32 ? kBf16 : TQ, DP, EXACT, true> : (const void*)fx_kv_tiles<HELD, TQ == kF32 ? kBf16 : TQ, DP, EXACT, false>)
+#define FX_KV_PAIR(DP, EXACT) Kernels{(const void*)fx_kv_rows<HELD, TQ, DP, EXACT>, TQ == kF32 ? nullptr : FX_KV_TILES(DP, EXACT)}
   if (depth == 64) return FX_KV_PAIR(64, true);
   if (depth == 128) return FX_KV_PAIR(128, true);
   if (depth == 256) return FX_KV_PAIR(256, true);
   if (depth < 128) return FX_KV_PAIR(128, false);
   return FX_KV_PAIR(256, false);
 #undef FX_KV_PAIR
+#undef FX_KV_TILES
 }
 template <int HELD>
 Kernels kernels_of(int type, int depth, bool wide) {

@@ -133,18 +133,17 @@ class PlainCache:
             pages = torch.where(ok, pages, 0)
             k = self.k[pages, :, j % P] * self.ks[pages][:, :, None]
             v = self.v[pages, :, j % P] * self.vs[pages][:, :, None]
-            for i in range(n):
-                p = L - n + i
-                sees = ok & (j <= p) & ((j > p - window) if window else True)
-                if not bool(sees.any()):
-                    continue
-                t = starts[b] + i
-                ki, vi = k[sees].repeat_interleave(hq // H, 1), v[sees].repeat_interleave(hq // H, 1)
-                s = (ki * q[t]).sum(-1) * scale
-                size[t] = ((ki * q[t]).abs().sum(-1) * scale).amax(0)
-                lse[t] = torch.logsumexp(s, 0)
-                w = torch.softmax(s, 0)[:, :, None]
-                out[t], spread[t] = (w * vi).sum(0), (w * vi.abs()).sum(0)
+            p = L - n + torch.arange(n)[:, None]
+            sees = ok & (j <= p) & ((j > p - window) if window else True)
+            k, v = torch.where(ok[:, None, None], k, 0.0), torch.where(ok[:, None, None], v, 0.0)
+            heads = lambda x: x.permute(1, 0, 2).repeat_interleave(hq // H, 0)  # noqa: E731
+            rows = slice(starts[b], starts[b] + n)
+            qb, kb, vb = q[rows].permute(1, 0, 2).contiguous(), heads(k).transpose(1, 2).contiguous(), heads(v).contiguous()
+            s = torch.where(sees, torch.bmm(qb, kb) * scale, -math.inf)
+            w = torch.nan_to_num(torch.softmax(s, 2), nan=0.0)               # (rows that see nothing)
+            size[rows] = torch.where(sees, torch.bmm(qb.abs(), kb.abs()) * scale, 0.0).amax(2).t()
+            lse[rows] = torch.logsumexp(s, 2).t()
+            out[rows], spread[rows] = torch.bmm(w, vb).permute(1, 0, 2), torch.bmm(w, vb.abs()).permute(1, 0, 2)
         return out, lse, spread, size
 
 
@@ -485,7 +484,7 @@ def check_attention(spec, held, kind, P, H, G, D, window=0, max_new=0, seed=1, c
     assert torch.equal(torch.isinf(l), torch.isinf(rl)) and bool((l[torch.isinf(rl)] < 0).all())
     assert bool((o[torch.isinf(rl)] == 0).all())
     fine = torch.isfinite(rl)
-    most, lmost = tolerance(kind, ref, torch.where(fine, rl, 0.0), spread, size, max(lens + [1]), D, any(n * G > 128 for _, n in spec))
+    most, lmost = tolerance(kind, ref, torch.where(fine, rl, 0.0), spread, size, max(lens + [1]), D, T * H * G >= 49152 and any(n * G > 128 for _, n in spec))
     worst = ((o - ref).abs() / most).max() if o.numel() else 0
     assert float(worst) <= 1, "out %.3g times its bound" % worst
     lw = ((l - rl).abs()[fine] / lmost[fine]).max() if bool(fine.any()) else 0
@@ -529,6 +528,18 @@ def test_prompts_on_pages_of_all_sizes(held, kind, P, G, D, window):
     """Requests of more rows than a tile beside short ones, on pages smaller and larger than a step of 64 tokens."""
     check_attention([(300, 140), (320, 270), (200, 1), (131, 129), (77, 60)], held, kind, P, 2, G, D, window=window, seed=P + D)
     check_attention([(700, 260)], held, kind, P, 1, G, D, window=window, seed=P + D + 1, strided=True)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("held", [E4M3, INT8])
+@pytest.mark.parametrize("kind", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("P,H,G,D,window", [(16, 90, 1, 64, 0), (32, 2, 45, 128, 70), (64, 3, 30, 128, 0), (128, 90, 1, 48, 33), (256, 9, 10, 80, 300), (16, 30, 3, 256, 40),
+                                            (64, 2, 47, 192, 0), (256, 90, 1, 128, 0), (64, 10, 9, 64, 1)])
+def test_many_rows(held, kind, P, H, G, D, window):
+    """Calls of so many rows that the long requests get large tiles: beside short ones and one that has nothing, with rows of no request."""
+    spec = [(300, 140), (320, 270), (200, 1), (0, 0), (131, 129), (77, 60), (5, 9)]
+    check_attention(spec, held, kind, P, H, G, D, window=window, seed=P + D, pad=3)
+    check_attention([(700, 600)], held, kind, P, H, G, D, window=window, seed=P + D + 1, strided=True, max_new=600)
 
 
 @pytest.mark.gpu
@@ -618,10 +629,10 @@ def test_what_a_row_does_not_see_has_no_influence(n, window):
 @pytest.mark.gpu
 @pytest.mark.parametrize("kind", [torch.float16, torch.bfloat16])
 @pytest.mark.parametrize("P", [16, 64, 256])
-@pytest.mark.parametrize("n", [6, 150])
-def test_nan_that_is_not_seen_and_nan_that_is(kind, P, n):
+@pytest.mark.parametrize("n,G", [(6, 2), (150, 2), (150, 330)])
+def test_nan_that_is_not_seen_and_nan_that_is(kind, P, n, G):
     """The same on pages of all kinds: codes behind the last token and before the window are NaN, then one value that some rows see."""
-    H, G, D, L, window = 1, 2, 128, 330, 100
+    H, D, L, window = 1, 128, 330, 100
     pages = -(-L // P)
     cache = filled(pages + 1, H, P, D, E4M3, 4)
     order = torch.randperm(pages + 1, generator=torch.Generator().manual_seed(P))[:pages].tolist()
