@@ -527,7 +527,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void fx_kv_rows(const FxKvA
 // changes them over.  Products go first (their waves' priority): what they wait for is longer.  Where a wave's registers are more than
 // half of a SIMD's (depths above 128) there is one group, which does one after the other.
 // Measured at 4 requests of 511 to 2 047 rows behind up to 6 001 cached tokens, 32 query heads on 8, depth 128, e4m3, bf16 (0.33
-// TFLOP): 380 us, 875 TFLOP/s, of 1 430 that a large library product reaches here.  Without the second group 438 us (before the next
+// TFLOP): 380 to 384 us, 870 TFLOP/s, of 1 430 that a large library product reaches here.  Without the second group 438 us (before the next
 // two steps), with a page a lane and group of 16 tokens (below) in place of one a step 421, without the priority 397.  A step takes about
 // 2 300 clocks for either half of its work: 1 024 of the matrix cores and their operands' way from LDS (64 reads of 16 bytes a
 // lane), or 1 750 of the vector units.

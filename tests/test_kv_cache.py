@@ -543,6 +543,19 @@ def test_many_rows(held, kind, P, H, G, D, window):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("n", [64, 65, 300])
+def test_many_requests_some_of_many_rows(n):
+    """Both kernels and their parts in one call, for more requests than a wave has lanes; the same bits in every call."""
+    rng = random.Random(n)
+    spec = [(L, min(L, rng.choice([0, 1, 1, 2, 7]))) for L in (rng.choice([0, 1, 17, 90, 200]) for _ in range(n))]
+    spec[n // 3], spec[n // 2], spec[n - 1], spec[5] = (1500, 300), (2600, 1), (900, 250), (400, 150)
+    first = check_attention(spec, INT8, torch.bfloat16, 32, 4, 16, 64, seed=n)
+    for _ in range(3):
+        again = check_attention(spec, INT8, torch.bfloat16, 32, 4, 16, 64, seed=n)
+        assert torch.equal(first[0], again[0]) and torch.equal(first[1], again[1])
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("max_new", [0, 1, 3, 500])
 def test_max_new_is_a_matter_of_speed(max_new):
     """Whatever it says, every row has its result."""
