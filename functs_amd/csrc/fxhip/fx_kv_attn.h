@@ -832,7 +832,9 @@ __global__ __launch_bounds__(64 * tile_waves(DP), tile_waves(DP) / 4) void fx_kv
         }
       }
     };
-    if (!late) {
+    // (a part without steps, the same in all waves: its rows see nothing, and there may be no table to send for)
+    if (n <= 0) {
+    } else if (!late) {
       for (int s = 0; s <= n; ++s) {
         __builtin_amdgcn_s_setprio(1);
         products(s, std::false_type());

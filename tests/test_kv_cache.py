@@ -712,6 +712,24 @@ def test_rows_of_no_request():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("D,heads", [(64, 90), (128, 90), (256, 90), (64, 2)])
+def test_rows_that_have_no_tokens(kind, D, heads):
+    """Tables of no columns, tables of one behind lengths of 0, and a request of many rows without tokens beside one that has some: zeros and
+    -inf, in calls of few rows (fx_kv_rows) and of many (16-bit ones of 49 152 rows and more: fx_kv_tiles)."""
+    n = 600
+    cache = filled(4, 2, 64, D, E4M3, 1)
+    q = torch.randn(n + 5, heads, D, generator=torch.Generator().manual_seed(1)).to(kind).cuda()
+    for table, lens, starts in (([[]], [700], [0, n]), ([[], []], [700, 3], [0, n, n + 2]), ([[1]], [0], [0, n]), ([[1], [-1]], [0, 0], [0, n, n + 2])):
+        table = torch.tensor(table, dtype=torch.int32).view(len(lens), len(table[0])).cuda()
+        out, lse = torch.full_like(q, 7.0), torch.full((n + 5, heads), 5.0, device="cuda")
+        for o, l, rest in (cache.attention(q, table, i32(lens), i32(starts)) + ((0.0, -math.inf),), cache.attention(q, table, i32(lens), i32(starts), out=out, lse=lse) + ((7.0, 5.0),)):
+            assert bool((o[:starts[-1]] == 0).all()) and bool((l[:starts[-1]] == -math.inf).all())
+            assert bool((o[starts[-1]:] == rest[0]).all()) and bool((l[starts[-1]:] == rest[1]).all())
+    check_attention([(0, 300), (200, 200), (0, 200)], E4M3, kind, 64, 2, heads // 2, D)
+
+
+@pytest.mark.gpu
 def test_views_and_strides():
     """A cache that is a layer of a larger one, queries that are a part of a joined product, a table that is a part of a wider one."""
     P, H, D, N = 32, 2, 64, 10
