@@ -29,6 +29,7 @@ namespace fxkv {
 typedef const __attribute__((address_space(4))) FxKvAttnArgs KernelArgs;   // where a kernel's arguments are
 constexpr float kInf = __builtin_inff(), kLn2 = 0.693147180559945309f;
 constexpr float kTiny = 1.17549435e-38f;   // in place of scales of 0 (memory that nobody has written): -inf and 0 stay what they are under it
+constexpr float kMost = 3.402823466e38f;   // of values' scales of infinity: the weight of a token that a row does not see stays 0
 enum { kBf16 = 0, kF16 = 1, kF32 = 2 };   // types of queries and results
 
 union Frag {   // eight 16-bit numbers of an operand
@@ -368,13 +369,13 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void fx_kv_rows(const FxKvA
         for (int e = 0; e < 4; ++e) s[r * 4 + e] = t[e];
       }
       load_keys(more ? step + W : step, pk);
-      float cs = fmaxf(ks * a.scale, kTiny), vscale = fmaxf(vs, kTiny);
+      float cs = fmaxf(ks * a.scale, kTiny), vscale = __builtin_amdgcn_fmed3f(vs, kTiny, kMost);   // (NaN: kTiny)
       const bool inside = base >= span.all_low && base + FX_KV_STEP <= span.all_high && __all(ok);
       if (!inside) {
         int hi_row_ = hi_row, lo_row_ = lo_row;
         asm volatile("" : "+v"(hi_row_), "+v"(lo_row_));   // (compared here, not ahead of the branch)
         const int t0 = base + kg * 16;
-        if (!ok || span.high <= t0) cs = vscale = 1.0f;   // (what lies there may be anything)
+        if (!ok || span.high <= t0 || t0 + 16 <= span.low) cs = vscale = 1.0f;   // (what lies there may be anything)
         const int h = ok ? hi_row_ - t0 : 0, b = lo_row_ - t0;
 #pragma unroll
         for (int e = 0; e < 16; ++e) s[e] = e < h && e >= b ? s[e] : -kInf;
@@ -775,7 +776,7 @@ __global__ __launch_bounds__(64 * tile_waves(DP), tile_waves(DP) / 4) void fx_kv
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
         cs[t] = fmaxf(ks[t % kP] * a.scale, kTiny);
-        cv[t] = fmaxf(vs[t % kP], kTiny);
+        cv[t] = __builtin_amdgcn_fmed3f(vs[t % kP], kTiny, kMost);   // (NaN: kTiny)
       }
       if (round < n) write_round(round);
       __builtin_amdgcn_sched_barrier(0);   // (what is loaded later stays out of registers that are not there)
@@ -789,7 +790,7 @@ __global__ __launch_bounds__(64 * tile_waves(DP), tile_waves(DP) / 4) void fx_kv
           for (int t = 0; t < 2; ++t) {
             const int t0 = base + (t * 2 + half) * 16;
             const bool ok = (t ? p1 : p0) >= 0;
-            if (!ok || mine.high <= t0) cs[t] = cv[t] = 1.0f;   // (what lies there may be anything)
+            if (!ok || mine.high <= t0 || t0 + 16 <= mine.low) cs[t] = cv[t] = 1.0f;   // (what lies there may be anything)
             const int h = ok ? hi_row_ - t0 : 0, b = lo_row_ - t0;
 #pragma unroll
             for (int e = 0; e < 16; ++e) r[t][e] = e < h && e >= b ? r[t][e] : -kInf;

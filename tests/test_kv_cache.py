@@ -669,6 +669,36 @@ def test_nan_that_is_not_seen_and_nan_that_is(kind, P, n, G):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("held", [E4M3, INT8])
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("P", [16, 32, 64])
+@pytest.mark.parametrize("n,G", [(1, 2), (6, 2), (150, 2), (150, 330)])
+def test_scales_that_are_not_seen(held, kind, P, n, G):
+    """Scales of every kind on pages that the table names and no row sees (before the window, in its first step of 64 tokens too, and
+    behind the last token), then an infinite scale of values that the last rows see and the others do not: the same bits."""
+    D, L, window = 64, 330, 80
+    pages = -(-L // P) + 1
+    cache = filled(pages, 1, P, D, held, 4)
+    order = torch.randperm(pages, generator=torch.Generator().manual_seed(P)).tolist()
+    q = torch.randn(n, G, D, generator=torch.Generator().manual_seed(n)).to(kind).cuda()
+    args = (q, i32([order]), i32([L]), i32([0, n]), 0.125, window)
+    out, lse = cache.attention(*args)
+    hidden = [order[p] for p in range(pages) if (p + 1) * P <= L - n + 1 - window or p * P >= L]
+    assert any((p + 1) * P > (L - n + 1 - window) // 64 * 64 for p in range(pages) if order[p] in hidden and p * P < L) or P == 64
+    for value in (math.inf, -math.inf, math.nan, 3.4e38, 0.0, -1.0):
+        for scales in (cache.k_scale, cache.v_scale):
+            scales[hidden] = value
+            again, lse2 = cache.attention(*args)
+            assert torch.equal(out, again) and torch.equal(lse, lse2), value
+    last = (L - 1) // P
+    see = L - last * P                                  # rows that see some of the last page
+    if n > see:
+        cache.v_scale[order[last]] = math.inf
+        again, lse2 = cache.attention(*args)
+        assert torch.equal(out[:n - see], again[:n - see]) and torch.equal(lse[:n - see], lse2[:n - see])
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("n", [1, 70])
 def test_memory_that_nobody_has_written(n):
     """A cache of zeros, its scales too, as a warm-up may have it: results are finite, and next to nothing."""
