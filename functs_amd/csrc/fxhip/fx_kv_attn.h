@@ -29,7 +29,12 @@ namespace fxkv {
 typedef const __attribute__((address_space(4))) FxKvAttnArgs KernelArgs;   // where a kernel's arguments are
 constexpr float kInf = __builtin_inff(), kLn2 = 0.693147180559945309f;
 constexpr float kTiny = 1.17549435e-38f;   // in place of scales of 0 (memory that nobody has written): -inf and 0 stay what they are under it
+// Weights are 2^(score - m) in base 2, at most 1: m is kHead above the largest score when it is set, and raised where a score is above it
+constexpr float kHead = 8.0f;
 constexpr float kMost = 3.402823466e38f;   // of values' scales of infinity: the weight of a token that a row does not see stays 0
+// Weights have the values' scale in their exponent.  Their sum is taken from them where the scale lies in this range, so that no weight that
+// counts leaves the range of normal numbers; under other scales from exponentials of its own (weight_sum)
+constexpr float kFoldLeast = 0x1p-64f, kFoldMost = 0x1p64f;
 enum { kBf16 = 0, kF16 = 1, kF32 = 2 };   // types of queries and results
 
 union Frag {   // eight 16-bit numbers of an operand
@@ -251,6 +256,16 @@ __device__ __forceinline__ void fill_rest(const FxKvAttnArgs& a) {
   }
 }
 
+// The sum of a lane's 16 weights without the values' scale
+template <class Scores>
+__device__ __forceinline__ float weight_sum(const Scores& s, float cs, float sub) {
+  float sum = 0.0f;
+#pragma unroll
+  for (int e = 0; e < 16; ++e) sum += __builtin_amdgcn_exp2f(__builtin_fmaf(s[e], cs, -sub));
+  return sum;
+}
+__device__ __forceinline__ bool folds(float scale) { return scale >= kFoldLeast && scale <= kFoldMost; }
+
 // the larger one; a NaN loses (fmaxf does the same and quiets what the matrix cores give it, an instruction for each)
 __device__ __forceinline__ float larger(float a, float b) { return __builtin_amdgcn_fmed3f(a, b, __builtin_inff()); }
 
@@ -395,15 +410,15 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void fx_kv_rows(const FxKvA
           nans = nans || __any(any != 0);
         }
       }
-      // running maximum: raised only where a score is 8 or more above it (weights stay below 2^8)
+      // running maximum: see kHead
       float top = larger(s[0], s[1]);
 #pragma unroll
       for (int e = 2; e < 16; ++e) top = larger(top, s[e]);
       top *= cs;
-      if (__any(top > m + 8.0f || (m == -kInf && top > -kInf))) {
+      if (__any(top > m)) {
         top = fmaxf(top, __shfl_xor(top, 16, 64));
         top = fmaxf(top, __shfl_xor(top, 32, 64));
-        const float now = fmaxf(m, top);
+        const float now = fmaxf(m, top + kHead);
         const float by = now == -kInf ? 1.0f : __builtin_amdgcn_exp2f(m - now);
         m = now;
         l *= by;
@@ -413,7 +428,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void fx_kv_rows(const FxKvA
           for (int e = 0; e < 4; ++e) acc[d][e] *= by;
       }
       const float sub = m == -kInf ? 0.0f : m;
-      // weights times the values' scale, a power of two: part of the exponent, and taken out of their sum again
+      // weights times the values' scale, a power of two: part of the exponent (see kFoldLeast), and taken out of their sum again
       Frag p[2][NP];
       float w[16], sum[2] = {0.0f, 0.0f};
       const float off = __builtin_amdgcn_logf(vscale) - sub;
@@ -422,7 +437,9 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void fx_kv_rows(const FxKvA
         w[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e], cs, off));
         sum[e & 1] += w[e];
       }
-      l = __builtin_fmaf(sum[0] + sum[1], __builtin_amdgcn_rcpf(vscale), l);
+      float add = (sum[0] + sum[1]) * __builtin_amdgcn_rcpf(vscale);
+      if (!__all(folds(vscale))) add = weight_sum(s, cs, sub);
+      l += add;
       split8<NP>(p[0], w);
       split8<NP>(p[1], w + 8);
 #pragma unroll
@@ -805,9 +822,9 @@ __global__ __launch_bounds__(64 * tile_waves(DP), tile_waves(DP) / 4) void fx_kv
           top[t] *= cs[t];
         }
         float up = fmaxf(top[0], top[1]);
-        if (__any(up > m + 8.0f || (m == -kInf && up > -kInf))) {
+        if (__any(up > m)) {
           up = fmaxf(up, __shfl_xor(up, 32, 64));
-          const float to_m = fmaxf(m, up);
+          const float to_m = fmaxf(m, up + kHead);
           const float by = to_m == -kInf ? 1.0f : __builtin_amdgcn_exp2f(m - to_m);
           m = to_m;
           l *= by;
@@ -817,7 +834,8 @@ __global__ __launch_bounds__(64 * tile_waves(DP), tile_waves(DP) / 4) void fx_kv
             for (int e = 0; e < 16; ++e) acc[d][e] *= by;
         }
         const float sub = m == -kInf ? 0.0f : m;
-        // weights times the values' scale, a power of two: part of the exponent, and taken out of their sum again
+        float add = 0.0f;
+        // weights times the values' scale, a power of two: part of the exponent (see kFoldLeast), and taken out of their sum again
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
           const float off = __builtin_amdgcn_logf(cv[t]) - sub;
@@ -827,10 +845,12 @@ __global__ __launch_bounds__(64 * tile_waves(DP), tile_waves(DP) / 4) void fx_kv
             w[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(r[t][e], cs[t], off));
             sum[e & 1] += w[e];
           }
-          l = __builtin_fmaf(sum[0] + sum[1], __builtin_amdgcn_rcpf(cv[t]), l);
+          add = __builtin_fmaf(sum[0] + sum[1], __builtin_amdgcn_rcpf(cv[t]), add);
           split8<NP>(p[t][0], w);
           split8<NP>(p[t][1], w + 8);
         }
+        if (!__all(folds(cv[0]) && folds(cv[1]))) add = weight_sum(r[0], cs[0], sub) + weight_sum(r[1], cs[1], sub);
+        l += add;
       }
     };
     // (a part without steps, the same in all waves: its rows see nothing, and there may be no table to send for)

@@ -584,8 +584,9 @@ int fx_kv_read(const fx_kv_cache* cache, const fx_kv_rows* rows, void* stream);
  * q [tokens][q_heads][depth], a depth contiguous; out [tokens][q_heads][depth] and lse [tokens][q_heads] contiguous.  Rows of no
  * request are left as they were, or get zeros and -infinity (clear_rest).  max_new: how many rows the longest request
  * has, at most, as far as the caller knows (0: unknown); it decides on forms, and so at most on how results are
- * rounded.  scale: 2^-26 to 32.  out does not overlap q.  Sums are fp32, and a token's weight in them is up to 2^8 before they are
- * divided: values of more than 2^120 / lens[b] in magnitude may become infinite.
+ * rounded.  scale: 2^-26 to 32.  out does not overlap q.  Sums are fp32, and a token's weight in them is 1 at most, and of the largest
+ * score 2^-8 at least, before they are divided: values of more than 2^127 / lens[b] in magnitude may become infinite, and a weight times a
+ * page's scale of values below 2^-126 adds nothing to out (to lse it does).
  * workspace: fx_kv_attention_workspace_bytes() of device memory for each call under way, 256-byte aligned; nothing is expected in it. */
 typedef struct fx_kv_attention_desc {
   const void* q;

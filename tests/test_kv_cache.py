@@ -850,6 +850,61 @@ def test_the_smallest_and_largest_scales(held, top, n):
         assert bool(((out.cpu().double() - ref).abs() <= bound).all()) and bool(((lse.cpu().double() - rl).abs() <= lbound).all())
 
 
+# n rows and query heads of a key head: one row, a few tiles of fx_kv_rows, and 49 152 rows and more (fx_kv_tiles, 16-bit queries)
+ROWS = [(1, 2), (140, 2), (150, 330)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("held", [E4M3, INT8])
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("n,G", ROWS)
+def test_small_weights_count_whatever_their_values_scale(held, kind, n, G):
+    """One token whose score is 18.375 above the 5 999 others (2^-26.5 of its weight each, 1.1e-4 together of those that pages of zeros hold),
+    whose pages hold zeros under scales from 0 to the largest.  Queries and keys have one column and a score is a product of two numbers of
+    few bits: 6 roundings of it (scale, log2(e) twice, the sum with the maximum, the way back by ln(2)), then sums as in tolerance()."""
+    L, P, D, scale = 6000, 64, 64, 147 / 64
+    for vs in (2.0 ** -100, 0.0, 2.0 ** -64, 1.0, 2.0 ** 64, 2.0 ** 100, 2.0 ** (119 if held == E4M3 else 121)):
+        c = filled(-(-L // P), 1, P, D, held, 5)
+        c.k.view(torch.uint8).zero_(), c.k_scale.fill_(1.0)
+        c.k.view(torch.uint8)[0, 0, 3, 0] = torch.tensor([8.0]).to(held).view(torch.uint8).item()
+        c.v.view(torch.uint8)[1:].zero_(), c.v_scale[1:].fill_(vs)
+        q = torch.zeros(n, 1, D)
+        q[:, :, 0] = 1.0
+        table, lens, starts = [list(range(c.k.size(0)))], [L], [0, n]
+        out, lse = c.attention(q.expand(n, G, D).to(kind).cuda(), i32(table), i32(lens), i32(starts), scale)
+        ref, rl, spread, size = PlainCache(c).attention(q, table, lens, starts, scale, 0)
+        bound, _ = tolerance(kind, ref, rl, spread, size, L, D, n * G >= 49152)
+        e = 2.0 ** -24
+        assert bool(((out.cpu().double() - ref).abs() <= bound).all()), vs
+        assert float((lse.cpu().double() - rl).abs().max()) <= 6 * e * 18.375 + 2.0 ** -22 + (L / 32 + 40) * e, vs
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("held", [E4M3, INT8])
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("n,G", ROWS)
+def test_the_smallest_and_largest_scales_of_values(held, kind, n, G):
+    """Pages under the ends of the range, alone and beside each other.  At the upper end codes are 0, 1 and -1, as values of more than 2^127
+    over the number of tokens may become infinite; what a token adds below 2^-126 may be lost, of sums whose weights are 2^-8 at least."""
+    L, P, D = 200, 64, 64
+    top = 119 if held == E4M3 else 121
+    small = kind == torch.float16                      # (its largest number is 65504)
+    for exps, most in (((-100,) * 4, 448), ((-100, -64, -10, -65), 448), ((top,) * 4, 0)) + (() if small else (((119,) * 4, 1), ((-100, 64, 0, 90), 448), ((65, -63, 100, 119), 1))):
+        c = filled(6, 1, P, D, held, 3)
+        codes = c.v.float()
+        c.v.copy_((codes.clamp(-most, most) if most != 1 else codes.sign() * (codes.abs() > 20)).to(held))
+        table, lens, starts = [[4, 1, 2, 0]], [L], [0, n]
+        for page, x in zip(table[0], exps):
+            c.v_scale[page] = 2.0 ** x
+        q = torch.randn(n, 1, D, generator=torch.Generator().manual_seed(n)).to(kind)
+        out, lse = c.attention(q.expand(n, G, D).cuda(), i32(table), i32(lens), i32(starts))
+        ref, rl, spread, size = PlainCache(c).attention(q, table, lens, starts, D ** -0.5, 0)
+        bound, lbound = tolerance(kind, ref, rl, spread, size, L, D, n * G >= 49152)
+        bound = bound + L * 448 * 2.0 ** -126 * 2.0 ** 8
+        assert bool(((out.cpu().double() - ref).abs() <= bound).all()), exps
+        assert bool(((lse.cpu().double() - rl).abs() <= lbound).all()), exps
+
+
 # ---- GPU: together ----
 
 def serve(steps, cache, table, free, tokens, seed, layers=1):
