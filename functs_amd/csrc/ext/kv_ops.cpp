@@ -56,6 +56,8 @@ int dtypeOf(const char* op, at::ScalarType t, const char* name) {
 
 // [pages, heads, page, depth] codes; a page's codes lie side by side, pages anywhere
 fx_kv_cache cacheOf(const char* op, const Tensor& k, const Tensor& v, const Tensor& ks, const Tensor& vs) {
+  TORCH_CHECK(k.dim() == 4, op, ": k_cache must be [pages, heads, page, depth], got ", k.sizes());
+  TORCH_CHECK(k.size(0) >= 1 && k.size(1) >= 1, op, ": a cache has at least one page and one head, got ", k.sizes());
   TORCH_CHECK(k.is_cuda(), op, " runs on the GPU only; k_cache is a ", k.device(), " tensor");
   const auto dev = k.device();
   onGpu(op, v, "v_cache", dev);
@@ -64,7 +66,6 @@ fx_kv_cache cacheOf(const char* op, const Tensor& k, const Tensor& v, const Tens
   noGrad(op, ks, "k_scale");
   noGrad(op, vs, "v_scale");
   TORCH_CHECK(k.scalar_type() == at::kFloat8_e4m3fn || k.scalar_type() == at::kChar, op, ": a cache holds float8_e4m3fn or int8, got ", k.scalar_type());
-  TORCH_CHECK(k.dim() == 4, op, ": k_cache must be [pages, heads, page, depth], got ", k.sizes());
   const int64_t N = k.size(0), H = k.size(1), P = k.size(2), D = k.size(3);
   TORCH_CHECK(v.scalar_type() == k.scalar_type() && v.dim() == 5 && v.size(0) == N && v.size(1) == H && v.size(2) * 16 == P && v.size(3) == D && v.size(4) == 16,
               op, ": v_cache must be [pages, heads, page / 16, depth, 16] of the type of k_cache, got ", v.scalar_type(), " ", v.sizes(), " beside ", k.sizes());

@@ -231,6 +231,27 @@ def test_tensors_on_the_host_are_refused():
             call()
 
 
+def refuse_empty_caches(dev):
+    c = KvCache.empty(2, 2, 16, 64, device=dev)
+    q, slots = torch.zeros(3, 4, 64, device=dev), torch.zeros(3, dtype=torch.long, device=dev)
+    for part in ((slice(None), slice(0, 0)), (slice(0, 0),), (slice(0, 0), slice(0, 0))):
+        x = KvCache(c.k[part], c.v[part], c.k_scale[part], c.v_scale[part])
+        k = q[:, :x.k.size(1)]
+        for call in (lambda: x.attention(q, i32([[0]], dev), i32([1], dev), i32([0, 3], dev)), lambda: x.attention(q[:0], i32([[0]], dev), i32([1], dev), i32([0, 0], dev)),
+                     lambda: x.store(k, k, slots), lambda: x.read(slots)):
+            with pytest.raises(RuntimeError, match="at least one page and one head"):
+                call()
+
+
+def test_caches_of_no_heads_or_pages_are_refused():
+    refuse_empty_caches("cpu")
+
+
+@pytest.mark.gpu
+def test_caches_of_no_heads_or_pages_are_refused_on_the_gpu():
+    refuse_empty_caches("cuda")
+
+
 class Cache(ctypes.Structure):
     _fields_ = [(n, ctypes.c_void_p) for n in ("k", "v", "k_scale", "v_scale")] + [(n, ctypes.c_int64) for n in ("ks", "vs", "kss", "vss")] + \
                [(n, ctypes.c_int32) for n in ("pages", "heads", "page_size", "depth", "held", "reserved")]
