@@ -38,6 +38,7 @@ void onGpu(const char* op, const Tensor& t, const char* name, c10::Device dev) {
 }
 void noGrad(const char* op, const Tensor& t, const char* name) {
   TORCH_CHECK(!(at::GradMode::is_enabled() && t.requires_grad()), op, " has no backward pass: ", name, " requires a gradient");
+  TORCH_CHECK(!t._fw_grad(0).defined(), op, " has no derivative: ", name, " carries a tangent");
 }
 int32_t sized(const char* op, int64_t n, const char* name) {
   TORCH_CHECK(n >= 0 && n <= INT32_MAX, op, ": ", name, " is out of range (", n, ")");
@@ -63,6 +64,8 @@ fx_kv_cache cacheOf(const char* op, const Tensor& k, const Tensor& v, const Tens
   onGpu(op, v, "v_cache", dev);
   onGpu(op, ks, "k_scale", dev);
   onGpu(op, vs, "v_scale", dev);
+  noGrad(op, k, "k_cache");
+  noGrad(op, v, "v_cache");
   noGrad(op, ks, "k_scale");
   noGrad(op, vs, "v_scale");
   TORCH_CHECK(k.scalar_type() == at::kFloat8_e4m3fn || k.scalar_type() == at::kChar, op, ": a cache holds float8_e4m3fn or int8, got ", k.scalar_type());

@@ -856,6 +856,38 @@ def test_more_refusals():
 
 
 @pytest.mark.gpu
+def test_derivatives_are_refused():
+    """Tangents of forward-mode differentiation on any operand, and codes that require a gradient."""
+    c = filled(4, 2, 16, 64, E4M3, 1)
+    table, lens, starts, slots = i32([[0, 1]]), i32([20]), i32([0, 2]), torch.tensor([3, 4]).cuda()
+    q, k, lse = torch.zeros(2, 4, 64, device="cuda"), torch.zeros(2, 2, 64, device="cuda"), torch.zeros(2, 4, device="cuda")
+
+    def refused(word, caches, store=(), attention=()):
+        for x in caches:
+            for call in (lambda: x.store(k, k, slots), lambda: x.read(slots), lambda: x.attention(q, table, lens, starts)):
+                with pytest.raises(RuntimeError, match=word):
+                    call()
+        for a in store:
+            with pytest.raises(RuntimeError, match=word):
+                c.store(*a, slots)
+        for a, kw in attention:
+            with pytest.raises(RuntimeError, match=word):
+                c.attention(a, table, lens, starts, **kw)
+
+    with torch.autograd.forward_ad.dual_level():
+        dual = lambda t: torch.autograd.forward_ad.make_dual(t.clone(), torch.ones_like(t))  # noqa: E731
+        refused("carries a tangent", (KvCache(c.k, c.v, dual(c.k_scale), c.v_scale), KvCache(c.k, c.v, c.k_scale, dual(c.v_scale))), ((dual(k), k), (k, dual(k))),
+                ((dual(q), {}), (q, dict(out=dual(q), lse=lse)), (q, dict(out=q.clone(), lse=dual(lse)))))
+        with torch.no_grad():
+            refused("carries a tangent", (), ((dual(k), k),), ((dual(q), {}),))
+    grown = lambda t: t.clone().requires_grad_()  # noqa: E731
+    caches = (KvCache(grown(c.k), c.v, c.k_scale, c.v_scale), KvCache(c.k, grown(c.v), c.k_scale, c.v_scale))
+    refused("requires a gradient", caches)
+    with torch.no_grad():
+        caches[0].read(slots), caches[1].attention(q, table, lens, starts)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("held,top", [(E4M3, 119), (INT8, 121)])
 @pytest.mark.parametrize("n", [1, 140])
 def test_the_smallest_and_largest_scales(held, top, n):
