@@ -1823,8 +1823,9 @@ int fx_kv_attention(const fx_kv_cache* cache, const fx_kv_attention_desc* desc, 
   const int64_t q_size = d.dtype == FX_DT_F32 ? 4 : 2;
   a.q_vec = ((uintptr_t)d.q & 15u) == 0 && d.q_token_stride * q_size % 16 == 0 && d.q_head_stride * q_size % 16 == 0;
   kv_workspace(a, l, c.depth, d.requests, (char*)d.workspace);
-  HIP_OK(fx_launch_kv_attention(a, l, (hipStream_t)stream));
-  return kv_launched((l.rows_grid > 0) + (l.tiles_grid > 0) + (l.shared ? 1 : 0));   // (fx_kv_offsets aside)
+  int launched = 0;
+  HIP_OK(fx_launch_kv_attention(a, l, (hipStream_t)stream, &launched));
+  return kv_launched(launched);
 }
 
 // ---- detection tail (fx_nms.hip) ----

@@ -79,4 +79,4 @@ struct FxKvLaunch {
   int64_t rows_grid, tiles_grid;    // workgroups of fx_kv_rows and fx_kv_tiles (0: not needed)
   FxKvParts rows_parts, tiles_parts;
 };
-hipError_t fx_launch_kv_attention(const FxKvAttnArgs& a, const FxKvLaunch& l, hipStream_t stream);
+hipError_t fx_launch_kv_attention(const FxKvAttnArgs& a, const FxKvLaunch& l, hipStream_t stream, int* launched);   // launched: how many kernels

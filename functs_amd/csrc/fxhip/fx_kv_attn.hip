@@ -65,26 +65,26 @@ __global__ __launch_bounds__(1024) void fx_kv_offsets(const FxKvAttnArgs a, int 
 
 namespace {
 template <class... A>
-hipError_t launch(const void* kernel, int64_t grid, int threads, hipStream_t stream, A... args) {
+hipError_t launch(int* launched, const void* kernel, int64_t grid, int threads, hipStream_t stream, A... args) {
   void* kargs[sizeof...(A)] = {(void*)&args...};
-  return hipLaunchKernel(kernel, dim3((unsigned)grid), dim3((unsigned)threads), kargs, 0, stream);
+  const hipError_t e = hipLaunchKernel(kernel, dim3((unsigned)grid), dim3((unsigned)threads), kargs, 0, stream);
+  *launched += e == hipSuccess;
+  return e;
 }
-hipError_t offsets(const FxKvAttnArgs& a, int tile_rows, int least, hipStream_t stream) {
+hipError_t offsets(int* launched, const FxKvAttnArgs& a, int tile_rows, int least, hipStream_t stream) {
   if (a.requests <= fxkv::kScanned) return hipSuccess;
-  FxKvAttnArgs args = a;
-  void* kargs[3] = {(void*)&args, (void*)&tile_rows, (void*)&least};
-  return hipLaunchKernel((const void*)fxkv::fx_kv_offsets, dim3(1), dim3(1024), kargs, 0, stream);
+  return launch(launched, (const void*)fxkv::fx_kv_offsets, 1, 1024, stream, a, tile_rows, least);
 }
-hipError_t join(const FxKvAttnArgs& a, const FxKvLaunch& l, hipStream_t stream) {
+hipError_t join(int* launched, const FxKvAttnArgs& a, const FxKvLaunch& l, hipStream_t stream) {
   const int type = l.type;
   const void* kernel = type == fxkv::kBf16 ? (const void*)fxkv::fx_kv_join<__bf16>
                        : type == fxkv::kF16 ? (const void*)fxkv::fx_kv_join<_Float16>
                                             : (const void*)fxkv::fx_kv_join<float>;
-  return launch(kernel, 2048, 256, stream, a, l.tiles_parts, l.rows_parts);
+  return launch(launched, kernel, 2048, 256, stream, a, l.tiles_parts, l.rows_parts);
 }
 }  // namespace
 
-hipError_t fx_launch_kv_attention(const FxKvAttnArgs& a, const FxKvLaunch& l, hipStream_t stream) {
+hipError_t fx_launch_kv_attention(const FxKvAttnArgs& a, const FxKvLaunch& l, hipStream_t stream, int* launched) {
   const bool wide = (1 << a.c.log_page) >= FX_KV_STEP;
   const fxkv::Kernels k = l.held == 0 ? fx_kv_kernels_e4m3(l.type, a.c.depth, wide) : fx_kv_kernels_int8(l.type, a.c.depth, wide);
   hipError_t e = hipSuccess;
@@ -93,16 +93,16 @@ hipError_t fx_launch_kv_attention(const FxKvAttnArgs& a, const FxKvLaunch& l, hi
     args.rows_above = l.rows_grid > 0 ? FX_KV_FEW : 0;
     args.rows_upto = int64_t{1} << 31;
     args.parts = l.tiles_parts;
-    if ((e = offsets(args, l.tiles_parts.tile_rows, fxkv::kTileLeast, stream)) != hipSuccess) return e;
-    if ((e = launch(k.tiles, l.tiles_grid, 2 * l.tiles_parts.tile_rows, stream, args)) != hipSuccess) return e;
+    if ((e = offsets(launched, args, l.tiles_parts.tile_rows, fxkv::kTileLeast, stream)) != hipSuccess) return e;
+    if ((e = launch(launched, k.tiles, l.tiles_grid, 2 * l.tiles_parts.tile_rows, stream, args)) != hipSuccess) return e;
     args.fill = 0;
   }
   if (l.rows_grid > 0) {
     args.rows_above = 0;
     args.rows_upto = l.tiles_grid > 0 ? FX_KV_FEW : int64_t{1} << 31;
     args.parts = l.rows_parts;
-    if ((e = offsets(args, FX_KV_ROWS, fxkv::kRowLeast, stream)) != hipSuccess) return e;
-    if ((e = launch(k.rows, l.rows_grid, 256, stream, args)) != hipSuccess) return e;
+    if ((e = offsets(launched, args, FX_KV_ROWS, fxkv::kRowLeast, stream)) != hipSuccess) return e;
+    if ((e = launch(launched, k.rows, l.rows_grid, 256, stream, args)) != hipSuccess) return e;
   }
-  return l.shared ? join(args, l, stream) : e;
+  return l.shared ? join(launched, args, l, stream) : e;
 }

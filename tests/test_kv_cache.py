@@ -577,6 +577,22 @@ def test_many_requests_some_of_many_rows(n):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("kind,heads,requests_,columns,launches", [(torch.float32, 2, 64, 5, 2), (torch.float32, 2, 65, 5, 3), (torch.float32, 2, 65, 4, 2),
+                                                                   (torch.bfloat16, 90, 64, 5, 3), (torch.bfloat16, 90, 65, 5, 5), (torch.bfloat16, 90, 1, 5, 2)])
+def test_every_launch_is_counted(kind, heads, requests_, columns, launches):
+    """fx_kv_rows, fx_kv_tiles beside it (16-bit calls of 49 152 rows and more of several requests), fx_kv_offsets ahead of either for more
+    than 64 requests, fx_kv_join where a table holds more than 256 tokens."""
+    c = filled(2, 2, 64, 64, E4M3, 1)
+    starts = [0] + [600] * requests_
+    q, table = torch.zeros(600, heads, 64, dtype=kind, device="cuda"), torch.zeros(requests_, columns, dtype=torch.int32, device="cuda")
+    counts = [ctypes.c_uint64(), ctypes.c_uint64()]
+    lib.fx_launch_stats(ctypes.byref(counts[0]), None)
+    c.attention(q, table, i32([columns * 64] * requests_), i32(starts))
+    lib.fx_launch_stats(ctypes.byref(counts[1]), None)
+    assert counts[1].value - counts[0].value == launches
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("max_new", [0, 1, 3, 500])
 def test_max_new_is_a_matter_of_speed(max_new):
     """Whatever it says, every row has its result."""
