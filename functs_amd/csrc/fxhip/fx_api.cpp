@@ -1675,7 +1675,9 @@ int kv_rows_of(const char* at, const FxKvCache& c, const fx_kv_rows* r, FxKvRows
   if (!kv_dtype(r->dtype)) return fail(FX_E_UNSUPPORTED, op + ": rows must be float32, float16 or bfloat16");
   if (r->tokens < 0) return fail(FX_E_INVALID, op + ": negative size");
   if (r->tokens > 0 && (!r->k || !r->v || !r->slots)) return fail(FX_E_INVALID, op + ": null argument");
-  if (r->tokens >= 1 << 30 || (int64_t)r->tokens * c.heads >= int64_t{1} << 32) return fail(FX_E_LIMIT, op + ": more rows than a launch holds");
+  // (a launch has fewer than 2^32 threads; the most are those of fx_kv_store, 512 for the tokens of a workgroup and a head)
+  if (r->tokens >= 1 << 30 || ((int64_t)r->tokens + FX_KV_STORE_MOST - 1) / FX_KV_STORE_MOST * c.heads >= int64_t{1} << 23)
+    return fail(FX_E_LIMIT, op + ": more rows than a launch holds (about 2^29 of all heads)");
   out = FxKvRows{r->k, r->v, r->k_token_stride, r->k_head_stride, r->v_token_stride, r->v_head_stride, r->slots, r->tokens, r->dtype};
   return FX_OK;
 }

@@ -33,6 +33,7 @@ struct FxKvRows {
   int32_t tokens, dtype;
 };
 
+#define FX_KV_STORE_MOST 63   // tokens that a workgroup of fx_kv_store takes at most: a lane each, and one for the token before them
 hipError_t fx_launch_kv_plan(const FxKvPlanArgs& a, hipStream_t stream);
 hipError_t fx_launch_kv_store(const FxKvCache& c, const FxKvRows& r, int held, hipStream_t stream);
 hipError_t fx_launch_kv_read(const FxKvCache& c, const FxKvRows& r, int held, hipStream_t stream);

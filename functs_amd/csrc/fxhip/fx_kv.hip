@@ -691,8 +691,8 @@ hipError_t fx_launch_kv_store(const FxKvCache& c, const FxKvRows& r, int held, h
       {(const void*)fx_kv_store_kernel<0, float>, (const void*)fx_kv_store_kernel<0, _Float16>, (const void*)fx_kv_store_kernel<0, __bf16>},
       {(const void*)fx_kv_store_kernel<1, float>, (const void*)fx_kv_store_kernel<1, _Float16>, (const void*)fx_kv_store_kernel<1, __bf16>}};
   const size_t size = r.dtype == FX_DT_F32 ? 4 : 2;
-  // (63: a lane each, and one for the token before them.  A workgroup for each 32 tokens took 96 us where 63 take 73)
-  int per = std::max(std::min(tokens_a_wave(c, r, 63) * kStoreWaves, 63), kStoreWaves);
+  // (a workgroup for each 32 tokens took 96 us where 63 take 73)
+  int per = std::max(std::min(tokens_a_wave(c, r, FX_KV_STORE_MOST) * kStoreWaves, FX_KV_STORE_MOST), kStoreWaves);
   int vec = aligned16(r.k, r.k_token, r.k_head, size) && aligned16(r.v, r.v_token, r.v_head, size);
   FxKvCache cache = c;
   FxKvRows rows = r;

@@ -571,7 +571,8 @@ typedef struct fx_kv_rows {
 /* Neighbours in `slots` that lie in one page are written together.  Where the first of them is the first of its page, the page
  * starts anew: its scale is that of these rows.  Otherwise the page keeps its scale or takes the larger one of these rows, and its
  * tokens before the first of them are rounded again to it; those behind are left as they were.  The rows of one page must be neighbours
- * (as fx_kv_plan lays them): two groups of rows for one page leave what either wrote.  Slots outside the cache are passed over. */
+ * (as fx_kv_plan lays them): two groups of rows for one page leave what either wrote.  Slots outside the cache are passed over.
+ * A call has fewer than 63 * 2^23 rows of all heads, fx_kv_read too. */
 int fx_kv_store(const fx_kv_cache* cache, const fx_kv_rows* rows, void* stream);
 /* The numbers at `slots`, in any order, rounded once to dtype; zeros for slots outside the cache. */
 int fx_kv_read(const fx_kv_cache* cache, const fx_kv_rows* rows, void* stream);

@@ -306,6 +306,17 @@ def test_the_c_abi_refuses_before_it_launches():
     assert lib.fx_kv_attention(ctypes.byref(Cache(**ok)), ctypes.byref(Attention(**{**att, "tokens": 0})), None) == 0
 
 
+@pytest.mark.parametrize("heads,tokens", [(2, 1 << 28), (64, 63 << 17), (65536, 63 << 7), (1, 63 << 23)])
+def test_more_rows_than_a_launch_holds_are_refused(heads, tokens):
+    """A launch has fewer than 2^32 threads: 512 for the 63 tokens of a workgroup and each head (addresses here are never read)."""
+    at = 4096
+    c = Cache(k=at, v=at, k_scale=at, v_scale=at, ks=heads * 256, vs=heads * 256, kss=heads, vss=heads, pages=2, heads=heads, page_size=16, depth=16, held=0)
+    rows = Rows(k=at, v=at, kt=heads * 16, kh=16, vt=heads * 16, vh=16, slots=at, tokens=tokens, dtype=C["FX_DT_BF16"])
+    assert -(-tokens // 63) * heads * 512 >= 2 ** 32
+    for call in (lib.fx_kv_store, lib.fx_kv_read):
+        assert call(ctypes.byref(c), ctypes.byref(rows), None) == C["FX_E_LIMIT"]
+
+
 def test_mutated_arguments_are_in_the_schemas():
     for name, written in (("kv_plan", {"block_table"}), ("kv_store", {"k_cache", "v_cache", "k_scale", "v_scale"}), ("kv_read", set()), ("kv_attention", set())):
         schema = getattr(torch.ops.functs, name).default._schema
