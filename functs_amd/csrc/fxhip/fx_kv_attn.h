@@ -120,10 +120,10 @@ __device__ __forceinline__ int64_t wave_total(int64_t v) {
   const bool endless = v >= int64_t{1} << 43;
   const int low = sum_upto((int)(v & 0xfffff)), high = sum_upto(endless ? 0 : (int)(v >> 20));
   const int64_t all = ((int64_t)__builtin_amdgcn_readlane(high, 63) << 20) + __builtin_amdgcn_readlane(low, 63);
-  return __any(endless) ? int64_t{1} << 60 : all;
+  return __any(endless) ? FX_KV_ENDLESS : all;
 }
 __device__ __forceinline__ int64_t all_steps(const FxKvAttnArgs& a, int64_t steps) {   // of all heads
-  return steps >= int64_t{1} << 60 ? steps : steps * a.c.heads;
+  return steps >= FX_KV_ENDLESS ? steps : steps * a.c.heads;
 }
 
 // Unit u of the call, or false behind the last one: every wave finds it by itself, in scalar registers, without a barrier.  Up
@@ -142,8 +142,9 @@ __device__ __forceinline__ bool unit_at(const FxKvAttnArgs& a, int tile_rows, in
   if (a.requests <= kScanned) {
     // (all three loads at once, whatever the lane)
     const int c = max(min(lane, a.requests - 1), 0), start = a.starts[c], end = a.starts[c + (a.requests > 0 ? 1 : 0)], len = a.requests > 0 ? a.lens[c] : 0;
-    const FxKvRequest r = request_of(a, start, lane < a.requests ? end : start, len, tile_rows);
-    chunk = fx_kv_chunk(all_steps(a, wave_total((int64_t)r.tiles * r.steps)), least);
+    const int behind = lane < a.requests ? end : start;
+    const FxKvRequest r = request_of(a, start, behind, len, tile_rows);
+    chunk = fx_kv_chunk(all_steps(a, wave_total(fx_kv_work(start, behind, r))), least);
     const int splits = fx_kv_parts(r.steps, chunk), items = r.tiles * a.c.heads, mine = items * splits, cut = splits > 1 ? (items << 16) + mine : 0;
     const int cuts = sum_upto(cut);
     int before = 0;
@@ -172,7 +173,7 @@ __device__ __forceinline__ bool unit_at(const FxKvAttnArgs& a, int tile_rows, in
     chunk = a.offsets[0];
     *shared_items = a.offsets[1];
     int lo = 0, hi = a.requests;
-    if (u >= units[hi]) return false;
+    if (u < 0 || u >= units[hi]) return false;
     while (hi - lo > 1) {
       const int step = (hi - lo + 63) >> 6, at = min(lo + lane * step, hi);
       const int last = 63 - __builtin_clzll(__ballot(at < hi && units[at] <= u));   // (lane 0 always)
@@ -189,10 +190,10 @@ __device__ __forceinline__ bool unit_at(const FxKvAttnArgs& a, int tile_rows, in
   x.request = scalar(x.request), rest = scalar(rest), parts = scalar(parts), chunk = scalar(chunk);
   x.r = FxKvRequest{scalar(x.r.start), scalar(x.r.rows), scalar(x.r.len), scalar(x.r.tiles), scalar(x.r.steps)};
   x.splits = scalar(fx_kv_parts(x.r.steps, chunk));
-  const int item = scalar(rest / x.splits);
+  int item;
+  if (!fx_kv_item(x.r, a.c.heads, x.splits, rest, &item, &x.tile, &x.head)) return false;
+  item = scalar(item), x.tile = scalar(x.tile), x.head = scalar(x.head);
   x.split = rest - item * x.splits;
-  x.tile = scalar(item / a.c.heads);
-  x.head = item - x.tile * a.c.heads;
   x.part = (parts & 0xffff) + item * x.splits;
   x.item = (int)((unsigned)parts >> 16) + item;
   return true;

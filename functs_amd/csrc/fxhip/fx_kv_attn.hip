@@ -11,7 +11,7 @@ __global__ __launch_bounds__(1024) void fx_kv_offsets(const FxKvAttnArgs a, int 
   int64_t work = 0;
   for (int b = (int)threadIdx.x; b < a.requests; b += 1024) {
     const FxKvRequest r = request_of(a, a.starts[b], a.starts[b + 1], a.lens[b], tile_rows);
-    work += (int64_t)r.tiles * r.steps;
+    work = min(work + fx_kv_work(a.starts[b], a.starts[b + 1], r), FX_KV_ENDLESS);
   }
   work = wave_total(work);
   if (lane == 0) s_work[wave] = work;
@@ -19,10 +19,10 @@ __global__ __launch_bounds__(1024) void fx_kv_offsets(const FxKvAttnArgs a, int 
   work = 0;
   bool endless = false;
   for (int w = 0; w < W; ++w) {
-    endless |= s_work[w] >= int64_t{1} << 60;
+    endless |= s_work[w] >= FX_KV_ENDLESS;
     work += s_work[w];
   }
-  const int chunk = fx_kv_chunk(all_steps(a, endless ? int64_t{1} << 60 : work), least);
+  const int chunk = fx_kv_chunk(all_steps(a, endless ? FX_KV_ENDLESS : work), least);
   int32_t* units_to = a.offsets + 2;
   int units = 0, cuts = 0;   // of the rounds before
   for (int b0 = 0; b0 < a.requests; b0 += 1024) {

@@ -35,12 +35,24 @@ FX_KV_HD FxKvRequest fx_kv_request(int start, int end, int len, int tokens, int 
   r.steps = (r.len + FX_KV_STEP - 1) / FX_KV_STEP - low / FX_KV_STEP;
   return r;
 }
+// Steps of a request's tiles, of one head, for the sum of a call.  Offsets that fall (there are none in a call that is meant) let requests
+// overlap, whose units may be more than 31 bits count: the work is endless then, so that nothing is cut and no part lies outside the workspace
+#define FX_KV_ENDLESS (int64_t{1} << 60)
+FX_KV_HD int64_t fx_kv_work(int start, int end, const FxKvRequest& r) { return start > end ? FX_KV_ENDLESS : (int64_t)r.tiles * r.steps; }
 // steps of a chunk, of `work` steps in all: a multiple of `least`
 FX_KV_HD int fx_kv_chunk(int64_t work, int least) {
   const int64_t steps = (work + FX_KV_TARGET - 1) / FX_KV_TARGET, chunk = (steps + least - 1) / least * least;
   return (int)(chunk < least ? least : chunk > (1 << 30) ? (1 << 30) : chunk);
 }
 FX_KV_HD int fx_kv_parts(int steps, int chunk) { return steps > chunk ? (steps + chunk - 1) / chunk : 1; }
+
+// Unit `rest` of a request, of `splits` for each item: false where it has none of that number
+FX_KV_HD bool fx_kv_item(const FxKvRequest& r, int heads, int splits, int rest, int* item, int* tile, int* head) {
+  *item = rest / splits;
+  *tile = *item / heads;
+  *head = *item - *tile * heads;
+  return rest >= 0 && *tile < r.tiles;
+}
 
 struct FxKvSpan {
   int low, high;            // tokens that some row of the tile sees: [low, high)

@@ -210,6 +210,28 @@ def test_every_step_is_taken_once_and_the_parts_fit_the_workspace(split, rows, l
         assert split.fx_kv_split_check(B, a, l, tokens, room, group, window, heads, rows, least, out) == 0, (case, starts[:9], lens[:9], group, window)
 
 
+def test_units_of_requests_that_overlap_stay_inside(tmp_path):
+    """Offsets that fall let requests overlap: their units may be more than 31 bits count.  Whatever the sums come to then, a unit that is found is one
+    of its request's and nothing is cut."""
+    so = str(tmp_path / "libkv_units.so")
+    subprocess.check_call(["g++", "-O2", "-std=c++17", "-fPIC", "-shared", os.path.join(os.path.dirname(os.path.abspath(__file__)), "support", "kv_units.cpp"), "-o", so])
+    check, shared = ctypes.CDLL(so).fx_kv_units_check, ctypes.c_int()
+    rng = random.Random(1)
+
+    def run(starts, lens, tokens, room, group, heads):
+        a, l = (ctypes.c_int * len(starts))(*starts), (ctypes.c_int * len(lens))(*lens)
+        return check(len(lens), a, l, tokens, room, group, heads, 16, 4, 1 << 20, ctypes.byref(shared))
+
+    for B, tokens, group, heads in ((2000, 1 << 20, 16, 4), (700, 1 << 22, 4, 16), (100, 5000, 8, 8)):
+        for falls in (True, False):
+            starts = [rng.randint(0, tokens) for _ in range(B + 1)]
+            starts[1], starts[2] = 0, tokens
+            lens = [rng.choice([0, 0, 1]) for _ in range(B)]
+            lens[B // 2], starts[B // 2 + 1] = 1 << 20, starts[B // 2] + 1      # one row and many tokens
+            assert run(starts if falls else sorted(starts), lens, tokens, 1 << 20, group, heads) == 0
+            assert not falls or shared.value == 0
+
+
 def test_entries_of_a_table_that_are_no_page(split):
     for entry, page in ((0, 0), (6, 6), (7, -1), (-1, -1), (2 ** 31 - 1, -1), (-2 ** 31, -1)):
         assert split.fx_kv_page_of(entry, 7) == page
@@ -585,6 +607,28 @@ def test_many_requests_some_of_many_rows(n):
     for _ in range(3):
         again = check_attention(spec, INT8, torch.bfloat16, 32, 4, 16, 64, seed=n)
         assert torch.equal(first[0], again[0]) and torch.equal(first[1], again[1])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind,H", [(torch.float32, 1), (torch.bfloat16, 42)])
+@pytest.mark.parametrize("n", [3, 70])
+def test_offsets_that_fall(kind, H, n):
+    """Requests that overlap by mistake: rows that are one request's alone have its results.  Rows behind the last offset are of no request, whatever the
+    offsets before it say, and may be cleared: 590 here."""
+    spec = [(900, 600), (700, 1), (300, 3)]
+    cache = filled(40, H, 64, 64, INT8, 5)
+    table, lens, starts = requests(spec, 64, 40, 1)
+    q = torch.randn(starts[-1], H * 2, 64, generator=torch.Generator().manual_seed(1)).to(kind).cuda()
+    table, lens = table + [[-1] * len(table[0])] * (n - 3), lens + [0] * (n - 3)
+    args = (q, i32(table), i32(lens))
+    rising = cache.attention(*args, i32(starts + [starts[-1]] * (n - 3)))
+    falling = cache.attention(*args, i32(starts[:3] + [590] + [590] * (n - 3)))         # the third request's end is in the first: it has no rows
+    ref, rl, spread, size = PlainCache(cache).attention(q, table, lens, starts + [starts[-1]] * (n - 3), 0.125, 0)
+    most, lmost = tolerance(kind, ref, rl, spread, size, 900, 64, True)
+    for (out, lse), rows in ((rising, starts[-1]), (falling, 590)):
+        assert bool(((out.cpu().double() - ref).abs() <= most)[:rows].all()) and bool(((lse.cpu().double() - rl).abs() <= lmost)[:rows].all())
+    wild = cache.attention(*args, i32([0, starts[1], 0, starts[1]] + [0] * (n - 3)))
+    assert bool(torch.isfinite(wild[0][:starts[1]].float()).all())
 
 
 @pytest.mark.gpu
