@@ -597,6 +597,14 @@ def test_many_rows(held, kind, P, H, G, D, window):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("held,kind", [(E4M3, torch.bfloat16), (INT8, torch.float16)])
+@pytest.mark.parametrize("P,H,G,D,window", [(16, 2, 45, 128, 0), (64, 1, 90, 64, 100), (256, 3, 30, 256, 7)])
+def test_many_rows_that_come_before_their_tokens(held, kind, P, H, G, D, window):
+    """Requests of more rows than tokens, in large tiles: the first rows see nothing, whole tiles of them too."""
+    check_attention([(100, 300), (200, 201), (1, 150)], held, kind, P, H, G, D, window=window, seed=P)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("n", [64, 65, 300])
 def test_many_requests_some_of_many_rows(n):
     """Both kernels and their parts in one call, for more requests than a wave has lanes; the same bits in every call."""
@@ -1155,6 +1163,37 @@ def test_a_captured_step_serves_other_lengths():
             assert torch.equal(a, b), new
         assert torch.equal(state["eager"]["table"], state["graph"]["table"])
         assert torch.equal(eager.k.view(torch.uint8), graphed.k.view(torch.uint8)) and torch.equal(eager.v_scale, graphed.v_scale)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [3, 70])
+def test_a_captured_call_of_both_kernels(n):
+    """A call of 49 152 rows and more, recorded once and replayed with other lengths, offsets, tables and queries, eager calls and waits in between: requests
+    that were long are short, empty or behind others, rows come before their tokens do, and every replay gives what an eager call gives."""
+    H, G, P, pages, rows = 2, 90, 32, 200, 300
+    cache = filled(pages, H, P, 64, E4M3, 3)
+    q, table, lens, starts = torch.zeros(rows, H * G, 64, dtype=torch.bfloat16, device="cuda"), i32([[-1] * 40] * n), i32([0] * n), i32([0] * (n + 1))
+    cache.attention(q, table, lens, starts, window=500)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = cache.attention(q, table, lens, starts, window=500)
+    for i, spec in enumerate(([(1200, 200), (1, 1), (900, 90)], [(0, 150), (100, 140), (3, 1)], [(5, 0)] * 3, [(1280, 1), (0, 0), (700, 299)], [(64, 1)] * 2 + [(1100, 260)])):
+        t, l, st = requests(spec, P, pages, i)
+        for b in range(3):
+            table[b] = i32(t[b][:40] + [-1] * (40 - len(t[b])))
+        lens.copy_(i32(l + [0] * (n - 3))), starts.copy_(i32(st + [st[-1]] * (n - 3)))
+        q.copy_(torch.randn(q.shape, generator=torch.Generator().manual_seed(i)).to(torch.bfloat16))
+        want = cache.attention(q, table, lens, starts, window=500)
+        for _ in range(2):
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]), spec
+        tb, ref = table.tolist(), PlainCache(cache)
+        part = slice(0, 2)                                # (two heads of each key head's: as many as a reference needs)
+        few = torch.cat([q[:, part], q[:, G:G + 2]], 1)
+        o, rl, spread, size = ref.attention(few, tb, lens.tolist(), starts.tolist(), 0.125, 500)
+        most, _ = tolerance(torch.bfloat16, o, torch.where(torch.isfinite(rl), rl, 0.0), spread, size, 1280, 64, True)
+        assert bool(((torch.cat([got[0][:, part], got[0][:, G:G + 2]], 1).cpu().double() - o).abs() <= most).all()), spec
 
 
 @pytest.mark.gpu
