@@ -47,6 +47,7 @@ FX_KV_HD int fx_kv_tile_rows(int depth) { return depth <= 128 ? 256 : 128; }
 //             96 000 rows 95 / 85, 192 000 rows 204 / 156; depth 256: 16 000 rows 76 / 86, 64 000 rows 447 / 368; depth 80: 32 000 rows 67 / 111
 //   requests  of 100 rows, 51 200 in all 46 / 71; of 128 rows, 65 536 in all 97 / 86, of 400 rows, 102 400 in all 116 / 84
 //   fp32      (three numbers for each query and weight) 64 000 rows 238 / 267, 192 000 rows 1 000 / 1 335, depth 256 517 / 1 002: fx_kv_rows always
+// Not measured on both sides: fp16, int8, pages of 16 and 32, depths below 64; they go by the same rule.
 #define FX_KV_FEW 128
 #define FX_KV_MANY 49152
 struct FxKvItem {   // rows whose cached tokens several workgroups shared

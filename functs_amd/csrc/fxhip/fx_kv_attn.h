@@ -11,8 +11,9 @@
 // Codes become bf16 (or f16) exactly; fp32 queries and the weights are sums of two or three such numbers:
 //   queries  bf16, f16: as they are;  fp32: three bf16 (24 bits)
 //   weights  fp32 results: three bf16;  f16: two (16 bits);  bf16: two in fx_kv_rows, which waits for memory anyway, one in
-//            fx_kv_tiles: weights of one bf16 are off by half a step each, no more than the result's own rounding is, and
-//            two took 721 us where one took 587 (prompts, before later steps).  Sums of the weights are fp32, of weights as they were
+//            fx_kv_tiles: weights of one bf16 are off by half a step each, no more than the result's own rounding is (2-norm of
+//            the error of prompts, against 64 bits: 0.0019, the result's rounding alone 0.0016), and two, as f16 calls have them,
+//            take 491 us where one takes 377.  Sums of the weights are fp32, of weights as they were
 #pragma once
 #include <type_traits>
 
@@ -546,10 +547,12 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void fx_kv_rows(const FxKvA
 // changes them over.  Products go first (their waves' priority): what they wait for is longer.  Where a wave's registers are more than
 // half of a SIMD's (depths above 128) there is one group, which does one after the other.
 // Measured at 4 requests of 511 to 2 047 rows behind up to 6 001 cached tokens, 32 query heads on 8, depth 128, e4m3, bf16 (0.33
-// TFLOP): 380 to 384 us, 870 TFLOP/s, of 1 430 that a large library product reaches here.  Without the second group 438 us (before the next
+// TFLOP): 375 to 384 us, 880 TFLOP/s, of 1 430 that a large library product reaches here.  Without the second group 438 us (before the next
 // two steps), with a page a lane and group of 16 tokens (below) in place of one a step 421, without the priority 397.  A step takes about
-// 2 300 clocks for either half of its work: 1 024 of the matrix cores and their operands' way from LDS (64 reads of 16 bytes a
-// lane), or 1 750 of the vector units.
+// 2 300 clocks for either half of its work: 1 024 of the matrix cores and their operands' way from LDS (32 reads of 16 bytes a
+// lane), or 1 750 of the vector units (265 instructions, 32 exponentials among them), the longer half.
+// Registers that do not fit, a lane: none at depth 64 and, with pages of 64 tokens and more, of bf16 calls at depth 128; f16 on e4m3 4; up to 143 in the
+// other forms (pages of 16 and 32, f16 on int8, depths that are not 64, 128 or 256, depth 256): 670 us for bf16 on int8 with pages of 16 where pages of 64 take 383.
 // In LDS a key's row of 16-byte pieces is permuted by its token (key_piece), which spreads the 32 rows of an operand over the banks; values
 // lie as [group][8 tokens of it][depth][8 tokens].
 typedef float fx_f32x16 __attribute__((ext_vector_type(16)));

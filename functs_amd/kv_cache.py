@@ -87,7 +87,8 @@ class KvCache:
         """Rows starts[b] to starts[b + 1] of q [tokens, query heads, depth] are the last tokens of request b's lens[b]; each sees
         the tokens up to its own (the last `window` of them, if not 0).  Returns the weighted values (type of q) and the logarithm of
         the sum of exponentials (fp32 [tokens, query heads]).  scale: depth ** -0.5 unless given, 2^-26 to 32.  max_new: the most rows of one request, if known (1
-        for a decoding step): a matter of speed alone.  With out and lse, rows of no request stay as they are there."""
+        for a decoding step): a matter of speed, and of how results are rounded, as the number of rows of a call is (fx_kv_attention in
+        include/fxhip.h).  With out and lse, rows of no request stay as they are there; out does not overlap q."""
         if scale is None:
             scale = self.k.size(3) ** -0.5
         args = (q, self.k, self.v, self.k_scale, self.v_scale, block_table, lens, starts, scale, window, max_new)

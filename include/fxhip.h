@@ -533,8 +533,8 @@ typedef struct fx_kv_cache {
 
 /* Request b has past[b] cached tokens and gets added[b] more, whose rows lie one request behind the other in arrays of `tokens`
  * rows.  A request is granted when past and added are not negative, past + added fits its row of the table
- * (columns * page_size), its rows fit `tokens`, and the free pages that are left for it (those of all requests
- * before it taken) are enough, or it needs none.
+ * (columns * page_size), its rows and those of all requests before it fit `tokens` (a request of no rows behind others that do not fit
+ * is not granted either), and the free pages that are left for it (those of all requests before it taken) are enough, or it needs none.
  *   starts[b]     first row of request b (at most `tokens`); starts[requests]: behind the last
  *   lens[b]       past + added if granted, else 0
  *   positions[t]  past + j for row j of a granted request, else -1 (rows behind the last request: -1)
@@ -581,11 +581,16 @@ int fx_kv_read(const fx_kv_cache* cache, const fx_kv_rows* rows, void* stream);
  * p = lens[b] - n + i and sees the tokens j <= p (window > 0: and j > p - window) whose page is in the cache.
  *   out = sum_j softmax_j(scale * q . k_j) v_j        lse = log sum_j exp(scale * q . k_j)   (fp32)
  * A row that sees nothing gets zeros and -infinity.  Query head h reads head h / (q_heads / heads).  What lies in the cache where
- * a row does not see it has no influence, NaN included.
- * q [tokens][q_heads][depth], a depth contiguous; out [tokens][q_heads][depth] and lse [tokens][q_heads] contiguous.  Rows of no
- * request are left as they were, or get zeros and -infinity (clear_rest).  max_new: how many rows the longest request
- * has, at most, as far as the caller knows (0: unknown); it decides on forms, and so at most on how results are
- * rounded.  scale: 2^-26 to 32.  out does not overlap q.  Sums are fp32, and a token's weight in them is 1 at most, and of the largest
+ * a row does not see it has no influence, codes and scales that are NaN or infinite included; the scales that it sees are finite, as
+ * fx_kv_store leaves them.
+ * q [tokens][q_heads][depth], a depth contiguous; out [tokens][q_heads][depth] (16-byte aligned) and lse [tokens][q_heads] contiguous.  starts
+ * do not fall; rows before the first and behind the last of them are of no request, and are left as they were or get zeros and -infinity
+ * (clear_rest).  scale: 2^-26 to 32.  out does not overlap q.
+ * max_new: how many rows the longest request has, at most, as far as the caller knows (0: unknown).  It decides on forms, and so does the number
+ * of rows of the whole call; results differ by how they are rounded.  Weights are off by 2^-22 of each at most (fp32 queries) or 2^-15; in bf16
+ * calls of 49 152 rows of all query heads and more, those of requests of more than 128 rows (tokens x query heads of a head) by 2^-8, half
+ * a step of the result's own type.
+ * Sums are fp32, those of the scores too (of queries times codes, before scales); a token's weight in them is 1 at most, and of the largest
  * score 2^-8 at least, before they are divided: values of more than 2^127 / lens[b] in magnitude may become infinite, and a weight times a
  * page's scale of values below 2^-126 adds nothing to out (to lse it does).
  * workspace: fx_kv_attention_workspace_bytes() of device memory for each call under way, 256-byte aligned; nothing is expected in it. */
