@@ -50,6 +50,7 @@ uint32_t fx_cmap_lds_bytes(const FxCmapLaunch& hl);
 uint32_t fx_cmap_chunk_rows();
 #include "fx_attn.h"
 #include "fx_kv.h"
+#include "fx_rotary.h"
 #include "fx_lstm_sched.h"
 int fx_launch_lstm_stack(const FxLstmArgs& a, int L, uint32_t* words_ctl, uint32_t* die_ctl, hipStream_t stream);
 int fx_lstm_ask(int form);
@@ -1828,6 +1829,38 @@ int fx_kv_attention(const fx_kv_cache* cache, const fx_kv_attention_desc* desc, 
   int launched = 0;
   HIP_OK(fx_launch_kv_attention(a, l, (hipStream_t)stream, &launched));
   return kv_launched(launched);
+}
+
+// ---- rotary positions (fx_rotary.hip) ----
+
+namespace {
+int rotary_of(const char* at, const fx_rotary_desc* desc, FxRotary& a) {
+  const std::string op(at);
+  if (!desc) return fail(FX_E_INVALID, op + ": null descriptor");
+  const fx_rotary_desc& d = *desc;
+  if (!kv_dtype(d.dtype)) return fail(FX_E_UNSUPPORTED, op + ": rows must be float32, float16 or bfloat16");
+  if (d.batch < 0 || d.tokens < 0 || d.heads < 1 || d.depth < 1) return fail(FX_E_INVALID, op + ": rows of no heads or columns, or a negative size");
+  if (d.pairs < 1 || (int64_t)d.pairs * 2 > d.depth)
+    return fail(FX_E_INVALID, op + ": at least one pair of columns turns, and " + std::to_string(d.depth) + " columns hold " + std::to_string(d.depth / 2) + " (got " + std::to_string(d.pairs) + ")");
+  if (d.pairs > FX_ROTARY_ANGLES) return fail(FX_E_UNSUPPORTED, op + ": more than " + std::to_string(FX_ROTARY_ANGLES) + " pairs");
+  if ((int64_t)d.heads * d.depth >= 1 << 28 || (int64_t)d.batch * d.tokens >= 1 << 30) return fail(FX_E_LIMIT, op + ": 2^28 numbers of a token, or 2^30 tokens");
+  a = FxRotary{FxTurns{d.positions, d.frequencies, d.pairs, d.positions_64 != 0, d.frequencies_32 != 0, d.interleaved != 0, d.back != 0, d.magnitude},
+               d.x, d.y, d.x_batch_stride, d.x_token_stride, d.x_head_stride, d.y_batch_stride, d.y_token_stride, d.y_head_stride, d.position_batch_stride,
+               d.batch, d.tokens, d.heads, d.depth, d.dtype};
+  if (d.batch == 0 || d.tokens == 0) return FX_OK;
+  if (!d.x || !d.y || !d.positions || !d.frequencies) return fail(FX_E_INVALID, op + ": null argument");
+  fx_rotary_shape(a);
+  if ((int64_t)a.blocks * a.slices >= 1 << 23) return fail(FX_E_LIMIT, op + ": more numbers than a launch holds");
+  return FX_OK;
+}
+}  // namespace
+
+int fx_rotary(const fx_rotary_desc* desc, void* stream) {
+  FxRotary a;
+  if (int rc = rotary_of("fx_rotary", desc, a)) return rc;
+  if (a.batch == 0 || a.tokens == 0) return FX_OK;
+  HIP_OK(fx_launch_rotary(a, (hipStream_t)stream));
+  return kv_launched(1);
 }
 
 // ---- detection tail (fx_nms.hip) ----

@@ -1,0 +1,125 @@
+// Rotary positions on the device.
+//
+// A pair (a, b) of a token at position p with frequency f becomes m (a cos pf - b sin pf, b cos pf + a sin pf); backward the
+// transposed matrix, which is sin with the other sign.  The angle is a product of 64 bits, less whole quarter turns: positions of
+// 2^31 are as exact as small ones (1e-7 of a turn at most).  What is left, up to pi / 4 either way, goes through polynomials in 32 bits
+// (least maximum error, found by exchange: sine 0.7 ulp, cosine 1.3 * 2^-24); products are 32 bits, rounded once at the end.
+#pragma once
+#include "fx_rotary.h"
+
+namespace {
+struct Turn { float c, s; };
+
+// (g: frequency times 2 / pi, quarter turns a token)
+__device__ __forceinline__ Turn turn_of(double p, double g, float magnitude, bool back) {
+  const double t = p * g, q = __builtin_rint(t);
+  const float r = (float)((t - q) * 1.57079632679489661923);
+  const int k = (int)(q - 4.0 * __builtin_rint(q * 0.25)) & 3;   // -2 .. 2
+  const float z = r * r;
+  float s = __builtin_fmaf(z, __builtin_fmaf(z, -0.000195169778f, 0.00833217613f), -0.166666552f);
+  s = __builtin_fmaf(r, z * s, r);
+  float c = __builtin_fmaf(z, __builtin_fmaf(z, 2.44380917e-05f, -0.00138873642f), 0.0416666456f);
+  c = __builtin_fmaf(z * z, c, __builtin_fmaf(z, -0.5f, 1.0f));
+  Turn w;
+  w.c = (k & 1) ? s : c;
+  w.s = (k & 1) ? c : s;
+  w.c = k == 1 || k == 2 ? -w.c : w.c;
+  w.s = (k >= 2) != back ? -w.s : w.s;
+  w.c *= magnitude;
+  w.s *= magnitude;
+  return w;
+}
+__device__ __forceinline__ double position_of(const FxTurns& t, int64_t i) {
+  return t.wide ? (double)((const int64_t*)t.positions)[i] : (double)((const int32_t*)t.positions)[i];
+}
+__device__ __forceinline__ double quarters_of(const FxTurns& t, int pair) {
+  return (t.narrow ? (double)((const float*)t.frequencies)[pair] : ((const double*)t.frequencies)[pair]) * 0.63661977236758134308;
+}
+__device__ __forceinline__ void turn_pair(float& a, float& b, const Turn& w) {
+  const float u = __builtin_fmaf(a, w.c, -(b * w.s)), v = __builtin_fmaf(b, w.c, a * w.s);
+  a = u;
+  b = v;
+}
+
+__device__ __forceinline__ unsigned divided(unsigned n, unsigned d, unsigned magic) { return magic ? __umulhi(n, magic) : n / d; }
+
+// N numbers from any address (rows of odd sizes begin anywhere)
+template <class T, int N>
+struct Some {
+  T e[N];
+  __device__ __forceinline__ void load(const T* p) { __builtin_memcpy(e, p, sizeof e); }
+  __device__ __forceinline__ void store(T* p) const { __builtin_memcpy(p, e, sizeof e); }
+};
+
+// A workgroup's share of the rows.  A unit is PV pairs of a head, or 2 PV of the columns that do not turn: two loads and two stores of
+// 16 bytes a lane where PV is 8 (16-bit types) or 4.  Where the units do not fit, the last one begins earlier and does some numbers
+// again.  Angles are computed once for all heads and kept in LDS, behind the first loads.
+template <class T, int PV, bool INTER>
+__device__ __forceinline__ void rotary_rows(const FxRotary& a, int block, int slice, Turn* s_turn) {
+  constexpr int kThreadsHere = 256, kUnits = 4;
+  const int tid = (int)threadIdx.x, pairs = a.turns.pairs, rest = a.depth - 2 * pairs, total = a.batch * a.tokens;
+  const int g0 = block * a.per, n = min(a.per, total - g0), row = a.units * a.heads, all = n * row;
+  T* const y = (T*)a.y;
+  bool first = true;
+  for (int base = slice * kThreadsHere * kUnits; base < all; base += a.slices * kThreadsHere * kUnits) {
+    Some<T, PV> lo[kUnits], hi[kUnits];
+    int64_t to[kUnits];              // the head's place in y
+    int at[kUnits], angle[kUnits];   // at: first pair or column; angle: place of the first pair's, -1: columns that do not turn, -2: few of them, -3: nothing
+#pragma unroll
+    for (int k = 0; k < kUnits; ++k) {
+      const int i = base + k * kThreadsHere + tid;
+      angle[k] = -3;
+      if (i >= all) continue;
+      const int j = (int)divided((unsigned)i, (unsigned)row, a.magic_token), in_row = i - j * row;
+      const int h = (int)divided((unsigned)in_row, (unsigned)a.units, a.magic_head), u = in_row - h * a.units;
+      const int g = g0 + j, b = a.batch == 1 ? 0 : g / a.tokens, t = g - b * a.tokens;
+      const T* x = (const T*)a.x + (int64_t)b * a.x_batch + (int64_t)t * a.x_token + (int64_t)h * a.x_head;
+      to[k] = (int64_t)b * a.y_batch + (int64_t)t * a.y_token + (int64_t)h * a.y_head;
+      if (u < a.turning) {
+        const int p = min(u * PV, pairs - PV);
+        at[k] = p;
+        angle[k] = j * pairs + p;
+        lo[k].load(x + (INTER ? 2 * p : p));
+        hi[k].load(x + (INTER ? 2 * p + PV : p + pairs));
+      } else if (rest >= 2 * PV) {
+        const int c = 2 * pairs + min((u - a.turning) * 2 * PV, rest - 2 * PV);
+        at[k] = c;
+        angle[k] = -1;
+        lo[k].load(x + c);
+        hi[k].load(x + c + PV);
+      } else {
+        angle[k] = -2;
+        for (int c = 2 * pairs; c < a.depth; ++c) y[to[k] + c] = x[c];
+      }
+    }
+    if (first) {
+      first = false;
+      for (int i = tid; i < n * pairs; i += kThreadsHere) {
+        const int j = (int)divided((unsigned)i, (unsigned)pairs, a.magic_pair), g = g0 + j, b = a.batch == 1 ? 0 : g / a.tokens;
+        s_turn[i] = turn_of(position_of(a.turns, (int64_t)b * a.position_batch + (g - b * a.tokens)), quarters_of(a.turns, i - j * pairs), a.turns.magnitude, a.turns.back != 0);
+      }
+      __syncthreads();
+    }
+#pragma unroll
+    for (int k = 0; k < kUnits; ++k) {
+      if (angle[k] < -1) continue;
+      if (angle[k] >= 0) {
+#pragma unroll
+        for (int i = 0; i < PV; ++i) {
+          T& ra = INTER ? (2 * i < PV ? lo[k].e[2 * i % PV] : hi[k].e[2 * i % PV]) : lo[k].e[i];
+          T& rb = INTER ? (2 * i + 1 < PV ? lo[k].e[(2 * i + 1) % PV] : hi[k].e[(2 * i + 1) % PV]) : hi[k].e[i];
+          float u = (float)ra, v = (float)rb;
+          turn_pair(u, v, s_turn[angle[k] + i]);
+          ra = (T)u;
+          rb = (T)v;
+        }
+        lo[k].store(y + to[k] + (INTER ? 2 * at[k] : at[k]));
+        hi[k].store(y + to[k] + (INTER ? 2 * at[k] + PV : at[k] + pairs));
+      } else {
+        lo[k].store(y + to[k] + at[k]);
+        hi[k].store(y + to[k] + at[k] + PV);
+      }
+    }
+  }
+}
+}  // namespace

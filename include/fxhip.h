@@ -616,6 +616,30 @@ typedef struct fx_kv_attention_desc {
 size_t fx_kv_attention_workspace_bytes(const fx_kv_cache* cache, const fx_kv_attention_desc* desc);
 int fx_kv_attention(const fx_kv_cache* cache, const fx_kv_attention_desc* desc, void* stream);
 
+/* ---- rotary positions ----
+ * Of a head's `depth` columns the first 2 * pairs turn, pair i of a token at position p by the angle p * frequencies[i]:
+ *   (a, b) -> magnitude * (a cos - b sin, b cos + a sin)          back: magnitude * (a cos + b sin, b cos - a sin), the gradient's
+ * where (a, b) are columns i and i + pairs, or 2 i and 2 i + 1 (interleaved); the other columns are copied.  y may not overlap x.
+ * The angle is formed in 64 bits (an error of about |p| frequency / 2^53), its cosine and sine are off by 2^-23 at most, products are fp32 and
+ * y is rounded once.  x [batch][tokens][heads][depth], a depth contiguous, strides in elements, any alignment of its numbers; positions int32, or
+ * int64 (positions_64), the tokens' side by side, position_batch_stride apart (0: all batches have the same); frequencies double, or float
+ * (frequencies_32): what they hold counts as exact.  1 <= pairs <= 2048, 2 * pairs <= depth, heads * depth < 2^28, batch * tokens < 2^30. */
+typedef struct fx_rotary_desc {
+  const void* x;
+  void* y;
+  const void* positions;
+  const void* frequencies;
+  int64_t x_batch_stride, x_token_stride, x_head_stride;
+  int64_t y_batch_stride, y_token_stride, y_head_stride;
+  int64_t position_batch_stride;
+  int32_t batch, tokens, heads, depth, pairs;
+  int32_t dtype; /* FX_DT_F32, FX_DT_F16, FX_DT_BF16 */
+  int32_t positions_64, frequencies_32, interleaved, back;
+  float magnitude;
+  int32_t reserved;
+} fx_rotary_desc;
+int fx_rotary(const fx_rotary_desc* desc, void* stream);
+
 /* ---- detection tail: score threshold + sort + class-aware greedy NMS + top-k, one launch ----
  * The step behind row compaction in the reference's detection programs, which it runs as ATen /
  * torchvision kernels with host synchronisations in between:
