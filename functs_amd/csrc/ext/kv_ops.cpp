@@ -3,6 +3,7 @@
 // many requests of different lengths.
 //   functs::kv_plan       pages, slots and offsets of a step's tokens, from lengths on the device
 //   functs::kv_store      writes keys and values
+//   functs::kv_append     the same with rotary positions: keys turn on the way, queries beside them
 //   functs::kv_read       gives them back as numbers
 //   functs::kv_attention  attention over them
 // Nothing here waits for the device or reads from it: a captured call serves other lengths when it is replayed.
@@ -11,7 +12,7 @@
 #include <cmath>
 #include <tuple>
 
-#include "op_checks.h"
+#include "rotary_ops.h"
 
 namespace functs {
 namespace {
@@ -149,6 +150,45 @@ void kvStore(const Tensor& k_, const Tensor& v_, Tensor k_cache, Tensor v_cache,
   for (const Tensor* t : {&k_cache, &v_cache, &k_scale, &v_scale}) written(*t);
 }
 
+Tensor kvAppend(const Tensor& q_, const Tensor& k_, const Tensor& v_, Tensor k_cache, Tensor v_cache, Tensor k_scale, Tensor v_scale, const Tensor& slots_,
+                const Tensor& positions_, const Tensor& frequencies_, double magnitude, bool interleaved) {
+  static const char op[] = "functs::kv_append";
+  const fx_kv_cache c = cacheOf(op, k_cache, v_cache, k_scale, v_scale);
+  const auto dev = k_cache.device();
+  const Tensor slots = slotsOf(op, slots_, dev);
+  const int32_t tokens = sized(op, slots.numel(), "the number of tokens");
+  rowsOf(op, k_, "k", c, tokens, dev);
+  rowsOf(op, v_, "v", c, tokens, dev);
+  onGpu(op, q_, "q", dev);
+  noGrad(op, q_, "q");
+  noGrad(op, k_, "k");
+  noGrad(op, v_, "v");
+  TORCH_CHECK(q_.dim() == 3 && q_.size(0) == tokens && q_.size(1) >= 1 && q_.size(2) == c.depth, op, ": q must be [", tokens, ", heads, ", c.depth, "], got ", q_.sizes());
+  TORCH_CHECK(k_.scalar_type() == v_.scalar_type() && q_.scalar_type() == k_.scalar_type(), op, ": q, k and v must be of one type, got ", q_.scalar_type(), ", ",
+              k_.scalar_type(), " and ", v_.scalar_type());
+  TORCH_CHECK(positions_.dim() == 1 && positions_.size(0) == tokens, op, ": positions must be [", tokens, "], got ", positions_.sizes());
+  const int dtype = dtypeOf(op, k_.scalar_type(), "k");
+  c10::DeviceGuard guard(dev);
+  const Tensor positions = positions_.contiguous(), frequencies = frequencies_.contiguous();
+  fx_rotary_desc d = rotaryDesc(op, positions, frequencies, magnitude, interleaved, c.depth, dev);
+  const Tensor q = q_.stride(2) == 1 ? q_ : q_.contiguous(), k = k_.stride(2) == 1 ? k_ : k_.contiguous(), v = v_.stride(2) == 1 ? v_ : v_.contiguous();
+  Tensor out = at::empty(q.sizes(), q.options().memory_format(at::MemoryFormat::Contiguous));
+  d.x = q.data_ptr();
+  d.y = out.data_ptr();
+  d.x_token_stride = q.stride(0);
+  d.x_head_stride = q.stride(1);
+  d.y_token_stride = out.stride(0);
+  d.y_head_stride = out.stride(1);
+  d.batch = 1;
+  d.tokens = tokens;
+  d.heads = sized(op, q.size(1), "the number of heads");
+  d.dtype = dtype;
+  const fx_kv_rows r = rowsDesc(k, v, slots, tokens, dtype);
+  FX_OK_OR_THROW(fx_kv_append(&c, &r, &d, streamOf(dev)));
+  for (const Tensor* t : {&k_cache, &v_cache, &k_scale, &v_scale}) written(*t);
+  return out;
+}
+
 std::tuple<Tensor, Tensor> kvRead(const Tensor& k_cache, const Tensor& v_cache, const Tensor& k_scale, const Tensor& v_scale, const Tensor& slots_,
                                   at::ScalarType dtype) {
   static const char op[] = "functs::kv_read";
@@ -250,6 +290,8 @@ TORCH_LIBRARY_FRAGMENT(functs, m) {
   m.def("kv_plan(Tensor past_lens, Tensor new_lens, Tensor(a!) block_table, Tensor free_pages, int page_size, int max_tokens, "
         "Tensor? free_start=None) -> (Tensor, Tensor, Tensor, Tensor, Tensor)", kvPlan);
   m.def("kv_store(Tensor k, Tensor v, Tensor(a!) k_cache, Tensor(b!) v_cache, Tensor(c!) k_scale, Tensor(d!) v_scale, Tensor slots) -> ()", kvStore);
+  m.def("kv_append(Tensor q, Tensor k, Tensor v, Tensor(a!) k_cache, Tensor(b!) v_cache, Tensor(c!) k_scale, Tensor(d!) v_scale, Tensor slots, "
+        "Tensor positions, Tensor frequencies, float magnitude=1.0, bool interleaved=False) -> Tensor", kvAppend);
   m.def("kv_read(Tensor k_cache, Tensor v_cache, Tensor k_scale, Tensor v_scale, Tensor slots, ScalarType dtype) -> (Tensor, Tensor)", kvRead);
   m.def("kv_attention(Tensor q, Tensor k_cache, Tensor v_cache, Tensor k_scale, Tensor v_scale, Tensor block_table, Tensor lens, Tensor starts, "
         "float scale, int window=0, int max_new=0) -> (Tensor, Tensor)", kvAttention);

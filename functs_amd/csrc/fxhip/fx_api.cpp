@@ -1734,6 +1734,37 @@ size_t kv_workspace(FxKvAttnArgs& a, FxKvLaunch& l, int depth, int requests, cha
 }
 }  // namespace
 
+// rotary positions (fx_rotary.hip)
+namespace {
+int rotary_of(const char* at, const fx_rotary_desc* desc, FxRotary& a) {
+  const std::string op(at);
+  if (!desc) return fail(FX_E_INVALID, op + ": null descriptor");
+  const fx_rotary_desc& d = *desc;
+  if (!kv_dtype(d.dtype)) return fail(FX_E_UNSUPPORTED, op + ": rows must be float32, float16 or bfloat16");
+  if (d.batch < 0 || d.tokens < 0 || d.heads < 1 || d.depth < 1) return fail(FX_E_INVALID, op + ": rows of no heads or columns, or a negative size");
+  if (d.pairs < 1 || (int64_t)d.pairs * 2 > d.depth)
+    return fail(FX_E_INVALID, op + ": at least one pair of columns turns, and " + std::to_string(d.depth) + " columns hold " + std::to_string(d.depth / 2) + " (got " + std::to_string(d.pairs) + ")");
+  if (d.pairs > FX_ROTARY_ANGLES) return fail(FX_E_UNSUPPORTED, op + ": more than " + std::to_string(FX_ROTARY_ANGLES) + " pairs");
+  if ((int64_t)d.heads * d.depth >= 1 << 28 || (int64_t)d.batch * d.tokens >= 1 << 30) return fail(FX_E_LIMIT, op + ": 2^28 numbers of a token, or 2^30 tokens");
+  a = FxRotary{FxTurns{d.positions, d.frequencies, d.pairs, d.positions_64 != 0, d.frequencies_32 != 0, d.interleaved != 0, d.back != 0, d.magnitude},
+               d.x, d.y, d.x_batch_stride, d.x_token_stride, d.x_head_stride, d.y_batch_stride, d.y_token_stride, d.y_head_stride, d.position_batch_stride,
+               d.batch, d.tokens, d.heads, d.depth, d.dtype};
+  if (d.batch == 0 || d.tokens == 0) return FX_OK;
+  if (!d.x || !d.y || !d.positions || !d.frequencies) return fail(FX_E_INVALID, op + ": null argument");
+  fx_rotary_shape(a);
+  if ((int64_t)a.blocks * a.slices >= 1 << 23) return fail(FX_E_LIMIT, op + ": more numbers than a launch holds");
+  return FX_OK;
+}
+}  // namespace
+
+int fx_rotary(const fx_rotary_desc* desc, void* stream) {
+  FxRotary a;
+  if (int rc = rotary_of("fx_rotary", desc, a)) return rc;
+  if (a.batch == 0 || a.tokens == 0) return FX_OK;
+  HIP_OK(fx_launch_rotary(a, (hipStream_t)stream));
+  return kv_launched(1);
+}
+
 int fx_kv_plan(const fx_kv_plan_desc* desc, void* stream) {
   if (!desc) return fail(FX_E_INVALID, "fx_kv_plan: null descriptor");
   const fx_kv_plan_desc& d = *desc;
@@ -1758,6 +1789,24 @@ int fx_kv_store(const fx_kv_cache* cache, const fx_kv_rows* rows, void* stream) 
   if (int rc = kv_rows_of("fx_kv_store", c, rows, r)) return rc;
   if (r.tokens == 0) return FX_OK;
   HIP_OK(fx_launch_kv_store(c, r, cache->held, (hipStream_t)stream));
+  return kv_launched(1);
+}
+
+int fx_kv_append(const fx_kv_cache* cache, const fx_kv_rows* rows, const fx_rotary_desc* queries, void* stream) {
+  static const char at[] = "fx_kv_append";
+  FxKvCache c;
+  FxKvRows r;
+  FxRotary q;
+  if (int rc = kv_cache_of(at, cache, c)) return rc;
+  if (int rc = kv_rows_of(at, c, rows, r)) return rc;
+  if (int rc = rotary_of(at, queries, q)) return rc;
+  if (q.batch != 1 || q.turns.back || q.tokens != r.tokens || q.depth != c.depth || q.dtype != r.dtype)
+    return fail(FX_E_INVALID, "fx_kv_append: queries are one batch of the rows' tokens, depth and type, and turn forward");
+  if (r.tokens == 0) return FX_OK;
+  // (a launch has fewer than 2^32 threads, 256 for each workgroup of either part)
+  if (((int64_t)r.tokens + FX_KV_STORE_MOST - 1) / FX_KV_STORE_MOST * c.heads * 2 + (int64_t)q.blocks * q.slices >= int64_t{1} << 24)
+    return fail(FX_E_LIMIT, "fx_kv_append: more rows than a launch holds");
+  HIP_OK(fx_launch_kv_append(c, r, q, cache->held, (hipStream_t)stream));
   return kv_launched(1);
 }
 
@@ -1829,38 +1878,6 @@ int fx_kv_attention(const fx_kv_cache* cache, const fx_kv_attention_desc* desc, 
   int launched = 0;
   HIP_OK(fx_launch_kv_attention(a, l, (hipStream_t)stream, &launched));
   return kv_launched(launched);
-}
-
-// ---- rotary positions (fx_rotary.hip) ----
-
-namespace {
-int rotary_of(const char* at, const fx_rotary_desc* desc, FxRotary& a) {
-  const std::string op(at);
-  if (!desc) return fail(FX_E_INVALID, op + ": null descriptor");
-  const fx_rotary_desc& d = *desc;
-  if (!kv_dtype(d.dtype)) return fail(FX_E_UNSUPPORTED, op + ": rows must be float32, float16 or bfloat16");
-  if (d.batch < 0 || d.tokens < 0 || d.heads < 1 || d.depth < 1) return fail(FX_E_INVALID, op + ": rows of no heads or columns, or a negative size");
-  if (d.pairs < 1 || (int64_t)d.pairs * 2 > d.depth)
-    return fail(FX_E_INVALID, op + ": at least one pair of columns turns, and " + std::to_string(d.depth) + " columns hold " + std::to_string(d.depth / 2) + " (got " + std::to_string(d.pairs) + ")");
-  if (d.pairs > FX_ROTARY_ANGLES) return fail(FX_E_UNSUPPORTED, op + ": more than " + std::to_string(FX_ROTARY_ANGLES) + " pairs");
-  if ((int64_t)d.heads * d.depth >= 1 << 28 || (int64_t)d.batch * d.tokens >= 1 << 30) return fail(FX_E_LIMIT, op + ": 2^28 numbers of a token, or 2^30 tokens");
-  a = FxRotary{FxTurns{d.positions, d.frequencies, d.pairs, d.positions_64 != 0, d.frequencies_32 != 0, d.interleaved != 0, d.back != 0, d.magnitude},
-               d.x, d.y, d.x_batch_stride, d.x_token_stride, d.x_head_stride, d.y_batch_stride, d.y_token_stride, d.y_head_stride, d.position_batch_stride,
-               d.batch, d.tokens, d.heads, d.depth, d.dtype};
-  if (d.batch == 0 || d.tokens == 0) return FX_OK;
-  if (!d.x || !d.y || !d.positions || !d.frequencies) return fail(FX_E_INVALID, op + ": null argument");
-  fx_rotary_shape(a);
-  if ((int64_t)a.blocks * a.slices >= 1 << 23) return fail(FX_E_LIMIT, op + ": more numbers than a launch holds");
-  return FX_OK;
-}
-}  // namespace
-
-int fx_rotary(const fx_rotary_desc* desc, void* stream) {
-  FxRotary a;
-  if (int rc = rotary_of("fx_rotary", desc, a)) return rc;
-  if (a.batch == 0 || a.tokens == 0) return FX_OK;
-  HIP_OK(fx_launch_rotary(a, (hipStream_t)stream));
-  return kv_launched(1);
 }
 
 // ---- detection tail (fx_nms.hip) ----

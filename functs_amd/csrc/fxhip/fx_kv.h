@@ -5,6 +5,7 @@
 
 #include "../../../include/fxhip.h"
 #include "fx_kv_split.h"
+#include "fx_rotary.h"
 
 // A cache as the kernels see it.  Keys [pages][heads][page][depth]; values [pages][heads][page / 16][depth][16]: the
 // second product of attention contracts over tokens, and a lane's operand is 8 or 16 of them side by side.
@@ -36,6 +37,7 @@ struct FxKvRows {
 #define FX_KV_STORE_MOST 63   // tokens that a workgroup of fx_kv_store takes at most: a lane each, and one for the token before them
 hipError_t fx_launch_kv_plan(const FxKvPlanArgs& a, hipStream_t stream);
 hipError_t fx_launch_kv_store(const FxKvCache& c, const FxKvRows& r, int held, hipStream_t stream);
+hipError_t fx_launch_kv_append(const FxKvCache& c, const FxKvRows& r, const FxRotary& q, int held, hipStream_t stream);
 hipError_t fx_launch_kv_read(const FxKvCache& c, const FxKvRows& r, int held, hipStream_t stream);
 
 #define FX_KV_ROWS 16   // rows (tokens of a request times query heads of a key head) of a tile of fx_kv_rows

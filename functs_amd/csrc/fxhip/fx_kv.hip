@@ -257,14 +257,6 @@ __global__ __launch_bounds__(kThreads) void fx_kv_read_kernel(const FxKvCache c,
   }
 }
 
-// tokens a wave takes: as many as leave some 8 192 waves (32 a CU), `most` at most
-int tokens_a_wave(const FxKvCache& c, const FxKvRows& r, int most) {
-  const int64_t per = (int64_t)r.tokens * c.heads * 2 / 8192;
-  return (int)(per < 1 ? 1 : per > most ? most : per);
-}
-bool aligned16(const void* p, int64_t a, int64_t b, size_t size) {
-  return ((uintptr_t)p & 15u) == 0 && a * (int64_t)size % 16 == 0 && b * (int64_t)size % 16 == 0;
-}
 }  // namespace
 
 hipError_t fx_launch_kv_plan(const FxKvPlanArgs& a, hipStream_t stream) {
@@ -278,15 +270,11 @@ hipError_t fx_launch_kv_store(const FxKvCache& c, const FxKvRows& r, int held, h
   static const void* const kernels[2][3] = {
       {(const void*)fx_kv_store_kernel<0, float>, (const void*)fx_kv_store_kernel<0, _Float16>, (const void*)fx_kv_store_kernel<0, __bf16>},
       {(const void*)fx_kv_store_kernel<1, float>, (const void*)fx_kv_store_kernel<1, _Float16>, (const void*)fx_kv_store_kernel<1, __bf16>}};
-  const size_t size = r.dtype == FX_DT_F32 ? 4 : 2;
-  // (a workgroup for each 32 tokens took 96 us where 63 take 73)
-  int per = std::max(std::min(tokens_a_wave(c, r, FX_KV_STORE_MOST) * kStoreWaves, FX_KV_STORE_MOST), kStoreWaves);
-  int vec = aligned16(r.k, r.k_token, r.k_head, size) && aligned16(r.v, r.v_token, r.v_head, size);
+  StoreShape shape = store_shape(c, r);
   FxKvCache cache = c;
   FxKvRows rows = r;
-  void* kargs[4] = {(void*)&cache, (void*)&rows, (void*)&per, (void*)&vec};
-  const int64_t grid = (int64_t)((r.tokens + per - 1) / per) * c.heads * 2;
-  return hipLaunchKernel(kernels[held][r.dtype == FX_DT_F32 ? 0 : r.dtype == FX_DT_F16 ? 1 : 2], dim3((unsigned)grid), dim3(kThreads), kargs, 0, stream);
+  void* kargs[4] = {(void*)&cache, (void*)&rows, (void*)&shape.per, (void*)&shape.vec};
+  return hipLaunchKernel(kernels[held][r.dtype == FX_DT_F32 ? 0 : r.dtype == FX_DT_F16 ? 1 : 2], dim3((unsigned)shape.blocks), dim3(kThreads), kargs, 0, stream);
 }
 
 hipError_t fx_launch_kv_read(const FxKvCache& c, const FxKvRows& r, int held, hipStream_t stream) {

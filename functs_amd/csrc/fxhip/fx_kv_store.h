@@ -1,6 +1,9 @@
 // How rows of keys and values become codes of the paged cache: the kernel of fx_kv_store (fx_kv.hip) and of
 // fx_kv_append (fx_kv_append.hip), whose keys turn on the way.
 #pragma once
+#include <algorithm>
+#include <type_traits>
+
 #include "fx_kv.h"
 #include "fx_kv_device.h"
 #include "fx_rotary_device.h"
@@ -130,16 +133,25 @@ __device__ __forceinline__ uint4 again16(uint4 w, float ratio, int n) {
 __device__ __forceinline__ int64_t lane_of(int64_t v, int lane) {   // in scalar registers
   return ((int64_t)__builtin_amdgcn_readlane((int)(v >> 32), lane) << 32) | (unsigned)__builtin_amdgcn_readlane((int)v, lane);
 }
-// One run, or a wave's share of it: rows [0, n) of `rows` go to offsets o0 on of a page (straight), or to those that `slots` says
-template <int HELD, class T, bool VALUES>
+// One run, or a wave's share of it: rows [0, n) of `rows` go to offsets o0 on of a page (straight), or to those that `slots` says.
+// TURN: keys turn by their tokens' positions ahead of all else, and are fp32 from then on.  The wave forms the angles of an iteration's rows
+// once (at most 256: 64 lanes of 8 columns, two to a pair) and keeps them in LDS; with halves apart a lane loads the other eight of its pairs too.
+// (Each lane forming its own eight angles: registers of 272 to 440 bytes a lane went through memory.)
+template <int HELD, class T, bool VALUES, bool TURN = false>
 struct StoreRun {
-  typedef typename Pack<T>::eight P8;
+  static_assert(!(VALUES && TURN), "values do not turn");
+  typedef std::conditional_t<TURN, float, T> N;   // what is kept of a number
+  typedef typename Pack<N>::eight P8;
   typedef typename Pack<T>::two P2;
   const T* rows;
   int64_t stride;
   int n, o0, D, lane;
   uint8_t* codes;
   bool vec;
+  const FxTurns* turns;    // TURN: what turns, the place of row 0's position, 2^32 / pairs, and where the wave keeps angles (kKept * 256 of them)
+  int64_t token;
+  unsigned magic_pair;
+  Turn* angles;
   // lane -> (row of an iteration, eight of its depth), or (group of an iteration, pair of columns)
   int width, abreast, sub, at, blocks, g0, count, iterations;
 
@@ -148,16 +160,104 @@ struct StoreRun {
     abreast = width >= 64 ? 1 : 64 / width;
     sub = lane / width;
     at = lane - sub * width;
+    if constexpr (TURN) sub = min(sub, abreast - 1);   // (all lanes form angles; those that are left over do the last row's columns again)
     blocks = width > 64 ? (width + 63) >> 6 : 1;   // (values of depth above 128)
     g0 = o0 >> 4;
     count = VALUES ? ((o0 + n + 15) >> 4) - g0 : n;
     iterations = (count + abreast - 1) / abreast * blocks;
   }
+  // column d of row j, as it is stored
+  __device__ __forceinline__ float number(int j, int d) const {
+    const T* p = rows + (int64_t)j * stride;
+    if constexpr (TURN) {
+      const int pairs = turns->pairs;
+      if (d < 2 * pairs) {
+        const bool upper = turns->interleaved ? (d & 1) != 0 : d >= pairs;
+        const int step = turns->interleaved ? 1 : pairs, pair = turns->interleaved ? d >> 1 : upper ? d - pairs : d;
+        float a = (float)p[upper ? d - step : d], b = (float)p[upper ? d : d + step];
+        turn_pair(a, b, turn_of(position_of(*turns, token + j), quarters_of(*turns, pair), turns->magnitude, false));
+        return upper ? b : a;
+      }
+    }
+    return (float)p[d];
+  }
+  // eight columns of a row as they are loaded, and the other eight of their pairs
+  struct Raw {
+    typename Pack<T>::eight own, other;
+  };
   // rows beyond the run: its last or first one again, which is in the maximum anyway and not written
-  __device__ __forceinline__ P8 load_eight(int k) const {
-    const T* p = rows + at * 8;
-    if ((k + 1) * abreast <= n) return load_numbers<T, 8, P8>(p + (int64_t)(k * abreast) * stride + (int64_t)sub * stride, vec);
-    return load_numbers<T, 8, P8>(p + (int64_t)min(k * abreast + sub, n - 1) * stride, vec);
+  __device__ __forceinline__ Raw load_raw(int k) const {
+    const int j = k * abreast + sub;
+    const T* p = rows + at * 8 + ((k + 1) * abreast <= n ? (int64_t)(k * abreast) * stride + (int64_t)sub * stride : (int64_t)min(j, n - 1) * stride);
+    Raw raw;
+    raw.own = load_numbers<T, 8, typename Pack<T>::eight>(p, vec);
+    if constexpr (TURN) {
+      const int pairs = turns->pairs, c0 = at * 8;
+      raw.other = raw.own;
+      if (!turns->interleaved && c0 < 2 * pairs) {
+        if (pairs % 8 == 0) {
+          raw.other = load_numbers<T, 8, typename Pack<T>::eight>(c0 < pairs ? p + pairs : p - pairs, vec);
+        } else {
+          union { typename Pack<T>::eight all; T e[8]; } w;
+          w.all = raw.own;
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (c0 + e < 2 * pairs) w.e[e] = p[c0 + e < pairs ? e + pairs : e - pairs];
+          raw.other = w.all;
+        }
+      }
+    }
+    return raw;
+  }
+  // the angles of iterations k0 on, `many` of them, to `angles`
+  __device__ __forceinline__ void form_angles(int k0, int many) const {
+    const int pairs = turns->pairs, row0 = k0 * abreast;
+    for (int i = lane; i < many * abreast * pairs; i += 64) {
+      const int j = (int)divided((unsigned)i, (unsigned)pairs, magic_pair);
+      angles[i] = turn_of(position_of(*turns, token + min(row0 + j, n - 1)), quarters_of(*turns, i - j * pairs), turns->magnitude, false);
+    }
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");   // (a wave's LDS accesses go in order)
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+  }
+  // k: of the iterations whose angles are kept
+  __device__ __forceinline__ P8 turned(const Raw& raw, int k) const {
+    if constexpr (!TURN) {
+      return raw.own;
+    } else {
+      union { P8 all; float x[8]; } y;
+      float other[8];
+      floats<T, 8>(y.x, raw.own);
+      floats<T, 8>(other, raw.other);
+      const int pairs = turns->pairs, c0 = at * 8;
+      const Turn* w = angles + (k * abreast + sub) * pairs;
+      if (c0 >= 2 * pairs) return y.all;
+      if (turns->interleaved) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (c0 + 2 * i < 2 * pairs) turn_pair(y.x[2 * i], y.x[2 * i + 1], w[c0 / 2 + i]);
+      } else if (pairs % 8 == 0) {
+        const bool upper = c0 >= pairs;
+        w += upper ? c0 - pairs : c0;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          float a = upper ? other[e] : y.x[e], b = upper ? y.x[e] : other[e];
+          turn_pair(a, b, w[e]);
+          y.x[e] = upper ? b : a;
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const bool upper = c0 + e >= pairs;
+          float a = upper ? other[e] : y.x[e], b = upper ? y.x[e] : other[e];
+          if (c0 + e < 2 * pairs) {
+            turn_pair(a, b, w[upper ? c0 + e - pairs : c0 + e]);
+            y.x[e] = upper ? b : a;
+          }
+        }
+      }
+      return y.all;
+    }
   }
   __device__ __forceinline__ int group_of(int k) const { return blocks > 1 ? k / blocks : k * abreast + sub; }
   __device__ __forceinline__ int pair_of(int k) const { return blocks > 1 ? at + (k % blocks) * 64 : at; }
@@ -182,7 +282,7 @@ struct StoreRun {
     const int j = k * abreast + sub;
     if (j >= n) return;
     float x[8];
-    floats<T, 8>(x, p);
+    floats<N, 8>(x, p);
     *(uint2*)(codes + (o0 + j) * D + at * 8) = make_uint2(codes4<HELD, PLAIN>(x, inv), codes4<HELD, PLAIN>(x + 4, inv));
   }
   template <bool PLAIN>
@@ -241,7 +341,8 @@ struct StoreRun {
         load_column(c, k);
         write_column<PLAIN>(k, c, inv, ratio);
       } else {
-        write_eight<PLAIN>(k, load_eight(k), inv);
+        if constexpr (TURN) form_angles(k, 1);
+        write_eight<PLAIN>(k, turned(load_raw(k), 0), inv);
       }
     }
   }
@@ -257,20 +358,28 @@ struct StoreRun {
       n = max(to - from, 0);
       o0 += from;
       rows += (int64_t)from * stride;
+      if constexpr (TURN) token += from;
     }
     shape();
     P8 kept8[VALUES ? 1 : kKept];
     P2 kept2[VALUES ? kKept : 1][16];
-    const bool keep = iterations <= kKept, used = sub < abreast;
+    const bool keep = iterations <= kKept, used = TURN || sub < abreast;
     unsigned m = 0;
     if (straight && used) {
       if (keep) {
+        Raw raw[VALUES ? 1 : kKept];
 #pragma unroll
         for (int k = 0; k < kKept; ++k) {
           if (k < iterations) {
             if constexpr (VALUES) load_column(kept2[k], k);
-            else kept8[k] = load_eight(k);
+            else raw[k] = load_raw(k);
           }
+        }
+        if constexpr (!VALUES) {
+          if constexpr (TURN) form_angles(0, iterations);
+#pragma unroll
+          for (int k = 0; k < kKept; ++k)
+            if (k < iterations) kept8[k] = turned(raw[k], k);
         }
 #pragma unroll
         for (int k = 0; k < kKept; ++k) {
@@ -279,7 +388,7 @@ struct StoreRun {
 #pragma unroll
               for (int e = 0; e < 16; ++e) m = Pack<T>::see(m, kept2[k][e]);
             } else {
-              m = Pack<T>::see(m, kept8[k]);
+              m = Pack<N>::see(m, kept8[k]);
             }
           }
         }
@@ -292,26 +401,27 @@ struct StoreRun {
 #pragma unroll
             for (int e = 0; e < 16; ++e) m = Pack<T>::see(m, c[e]);
           } else {
-            m = Pack<T>::see(m, load_eight(k));
+            if constexpr (TURN) form_angles(k, 1);
+            m = Pack<N>::see(m, turned(load_raw(k), 0));
           }
         }
       }
     }
-    m = wave_largest<sizeof(T) == 2>(m);
+    m = wave_largest<sizeof(N) == 2>(m);
     if (tops) {
       if (lane == 0) tops[wave] = m;
       __syncthreads();   // (and the scale has been read)
       m = 0;
 #pragma unroll
-      for (int w = 0; w < kStoreWaves; ++w) m = Pack<T>::larger(m, tops[w]);
+      for (int w = 0; w < kStoreWaves; ++w) m = Pack<N>::larger(m, tops[w]);
     }
-    float top = Pack<T>::value(m);
+    float top = Pack<N>::value(m);
     constexpr float kMost = HELD == 0 ? 448.0f * 0x1p119f : 127.0f * 0x1p121f;
     const bool plain = straight && top <= kMost;
     if (!plain) {   // infinities or NaN (or slots in any order): the largest finite one
       float t = 0.0f;
       for (int j = 0; j < n; ++j)
-        for (int d = lane; d < D; d += 64) t = fmaxf(t, finite_abs((float)rows[(int64_t)j * stride + d]));
+        for (int d = lane; d < D; d += 64) t = fmaxf(t, finite_abs(number(j, d)));
       top = wave_max64(t);
       if (tops) {
         __syncthreads();
@@ -348,7 +458,7 @@ struct StoreRun {
     for (int j = 0; j < n; ++j) {
       const int o = (int)(slots[j] & page_mask);
       for (int d = lane; d < D; d += 64) {
-        const float x[4] = {(float)rows[(int64_t)j * stride + d] * inv, 0.0f, 0.0f, 0.0f};
+        const float x[4] = {number(j, d) * inv, 0.0f, 0.0f, 0.0f};
         const uint8_t code = (uint8_t)encode4<HELD>(x);
         if (VALUES) codes[((o >> 4) * D + d) * 16 + (o & 15)] = code;
         else codes[o * D + d] = code;
@@ -357,12 +467,12 @@ struct StoreRun {
   }
 };
 
-template <int HELD, class T>
-__global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 5 : 4) void fx_kv_store_kernel(const FxKvCache c, const FxKvRows r, int per, int vec) {
-  __shared__ unsigned s_tops[2][kStoreWaves];
+// A workgroup's keys or values of one head.  q, angles (4 * kKept * 256 of them): of keys that turn (TURN), by the positions of all tokens
+template <int HELD, class T, bool TURN>
+__device__ __forceinline__ void store_chunk(const FxKvCache& c, const FxKvRows& r, int per, int vec, unsigned block, const FxRotary* q, Turn* angles, unsigned (*s_tops)[kStoreWaves]) {
   const int lane = (int)threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-  const unsigned chunk_head = blockIdx.x >> 1;
-  const int half = (int)(blockIdx.x & 1), chunk = (int)(chunk_head / (unsigned)c.heads), head = (int)(chunk_head - (unsigned)chunk * (unsigned)c.heads);
+  const unsigned chunk_head = block >> 1;
+  const int half = (int)(block & 1), chunk = (int)(chunk_head / (unsigned)c.heads), head = (int)(chunk_head - (unsigned)chunk * (unsigned)c.heads);
   const int D = c.depth, page = 1 << c.log_page;
   const int64_t n_slots = (int64_t)c.pages << c.log_page;
   const int t0 = chunk * per, t1 = min(r.tokens, t0 + per);
@@ -400,11 +510,12 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 5 : 4) void fx_kv_store_
     const int o0 = (int)(s0 & (page - 1));
     const int64_t in_page = (int64_t)head * page * D;
     if (half == 0) {
-      StoreRun<HELD, T, false> run;
+      StoreRun<HELD, T, false, TURN> run;
       run.rows = (const T*)r.k + (int64_t)t * r.k_token + (int64_t)head * r.k_head;
       run.stride = r.k_token;
       run.n = n, run.o0 = o0, run.D = D, run.vec = vec != 0;
       run.codes = c.k + p * c.k_stride + in_page;
+      if constexpr (TURN) run.turns = &q->turns, run.token = t, run.magic_pair = q->magic_pair, run.angles = angles + wave * (4 * 256);
       run.run(straight, r.slots + t, page - 1, c.k_scale + p * c.ks_stride + head, tops);
     } else {
       StoreRun<HELD, T, true> run;
@@ -415,5 +526,34 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 5 : 4) void fx_kv_store_
       run.run(straight, r.slots + t, page - 1, c.v_scale + p * c.vs_stride + head, tops);
     }
   }
+}
+
+template <int HELD, class T>
+__global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 5 : 4) void fx_kv_store_kernel(const FxKvCache c, const FxKvRows r, int per, int vec) {
+  __shared__ unsigned s_tops[2][kStoreWaves];
+  store_chunk<HELD, T, false>(c, r, per, vec, blockIdx.x, nullptr, nullptr, s_tops);
+}
+
+// tokens a wave takes: as many as leave some 8 192 waves (32 a CU), `most` at most
+inline int tokens_a_wave(const FxKvCache& c, const FxKvRows& r, int most) {
+  const int64_t per = (int64_t)r.tokens * c.heads * 2 / 8192;
+  return (int)(per < 1 ? 1 : per > most ? most : per);
+}
+inline bool aligned16(const void* p, int64_t a, int64_t b, size_t size) {
+  return ((uintptr_t)p & 15u) == 0 && a * (int64_t)size % 16 == 0 && b * (int64_t)size % 16 == 0;
+}
+// How the tokens of a call that stores are dealt out: `per` tokens a workgroup, a key head, keys and values apart
+struct StoreShape {
+  int per, vec;
+  int64_t blocks;
+};
+inline StoreShape store_shape(const FxKvCache& c, const FxKvRows& r) {
+  const size_t size = r.dtype == FX_DT_F32 ? 4 : 2;
+  StoreShape s;
+  // (a workgroup for each 32 tokens took 96 us where 63 take 73)
+  s.per = std::max(std::min(tokens_a_wave(c, r, FX_KV_STORE_MOST) * kStoreWaves, FX_KV_STORE_MOST), kStoreWaves);
+  s.vec = aligned16(r.k, r.k_token, r.k_head, size) && aligned16(r.v, r.v_token, r.v_head, size);
+  s.blocks = (int64_t)((r.tokens + s.per - 1) / s.per) * c.heads * 2;
+  return s;
 }
 }  // namespace

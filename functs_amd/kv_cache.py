@@ -7,10 +7,11 @@ pages, keys and values are codes of one byte (float8_e4m3fn or int8) under a sca
     cache = KvCache.empty(pages, heads, page_size, depth)
     step = cache.plan(past_lens, new_lens, block_table, free_pages, max_tokens)   # once a step
     cache.store(k, v, step.slots)                                                 # in every layer
+    q = cache.append(q, k, v, step.slots, step.positions, frequencies)            # (the same for a model with rotary positions)
     out, lse = cache.attention(q, block_table, step.lens, step.starts)
     k, v = cache.read(slots, torch.bfloat16)                                      # the numbers again
 
-The same four calls are TorchScript operators on the cache's tensors: torch.ops.functs.kv_plan, kv_store, kv_read,
+The same calls are TorchScript operators on the cache's tensors: torch.ops.functs.kv_plan, kv_store, kv_append, kv_read,
 kv_attention.  Lengths, tables and slots are read on the device and nothing waits for it: a step captured into a graph
 serves any lengths that fit its tensors.  include/fxhip.h defines the layout, the codes and every rule.
 
@@ -77,6 +78,12 @@ class KvCache:
         """Writes rows k, v [tokens, heads, depth] to `slots`.  The rows of one page are neighbours, as plan() lays them; a page
         starts anew where the first of them is its first token."""
         torch.ops.functs.kv_store(k, v, self.k, self.v, self.k_scale, self.v_scale, slots)
+
+    def append(self, q: Tensor, k: Tensor, v: Tensor, slots: Tensor, positions: Tensor, frequencies: Tensor, magnitude: float = 1.0,
+               interleaved: bool = False) -> Tensor:
+        """store() of keys that turn by their tokens' positions on the way (functs_amd.rotary), in fp32 and rounded once, to their codes.  Returns
+        the queries q [tokens, query heads, depth] turned, as rotary.rotary() gives them; one launch for all."""
+        return torch.ops.functs.kv_append(q, k, v, self.k, self.v, self.k_scale, self.v_scale, slots, positions, frequencies, magnitude, interleaved)
 
     def read(self, slots: Tensor, dtype: torch.dtype = torch.float32) -> Tuple[Tensor, Tensor]:
         """Keys and values [tokens, heads, depth] at `slots`, as numbers; zeros for slots outside the cache."""

@@ -496,12 +496,37 @@ int fx_attention_steps(const float* x, const float* k, const float* v, const flo
                        const float* wo, float* k_out, float* v_out, float* x_out, int batch, int heads, int depth, int rows,
                        int start, int steps, float scale, float k_add, float v_add, void* stream);
 
+/* ---- rotary positions ----
+ * Of a head's `depth` columns the first 2 * pairs turn, pair i of a token at position p by the angle p * frequencies[i]:
+ *   (a, b) -> magnitude * (a cos - b sin, b cos + a sin)          back: magnitude * (a cos + b sin, b cos - a sin), the gradient's
+ * where (a, b) are columns i and i + pairs, or 2 i and 2 i + 1 (interleaved); the other columns are copied.  y may not overlap x.
+ * The angle is formed in 64 bits (an error of about |p| frequency / 2^53), its cosine and sine are off by 2^-23 at most, products are fp32 and
+ * y is rounded once.  x [batch][tokens][heads][depth], a depth contiguous, strides in elements, any alignment of its numbers; positions int32, or
+ * int64 (positions_64), the tokens' side by side, position_batch_stride apart (0: all batches have the same); frequencies double, or float
+ * (frequencies_32): what they hold counts as exact.  1 <= pairs <= 2048, 2 * pairs <= depth, heads * depth < 2^28, batch * tokens < 2^30. */
+typedef struct fx_rotary_desc {
+  const void* x;
+  void* y;
+  const void* positions;
+  const void* frequencies;
+  int64_t x_batch_stride, x_token_stride, x_head_stride;
+  int64_t y_batch_stride, y_token_stride, y_head_stride;
+  int64_t position_batch_stride;
+  int32_t batch, tokens, heads, depth, pairs;
+  int32_t dtype; /* FX_DT_F32, FX_DT_F16, FX_DT_BF16 */
+  int32_t positions_64, frequencies_32, interleaved, back;
+  float magnitude;
+  int32_t reserved;
+} fx_rotary_desc;
+int fx_rotary(const fx_rotary_desc* desc, void* stream);
+
 /* ---- a paged key / value cache held in 8 bits ----
  * What fx_attention_steps keeps in two fp32 tensors of one length (functs/benchmark/simpleops/attention/attention.py:38-58),
  * for many requests of any length: pages of `page_size` tokens that requests share, a table of pages for each
  * request, keys and values in 8 bits with a scale for each page and head.
  *   fx_kv_plan       where the tokens of a step go: pages, slots, positions, offsets, from the requests' lengths
  *   fx_kv_store      writes keys and values
+ *   fx_kv_append     the same with rotary positions: keys turn on the way, queries beside them
  *   fx_kv_read       gives them back as numbers
  *   fx_kv_attention  attention over them: single tokens, a few, or whole prompts behind what is cached
  * Everything that changes from step to step (lengths, tables, slots) is read on the device: a captured call serves any lengths
@@ -574,6 +599,11 @@ typedef struct fx_kv_rows {
  * (as fx_kv_plan lays them): two groups of rows for one page leave what either wrote.  Slots outside the cache are passed over.
  * A call has fewer than 63 * 2^23 rows of all heads, fx_kv_read too. */
 int fx_kv_store(const fx_kv_cache* cache, const fx_kv_rows* rows, void* stream);
+/* fx_kv_store of keys that turn (fx_rotary) by their tokens' positions, and the queries of the same tokens turned, in one launch.
+ * queries: a descriptor of fx_rotary with batch 1, back 0 and the rows' tokens, depth and dtype; any number of heads.  Its positions, frequencies,
+ * magnitude and layout are the keys' as well, and its y holds fx_rotary's results bit for bit.  Keys turn in fp32 and are rounded once, to their
+ * codes, and their scales are of the turned numbers.  Rows whose slot is outside the cache turn all the same. */
+int fx_kv_append(const fx_kv_cache* cache, const fx_kv_rows* rows, const fx_rotary_desc* queries, void* stream);
 /* The numbers at `slots`, in any order, rounded once to dtype; zeros for slots outside the cache. */
 int fx_kv_read(const fx_kv_cache* cache, const fx_kv_rows* rows, void* stream);
 
@@ -615,30 +645,6 @@ typedef struct fx_kv_attention_desc {
 } fx_kv_attention_desc;
 size_t fx_kv_attention_workspace_bytes(const fx_kv_cache* cache, const fx_kv_attention_desc* desc);
 int fx_kv_attention(const fx_kv_cache* cache, const fx_kv_attention_desc* desc, void* stream);
-
-/* ---- rotary positions ----
- * Of a head's `depth` columns the first 2 * pairs turn, pair i of a token at position p by the angle p * frequencies[i]:
- *   (a, b) -> magnitude * (a cos - b sin, b cos + a sin)          back: magnitude * (a cos + b sin, b cos - a sin), the gradient's
- * where (a, b) are columns i and i + pairs, or 2 i and 2 i + 1 (interleaved); the other columns are copied.  y may not overlap x.
- * The angle is formed in 64 bits (an error of about |p| frequency / 2^53), its cosine and sine are off by 2^-23 at most, products are fp32 and
- * y is rounded once.  x [batch][tokens][heads][depth], a depth contiguous, strides in elements, any alignment of its numbers; positions int32, or
- * int64 (positions_64), the tokens' side by side, position_batch_stride apart (0: all batches have the same); frequencies double, or float
- * (frequencies_32): what they hold counts as exact.  1 <= pairs <= 2048, 2 * pairs <= depth, heads * depth < 2^28, batch * tokens < 2^30. */
-typedef struct fx_rotary_desc {
-  const void* x;
-  void* y;
-  const void* positions;
-  const void* frequencies;
-  int64_t x_batch_stride, x_token_stride, x_head_stride;
-  int64_t y_batch_stride, y_token_stride, y_head_stride;
-  int64_t position_batch_stride;
-  int32_t batch, tokens, heads, depth, pairs;
-  int32_t dtype; /* FX_DT_F32, FX_DT_F16, FX_DT_BF16 */
-  int32_t positions_64, frequencies_32, interleaved, back;
-  float magnitude;
-  int32_t reserved;
-} fx_rotary_desc;
-int fx_rotary(const fx_rotary_desc* desc, void* stream);
 
 /* ---- detection tail: score threshold + sort + class-aware greedy NMS + top-k, one launch ----
  * The step behind row compaction in the reference's detection programs, which it runs as ATen /
