@@ -6,38 +6,32 @@
 #include "fx_kv_store.h"
 
 namespace {
-template <int HELD, class T>
+template <int HELD, class T, bool INTER>
 __global__ __launch_bounds__(kThreads, 3) void fx_kv_append_kernel(const FxKvCache c, const FxKvRows r, int per, int vec, unsigned stores, const FxRotary q) {
   __shared__ unsigned s_tops[2][kStoreWaves];
-  __shared__ Turn s_turn[kStoreWaves * 4 * 256];
-  static_assert(kStoreWaves * 4 * 256 >= FX_ROTARY_ANGLES, "both parts' angles");
+  __shared__ Turn s_turn[FX_ROTARY_ANGLES];
   constexpr int PV = sizeof(T) == 4 ? 4 : 8;
   if (blockIdx.x < stores) {
-    store_chunk<HELD, T, true>(c, r, per, vec, blockIdx.x, &q, s_turn, s_tops);
+    store_chunk<HELD, T, true, INTER>(c, r, per, vec, blockIdx.x, &q.turns, s_tops);
     return;
   }
   const unsigned share = blockIdx.x - stores;
   const int block = (int)(share / (unsigned)q.slices), slice = (int)(share % (unsigned)q.slices);
-  if (q.turns.pairs >= PV) {
-    if (q.turns.interleaved) rotary_rows<T, PV, true>(q, block, slice, s_turn);
-    else rotary_rows<T, PV, false>(q, block, slice, s_turn);
-  } else {
-    if (q.turns.interleaved) rotary_rows<T, 1, true>(q, block, slice, s_turn);
-    else rotary_rows<T, 1, false>(q, block, slice, s_turn);
-  }
+  if (q.turns.pairs >= PV) rotary_rows<T, PV, INTER>(q, block, slice, s_turn);
+  else rotary_rows<T, 1, INTER>(q, block, slice, s_turn);
 }
 }  // namespace
 
 hipError_t fx_launch_kv_append(const FxKvCache& c, const FxKvRows& r, const FxRotary& q, int held, hipStream_t stream) {
-  static const void* const kernels[2][3] = {
-      {(const void*)fx_kv_append_kernel<0, float>, (const void*)fx_kv_append_kernel<0, _Float16>, (const void*)fx_kv_append_kernel<0, __bf16>},
-      {(const void*)fx_kv_append_kernel<1, float>, (const void*)fx_kv_append_kernel<1, _Float16>, (const void*)fx_kv_append_kernel<1, __bf16>}};
+#define FX_ROW(H, T) {(const void*)fx_kv_append_kernel<H, T, false>, (const void*)fx_kv_append_kernel<H, T, true>}
+  static const void* const kernels[2][3][2] = {{FX_ROW(0, float), FX_ROW(0, _Float16), FX_ROW(0, __bf16)}, {FX_ROW(1, float), FX_ROW(1, _Float16), FX_ROW(1, __bf16)}};
+#undef FX_ROW
   StoreShape shape = store_shape(c, r);
   FxKvCache cache = c;
   FxKvRows rows = r;
   FxRotary queries = q;
   unsigned stores = (unsigned)shape.blocks;
   void* kargs[6] = {(void*)&cache, (void*)&rows, (void*)&shape.per, (void*)&shape.vec, (void*)&stores, (void*)&queries};
-  return hipLaunchKernel(kernels[held][r.dtype == FX_DT_F32 ? 0 : r.dtype == FX_DT_F16 ? 1 : 2], dim3(stores + (unsigned)q.blocks * (unsigned)q.slices), dim3(kThreads),
-                         kargs, 0, stream);
+  const int type = r.dtype == FX_DT_F32 ? 0 : r.dtype == FX_DT_F16 ? 1 : 2;
+  return hipLaunchKernel(kernels[held][type][q.turns.interleaved ? 1 : 0], dim3(stores + (unsigned)q.blocks * (unsigned)q.slices), dim3(kThreads), kargs, 0, stream);
 }

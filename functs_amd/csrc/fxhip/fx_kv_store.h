@@ -134,10 +134,12 @@ __device__ __forceinline__ int64_t lane_of(int64_t v, int lane) {   // in scalar
   return ((int64_t)__builtin_amdgcn_readlane((int)(v >> 32), lane) << 32) | (unsigned)__builtin_amdgcn_readlane((int)v, lane);
 }
 // One run, or a wave's share of it: rows [0, n) of `rows` go to offsets o0 on of a page (straight), or to those that `slots` says.
-// TURN: keys turn by their tokens' positions ahead of all else, and are fp32 from then on.  The wave forms the angles of an iteration's rows
-// once (at most 256: 64 lanes of 8 columns, two to a pair) and keeps them in LDS; with halves apart a lane loads the other eight of its pairs too.
-// (Each lane forming its own eight angles: registers of 272 to 440 bytes a lane went through memory.)
-template <int HELD, class T, bool VALUES, bool TURN = false>
+// TURN: keys turn by their tokens' positions ahead of all else, and are fp32 from then on.  A lane has 8 pairs of a row (16 of its columns, or 16
+// that do not turn), forms their angles by itself and keeps the turned numbers of two iterations; where the units of a row do not fit, the last one
+// begins earlier and does some columns again.  INTER: pairs are neighbours.  Angles are formed for each head anew: 2 us of the chip's vector units for
+// 10 565 tokens, 8 heads and 32 pairs, of 69.  Slower, with queries, keys and values of that call: 8 columns a lane, angles shared by a wave in LDS and
+// numbers in registers 82 us, numbers in LDS as well 88; four waves a SIMD instead of three (registers go through memory) 76.
+template <int HELD, class T, bool VALUES, bool TURN = false, bool INTER = false>
 struct StoreRun {
   static_assert(!(VALUES && TURN), "values do not turn");
   typedef std::conditional_t<TURN, float, T> N;   // what is kept of a number
@@ -148,23 +150,48 @@ struct StoreRun {
   int n, o0, D, lane;
   uint8_t* codes;
   bool vec;
-  const FxTurns* turns;    // TURN: what turns, the place of row 0's position, 2^32 / pairs, and where the wave keeps angles (kKept * 256 of them)
+  const FxTurns* turns;    // TURN: what turns, and the place of row 0's position
   int64_t token;
-  unsigned magic_pair;
-  Turn* angles;
+  double quarters[TURN ? 8 : 1];
+  int lo, hi, n_lo, n_hi;  // the lane's columns: n_lo from lo on, n_hi from hi on, 8 each but at the ends
+  bool turning;
   // lane -> (row of an iteration, eight of its depth), or (group of an iteration, pair of columns)
   int width, abreast, sub, at, blocks, g0, count, iterations;
 
   __device__ __forceinline__ void shape() {
     width = VALUES ? D >> 1 : D >> 3;
+    if constexpr (TURN) {
+      const int pairs = turns->pairs, rest = D - 2 * pairs;
+      width = ((pairs + 7) >> 3) + ((rest + 15) >> 4);
+    }
     abreast = width >= 64 ? 1 : 64 / width;
     sub = lane / width;
     at = lane - sub * width;
-    if constexpr (TURN) sub = min(sub, abreast - 1);   // (all lanes form angles; those that are left over do the last row's columns again)
     blocks = width > 64 ? (width + 63) >> 6 : 1;   // (values of depth above 128)
     g0 = o0 >> 4;
     count = VALUES ? ((o0 + n + 15) >> 4) - g0 : n;
     iterations = (count + abreast - 1) / abreast * blocks;
+    if constexpr (TURN) {
+      const int pairs = turns->pairs, rest = D - 2 * pairs, units = (pairs + 7) >> 3;
+      turning = at < units;
+      if (turning) {
+        const int first = max(min(at * 8, pairs - 8), 0), some = min(pairs, 8);
+        lo = INTER ? 2 * first : first;
+        hi = INTER ? lo + 8 : first + pairs;
+        n_lo = INTER ? min(2 * some, 8) : some;
+        n_hi = INTER ? 2 * some - n_lo : some;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) quarters[i] = quarters_of(*turns, min(first + i, pairs - 1));
+      } else {
+        const int some = min(rest, 16);
+        lo = 2 * pairs + max(min((at - units) * 16, rest - 16), 0);
+        hi = lo + 8;
+        n_lo = min(some, 8);
+        n_hi = some - n_lo;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) quarters[i] = 0.0;
+      }
+    }
   }
   // column d of row j, as it is stored
   __device__ __forceinline__ float number(int j, int d) const {
@@ -181,83 +208,78 @@ struct StoreRun {
     }
     return (float)p[d];
   }
-  // eight columns of a row as they are loaded, and the other eight of their pairs
-  struct Raw {
-    typename Pack<T>::eight own, other;
-  };
   // rows beyond the run: its last or first one again, which is in the maximum anyway and not written
-  __device__ __forceinline__ Raw load_raw(int k) const {
-    const int j = k * abreast + sub;
-    const T* p = rows + at * 8 + ((k + 1) * abreast <= n ? (int64_t)(k * abreast) * stride + (int64_t)sub * stride : (int64_t)min(j, n - 1) * stride);
-    Raw raw;
-    raw.own = load_numbers<T, 8, typename Pack<T>::eight>(p, vec);
-    if constexpr (TURN) {
-      const int pairs = turns->pairs, c0 = at * 8;
-      raw.other = raw.own;
-      if (!turns->interleaved && c0 < 2 * pairs) {
-        if (pairs % 8 == 0) {
-          raw.other = load_numbers<T, 8, typename Pack<T>::eight>(c0 < pairs ? p + pairs : p - pairs, vec);
-        } else {
-          union { typename Pack<T>::eight all; T e[8]; } w;
-          w.all = raw.own;
-#pragma unroll
-          for (int e = 0; e < 8; ++e)
-            if (c0 + e < 2 * pairs) w.e[e] = p[c0 + e < pairs ? e + pairs : e - pairs];
-          raw.other = w.all;
-        }
-      }
-    }
-    return raw;
+  __device__ __forceinline__ typename Pack<T>::eight load_eight(int k) const {
+    typedef typename Pack<T>::eight P;
+    const T* p = rows + at * 8;
+    if ((k + 1) * abreast <= n) return load_numbers<T, 8, P>(p + (int64_t)(k * abreast) * stride + (int64_t)sub * stride, vec);
+    return load_numbers<T, 8, P>(p + (int64_t)min(k * abreast + sub, n - 1) * stride, vec);
   }
-  // the angles of iterations k0 on, `many` of them, to `angles`
-  __device__ __forceinline__ void form_angles(int k0, int many) const {
-    const int pairs = turns->pairs, row0 = k0 * abreast;
-    for (int i = lane; i < many * abreast * pairs; i += 64) {
-      const int j = (int)divided((unsigned)i, (unsigned)pairs, magic_pair);
-      angles[i] = turn_of(position_of(*turns, token + min(row0 + j, n - 1)), quarters_of(*turns, i - j * pairs), turns->magnitude, false);
-    }
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");   // (a wave's LDS accesses go in order)
-    __builtin_amdgcn_wave_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-  }
-  // k: of the iterations whose angles are kept
-  __device__ __forceinline__ P8 turned(const Raw& raw, int k) const {
-    if constexpr (!TURN) {
-      return raw.own;
+  // TURN: the lane's columns of a row as they are loaded
+  struct Raw { typename Pack<T>::eight lo, hi; };
+  __device__ __forceinline__ int row_of(int k) const { return min(k * abreast + sub, n - 1); }
+  __device__ __forceinline__ void load_sixteen(Raw& raw, int k) const {
+    const T* p = rows + (int64_t)row_of(k) * stride;
+    if (n_lo + n_hi == 16) {
+      __builtin_memcpy(&raw.lo, p + lo, sizeof raw.lo);
+      __builtin_memcpy(&raw.hi, p + hi, sizeof raw.hi);
     } else {
-      union { P8 all; float x[8]; } y;
-      float other[8];
-      floats<T, 8>(y.x, raw.own);
-      floats<T, 8>(other, raw.other);
-      const int pairs = turns->pairs, c0 = at * 8;
-      const Turn* w = angles + (k * abreast + sub) * pairs;
-      if (c0 >= 2 * pairs) return y.all;
-      if (turns->interleaved) {
+      union { typename Pack<T>::eight all; T e[8]; } a, b;
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (c0 + 2 * i < 2 * pairs) turn_pair(y.x[2 * i], y.x[2 * i + 1], w[c0 / 2 + i]);
-      } else if (pairs % 8 == 0) {
-        const bool upper = c0 >= pairs;
-        w += upper ? c0 - pairs : c0;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          float a = upper ? other[e] : y.x[e], b = upper ? y.x[e] : other[e];
-          turn_pair(a, b, w[e]);
-          y.x[e] = upper ? b : a;
-        }
-      } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const bool upper = c0 + e >= pairs;
-          float a = upper ? other[e] : y.x[e], b = upper ? y.x[e] : other[e];
-          if (c0 + e < 2 * pairs) {
-            turn_pair(a, b, w[upper ? c0 + e - pairs : c0 + e]);
-            y.x[e] = upper ? b : a;
-          }
-        }
+      for (int i = 0; i < 8; ++i) {
+        a.e[i] = i < n_lo ? p[lo + i] : (T)0.0f;
+        b.e[i] = i < n_hi ? p[hi + i] : (T)0.0f;
       }
-      return y.all;
+      raw.lo = a.all;
+      raw.hi = b.all;
     }
+  }
+  // x: the first of each pair, then the others (of columns that do not turn: in the same order)
+  __device__ __forceinline__ void turn_sixteen(float (&x)[16], const Raw& raw, double position) const {
+    float u[8], v[8];
+    floats<T, 8>(u, raw.lo);
+    floats<T, 8>(v, raw.hi);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      x[i] = INTER ? (i < 4 ? u[2 * i % 8] : v[2 * i % 8]) : u[i];
+      x[8 + i] = INTER ? (i < 4 ? u[(2 * i + 1) % 8] : v[(2 * i + 1) % 8]) : v[i];
+    }
+    if (turning) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        turn_pair(x[i], x[8 + i], turn_of(position, quarters[i], turns->magnitude, false));
+        if (i % 2 == 1) __builtin_amdgcn_sched_barrier(0);   // (eight angles at once take 40 registers more)
+      }
+    }
+  }
+  template <bool PLAIN>
+  __device__ __forceinline__ void write_sixteen(int k, const float (&x)[16], float inv) const {
+    const int j = k * abreast + sub;
+    if (j >= n || sub >= abreast) return;
+    float y[16];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      y[INTER ? 2 * i : i] = x[i];
+      y[INTER ? 2 * i + 1 : 8 + i] = x[8 + i];
+    }
+    uint8_t* to = codes + (o0 + j) * D;
+    const unsigned u[4] = {codes4<HELD, PLAIN>(y, inv), codes4<HELD, PLAIN>(y + 4, inv), codes4<HELD, PLAIN>(y + 8, inv), codes4<HELD, PLAIN>(y + 12, inv)};
+    if (n_lo + n_hi == 16) {
+      __builtin_memcpy(to + lo, u, 8);
+      __builtin_memcpy(to + hi, u + 2, 8);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        if (i < n_lo) to[lo + i] = (uint8_t)(u[i >> 2] >> (8 * (i & 3)));
+        if (i < n_hi) to[hi + i] = (uint8_t)(u[2 + (i >> 2)] >> (8 * (i & 3)));
+      }
+    }
+  }
+  static constexpr int kTurned = 2;   // iterations whose turned numbers stay in registers
+  static __device__ __forceinline__ unsigned largest_of(unsigned m, const float (&x)[16]) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) m = max(m, __float_as_uint(x[i]) & 0x7fffffffu);
+    return m;
   }
   __device__ __forceinline__ int group_of(int k) const { return blocks > 1 ? k / blocks : k * abreast + sub; }
   __device__ __forceinline__ int pair_of(int k) const { return blocks > 1 ? at + (k % blocks) * 64 : at; }
@@ -323,7 +345,23 @@ struct StoreRun {
   }
   static constexpr int kKept = VALUES ? 1 : 4;   // iterations whose numbers stay in registers: more of them cost waves
   template <bool PLAIN>
-  __device__ __forceinline__ void write(const P8 (&kept8)[VALUES ? 1 : kKept], const P2 (&kept2)[VALUES ? kKept : 1][16], bool keep, float inv, float ratio) const {
+  __device__ __forceinline__ void write(const P8 (&kept8)[VALUES ? 1 : kKept], const P2 (&kept2)[VALUES ? kKept : 1][16], const float (&turned16)[TURN ? kTurned : 1][16], bool keep, float inv, float ratio) const {
+    if constexpr (TURN) {
+      if (iterations <= kTurned) {
+#pragma unroll
+        for (int k = 0; k < kTurned; ++k)
+          if (k < iterations) write_sixteen<PLAIN>(k, turned16[k], inv);
+        return;
+      }
+#pragma unroll 1
+      for (int k = 0; k < iterations; ++k) {
+        Raw raw;
+        load_sixteen(raw, k);
+        float x[16];
+        turn_sixteen(x, raw, position_of(*turns, token + row_of(k)));
+        write_sixteen<PLAIN>(k, x, inv);
+      }
+    } else {
     if (keep) {
 #pragma unroll
       for (int k = 0; k < kKept; ++k) {
@@ -341,9 +379,9 @@ struct StoreRun {
         load_column(c, k);
         write_column<PLAIN>(k, c, inv, ratio);
       } else {
-        if constexpr (TURN) form_angles(k, 1);
-        write_eight<PLAIN>(k, turned(load_raw(k), 0), inv);
+        write_eight<PLAIN>(k, load_eight(k), inv);
       }
+    }
     }
   }
 
@@ -363,23 +401,44 @@ struct StoreRun {
     shape();
     P8 kept8[VALUES ? 1 : kKept];
     P2 kept2[VALUES ? kKept : 1][16];
-    const bool keep = iterations <= kKept, used = TURN || sub < abreast;
+    float turned16[TURN ? kTurned : 1][16];
+    const bool keep = iterations <= kKept, used = sub < abreast;
     unsigned m = 0;
     if (straight && used) {
-      if (keep) {
-        Raw raw[VALUES ? 1 : kKept];
+      if constexpr (TURN) {
+        if (iterations <= kTurned) {
+          Raw raw[kTurned];
+          double position[kTurned];
+#pragma unroll
+          for (int k = 0; k < kTurned; ++k) {
+            if (k < iterations) {
+              load_sixteen(raw[k], k);
+              position[k] = position_of(*turns, token + row_of(k));
+            }
+          }
+#pragma unroll
+          for (int k = 0; k < kTurned; ++k) {
+            if (k < iterations) {
+              turn_sixteen(turned16[k], raw[k], position[k]);
+              m = largest_of(m, turned16[k]);
+            }
+          }
+        } else {
+#pragma unroll 1
+          for (int k = 0; k < iterations; ++k) {
+            Raw raw;
+            load_sixteen(raw, k);
+            turn_sixteen(turned16[0], raw, position_of(*turns, token + row_of(k)));
+            m = largest_of(m, turned16[0]);
+          }
+        }
+      } else if (keep) {
 #pragma unroll
         for (int k = 0; k < kKept; ++k) {
           if (k < iterations) {
             if constexpr (VALUES) load_column(kept2[k], k);
-            else raw[k] = load_raw(k);
+            else kept8[k] = load_eight(k);
           }
-        }
-        if constexpr (!VALUES) {
-          if constexpr (TURN) form_angles(0, iterations);
-#pragma unroll
-          for (int k = 0; k < kKept; ++k)
-            if (k < iterations) kept8[k] = turned(raw[k], k);
         }
 #pragma unroll
         for (int k = 0; k < kKept; ++k) {
@@ -388,7 +447,7 @@ struct StoreRun {
 #pragma unroll
               for (int e = 0; e < 16; ++e) m = Pack<T>::see(m, kept2[k][e]);
             } else {
-              m = Pack<N>::see(m, kept8[k]);
+              m = Pack<T>::see(m, kept8[k]);
             }
           }
         }
@@ -401,8 +460,7 @@ struct StoreRun {
 #pragma unroll
             for (int e = 0; e < 16; ++e) m = Pack<T>::see(m, c[e]);
           } else {
-            if constexpr (TURN) form_angles(k, 1);
-            m = Pack<N>::see(m, turned(load_raw(k), 0));
+            m = Pack<T>::see(m, load_eight(k));
           }
         }
       }
@@ -449,8 +507,8 @@ struct StoreRun {
     const float inv = 1.0f / scale;   // (a power of two: exact)
     if (straight) {
       if (!used) return;
-      if (plain) write<true>(kept8, kept2, keep, inv, ratio);
-      else write<false>(kept8, kept2, keep, inv, ratio);
+      if (plain) write<true>(kept8, kept2, turned16, keep, inv, ratio);
+      else write<false>(kept8, kept2, turned16, keep, inv, ratio);
       return;
     }
     // slots in any order: token by token, so that of two rows for one slot the later one stays
@@ -467,9 +525,9 @@ struct StoreRun {
   }
 };
 
-// A workgroup's keys or values of one head.  q, angles (4 * kKept * 256 of them): of keys that turn (TURN), by the positions of all tokens
-template <int HELD, class T, bool TURN>
-__device__ __forceinline__ void store_chunk(const FxKvCache& c, const FxKvRows& r, int per, int vec, unsigned block, const FxRotary* q, Turn* angles, unsigned (*s_tops)[kStoreWaves]) {
+// A workgroup's keys or values of one head.  turns: of keys that turn (TURN), by the positions of all tokens
+template <int HELD, class T, bool TURN, bool INTER>
+__device__ __forceinline__ void store_chunk(const FxKvCache& c, const FxKvRows& r, int per, int vec, unsigned block, const FxTurns* turns, unsigned (*s_tops)[kStoreWaves]) {
   const int lane = (int)threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const unsigned chunk_head = block >> 1;
   const int half = (int)(block & 1), chunk = (int)(chunk_head / (unsigned)c.heads), head = (int)(chunk_head - (unsigned)chunk * (unsigned)c.heads);
@@ -510,12 +568,12 @@ __device__ __forceinline__ void store_chunk(const FxKvCache& c, const FxKvRows& 
     const int o0 = (int)(s0 & (page - 1));
     const int64_t in_page = (int64_t)head * page * D;
     if (half == 0) {
-      StoreRun<HELD, T, false, TURN> run;
+      StoreRun<HELD, T, false, TURN, INTER> run;
       run.rows = (const T*)r.k + (int64_t)t * r.k_token + (int64_t)head * r.k_head;
       run.stride = r.k_token;
       run.n = n, run.o0 = o0, run.D = D, run.vec = vec != 0;
       run.codes = c.k + p * c.k_stride + in_page;
-      if constexpr (TURN) run.turns = &q->turns, run.token = t, run.magic_pair = q->magic_pair, run.angles = angles + wave * (4 * 256);
+      if constexpr (TURN) run.turns = turns, run.token = t;
       run.run(straight, r.slots + t, page - 1, c.k_scale + p * c.ks_stride + head, tops);
     } else {
       StoreRun<HELD, T, true> run;
@@ -531,7 +589,7 @@ __device__ __forceinline__ void store_chunk(const FxKvCache& c, const FxKvRows& 
 template <int HELD, class T>
 __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 5 : 4) void fx_kv_store_kernel(const FxKvCache c, const FxKvRows r, int per, int vec) {
   __shared__ unsigned s_tops[2][kStoreWaves];
-  store_chunk<HELD, T, false>(c, r, per, vec, blockIdx.x, nullptr, nullptr, s_tops);
+  store_chunk<HELD, T, false, false>(c, r, per, vec, blockIdx.x, nullptr, s_tops);
 }
 
 // tokens a wave takes: as many as leave some 8 192 waves (32 a CU), `most` at most
