@@ -49,6 +49,7 @@ hipError_t fx_cmap_resident(uint32_t lds_bytes, uint32_t* wide, uint32_t* narrow
 uint32_t fx_cmap_lds_bytes(const FxCmapLaunch& hl);
 uint32_t fx_cmap_chunk_rows();
 #include "fx_attn.h"
+#include "fx_beam.h"
 #include "fx_kv.h"
 #include "fx_rotary.h"
 #include "fx_lstm_sched.h"
@@ -1878,6 +1879,67 @@ int fx_kv_attention(const fx_kv_cache* cache, const fx_kv_attention_desc* desc, 
   int launched = 0;
   HIP_OK(fx_launch_kv_attention(a, l, (hipStream_t)stream, &launched));
   return kv_launched(launched);
+}
+
+// ---- a beam search's selection (fx_beam.hip) ----
+
+namespace {
+int beam_of(const fx_beam_select_desc* desc, FxBeamArgs& a) {
+  static const std::string op = "fx_beam_select";
+  if (!desc) return fail(FX_E_INVALID, op + ": null descriptor");
+  const fx_beam_select_desc& d = *desc;
+  if (!kv_dtype(d.dtype)) return fail(FX_E_UNSUPPORTED, op + ": logits must be float32, float16 or bfloat16");
+  if (d.requests < 0) return fail(FX_E_INVALID, op + ": negative size");
+  if (d.beams < 1 || d.beams > FX_BEAM_MAX_BEAMS || d.count < 1 || d.count > FX_BEAM_MAX_COUNT || d.words < 1 || d.words > FX_BEAM_MAX_WORDS)
+    return fail(FX_E_UNSUPPORTED, op + ": 1 to " + std::to_string(FX_BEAM_MAX_BEAMS) + " beams, 1 to " + std::to_string(FX_BEAM_MAX_COUNT) + " continuations and 1 to " +
+                                      std::to_string(FX_BEAM_MAX_WORDS) + " words (got " + std::to_string(d.beams) + ", " + std::to_string(d.count) + ", " + std::to_string(d.words) + ")");
+  memset(&a, 0, sizeof a);
+  a.logits = d.logits;
+  a.l_request = d.request_stride;
+  a.l_beam = d.beam_stride;
+  a.scores = d.scores;
+  a.ended = d.ended;
+  a.out_scores = d.out_scores;
+  a.out_beams = d.out_beams;
+  a.out_words = d.out_words;
+  a.end_word = d.end_word;
+  a.requests = d.requests;
+  a.beams = d.beams;
+  a.words = d.words;
+  a.count = d.count;
+  a.dtype = d.dtype;
+  fx_beam_shape(a);
+  // (a launch has fewer than 2^32 threads: 64 for each part of a row, 1 024 for each request)
+  if ((int64_t)d.requests * d.beams * a.chunks >= (int64_t{1} << 26) - 4 || d.requests >= 1 << 22) return fail(FX_E_LIMIT, op + ": more rows than a launch holds");
+  return FX_OK;
+}
+size_t beam_workspace(FxBeamArgs& a, char* base) {
+  const size_t parts = (size_t)a.requests * a.beams * a.chunks;
+  a.parts = (FxBeamPart*)base;
+  a.lists = (FxBeamWord*)(base + parts * sizeof(FxBeamPart));
+  return parts * (sizeof(FxBeamPart) + a.count * sizeof(FxBeamWord));
+}
+}  // namespace
+
+size_t fx_beam_select_workspace_bytes(const fx_beam_select_desc* desc) {
+  FxBeamArgs a;
+  if (beam_of(desc, a) != FX_OK) return 0;
+  return std::max<size_t>(beam_workspace(a, nullptr), 16);
+}
+
+int fx_beam_select(const fx_beam_select_desc* desc, void* stream) {
+  FxBeamArgs a;
+  if (int rc = beam_of(desc, a)) return rc;
+  if (a.requests == 0) return FX_OK;
+  if (!a.logits || !a.scores || !a.out_scores || !a.out_beams || !a.out_words) return fail(FX_E_INVALID, "fx_beam_select: null argument");
+  if (!desc->workspace || ((uintptr_t)desc->workspace & 15u) != 0 || desc->workspace_bytes < fx_beam_select_workspace_bytes(desc))
+    return fail(FX_E_INVALID, "fx_beam_select: workspace must be 16-byte aligned and hold fx_beam_select_workspace_bytes()");
+  beam_workspace(a, (char*)desc->workspace);
+  int launched = 0;
+  const hipError_t e = fx_launch_beam_select(a, (hipStream_t)stream, &launched);
+  kv_launched(launched);
+  HIP_OK(e);
+  return FX_OK;
 }
 
 // ---- detection tail (fx_nms.hip) ----

@@ -646,6 +646,37 @@ typedef struct fx_kv_attention_desc {
 size_t fx_kv_attention_workspace_bytes(const fx_kv_cache* cache, const fx_kv_attention_desc* desc);
 int fx_kv_attention(const fx_kv_cache* cache, const fx_kv_attention_desc* desc, void* stream);
 
+/* ---- a beam search's selection ----
+ * Of each request the `count` best continuations of all its beams: candidate (beam k, word w) has the total
+ *   scores[k] + (logits[k][w] - log sum_v exp(logits[k][v]))
+ * formed in 64 bits (the sum's terms, exp(logit - largest), in fp32) and rounded to fp32 for out_scores.  Larger totals go first, equal ones by beam, within a
+ * beam larger logits, then lower words.  No candidates have: words whose logit is -infinity (masked), rows of nothing else, rows that hold a NaN or +infinity,
+ * beams whose score is -infinity or NaN (there is none yet, or none any more).  A beam that has ended (ended: one byte each, or null) has one candidate, end_word
+ * with the beam's score, whatever its logits are, which are not read.  Where there are fewer than `count`, the places behind have -infinity, beam -1 and word -1.
+ * logits [requests][beams][words], a beam's words side by side, strides in elements, any alignment of its numbers; scores and ended [requests][beams], out_* [requests][count]
+ * contiguous.  beams: 1 to 32, count: 1 to 64, words: 1 to 2^18.
+ * workspace: fx_beam_select_workspace_bytes() of device memory for each call under way, 16-byte aligned; nothing is expected in it.  Two launches. */
+#define FX_BEAM_MAX_BEAMS 32
+#define FX_BEAM_MAX_COUNT 64
+#define FX_BEAM_MAX_WORDS 262144
+typedef struct fx_beam_select_desc {
+  const void* logits;
+  const float* scores;
+  const uint8_t* ended;
+  int64_t request_stride, beam_stride;
+  int64_t end_word;
+  float* out_scores;
+  int32_t* out_beams;
+  int64_t* out_words;
+  int32_t requests, beams, words, count;
+  int32_t dtype; /* of the logits: FX_DT_F32, FX_DT_F16, FX_DT_BF16 */
+  int32_t reserved;
+  void* workspace;
+  size_t workspace_bytes;
+} fx_beam_select_desc;
+size_t fx_beam_select_workspace_bytes(const fx_beam_select_desc* desc);
+int fx_beam_select(const fx_beam_select_desc* desc, void* stream);
+
 /* ---- detection tail: score threshold + sort + class-aware greedy NMS + top-k, one launch ----
  * The step behind row compaction in the reference's detection programs, which it runs as ATen /
  * torchvision kernels with host synchronisations in between:
