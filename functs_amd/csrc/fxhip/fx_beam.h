@@ -5,7 +5,8 @@
 
 #include "../../../include/fxhip.h"
 
-// What a wave finds in its part of a row: the largest logit, the sum of exp(logit - top), and behind it the best `count` (x, word), best first
+// What a wave finds in its part of a row: the largest logit, the sum of 2^(x c - r) (NaN where there is one in the part), and in a list of its own
+// the best `count` (x, word), best first
 struct FxBeamPart {
   float top;
   float unused;
