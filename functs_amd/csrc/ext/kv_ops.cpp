@@ -6,11 +6,14 @@
 //   functs::kv_append     the same with rotary positions: keys turn on the way, queries beside them
 //   functs::kv_read       gives them back as numbers
 //   functs::kv_attention  attention over them
+//   functs::kv_fork       the tables behind a beam search's selection: pages shared, to be copied, free again
+//   functs::kv_copy       copies pages, in all layers at once
 // Nothing here waits for the device or reads from it: a captured call serves other lengths when it is replayed.
 #include <torch/library.h>
 
 #include <cmath>
 #include <tuple>
+#include <vector>
 
 #include "rotary_ops.h"
 
@@ -269,6 +272,77 @@ void attend(const Tensor& q_, const Tensor& k_cache, const Tensor& v_cache, cons
   FX_OK_OR_THROW(fx_kv_attention(&c, &d, streamOf(dev)));
 }
 
+std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> kvFork(const Tensor& parents_, const Tensor& lens_, Tensor block_table, const Tensor& free_pages, int64_t page_size,
+                                                          const std::optional<Tensor>& free_start) {
+  static const char op[] = "functs::kv_fork";
+  TORCH_CHECK(block_table.is_cuda(), op, " runs on the GPU only; block_table is a ", block_table.device(), " tensor");
+  const auto dev = block_table.device();
+  onGpu(op, parents_, "parents", dev);
+  TORCH_CHECK(parents_.scalar_type() == at::kInt && parents_.dim() == 2, op, ": parents must be int32 [groups, beams], got ", parents_.scalar_type(), " ", parents_.sizes());
+  const int64_t G = parents_.size(0), K = parents_.size(1);
+  TORCH_CHECK(block_table.scalar_type() == at::kInt && block_table.dim() == 2 && block_table.size(0) == G * K && (block_table.size(1) <= 1 || block_table.stride(1) == 1), op,
+              ": block_table must be int32 [", G * K, ", columns], columns side by side, got ", block_table.scalar_type(), " ", block_table.sizes());
+  c10::DeviceGuard guard(dev);
+  const Tensor parents = parents_.contiguous(), lens = ints(op, lens_, "lens", G * K, dev), pages = ints(op, free_pages, "free_pages", -1, dev);
+  Tensor from;
+  if (free_start && free_start->defined()) {
+    onGpu(op, *free_start, "free_start", dev);
+    TORCH_CHECK(free_start->scalar_type() == at::kInt && free_start->numel() == 1, op, ": free_start must be one int32");
+    from = *free_start;
+  }
+  TORCH_CHECK(page_size >= 16 && page_size <= 256, op, ": page_size must be 16, 32, 64, 128 or 256, got ", page_size);
+  fx_kv_fork_desc d;
+  memset(&d, 0, sizeof d);
+  d.groups = sized(op, G, "the number of groups");
+  d.beams = sized(op, K, "the number of beams");
+  d.columns = sized(op, block_table.size(1), "the number of columns");
+  d.n_free = sized(op, pages.numel(), "the number of free pages");
+  d.page_size = (int32_t)page_size;
+  const size_t bytes = fx_kv_fork_workspace_bytes(&d);
+  TORCH_CHECK(bytes > 0, "fxhip: ", fx_last_error(), " (", op, ")");
+  const auto i32 = at::TensorOptions().dtype(at::kInt).device(dev);
+  const Tensor ws = at::empty({(int64_t)bytes}, i32.dtype(at::kByte));
+  Tensor out_lens = at::empty({G * K}, i32), copies = at::empty({G * K, 3}, i32), taken = at::empty({1}, i32), freed = at::empty({G * K * block_table.size(1)}, i32),
+         n_freed = at::empty({1}, i32);
+  d.parents = parents.data_ptr<int32_t>();
+  d.lens = lens.data_ptr<int32_t>();
+  d.table = block_table.data_ptr<int32_t>();
+  d.table_stride = block_table.stride(0);
+  d.free_pages = pages.data_ptr<int32_t>();
+  d.free_start = from.defined() ? from.data_ptr<int32_t>() : nullptr;
+  d.out_lens = out_lens.data_ptr<int32_t>();
+  d.copies = copies.data_ptr<int32_t>();
+  d.taken = taken.data_ptr<int32_t>();
+  d.freed = freed.data_ptr<int32_t>();
+  d.n_freed = n_freed.data_ptr<int32_t>();
+  d.workspace = ws.data_ptr();
+  d.workspace_bytes = bytes;
+  FX_OK_OR_THROW(fx_kv_fork(&d, streamOf(dev)));
+  written(block_table);
+  return {out_lens, copies, taken, freed, n_freed};
+}
+
+void kvCopy(at::TensorList k_caches, at::TensorList v_caches, at::TensorList k_scales, at::TensorList v_scales, const Tensor& copies_) {
+  static const char op[] = "functs::kv_copy";
+  const size_t L = k_caches.size();
+  TORCH_CHECK(v_caches.size() == L && k_scales.size() == L && v_scales.size() == L, op, ": as many k_caches as v_caches, k_scales and v_scales, got ", L, ", ", v_caches.size(),
+              ", ", k_scales.size(), " and ", v_scales.size());
+  TORCH_CHECK(copies_.is_cuda(), op, " runs on the GPU only; copies is a ", copies_.device(), " tensor");
+  const auto dev = copies_.device();
+  TORCH_CHECK(copies_.scalar_type() == at::kInt && copies_.dim() == 2 && copies_.size(1) == 3, op, ": copies must be int32 [rows, 3], got ", copies_.scalar_type(), " ",
+              copies_.sizes());
+  std::vector<fx_kv_cache> caches;
+  for (size_t i = 0; i < L; ++i) {
+    caches.push_back(cacheOf(op, k_caches[i], v_caches[i], k_scales[i], v_scales[i]));
+    onGpu(op, k_caches[i], "k_caches", dev);
+  }
+  c10::DeviceGuard guard(dev);
+  const Tensor copies = copies_.contiguous();
+  FX_OK_OR_THROW(fx_kv_copy(caches.data(), sized(op, (int64_t)L, "the number of caches"), copies.data_ptr<int32_t>(), sized(op, copies.size(0), "the number of rows"), streamOf(dev)));
+  for (const at::TensorList& list : {k_caches, v_caches, k_scales, v_scales})
+    for (const Tensor& t : list) written(t);
+}
+
 std::tuple<Tensor, Tensor> kvAttention(const Tensor& q, const Tensor& k_cache, const Tensor& v_cache, const Tensor& k_scale, const Tensor& v_scale,
                                        const Tensor& block_table, const Tensor& lens, const Tensor& starts, double scale, int64_t window, int64_t max_new) {
   Tensor out, lse;
@@ -293,6 +367,9 @@ TORCH_LIBRARY_FRAGMENT(functs, m) {
   m.def("kv_append(Tensor q, Tensor k, Tensor v, Tensor(a!) k_cache, Tensor(b!) v_cache, Tensor(c!) k_scale, Tensor(d!) v_scale, Tensor slots, "
         "Tensor positions, Tensor frequencies, float magnitude=1.0, bool interleaved=False) -> Tensor", kvAppend);
   m.def("kv_read(Tensor k_cache, Tensor v_cache, Tensor k_scale, Tensor v_scale, Tensor slots, ScalarType dtype) -> (Tensor, Tensor)", kvRead);
+  m.def("kv_fork(Tensor parents, Tensor lens, Tensor(a!) block_table, Tensor free_pages, int page_size, Tensor? free_start=None) -> "
+        "(Tensor, Tensor, Tensor, Tensor, Tensor)", kvFork);
+  m.def("kv_copy(Tensor(a!)[] k_caches, Tensor(b!)[] v_caches, Tensor(c!)[] k_scales, Tensor(d!)[] v_scales, Tensor copies) -> ()", kvCopy);
   m.def("kv_attention(Tensor q, Tensor k_cache, Tensor v_cache, Tensor k_scale, Tensor v_scale, Tensor block_table, Tensor lens, Tensor starts, "
         "float scale, int window=0, int max_new=0) -> (Tensor, Tensor)", kvAttention);
   m.def("kv_attention.out(Tensor q, Tensor k_cache, Tensor v_cache, Tensor k_scale, Tensor v_scale, Tensor block_table, Tensor lens, Tensor starts, "

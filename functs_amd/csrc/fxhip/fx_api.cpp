@@ -51,6 +51,7 @@ uint32_t fx_cmap_chunk_rows();
 #include "fx_attn.h"
 #include "fx_beam.h"
 #include "fx_kv.h"
+#include "fx_kv_fork.h"
 #include "fx_rotary.h"
 #include "fx_lstm_sched.h"
 int fx_launch_lstm_stack(const FxLstmArgs& a, int L, uint32_t* words_ctl, uint32_t* die_ctl, hipStream_t stream);
@@ -1879,6 +1880,108 @@ int fx_kv_attention(const fx_kv_cache* cache, const fx_kv_attention_desc* desc, 
   int launched = 0;
   HIP_OK(fx_launch_kv_attention(a, l, (hipStream_t)stream, &launched));
   return kv_launched(launched);
+}
+
+// ---- pages behind a beam search's selection (fx_kv_fork.hip) ----
+
+namespace {
+int fork_of(const fx_kv_fork_desc* desc, FxKvForkArgs& a) {
+  static const std::string op = "fx_kv_fork";
+  if (!desc) return fail(FX_E_INVALID, op + ": null descriptor");
+  const fx_kv_fork_desc& d = *desc;
+  const int log_page = log_page_of(d.page_size);
+  if (log_page < 0) return fail(FX_E_UNSUPPORTED, op + ": page_size must be 16, 32, 64, 128 or 256 (got " + std::to_string(d.page_size) + ")");
+  if (d.beams < 1 || d.beams > FX_BEAM_MAX_BEAMS)
+    return fail(FX_E_UNSUPPORTED, op + ": 1 to " + std::to_string(FX_BEAM_MAX_BEAMS) + " beams a group (got " + std::to_string(d.beams) + ")");
+  if (d.groups < 0 || d.columns < 0 || d.n_free < 0) return fail(FX_E_INVALID, op + ": negative size");
+  const int64_t blocks = ((int64_t)d.columns + FX_KV_FORK_COLUMNS - 1) / FX_KV_FORK_COLUMNS;
+  // (a launch has fewer than 2^32 threads, 256 for each block of columns of a group; freed pages are counted in 31 bits)
+  if ((int64_t)d.groups * d.beams >= 1 << 26 || (int64_t)d.groups * blocks >= 1 << 24 || (int64_t)d.groups * d.beams * d.columns >= int64_t{1} << 31 ||
+      ((int64_t)d.columns << log_page) > int64_t{1} << 30)
+    return fail(FX_E_LIMIT, op + ": 2^26 rows, 2^31 entries, or more than 2^30 tokens of one row");
+  memset(&a, 0, sizeof a);
+  a.parents = d.parents;
+  a.lens = d.lens;
+  a.free_pages = d.free_pages;
+  a.free_start = d.free_start;
+  a.table = d.table;
+  a.out_lens = d.out_lens;
+  a.copies = d.copies;
+  a.taken = d.taken;
+  a.freed = d.freed;
+  a.n_freed = d.n_freed;
+  a.table_stride = d.table_stride;
+  a.groups = d.groups;
+  a.beams = d.beams;
+  a.columns = d.columns;
+  a.n_free = d.n_free;
+  a.log_page = log_page;
+  a.blocks = (int32_t)blocks;
+  return FX_OK;
+}
+size_t fork_workspace(FxKvForkArgs& a, char* base) {
+  const size_t rows = (size_t)a.groups * a.beams, units = (size_t)a.groups * a.blocks;
+  a.rows = (FxKvForkRow*)base;
+  a.counts = (int32_t*)(base + rows * sizeof(FxKvForkRow));
+  a.lists = a.counts + units;
+  return rows * sizeof(FxKvForkRow) + units * (1 + (size_t)a.beams * FX_KV_FORK_COLUMNS) * sizeof(int32_t);
+}
+}  // namespace
+
+size_t fx_kv_fork_workspace_bytes(const fx_kv_fork_desc* desc) {
+  FxKvForkArgs a;
+  if (fork_of(desc, a) != FX_OK) return 0;
+  return std::max<size_t>(fork_workspace(a, nullptr), 16);
+}
+
+int fx_kv_fork(const fx_kv_fork_desc* desc, void* stream) {
+  FxKvForkArgs a;
+  if (int rc = fork_of(desc, a)) return rc;
+  const bool rows = a.groups > 0, entries = rows && a.columns > 0;
+  if (!a.taken || !a.n_freed || (rows && (!a.parents || !a.lens || !a.out_lens || !a.copies)) || (entries && (!a.table || !a.freed)) || (a.n_free > 0 && !a.free_pages))
+    return fail(FX_E_INVALID, "fx_kv_fork: null argument");
+  if ((int64_t)a.groups * a.beams > 1 && a.table_stride < a.columns) return fail(FX_E_INVALID, "fx_kv_fork: rows of the table overlap");
+  if (!desc->workspace || ((uintptr_t)desc->workspace & 15u) != 0 || desc->workspace_bytes < fx_kv_fork_workspace_bytes(desc))
+    return fail(FX_E_INVALID, "fx_kv_fork: workspace must be 16-byte aligned and hold fx_kv_fork_workspace_bytes()");
+  fork_workspace(a, (char*)desc->workspace);
+  int launched = 0;
+  const hipError_t e = fx_launch_kv_fork(a, (hipStream_t)stream, &launched);
+  kv_launched(launched);
+  HIP_OK(e);
+  return FX_OK;
+}
+
+int fx_kv_copy(const fx_kv_cache* caches, int n_caches, const int32_t* copies, int rows, void* stream) {
+  static const char at[] = "fx_kv_copy";
+  if (n_caches < 0 || rows < 0) return fail(FX_E_INVALID, "fx_kv_copy: negative size");
+  if (n_caches == 0) return FX_OK;
+  if (!caches || (rows > 0 && !copies)) return fail(FX_E_INVALID, "fx_kv_copy: null argument");
+  if (rows >= 1 << 26) return fail(FX_E_LIMIT, "fx_kv_copy: 2^26 rows");
+  FxKvCopyArgs a;
+  memset(&a, 0, sizeof a);
+  for (int i = 0; i < n_caches; ++i) {   // all of them are looked at before the first launch
+    FxKvCache c;
+    if (int rc = kv_cache_of(at, caches + i, c)) return rc;
+    if (i == 0) a.c = c;
+    if (c.pages != a.c.pages || c.heads != a.c.heads || c.depth != a.c.depth || c.log_page != a.c.log_page || c.k_stride != a.c.k_stride || c.v_stride != a.c.v_stride ||
+        c.ks_stride != a.c.ks_stride || c.vs_stride != a.c.vs_stride || caches[i].held != caches[0].held)
+      return fail(FX_E_INVALID, "fx_kv_copy: the caches must have the same sizes, types and strides");
+  }
+  if (rows == 0) return FX_OK;
+  a.copies = copies;
+  a.rows = rows;
+  a.heads_a_unit = std::max(std::max(16384 / ((1 << a.c.log_page) * a.c.depth), 1), (a.c.heads + 63) / 64);
+  a.units_a_page = (a.c.heads + a.heads_a_unit - 1) / a.heads_a_unit;
+  for (int i = 0; i < n_caches; i += FX_KV_COPY_LAYERS) {
+    a.layers = std::min(n_caches - i, FX_KV_COPY_LAYERS);
+    for (int l = 0; l < a.layers; ++l) {
+      const fx_kv_cache& c = caches[i + l];
+      a.layer[l] = {(uint8_t*)c.k, (uint8_t*)c.v, c.k_scale, c.v_scale};
+    }
+    HIP_OK(fx_launch_kv_copy(a, (hipStream_t)stream));
+    kv_launched(1);
+  }
+  return FX_OK;
 }
 
 // ---- a beam search's selection (fx_beam.hip) ----

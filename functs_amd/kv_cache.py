@@ -10,14 +10,16 @@ pages, keys and values are codes of one byte (float8_e4m3fn or int8) under a sca
     q = cache.append(q, k, v, step.slots, step.positions, frequencies)            # (the same for a model with rotary positions)
     out, lse = cache.attention(q, block_table, step.lens, step.starts)
     k, v = cache.read(slots, torch.bfloat16)                                      # the numbers again
+    fork = cache.fork(parents, lens, block_table, free_pages)                     # beams: behind their selection (functs_amd.beam)
+    copy_pages(layers, fork.copies)                                               # in all layers at once
 
 The same calls are TorchScript operators on the cache's tensors: torch.ops.functs.kv_plan, kv_store, kv_append, kv_read,
-kv_attention.  Lengths, tables and slots are read on the device and nothing waits for it: a step captured into a graph
+kv_attention, kv_fork, kv_copy.  Lengths, tables and slots are read on the device and nothing waits for it: a step captured into a graph
 serves any lengths that fit its tensors.  include/fxhip.h defines the layout, the codes and every rule.
 
 GPU tensors only: there is no host fallback, and no backward pass (codes are steps).
 """
-from typing import NamedTuple, Optional, Tuple
+from typing import NamedTuple, Optional, Sequence, Tuple
 
 import torch
 from torch import Tensor
@@ -39,6 +41,22 @@ class Step(NamedTuple):
     starts: Tensor
     lens: Tensor
     taken: Tensor
+
+
+class Fork(NamedTuple):
+    """What KvCache.fork says.  lens [rows]: tokens of the new rows, 0 where a row continues none or got no page; copies [rows, 3]: (page, to page, tokens) for copy_pages,
+    -1, -1, 0 where nothing is to be copied; taken [1]: how many of the free pages were given out; freed [rows * columns]: pages that no row has any more, the first
+    n_freed[0] of them, -1 behind."""
+    lens: Tensor
+    copies: Tensor
+    taken: Tensor
+    freed: Tensor
+    n_freed: Tensor
+
+
+def copy_pages(caches: Sequence["KvCache"], copies: Tensor) -> None:
+    """Copies pages as Fork.copies says, in all caches (layers of a model, of the same sizes) at once."""
+    torch.ops.functs.kv_copy([c.k for c in caches], [c.v for c in caches], [c.k_scale for c in caches], [c.v_scale for c in caches], copies)
 
 
 class KvCache:
@@ -73,6 +91,12 @@ class KvCache:
         other in arrays of max_tokens rows.  New pages come from free_pages (from free_pages[free_start[0]] on), request by request,
         and are entered in block_table [requests, columns]; a request that does not fit gets nothing."""
         return Step(*torch.ops.functs.kv_plan(past_lens, new_lens, block_table, free_pages, self.page_size, max_tokens, free_start))
+
+    def fork(self, parents: Tensor, lens: Tensor, block_table: Tensor, free_pages: Tensor, free_start: Optional[Tensor] = None) -> Fork:
+        """The tables of beams behind a selection: row g * beams + j of block_table [groups * beams, columns] continues row g * beams + parents[g, j] (int32 [groups, beams], as
+        beam.select() gives them) with its lens[] tokens.  Full pages are shared; a partly filled one has one owner, the other rows that continue it get pages of rows that
+        nobody continues, or free ones, and are to be copied.  Call it once a step, and copy_pages() for all layers before anything is stored."""
+        return Fork(*torch.ops.functs.kv_fork(parents, lens, block_table, free_pages, self.page_size, free_start))
 
     def store(self, k: Tensor, v: Tensor, slots: Tensor) -> None:
         """Writes rows k, v [tokens, heads, depth] to `slots`.  The rows of one page are neighbours, as plan() lays them; a page

@@ -529,6 +529,8 @@ int fx_rotary(const fx_rotary_desc* desc, void* stream);
  *   fx_kv_append     the same with rotary positions: keys turn on the way, queries beside them
  *   fx_kv_read       gives them back as numbers
  *   fx_kv_attention  attention over them: single tokens, a few, or whole prompts behind what is cached
+ *   fx_kv_fork       behind a beam search's selection: which pages each beam has now, which have to be copied, which are free again
+ *   fx_kv_copy       copies them, in all layers at once
  * Everything that changes from step to step (lengths, tables, slots) is read on the device: a captured call serves any lengths
  * that fit its tensors.  Indices are checked there: pages and slots outside the cache are passed over.
  *
@@ -645,6 +647,45 @@ typedef struct fx_kv_attention_desc {
 } fx_kv_attention_desc;
 size_t fx_kv_attention_workspace_bytes(const fx_kv_cache* cache, const fx_kv_attention_desc* desc);
 int fx_kv_attention(const fx_kv_cache* cache, const fx_kv_attention_desc* desc, void* stream);
+
+/* Rows of the table are beams, `beams` of each group (request); new row j of group g continues the group's old row parents[g][j], with all its lens[] tokens
+ * (lens: of the old rows, outside 0 .. columns * page_size counts as 0; a row has the pages of its table that its tokens lie in).
+ *   Pages that are full are shared: table rows name the same ones.  A page that is partly filled belongs to one row: of the new rows that continue it the first
+ *   keeps it, each other one gets a page of its own, into which its tokens have to be copied: one of those of its group's old rows that nobody continues
+ *   (in their order), else the next of free_pages (from free_pages[free_start[0]] on; free_start null: 0), group by group, row by row.
+ *   out_lens[r]   tokens of the new row: 0 where parents is outside 0 .. beams - 1, or no page was left for it; its row of the table is left as it was then
+ *   copies[r]     (page, to page, tokens) that the row needs copied, or (-1, -1, 0)
+ *   taken[0]      how many of free_pages were given out
+ *   freed, n_freed[0]   pages that an old row of a group had and no new one has, each once: group by group, column by column, row by row; -1 behind them
+ * Pages are told apart by their numbers, column by column within a group: a page stands in one column, and in the rows of one group.  Entries below 0 are no pages:
+ * they are moved with the others, and neither copied nor freed.
+ * The table is changed in place (rows table_stride apart, entries behind a row's tokens left as they were).  All arrays are int32 on the device: parents, lens, out_lens
+ * [groups * beams], copies [groups * beams][3], freed [groups * beams * columns].  beams: 1 to 32.
+ * workspace: fx_kv_fork_workspace_bytes() of device memory for each call under way, 16-byte aligned; nothing is expected in it.  Three launches. */
+typedef struct fx_kv_fork_desc {
+  const int32_t* parents;
+  const int32_t* lens;
+  int32_t* table;
+  int64_t table_stride;
+  const int32_t* free_pages;
+  const int32_t* free_start;
+  int32_t* out_lens;
+  int32_t* copies;
+  int32_t* taken;
+  int32_t* freed;
+  int32_t* n_freed;
+  int32_t groups, beams, columns, n_free, page_size;
+  int32_t reserved;
+  void* workspace;
+  size_t workspace_bytes;
+} fx_kv_fork_desc;
+size_t fx_kv_fork_workspace_bytes(const fx_kv_fork_desc* desc);
+int fx_kv_fork(const fx_kv_fork_desc* desc, void* stream);
+/* In each of n_caches caches of the same sizes, types and strides (the layers of a model): for each of `rows` rows of copies [rows][3] the keys of the first `tokens`
+ * tokens of a page, the values of their groups of 16, and both scales go to another page.  Rows with a page outside the cache, and of a page to itself, copy nothing;
+ * tokens are held to 0 .. page_size.  A page that is copied to is copied from by no row of the call, and copied to by one (as fx_kv_fork lays them).
+ * One launch for each 32 caches. */
+int fx_kv_copy(const fx_kv_cache* caches, int n_caches, const int32_t* copies, int rows, void* stream);
 
 /* ---- a beam search's selection ----
  * Of each request the `count` best continuations of all its beams: candidate (beam k, word w) has the total
