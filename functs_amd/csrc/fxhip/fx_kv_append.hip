@@ -7,12 +7,13 @@
 
 namespace {
 template <int HELD, class T, bool INTER>
-__global__ __launch_bounds__(kThreads, 3) void fx_kv_append_kernel(const FxKvCache c, const FxKvRows r, int per, int vec, unsigned stores, const FxRotary q) {
+__global__ __launch_bounds__(kThreads, 4) void fx_kv_append_kernel(const FxKvCache c, const FxKvRows r, int per, int vec, unsigned stores, const FxRotary q) {
   __shared__ unsigned s_tops[2][kStoreWaves];
   __shared__ Turn s_turn[FX_ROTARY_ANGLES];
   constexpr int PV = sizeof(T) == 4 ? 4 : 8;
   if (blockIdx.x < stores) {
-    store_chunk<HELD, T, true, INTER>(c, r, per, vec, blockIdx.x, &q.turns, s_tops);
+    static_assert(sizeof s_turn >= kTurnPairs * sizeof(double), "either part's numbers");
+    store_chunk<HELD, T, true, INTER>(c, r, per, vec, blockIdx.x, &q.turns, (double*)s_turn, s_tops);
     return;
   }
   const unsigned share = blockIdx.x - stores;

@@ -152,7 +152,8 @@ struct StoreRun {
   bool vec;
   const FxTurns* turns;    // TURN: what turns, and the place of row 0's position
   int64_t token;
-  double quarters[TURN ? 8 : 1];
+  const double* quarters;  // (LDS) of all pairs
+  int pair0;               // the lane's first
   int lo, hi, n_lo, n_hi;  // the lane's columns: n_lo from lo on, n_hi from hi on, 8 each but at the ends
   bool turning;
   // lane -> (row of an iteration, eight of its depth), or (group of an iteration, pair of columns)
@@ -180,16 +181,14 @@ struct StoreRun {
         hi = INTER ? lo + 8 : first + pairs;
         n_lo = INTER ? min(2 * some, 8) : some;
         n_hi = INTER ? 2 * some - n_lo : some;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) quarters[i] = quarters_of(*turns, min(first + i, pairs - 1));
+        pair0 = first;
       } else {
         const int some = min(rest, 16);
         lo = 2 * pairs + max(min((at - units) * 16, rest - 16), 0);
         hi = lo + 8;
         n_lo = min(some, 8);
         n_hi = some - n_lo;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) quarters[i] = 0.0;
+        pair0 = 0;
       }
     }
   }
@@ -216,29 +215,42 @@ struct StoreRun {
     return load_numbers<T, 8, P>(p + (int64_t)min(k * abreast + sub, n - 1) * stride, vec);
   }
   // TURN: the lane's columns of a row as they are loaded
-  struct Raw { typename Pack<T>::eight lo, hi; };
+  struct Raw { unsigned u[sizeof(T) * 4]; };   // (whole words: halves would take a register each)
   __device__ __forceinline__ int row_of(int k) const { return min(k * abreast + sub, n - 1); }
   __device__ __forceinline__ void load_sixteen(Raw& raw, int k) const {
     const T* p = rows + (int64_t)row_of(k) * stride;
     if (n_lo + n_hi == 16) {
-      __builtin_memcpy(&raw.lo, p + lo, sizeof raw.lo);
-      __builtin_memcpy(&raw.hi, p + hi, sizeof raw.hi);
+      __builtin_memcpy(raw.u, p + lo, sizeof raw.u / 2);
+      __builtin_memcpy(raw.u + sizeof(T) * 2, p + hi, sizeof raw.u / 2);
     } else {
-      union { typename Pack<T>::eight all; T e[8]; } a, b;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        a.e[i] = i < n_lo ? p[lo + i] : (T)0.0f;
-        b.e[i] = i < n_hi ? p[hi + i] : (T)0.0f;
+      for (int i = 0; i < 16; ++i) {
+        const bool there = i < 8 ? i < n_lo : i - 8 < n_hi;
+        const T* from = p + (i < 8 ? lo + i : hi + i - 8);
+        if constexpr (sizeof(T) == 4) {
+          raw.u[i] = there ? __builtin_bit_cast(unsigned, *from) : 0u;
+        } else {
+          const unsigned w = there ? (unsigned)__builtin_bit_cast(unsigned short, *from) : 0u;
+          raw.u[i / 2] = i % 2 == 0 ? w : raw.u[i / 2] | w << 16;
+        }
       }
-      raw.lo = a.all;
-      raw.hi = b.all;
     }
   }
   // x: the first of each pair, then the others (of columns that do not turn: in the same order)
-  __device__ __forceinline__ void turn_sixteen(float (&x)[16], const Raw& raw, double position) const {
+  __device__ __forceinline__ void turn_sixteen(float (&x)[16], Raw& raw, double position) const {
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) * 4; ++i) asm volatile("" : "+v"(raw.u[i]));
     float u[8], v[8];
-    floats<T, 8>(u, raw.lo);
-    floats<T, 8>(v, raw.hi);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if constexpr (sizeof(T) == 4) {
+        u[i] = __uint_as_float(raw.u[i]);
+        v[i] = __uint_as_float(raw.u[8 + i]);
+      } else {
+        u[i] = (float)__builtin_bit_cast(T, (unsigned short)(raw.u[i / 2] >> (i % 2 * 16)));
+        v[i] = (float)__builtin_bit_cast(T, (unsigned short)(raw.u[4 + i / 2] >> (i % 2 * 16)));
+      }
+    }
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       x[i] = INTER ? (i < 4 ? u[2 * i % 8] : v[2 * i % 8]) : u[i];
@@ -247,7 +259,7 @@ struct StoreRun {
     if (turning) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        turn_pair(x[i], x[8 + i], turn_of(position, quarters[i], turns->magnitude, false));
+        turn_pair(x[i], x[8 + i], turn_of(position, quarters[pair0 + i], turns->magnitude, false));
         if (i % 2 == 1) __builtin_amdgcn_sched_barrier(0);   // (eight angles at once take 40 registers more)
       }
     }
@@ -525,15 +537,22 @@ struct StoreRun {
   }
 };
 
-// A workgroup's keys or values of one head.  turns: of keys that turn (TURN), by the positions of all tokens
+// A workgroup's keys or values of one head.  turns, quarters (LDS, kTurnPairs): of keys that turn (TURN), by the positions of all tokens
+constexpr int kTurnPairs = FX_KV_MAX_DEPTH / 2 + 8;
 template <int HELD, class T, bool TURN, bool INTER>
-__device__ __forceinline__ void store_chunk(const FxKvCache& c, const FxKvRows& r, int per, int vec, unsigned block, const FxTurns* turns, unsigned (*s_tops)[kStoreWaves]) {
+__device__ __forceinline__ void store_chunk(const FxKvCache& c, const FxKvRows& r, int per, int vec, unsigned block, const FxTurns* turns, double* quarters, unsigned (*s_tops)[kStoreWaves]) {
   const int lane = (int)threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const unsigned chunk_head = block >> 1;
   const int half = (int)(block & 1), chunk = (int)(chunk_head / (unsigned)c.heads), head = (int)(chunk_head - (unsigned)chunk * (unsigned)c.heads);
   const int D = c.depth, page = 1 << c.log_page;
   const int64_t n_slots = (int64_t)c.pages << c.log_page;
   const int t0 = chunk * per, t1 = min(r.tokens, t0 + per);
+  if constexpr (TURN) {   // (with the pairs behind the last, which a lane reads of fewer than 8)
+    if (half == 0) {
+      for (int i = (int)threadIdx.x; i < turns->pairs + 8; i += kThreads) quarters[i] = quarters_of(*turns, min(i, turns->pairs - 1));
+      __syncthreads();
+    }
+  }
   // lane i: the slot of token t0 - 1 + i, which a run that begins in the chunk needs (the first 64 - per of it, at least)
   auto slot_of = [&](int t) -> int64_t {
     const int64_t s = t >= 0 && t < r.tokens ? r.slots[min(max(t, 0), r.tokens - 1)] : -1;
@@ -573,7 +592,7 @@ __device__ __forceinline__ void store_chunk(const FxKvCache& c, const FxKvRows& 
       run.stride = r.k_token;
       run.n = n, run.o0 = o0, run.D = D, run.vec = vec != 0;
       run.codes = c.k + p * c.k_stride + in_page;
-      if constexpr (TURN) run.turns = turns, run.token = t;
+      if constexpr (TURN) run.turns = turns, run.token = t, run.quarters = quarters;
       run.run(straight, r.slots + t, page - 1, c.k_scale + p * c.ks_stride + head, tops);
     } else {
       StoreRun<HELD, T, true> run;
@@ -589,7 +608,7 @@ __device__ __forceinline__ void store_chunk(const FxKvCache& c, const FxKvRows& 
 template <int HELD, class T>
 __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 5 : 4) void fx_kv_store_kernel(const FxKvCache c, const FxKvRows r, int per, int vec) {
   __shared__ unsigned s_tops[2][kStoreWaves];
-  store_chunk<HELD, T, false, false>(c, r, per, vec, blockIdx.x, nullptr, s_tops);
+  store_chunk<HELD, T, false, false>(c, r, per, vec, blockIdx.x, nullptr, nullptr, s_tops);
 }
 
 // tokens a wave takes: as many as leave some 8 192 waves (32 a CU), `most` at most
