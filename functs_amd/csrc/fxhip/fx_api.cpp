@@ -2013,14 +2013,14 @@ int beam_of(const fx_beam_select_desc* desc, FxBeamArgs& a) {
   a.dtype = d.dtype;
   fx_beam_shape(a);
   // (a launch has fewer than 2^32 threads: 64 for each part of a row, 1 024 for each request)
-  if ((int64_t)d.requests * d.beams * a.chunks >= (int64_t{1} << 26) - 4 || d.requests >= 1 << 22) return fail(FX_E_LIMIT, op + ": more rows than a launch holds");
+  if ((int64_t)d.requests * d.beams * a.parts_a_row >= (int64_t{1} << 26) - 4 || d.requests >= 1 << 22) return fail(FX_E_LIMIT, op + ": more rows than a launch holds");
   return FX_OK;
 }
 size_t beam_workspace(FxBeamArgs& a, char* base) {
-  const size_t parts = (size_t)a.requests * a.beams * a.chunks;
+  const size_t parts = (size_t)a.requests * a.beams * a.parts_a_row;
   a.parts = (FxBeamPart*)base;
-  a.lists = (FxBeamWord*)(base + parts * sizeof(FxBeamPart));
-  return parts * (sizeof(FxBeamPart) + a.count * sizeof(FxBeamWord));
+  a.tops = (int32_t*)(base + parts * sizeof(FxBeamPart));
+  return parts * (sizeof(FxBeamPart) + FX_BEAM_SEGMENTS * sizeof(int32_t));
 }
 }  // namespace
 

@@ -5,16 +5,12 @@
 
 #include "../../../include/fxhip.h"
 
-// What a wave finds in its part of a row: the largest logit, the sum of 2^(x c - r) (NaN where there is one in the part), and in a list of its own
-// the best `count` (x, word), best first
+#define FX_BEAM_SEGMENTS 16   // of a wave's words: those of 16 lanes' loads, side by side
+// What a wave finds in its words: the largest logit and the sum of 2^(x c - r) (NaN where there is one)
 struct FxBeamPart {
   float top;
   float unused;
   double sum;
-};
-struct FxBeamWord {
-  float x;        // -infinity: none
-  uint32_t word;
 };
 struct FxBeamArgs {
   const void* logits;                  // [requests][beams][words], a beam's words side by side
@@ -25,9 +21,9 @@ struct FxBeamArgs {
   int32_t* out_beams;
   int64_t* out_words;
   int64_t end_word;
-  FxBeamPart* parts;                   // [requests * beams][chunks]
-  FxBeamWord* lists;                   // [requests * beams][chunks][count]
-  int32_t requests, beams, words, count, dtype, chunks, loads;   // loads: of 16 bytes that a lane has under way
+  FxBeamPart* parts;                   // [requests * beams][parts_a_row]
+  int32_t* tops;                       // [requests * beams][parts_a_row][FX_BEAM_SEGMENTS]: the largest of each segment, as a whole number in the order of floats
+  int32_t requests, beams, words, count, dtype, parts_a_row;
 };
-void fx_beam_shape(FxBeamArgs& a);     // chunks and loads
+void fx_beam_shape(FxBeamArgs& a);     // parts_a_row
 hipError_t fx_launch_beam_select(const FxBeamArgs& a, hipStream_t stream, int* launched);

@@ -1,22 +1,27 @@
 // A beam search's selection: of each request the `count` best continuations of all its beams and words, by score + logit - log sum exp(logits).
 //
-// Two launches.  fx_beam_scan reads the logits once: a wave takes up to 8 192 words of a row, holds them in registers, and leaves their largest, their
-// sum of exponentials and their best `count`, in order.  fx_beam_join, a workgroup a request, merges the parts of a row (a wave a row), then ranks the
-// rows' candidates.
+// Two launches.  fx_beam_scan reads the logits once; a wave leaves the sum of exponentials of its 2 048 (16-bit types) or 1 024 words and the largest of each
+// sixteenth of them.  fx_beam_join, a workgroup a request and a wave a row, finds from these which few segments the best words can lie in, reads those again (from the caches, as a
+// rule) and takes their best; then it ranks the rows' candidates.  (The best words of every part found by fx_beam_scan itself: 31 us for 488 rows of 128 001 words,
+// half of them instructions of that search.)
 //
 // What is compared within a row are its logits; between rows score + (logit - lse) in 64 bits.  Sums of exponentials: eight at a time in fp32, these in
 // 64 bits, so that lse is off by some 1e-8 and rows change places only where they are as near as that.
 //
-// The best `count` of a wave's words: the largest of each of 256 groups of words are compared with a bound that is halved until `count` groups, and hardly
-// more, have one above it; the words above it are a few more than `count`, and are ranked by counting.  Equal numbers: lower words go first, and so as
-// many as there may be of them never need more than the list's 256 places (it is cut to the best `count` when it fills up).
+// The best `count` words: a bound is halved until at least `count` of 256 groups of segments, and hardly more, have a word at or above it; the words at or above it are a
+// few more than `count`, and are ranked by counting.  Equal numbers: lower words go first, and so as many as there may be of them never need more than a list's
+// 256 places (it is cut to the best `count` when it fills up).
 #include <algorithm>
 
 #include "fx_beam.h"
 
 namespace {
 constexpr int kThreads = 256, kWaves = kThreads / 64;
+constexpr int kLoads = 4;    // of 16 bytes that a lane of fx_beam_scan has under way (8: rows of an odd number of words took 23 us where four take 18, and little else)
 constexpr int kList = 256;   // candidates that a wave keeps: the best FX_BEAM_MAX_COUNT and two steps' of 64
+constexpr int kSegments = 512;   // that it lists before it looks at them
+constexpr int kJoinWaves = 8;    // rows of a request at a time, at most
+constexpr float kLowest = -3.402823466e38f;   // (-infinity is none)
 
 __device__ __forceinline__ float wave_max(float m) {
   const auto step = [](float m, int s) { return fmaxf(m, __uint_as_float((unsigned)s)); };
@@ -51,12 +56,8 @@ __device__ __forceinline__ int ordered(float x) {
 __device__ __forceinline__ float unordered(int i) { return __uint_as_float((unsigned)(i ^ ((i >> 31) & 0x7fffffff))); }
 // larger keys go first: larger numbers (-0 is 0), then lower words
 __device__ __forceinline__ uint64_t key_of(float x, uint32_t word) { return ((uint64_t)((unsigned)ordered(x + 0.0f) ^ 0x80000000u) << 32) | (0xffffffffu - word); }
-__device__ __forceinline__ FxBeamWord word_of(uint64_t key) {
-  FxBeamWord w;
-  w.x = unordered((int)((unsigned)(key >> 32) ^ 0x80000000u));
-  w.word = 0xffffffffu - (unsigned)key;
-  return w;
-}
+__device__ __forceinline__ float x_of(uint64_t key) { return unordered((int)((unsigned)(key >> 32) ^ 0x80000000u)); }
+__device__ __forceinline__ uint32_t word_of(uint64_t key) { return 0xffffffffu - (unsigned)key; }
 __device__ __forceinline__ int below(uint64_t mask) {   // set lanes below this one
   return (int)__builtin_amdgcn_mbcnt_hi((unsigned)(mask >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)mask, 0u));
 }
@@ -68,7 +69,7 @@ __device__ __forceinline__ void rank_keys(const uint64_t* keys, int n, int lane,
     mine[i] = lane + 64 * i < n ? keys[lane + 64 * i] : 0;
     rank[i] = 0;
   }
-#pragma unroll 4
+#pragma unroll 8
   for (int j = 0; j < n; ++j) {
     const uint64_t k = keys[j];
     rank[0] += k > mine[0] ? 1 : 0;
@@ -96,243 +97,180 @@ template <> struct Load<__bf16> {
   unsigned u[4];
   __device__ __forceinline__ float operator[](int e) const { return __uint_as_float(e % 2 ? u[e / 2] & 0xffff0000u : u[e / 2] << 16); }
 };
-// (between two passes over the words: without it the compiler keeps them as floats as well)
-template <class T>
-__device__ __forceinline__ void as_loaded(Load<T>& w) { asm volatile("" : "+v"(w.u[0]), "+v"(w.u[1]), "+v"(w.u[2]), "+v"(w.u[3])); }
-
 // Terms 2^(x c - r), r the whole number next to the largest x c: product and difference are rounded once.  c is log2 e (1 + 1.3e-8), for which the sum's
 // logarithm is put right.  Numbers whose x c may be infinite: by their difference to the largest.
 constexpr float kC = 1.44269504088896340736f;
 __device__ __forceinline__ bool far_from(float top) { return __builtin_fabsf(top) > 1e30f; }
 __device__ __forceinline__ float whole_of(float top) { return __builtin_rintf(top * kC); }
-__device__ __forceinline__ double lse_of(float top, double sum) {
-  if (!(top > -INFINITY)) return sum == 0.0 ? -INFINITY : sum;   // (no words, or NaN)
-  const double r = far_from(top) ? (double)top * (double)kC : (double)whole_of(top);
-  return r * 0.69314718055994530942 + log(sum) - ((double)kC / 1.44269504088896340736 - 1.0) * (double)top;
+// 2^(reference of a - that of b), a no more than b: exact between whole ones, and of far ones, which are the same or 2^70 apart at least, 1 or 0
+__device__ __forceinline__ double between(float a, float b) {
+  if (far_from(a) || far_from(b)) return a == b ? 1.0 : 0.0;
+  return __builtin_amdgcn_ldexp(1.0, (int)fmaxf(whole_of(a) - whole_of(b), -4000.0f));
+}
+// a part's sum under the reference of `most`, the row's largest logit
+__device__ __forceinline__ double part_of(const FxBeamPart& p, float most) { return p.top > -INFINITY ? p.sum * between(p.top, most) : p.sum; }   // (of no words: 0, or NaN)
+__device__ __forceinline__ double lse_of(float most, double sum) {
+  const double r = far_from(most) ? (double)most * (double)kC : (double)whole_of(most);
+  return r * 0.69314718055994530942 + log(sum) - ((double)kC / 1.44269504088896340736 - 1.0) * (double)most;
 }
 
-// A wave: 64 * LOADS loads of 16 bytes
-template <class T, int LOADS>
-__global__ __launch_bounds__(kThreads, LOADS > 8 ? 3 : LOADS > 4 ? 5 : 6) void fx_beam_scan(const FxBeamArgs a) {
-  constexpr int kVec = 16 / (int)sizeof(T), kGroups = 4, kPerGroup = LOADS / kGroups, kWords = 64 * kVec * LOADS;
-  constexpr unsigned kNone = Load<T>::kNone;
-  __shared__ uint64_t s_keys[kWaves][kList];
-  __shared__ uint4 s_loads[kWaves][64];
-  __shared__ int s_places[kWaves][64];
+// Words of a row: load l of a part, in its lane.  Loads that would begin in a row's last words lie at its end (at), less the first ones, which are other lanes'
+template <class T>
+struct Words {
+  static constexpr int kVec = 16 / (int)sizeof(T), kPart = 64 * kVec * kLoads, kSegment = 16 * kVec;
+  const T* x;
+  int words;
+  __device__ __forceinline__ int at(int place) const { return min(place, words - kVec); }
+  // the numbers from `place` on, -infinity for those that are not the lane's
+  __device__ __forceinline__ Load<T> load(int place) const {
+    Load<T> v;
+    __builtin_memcpy(v.u, (const char*)x + (unsigned)at(place) * (unsigned)sizeof(T), 16);
+    return v;
+  }
+  __device__ __forceinline__ void mask(Load<T>& v, int place) const {
+    const int skip = place - at(place);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (sizeof(T) == 4) v.u[i] = skip > i ? Load<T>::kNone : v.u[i];
+      else v.u[i] = skip > 2 * i + 1 ? Load<T>::kNone : skip == 2 * i + 1 ? (v.u[i] & 0xffff0000u) | (Load<T>::kNone & 0xffffu) : v.u[i];
+    }
+  }
+  // of a row that is shorter than a load: all of it
+  __device__ __forceinline__ Load<T> load_tiny() const {
+    T few[kVec];
+#pragma unroll
+    for (int e = 0; e < kVec; ++e) few[e] = e < words ? x[e] : (T)(-INFINITY);
+    Load<T> v;
+    __builtin_memcpy(v.u, few, 16);
+    return v;
+  }
+};
+template <class T>
+__device__ __forceinline__ Words<T> words_of(const FxBeamArgs& a, int64_t row) {
+  const int64_t request = row / a.beams;
+  Words<T> w;
+  w.x = (const T*)a.logits + request * a.l_request + (row - request * a.beams) * a.l_beam;
+  w.words = a.words;
+  return w;
+}
+// the largest of the lane's 16 lanes, in the last of them (of whole numbers the compiler makes one instruction a step)
+__device__ __forceinline__ int segment_max(int m) {
+#define FX_STEP(ctrl) m = max(m, __builtin_amdgcn_update_dpp((int)0x80000000, m, ctrl, 0xf, 0xf, false));
+  FX_STEP(0x111) FX_STEP(0x112) FX_STEP(0x114) FX_STEP(0x118)
+#undef FX_STEP
+  return m;
+}
+
+// Bound: HBM.  A wave a part; nothing is shared between waves.
+template <class T>
+__global__ __launch_bounds__(kThreads, 8) void fx_beam_scan(const FxBeamArgs a) {
+  typedef Words<T> W;
   const int lane = (int)threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-  const int unit = (int)blockIdx.x * kWaves + wave, row = unit / a.chunks, chunk = unit - row * a.chunks;
-  if (row >= a.requests * a.beams) return;   // (waves of a workgroup do not wait for each other)
-  // beams with no continuations of their own: known ahead of the logits, which need not be read then, or with them where there is little to read
-  const bool idle = (a.ended && a.ended[row]) || !(a.scores[row] > -INFINITY);
-  if (LOADS > 4 && idle) return;
-  const int request = row / a.beams;
-  const T* x = (const T*)a.logits + (int64_t)request * a.l_request + (int64_t)(row - request * a.beams) * a.l_beam;
-  const int from = chunk * kWords;
-
-  // load l: words at_of(l) on.  Loads that would begin in a row's last words lie at its end, less the first ones, which are other lanes'
-  const auto place_of = [&](int l) { return from + (l * 64 + lane) * kVec; };
-  const auto at_of = [&](int l) { return min(place_of(l), a.words - kVec); };
-  Load<T> v[LOADS];
-  if (a.words >= kVec) {
+  const int unit = (int)blockIdx.x * kWaves + wave, row = unit / a.parts_a_row, part = unit - row * a.parts_a_row;
+  if (row >= a.requests * a.beams) return;
+  // (beams with no continuations of their own are not read)
+  if ((a.ended && a.ended[row]) || !(a.scores[row] > -INFINITY)) return;
+  const W w = words_of<T>(a, row);
+  const int begin = part * W::kPart + lane * W::kVec;   // load l: words begin + l * 64 * kVec on
+  Load<T> v[kLoads];
+  if (w.words >= W::kVec) {
 #pragma unroll
-    for (int l = 0; l < LOADS; ++l) __builtin_memcpy(v[l].u, (const char*)x + (unsigned)at_of(l) * (unsigned)sizeof(T), 16);
-  } else {   // fewer words than a load
+    for (int l = 0; l < kLoads; ++l) v[l] = w.load(begin + l * 64 * W::kVec);
+    if ((part + 1) * W::kPart > w.words) {
 #pragma unroll
-    for (int l = 0; l < LOADS; ++l) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) v[l].u[i] = kNone;
+      for (int l = 0; l < kLoads; ++l) w.mask(v[l], begin + l * 64 * W::kVec);
     }
-    if (lane == 0) {
-      T few[kVec];
+  } else {
 #pragma unroll
-      for (int e = 0; e < kVec; ++e) few[e] = e < a.words ? x[e] : (T)(-INFINITY);
-      __builtin_memcpy(v[0].u, few, 16);
+    for (int l = 0; l < kLoads; ++l) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[l].u[i] = Load<T>::kNone;
     }
+    if (lane == 0) v[0] = w.load_tiny();
   }
-  if (LOADS <= 4 && idle) return;
-
-  const int count = a.count;
-  uint64_t* keys = s_keys[wave];
-  uint4* loads = s_loads[wave];
-  int* places = s_places[wave];
-  int n = 0;                        // candidates so far
-  float bound = -INFINITY;
-  uint32_t last = 0xffffffffu;      // of words equal to the bound, those up to this one
-  const auto cut = [&]() {          // to the best `count`, in order; what comes has to be better than the last of them
-    uint64_t mine[kList / 64];
-    int rank[kList / 64];
-    in_wave();
-    rank_keys(keys, n, lane, mine, rank);
-    in_wave();
+  float x[kLoads][W::kVec];
+  int all = (int)0x80000000;
+  int* const tops = a.tops + (int64_t)unit * FX_BEAM_SEGMENTS + (lane >> 4);
 #pragma unroll
-    for (int i = 0; i < kList / 64; ++i)
-      if (lane + 64 * i < n && rank[i] < count) keys[rank[i]] = mine[i];
-    in_wave();
-    n = min(n, count);
-    if (n == count) {
-      const FxBeamWord worst = word_of(keys[n - 1]);
-      bound = worst.x;
-      last = worst.word;
-    }
-  };
-  if (a.words >= kVec && from + kWords > a.words) {
-#pragma unroll
-    for (int l = 0; l < LOADS; ++l) {
-      const int skip = place_of(l) - at_of(l);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if (sizeof(T) == 4) v[l].u[i] = skip > i ? kNone : v[l].u[i];
-        else v[l].u[i] = skip > 2 * i + 1 ? kNone : skip == 2 * i + 1 ? (v[l].u[i] & 0xffff0000u) | (kNone & 0xffffu) : v[l].u[i];
-      }
-    }
-  }
-  float best[LOADS];   // of each load
-#pragma unroll
-  for (int l = 0; l < LOADS; ++l) {
+  for (int l = 0; l < kLoads; ++l) {
     float m = -INFINITY;
-    as_loaded(v[l]);
 #pragma unroll
-    for (int e = 0; e < kVec; ++e) m = fmaxf(m, v[l][e]);   // (NaN is passed over here, and is in the sum)
-    best[l] = m;
-    __builtin_amdgcn_sched_barrier(0);   // (one load's words after the other: all of them as floats do not fit)
+    for (int e = 0; e < W::kVec; ++e) {
+      x[l][e] = v[l][e];
+      m = fmaxf(m, x[l][e]);   // (NaN is passed over here, and is in the sum)
+    }
+    const int segment = segment_max(ordered(m));
+    if ((lane & 15) == 15) tops[l * 4] = segment;
+    all = max(all, segment);
   }
-  float group[kGroups], most = -INFINITY;
-#pragma unroll
-  for (int g = 0; g < kGroups; ++g) {
-    group[g] = -INFINITY;
-#pragma unroll
-    for (int l = 0; l < kPerGroup; ++l) group[g] = fmaxf(group[g], best[g * kPerGroup + l]);
-    most = fmaxf(most, group[g]);
-  }
-  most = wave_max(most);
-
+  const float most = unordered(max(max(__builtin_amdgcn_readlane(all, 15), __builtin_amdgcn_readlane(all, 31)), max(__builtin_amdgcn_readlane(all, 47), __builtin_amdgcn_readlane(all, 63))));
   const bool far = far_from(most);
   const float r = most > -INFINITY ? whole_of(most) : 0.0f;
   double sum = 0.0;
   if (!far) {
 #pragma unroll
-    for (int l = 0; l < LOADS; ++l) {
+    for (int l = 0; l < kLoads; ++l) {
       float some = 0.0f;
-      as_loaded(v[l]);
 #pragma unroll
-      for (int e = 0; e < kVec; ++e) some += __builtin_amdgcn_exp2f(__builtin_fmaf(v[l][e], kC, -r));
+      for (int e = 0; e < W::kVec; ++e) some += __builtin_amdgcn_exp2f(__builtin_fmaf(x[l][e], kC, -r));
       sum += (double)some;
-      __builtin_amdgcn_sched_barrier(0);
     }
   } else {
     const float least = most > -INFINITY ? most : 0.0f;
 #pragma unroll
-    for (int l = 0; l < LOADS; ++l) {
+    for (int l = 0; l < kLoads; ++l) {
       float some = 0.0f;
-      as_loaded(v[l]);
 #pragma unroll
-      for (int e = 0; e < kVec; ++e) some += __builtin_amdgcn_exp2f((v[l][e] - least) * kC);
+      for (int e = 0; e < W::kVec; ++e) some += __builtin_amdgcn_exp2f((x[l][e] - least) * kC);
       sum += (double)some;
-      __builtin_amdgcn_sched_barrier(0);
     }
-  }
-  if (most > -INFINITY) {
-    // a bound with at least `count` groups at or above it (all are at or above the least), and hopefully few more
-    float least = fminf(fminf(group[0], group[1]), fminf(group[2], group[3])), high = most;
-    least = -wave_max(-least);
-    const auto above = [&](float b) {
-      int some = 0;
-#pragma unroll
-      for (int g = 0; g < kGroups; ++g) some += __builtin_popcountll(__ballot(group[g] >= b));
-      return some;
-    };
-    float low = fmaxf(least, most - 64.0f);
-    if (above(low) < count) low = least;
-#pragma unroll 1
-    for (int i = 0; i < 12; ++i) {
-      const float mid = 0.5f * low + 0.5f * high;
-      if (!(mid > low)) break;
-      const int some = above(mid);
-      if (some >= count) low = mid;
-      else high = mid;
-      if (some >= count && some <= count + 6) break;
-    }
-    bound = fmaxf(low, -3.402823466e38f);   // (-infinity is none)
-    // The loads that have a word above the bound go to LDS, 64 at most, and from there each of their words to a lane.  More than 64 (of equal words):
-    // all loads take that way, read again.
-    int found = 0;
-#pragma unroll
-    for (int l = 0; l < LOADS; ++l) {
-      const uint64_t lanes = __ballot(best[l] >= bound);
-      if (lanes == 0) continue;
-      const int to = found + below(lanes);
-      if (best[l] >= bound && to < 64) {
-        loads[to] = make_uint4(v[l].u[0], v[l].u[1], v[l].u[2], v[l].u[3]);
-        places[to] = a.words >= kVec ? at_of(l) : 0;
-      }
-      found += __builtin_popcountll(lanes);
-    }
-    const bool few = found <= 64;   // (rows shorter than a load have one)
-#pragma unroll 1
-    for (int l = 0; l < (few ? 1 : LOADS); ++l) {
-      int skip = 0;
-      if (!few) {
-        in_wave();
-        uint4 w;
-        __builtin_memcpy(&w, (const char*)x + (unsigned)at_of(l) * (unsigned)sizeof(T), 16);
-        loads[lane] = w;
-        places[lane] = at_of(l);
-        skip = from + l * 64 * kVec;   // (words before it are other lanes' or an earlier load's)
-        found = 64;
-      }
-      in_wave();
-#pragma unroll 1
-      for (int i0 = 0; i0 < found; i0 += 64 / kVec) {
-        if (n > kList - 64) cut();   // (no room for a word of each lane)
-        const int i = i0 + lane / kVec, e = lane % kVec;
-        float z = -INFINITY;
-        uint32_t word = 0;
-        if (i < found) {
-          z = (float)((const T*)loads)[i * kVec + e];
-          const int at = places[i];
-          word = (uint32_t)(at + e);
-          if (at + e < skip + (few ? 0 : i * kVec)) z = -INFINITY;
-        }
-        const bool hit = z > bound || (z == bound && word <= last);
-        const uint64_t lanes = __ballot(hit);
-        if (hit) keys[n + below(lanes)] = key_of(z, word);
-        n += __builtin_popcountll(lanes);
-      }
-    }
-    cut();
   }
   sum = wave_sum(sum);
-  const int64_t part = (int64_t)row * a.chunks + chunk;
   if (lane == 0) {
-    a.parts[part].top = most;
-    a.parts[part].sum = sum;
-  }
-  if (lane < count) {
-    FxBeamWord none;
-    none.x = -INFINITY;
-    none.word = 0;
-    a.lists[part * count + lane] = lane < n ? word_of(keys[lane]) : none;
+    a.parts[unit].top = most;
+    a.parts[unit].sum = sum;
   }
 }
 
-// Each wave has the lists of a row in LDS: [waves][chunks * count], and there are the rows' best [beams][count]
-__global__ __launch_bounds__(1024) void fx_beam_join(const FxBeamArgs a) {
+// Bound: latency.  A row is a chain of some ten steps, and the code of each arrives for the first time: loops are not unrolled where they need not be (16 segments' loads in
+// registers, 28 KB of code, took 2 us more than this).
+template <class T>
+__global__ __launch_bounds__(512) void fx_beam_join(const FxBeamArgs a) {
+  typedef Words<T> W;
   extern __shared__ uint4 s_join[];
-  const int count = a.count, K = a.beams, entries = a.chunks * count;
-  const int lane = (int)threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), waves = (int)blockDim.x >> 6;
-  double* score = (double*)s_join;                    // [beams][count]
-  uint32_t* word = (uint32_t*)(score + K * count);    // [beams][count]
-  FxBeamWord* mine = (FxBeamWord*)(word + ((K * count + 1) & ~1)) + (size_t)wave * entries;
+  const int count = a.count, K = a.beams, lane = (int)threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), waves = (int)blockDim.x >> 6;
+  uint4* loads = s_join + wave * 64;                               // [waves][64]
+  double* score = (double*)(s_join + waves * 64);                  // [beams][count]
+  uint64_t* keys = (uint64_t*)score + K * count + wave * kList;    // [waves][kList]
+  uint32_t* word = (uint32_t*)((uint64_t*)score + K * count + waves * kList);   // [beams][count]
+  int* list = (int*)(word + K * count) + wave * kSegments;         // [waves][kSegments]
+  int* places = (int*)(word + K * count) + waves * kSegments + wave * 64;       // [waves][64]
   const int64_t request = blockIdx.x;
+  const int fours = a.parts_a_row * (FX_BEAM_SEGMENTS / 4);        // of segments of a row
   for (int k = wave; k < K; k += waves) {
     const int64_t row = request * K + k;
     // (all loads at once: what beams with no candidates of their own have there is never looked at)
     const float before = a.scores[row];
     const bool over = a.ended && a.ended[row];
-    const FxBeamPart p = lane < a.chunks ? a.parts[row * a.chunks + lane] : FxBeamPart{-INFINITY, 0.0f, 0.0};
-    in_wave();
-    for (int i = lane; i < entries; i += 64) mine[i] = a.lists[row * entries + i];
-    in_wave();
+    const int4* tops = (const int4*)a.tops + row * fours;
+    const FxBeamPart* parts = a.parts + row * a.parts_a_row;
+    const FxBeamPart none{-INFINITY, 0.0f, 0.0};
+    const FxBeamPart first = lane < a.parts_a_row ? parts[lane] : none;
+    float group[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};   // 256 groups of segments: four to a lane
+#pragma unroll 1
+    for (int i0 = 0; i0 < fours; i0 += 256) {
+      int4 t[4];
+#pragma unroll
+      for (int g = 0; g < 4; ++g) t[g] = tops[min(i0 + 64 * g + lane, fours - 1)];   // (the last one again)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const bool some = i0 + 64 * g + lane < fours;
+        group[0] = fmaxf(group[0], some ? unordered(t[g].x) : -INFINITY);
+        group[1] = fmaxf(group[1], some ? unordered(t[g].y) : -INFINITY);
+        group[2] = fmaxf(group[2], some ? unordered(t[g].z) : -INFINITY);
+        group[3] = fmaxf(group[3], some ? unordered(t[g].w) : -INFINITY);
+      }
+    }
     const bool live = before > -INFINITY;
     int n = 0;
     if (over) {
@@ -342,52 +280,171 @@ __global__ __launch_bounds__(1024) void fx_beam_join(const FxBeamArgs a) {
       }
       n = live ? 1 : 0;
     } else if (live) {
-      const float top = wave_max(p.top);
-      const double most = (double)top;
-      const double part = lse_of(p.top, p.sum);
-      const double sum = wave_sum(part == -INFINITY ? 0.0 : exp(part - most));   // (NaN stays)
-      const double lse = log(sum) + most;
-      if (top > -INFINITY && lse - lse == 0.0) {   // (a row with NaN or +infinity has none)
-        int at = 0;                                 // the lane's place in the list of its part
-        float x = -INFINITY;
-        uint32_t w = 0;
-        const auto next = [&]() {
-          x = -INFINITY;
-          if (lane < a.chunks && at < count) {
-            const FxBeamWord e = mine[lane * count + at];
-            x = e.x;
-            w = e.word;
-          }
+      const float top = wave_max(fmaxf(fmaxf(group[0], group[1]), fmaxf(group[2], group[3])));
+      if (top > -INFINITY) {
+        // a bound with at least `count` groups at or above it (all are at or above the least), and hopefully few more
+        float low = -wave_max(-fminf(fminf(group[0], group[1]), fminf(group[2], group[3]))), high = top;
+        const auto above = [&](float b) {
+          int some = 0;
+#pragma unroll
+          for (int g = 0; g < 4; ++g) some += __builtin_popcountll(__ballot(group[g] >= b));
+          return some;
         };
-        next();
-        for (; n < count; ++n) {
-          const float m = wave_max(x);
-          if (!(m > -INFINITY)) break;
-          const int first = __builtin_ctzll(__ballot(x == m));   // (parts are in the order of their words)
-          if (lane == first) {
-            score[k * count + n] = (double)before + ((double)x - lse);
-            word[k * count + n] = w;
-            ++at;
-            next();
+        if (high - 64.0f > low && above(high - 64.0f) >= count) low = high - 64.0f;
+        // (quarters instead of halves, whose counts do not wait for each other; fewer segments than 12 take as long as so many)
+#pragma unroll 1
+        for (int i = 0; i < 10; ++i) {
+          const float mid = 0.5f * low + 0.5f * high, one = 0.5f * low + 0.5f * mid, three = 0.5f * mid + 0.5f * high;
+          if (!(mid > low)) break;
+          const int at_one = above(one), at_mid = above(mid), at_three = above(three);
+          int some = at_one;
+          if (at_three >= count) low = three, some = at_three;
+          else if (at_mid >= count) low = mid, high = three, some = at_mid;
+          else if (at_one >= count) low = one, high = mid;
+          else high = one;
+          if (some >= count && some <= max(count + 2, 12)) break;
+        }
+        float bound = fmaxf(low, kLowest);
+        uint32_t last = 0xffffffffu;      // of words equal to the bound, those up to this one
+        const W w = words_of<T>(a, row);
+        const bool tiny = w.words < W::kVec;
+        double lse = 0.0;
+#pragma unroll 1
+        for (int seen = 0; seen < fours;) {
+          int listed = 0;
+#pragma unroll 1
+          for (; seen < fours && listed <= kSegments - 256; seen += 64) {
+            const int i0 = seen;
+            const int4 t = tops[min(i0 + lane, fours - 1)];
+            const float each[4] = {unordered(t.x), unordered(t.y), unordered(t.z), unordered(t.w)};
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              const bool some = i0 + lane < fours && each[q] >= bound;
+              const uint64_t lanes = __ballot(some);
+              if (some) list[listed + below(lanes)] = (i0 + lane) * 4 + q;
+              listed += __builtin_popcountll(lanes);
+            }
+          }
+          in_wave();
+          // The words of the listed segments, 16 lanes a segment, four loads under way.  Of the loads those that have a word above the bound go to LDS, 64 at most,
+          // and from there each of their words to a lane.  More than 64 (of equal words): all loads take that way, four segments at a time.
+          const auto place_of = [&](int i) {   // (of none: behind the last word, where nothing is the lane's)
+            return i < listed ? list[i] * W::kSegment + (lane & 15) * W::kVec : a.words;
+          };
+          const auto load = [&](int place) {
+            if (!tiny) return w.load(place);
+            Load<T> v = w.load_tiny();
+            if (place != 0) v.u[0] = v.u[1] = v.u[2] = v.u[3] = Load<T>::kNone;
+            return v;
+          };
+          int found = 0;
+#pragma unroll 1
+          for (int i0 = 0; i0 < listed; i0 += 16) {
+            Load<T> v[4];
+            int place[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+              place[u] = place_of(i0 + 4 * u + (lane >> 4));
+              v[u] = load(place[u]);
+            }
+            if (lse == 0.0) {   // (the first time, while they are under way)
+              double sum = part_of(first, top);
+#pragma unroll 1
+              for (int i = lane + 64; i < a.parts_a_row; i += 64) sum += part_of(parts[i], top);
+              lse = lse_of(top, wave_sum(sum));
+              if (!(lse - lse == 0.0)) listed = 0, seen = fours;   // (a row with NaN or +infinity has no candidates)
+            }
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+              float m = v[u][0];   // (of words that are other lanes', too: they are passed over below)
+#pragma unroll
+              for (int e = 1; e < W::kVec; ++e) m = fmaxf(m, v[u][e]);
+              const bool some = m >= bound && place[u] < a.words;
+              const uint64_t lanes = __ballot(some);
+              const int to = found + below(lanes);
+              if (some && to < 64) {
+                loads[to] = make_uint4(v[u].u[0], v[u].u[1], v[u].u[2], v[u].u[3]);
+                places[to] = place[u];
+              }
+              found += __builtin_popcountll(lanes);
+            }
+          }
+          if (listed == 0) found = 0;
+          const bool few = found <= 64;
+          int i0 = 0;    // of the segments, where they come four at a time
+#pragma unroll 1
+          while (found > 0) {
+            if (!few) {
+              in_wave();
+              const int place = place_of(i0 + (lane >> 4));
+              const Load<T> v = load(place);
+              loads[lane] = make_uint4(v.u[0], v.u[1], v.u[2], v.u[3]);
+              places[lane] = place;
+              found = 64;
+            }
+            in_wave();
+#pragma unroll 1
+            for (int i1 = 0; i1 < found + 64 / W::kVec; i1 += 64 / W::kVec) {   // (and once more, for what is left in the list)
+              if (n > kList - 64 || i1 >= found) {
+                // no room for a word of each lane, or the end: the best `count`, in order; what comes has to be better than the last of them
+                uint64_t mine[kList / 64];
+                int rank[kList / 64];
+                in_wave();
+                rank_keys(keys, n, lane, mine, rank);
+                in_wave();
+#pragma unroll
+                for (int i = 0; i < kList / 64; ++i)
+                  if (lane + 64 * i < n && rank[i] < count) keys[rank[i]] = mine[i];
+                in_wave();
+                n = min(n, count);
+                if (n == count) {
+                  const uint64_t worst = keys[n - 1];
+                  bound = x_of(worst);
+                  last = word_of(worst);
+                }
+              }
+              const int i = i1 + lane / W::kVec, e = lane % W::kVec;
+              float z = -INFINITY;
+              uint32_t here = 0;
+              if (i < found) {
+                const int place = places[i], at = tiny ? 0 : w.at(place);
+                here = (uint32_t)(at + e);
+                if (at + e >= place && place < a.words) z = (float)((const T*)loads)[i * W::kVec + e];
+              }
+              const bool hit = z > bound || (z == bound && here <= last);
+              const uint64_t lanes = __ballot(hit);
+              if (hit) keys[n + below(lanes)] = key_of(z, here);
+              n += __builtin_popcountll(lanes);
+            }
+            i0 += 4;
+            if (few || i0 >= listed) break;
           }
         }
+        in_wave();
+        for (int i = lane; i < n; i += 64) {
+          score[k * count + i] = (double)before + ((double)x_of(keys[i]) - lse);
+          word[k * count + i] = word_of(keys[i]);
+        }
+        in_wave();
       }
     }
     for (int i = n + lane; i < count; i += 64) score[k * count + i] = -INFINITY;
   }
   __syncthreads();
-  // the place of a candidate: how many are better, or as good and before it
-  const int all = K * count;
-  for (int i = (int)threadIdx.x; i < all; i += (int)blockDim.x) {
+  // the place of a candidate: how many are better, or as good and before it; eight lanes to a candidate
+  const int all = K * count, eighth = (int)threadIdx.x & 7;
+  for (int i = (int)threadIdx.x >> 3; i < all; i += (int)blockDim.x >> 3) {
     const double s = score[i];
-    if (!(s > -INFINITY)) continue;
     int rank = 0;
-#pragma unroll 8
-    for (int j = 0; j < all; ++j) {
+#pragma unroll 4
+    for (int j = eighth; j < all; j += 8) {
       const double t = score[j];
       rank += t > s || (t == s && j < i) ? 1 : 0;
     }
-    if (rank >= count) continue;
+    rank += __shfl_xor(rank, 1, 64);
+    rank += __shfl_xor(rank, 2, 64);
+    rank += __shfl_xor(rank, 4, 64);
+    if (eighth != 0 || rank >= count || !(s > -INFINITY)) continue;
     const int k = i / count;
     const int64_t to = request * count + rank;
     a.out_scores[to] = (float)s;
@@ -408,35 +465,27 @@ __global__ __launch_bounds__(1024) void fx_beam_join(const FxBeamArgs a) {
     }
   }
 }
-
-int chunks_of(const FxBeamArgs& a, int loads) {
-  const int words = 64 * (a.dtype == FX_DT_F32 ? 4 : 8) * loads;
-  return (a.words + words - 1) / words;
-}
 }  // namespace
 
 void fx_beam_shape(FxBeamArgs& a) {
-  // few rows: shorter parts; a row has no more of them than a wave of fx_beam_join has lanes
-  a.loads = chunks_of(a, 4) <= 64 && (int64_t)a.requests * a.beams * chunks_of(a, 4) <= 8192 ? 4 : chunks_of(a, 8) <= 64 ? 8 : 16;
-  a.chunks = chunks_of(a, a.loads);
+  const int words = 64 * (a.dtype == FX_DT_F32 ? 4 : 8) * kLoads;
+  a.parts_a_row = (a.words + words - 1) / words;
 }
 
 hipError_t fx_launch_beam_select(const FxBeamArgs& a, hipStream_t stream, int* launched) {
-  static const void* const scans[2][3] = {{(const void*)fx_beam_scan<float, 4>, (const void*)fx_beam_scan<_Float16, 4>, (const void*)fx_beam_scan<__bf16, 4>},
-                                          {(const void*)fx_beam_scan<float, 8>, (const void*)fx_beam_scan<_Float16, 8>, (const void*)fx_beam_scan<__bf16, 8>}};
-  // (16: 64 parts of 16-bit rows are 2^18 words with 8)
-  const void* const scan = a.loads == 16 ? (const void*)fx_beam_scan<float, 16> : scans[a.loads == 8][a.dtype == FX_DT_F32 ? 0 : a.dtype == FX_DT_F16 ? 1 : 2];
+  static const void* const scans[3] = {(const void*)fx_beam_scan<float>, (const void*)fx_beam_scan<_Float16>, (const void*)fx_beam_scan<__bf16>};
+  static const void* const joins[3] = {(const void*)fx_beam_join<float>, (const void*)fx_beam_join<_Float16>, (const void*)fx_beam_join<__bf16>};
+  const int type = a.dtype == FX_DT_F32 ? 0 : a.dtype == FX_DT_F16 ? 1 : 2;
   FxBeamArgs args = a;
   void* kargs[1] = {(void*)&args};
-  const int64_t units = (int64_t)a.requests * a.beams * a.chunks;
+  const int64_t units = (int64_t)a.requests * a.beams * a.parts_a_row;
   *launched = 0;
-  const hipError_t e = hipLaunchKernel(scan, dim3((unsigned)((units + kWaves - 1) / kWaves)), dim3(kThreads), kargs, 0, stream);
+  const hipError_t e = hipLaunchKernel(scans[type], dim3((unsigned)((units + kWaves - 1) / kWaves)), dim3(kThreads), kargs, 0, stream);
   if (e != hipSuccess) return e;
   *launched = 1;
-  // (64 KiB of LDS a workgroup: at most 32 * 64 candidates of 12 bytes, and one row's lists of 64 * 64 words of 8)
-  const size_t rows = (size_t)a.beams * a.count * 12 + 8, lists = (size_t)a.chunks * a.count * sizeof(FxBeamWord);
-  const int waves = std::max(1, std::min(std::min(a.beams, 16), (int)((65536 - rows) / lists)));
-  const hipError_t f = hipLaunchKernel((const void*)fx_beam_join, dim3((unsigned)a.requests), dim3((unsigned)waves * 64), kargs, rows + (size_t)waves * lists, stream);
+  // (64 KiB of LDS a workgroup)
+  const int a_wave = 64 * 20 + kList * 8 + kSegments * 4, waves = std::min(std::min(a.beams, kJoinWaves), (65536 - a.beams * a.count * 12) / a_wave);
+  const hipError_t f = hipLaunchKernel(joins[type], dim3((unsigned)a.requests), dim3((unsigned)waves * 64), kargs, (size_t)(a.beams * a.count * 12 + waves * a_wave), stream);
   if (f == hipSuccess) *launched = 2;
   return f;
 }
