@@ -5,7 +5,7 @@
 
 #include "../../../include/fxhip.h"
 
-#define FX_BEAM_SEGMENTS 16   // of a wave's words: those of 16 lanes' loads, side by side
+#define FX_BEAM_SEGMENTS 8   // of a wave's words: what 16 lanes have loaded in two neighbouring loads
 // What a wave finds in its words: the largest logit and the sum of 2^(x c - r) (NaN where there is one)
 struct FxBeamPart {
   float top;

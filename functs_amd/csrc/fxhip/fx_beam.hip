@@ -1,7 +1,7 @@
 // A beam search's selection: of each request the `count` best continuations of all its beams and words, by score + logit - log sum exp(logits).
 //
 // Two launches.  fx_beam_scan reads the logits once; a wave leaves the sum of exponentials of its 2 048 (16-bit types) or 1 024 words and the largest of each
-// sixteenth of them.  fx_beam_join, a workgroup a request and a wave a row, finds from these which few segments the best words can lie in, reads those again (from the caches, as a
+// eighth of them.  fx_beam_join, a workgroup a request and a wave a row, finds from these which few segments the best words can lie in, reads those again (from the caches, as a
 // rule) and takes their best; then it ranks the rows' candidates.  (The best words of every part found by fx_beam_scan itself: 31 us for 488 rows of 128 001 words,
 // half of them instructions of that search.)
 //
@@ -20,6 +20,8 @@ constexpr int kThreads = 256, kWaves = kThreads / 64;
 constexpr int kLoads = 4;    // of 16 bytes that a lane of fx_beam_scan has under way (8: rows of an odd number of words took 23 us where four take 18, and little else)
 constexpr int kList = 256;   // candidates that a wave keeps: the best FX_BEAM_MAX_COUNT and two steps' of 64
 constexpr int kSegments = 512;   // that it lists before it looks at them
+constexpr int kPer = kLoads * 4 / FX_BEAM_SEGMENTS;   // loads of 16 lanes that are a segment (1: fx_beam_scan 25.4 us instead of 24.4; 4: 22.5, but fx_beam_join 2.5 us more)
+constexpr int kUnder = 6;        // loads of a lane of fx_beam_join under way: 12 segments
 constexpr int kJoinWaves = 8;    // rows of a request at a time, at most
 constexpr float kLowest = -3.402823466e38f;   // (-infinity is none)
 
@@ -117,7 +119,7 @@ __device__ __forceinline__ double lse_of(float most, double sum) {
 // Words of a row: load l of a part, in its lane.  Loads that would begin in a row's last words lie at its end (at), less the first ones, which are other lanes'
 template <class T>
 struct Words {
-  static constexpr int kVec = 16 / (int)sizeof(T), kPart = 64 * kVec * kLoads, kSegment = 16 * kVec;
+  static constexpr int kVec = 16 / (int)sizeof(T), kPart = 64 * kVec * kLoads;
   const T* x;
   int words;
   __device__ __forceinline__ int at(int place) const { return min(place, words - kVec); }
@@ -190,6 +192,7 @@ __global__ __launch_bounds__(kThreads, 8) void fx_beam_scan(const FxBeamArgs a) 
   }
   float x[kLoads][W::kVec];
   int all = (int)0x80000000;
+  float pair = -INFINITY;
   int* const tops = a.tops + (int64_t)unit * FX_BEAM_SEGMENTS + (lane >> 4);
 #pragma unroll
   for (int l = 0; l < kLoads; ++l) {
@@ -199,9 +202,13 @@ __global__ __launch_bounds__(kThreads, 8) void fx_beam_scan(const FxBeamArgs a) 
       x[l][e] = v[l][e];
       m = fmaxf(m, x[l][e]);   // (NaN is passed over here, and is in the sum)
     }
-    const int segment = segment_max(ordered(m));
-    if ((lane & 15) == 15) tops[l * 4] = segment;
-    all = max(all, segment);
+    pair = fmaxf(pair, m);
+    if (l % kPer == kPer - 1) {
+      const int segment = segment_max(ordered(pair));
+      if ((lane & 15) == 15) tops[l / kPer * 4] = segment;
+      all = max(all, segment);
+      pair = -INFINITY;
+    }
   }
   const float most = unordered(max(max(__builtin_amdgcn_readlane(all, 15), __builtin_amdgcn_readlane(all, 31)), max(__builtin_amdgcn_readlane(all, 47), __builtin_amdgcn_readlane(all, 63))));
   const bool far = far_from(most);
@@ -326,10 +333,12 @@ __global__ __launch_bounds__(512) void fx_beam_join(const FxBeamArgs a) {
             }
           }
           in_wave();
-          // The words of the listed segments, 16 lanes a segment, four loads under way.  Of the loads those that have a word above the bound go to LDS, 64 at most,
+          // The words of the listed segments, 32 lanes a segment, six loads under way.  Of the loads those that have a word above the bound go to LDS, 64 at most,
           // and from there each of their words to a lane.  More than 64 (of equal words): all loads take that way, four segments at a time.
           const auto place_of = [&](int i) {   // (of none: behind the last word, where nothing is the lane's)
-            return i < listed ? list[i] * W::kSegment + (lane & 15) * W::kVec : a.words;
+            if (i >= listed) return a.words;
+            const int s = list[i], part = s / FX_BEAM_SEGMENTS, first = s % FX_BEAM_SEGMENTS / 4 * kPer + ((lane >> 4) & (kPer - 1));   // the load of the part
+            return part * W::kPart + (first * 64 + (s & 3) * 16 + (lane & 15)) * W::kVec;
           };
           const auto load = [&](int place) {
             if (!tiny) return w.load(place);
@@ -339,12 +348,12 @@ __global__ __launch_bounds__(512) void fx_beam_join(const FxBeamArgs a) {
           };
           int found = 0;
 #pragma unroll 1
-          for (int i0 = 0; i0 < listed; i0 += 16) {
-            Load<T> v[4];
-            int place[4];
+          for (int i0 = 0; i0 < listed; i0 += kUnder * 4 / kPer) {
+            Load<T> v[kUnder];
+            int place[kUnder];
 #pragma unroll
-            for (int u = 0; u < 4; ++u) {
-              place[u] = place_of(i0 + 4 * u + (lane >> 4));
+            for (int u = 0; u < kUnder; ++u) {
+              place[u] = place_of(i0 + (4 * u + (lane >> 4)) / kPer);
               v[u] = load(place[u]);
             }
             if (lse == 0.0) {   // (the first time, while they are under way)
@@ -355,7 +364,7 @@ __global__ __launch_bounds__(512) void fx_beam_join(const FxBeamArgs a) {
               if (!(lse - lse == 0.0)) listed = 0, seen = fours;   // (a row with NaN or +infinity has no candidates)
             }
 #pragma unroll
-            for (int u = 0; u < 4; ++u) {
+            for (int u = 0; u < kUnder; ++u) {
               float m = v[u][0];   // (of words that are other lanes', too: they are passed over below)
 #pragma unroll
               for (int e = 1; e < W::kVec; ++e) m = fmaxf(m, v[u][e]);
@@ -376,7 +385,7 @@ __global__ __launch_bounds__(512) void fx_beam_join(const FxBeamArgs a) {
           while (found > 0) {
             if (!few) {
               in_wave();
-              const int place = place_of(i0 + (lane >> 4));
+              const int place = place_of(i0 + (lane >> 4) / kPer);
               const Load<T> v = load(place);
               loads[lane] = make_uint4(v.u[0], v.u[1], v.u[2], v.u[3]);
               places[lane] = place;
@@ -416,7 +425,7 @@ __global__ __launch_bounds__(512) void fx_beam_join(const FxBeamArgs a) {
               if (hit) keys[n + below(lanes)] = key_of(z, here);
               n += __builtin_popcountll(lanes);
             }
-            i0 += 4;
+            i0 += 4 / kPer;
             if (few || i0 >= listed) break;
           }
         }

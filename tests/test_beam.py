@@ -119,10 +119,10 @@ def test_the_c_abi_refuses_before_it_launches():
             assert lib.fx_beam_select_workspace_bytes(ctypes.byref(d)) == 0
     assert lib.fx_beam_select(None, None) == C["FX_E_INVALID"] and lib.fx_beam_select_workspace_bytes(None) == 0
     assert lib.fx_beam_select(ctypes.byref(Desc(**{**ok, "requests": 0})), None) == 0   # nothing to do
-    # each 256 loads of 16 bytes of a row: 16 bytes, and 4 for each of 16 segments
+    # each 256 loads of 16 bytes of a row: 16 bytes, and 4 for each of 8 segments
     for words, dtype, parts in ((10, "FX_DT_BF16", 1), (2049, "FX_DT_BF16", 2), (131072, "FX_DT_F16", 64), (131073, "FX_DT_F16", 65), (262144, "FX_DT_F32", 256), (1025, "FX_DT_F32", 2)):
         d = Desc(**{**ok, "words": words, "dtype": C[dtype]})
-        assert lib.fx_beam_select_workspace_bytes(ctypes.byref(d)) == 8 * parts * (16 + 4 * 16)
+        assert lib.fx_beam_select_workspace_bytes(ctypes.byref(d)) == 8 * parts * (16 + 4 * 8)
 
 
 # ---- GPU ----
