@@ -18,11 +18,13 @@
 namespace {
 constexpr int kThreads = 256, kWaves = kThreads / 64;
 constexpr int kLoads = 4;    // of 16 bytes that a lane of fx_beam_scan has under way (8: rows of an odd number of words took 23 us where four take 18, and little else)
-constexpr int kList = 256;   // candidates that a wave keeps: the best FX_BEAM_MAX_COUNT and two steps' of 64
-constexpr int kSegments = 512;   // that it lists before it looks at them
+constexpr int kMore = 128;   // candidates that a wave keeps besides the best `count`: two steps' of 64
+constexpr int kList = FX_BEAM_MAX_COUNT + kMore;
+constexpr int kSegments = 384;   // that it lists before it looks at them
 constexpr int kPer = kLoads * 4 / FX_BEAM_SEGMENTS;   // loads of 16 lanes that are a segment (1: fx_beam_scan 25.4 us instead of 24.4; 4: 22.5, but fx_beam_join 2.5 us more)
 constexpr int kUnder = 6;        // loads of a lane of fx_beam_join under way: 12 segments
-constexpr int kJoinWaves = 8;    // rows of a request at a time, at most
+constexpr int kJoinWaves = 16;   // rows of a request at a time, at most
+constexpr int kLinear = 128;     // candidates of a request that are ranked against each other; more are joined in pairs of rows
 constexpr float kLowest = -3.402823466e38f;   // (-infinity is none)
 
 __device__ __forceinline__ float wave_max(float m) {
@@ -242,16 +244,17 @@ __global__ __launch_bounds__(kThreads, 8) void fx_beam_scan(const FxBeamArgs a) 
 // Bound: latency.  A row is a chain of some ten steps, and the code of each arrives for the first time: loops are not unrolled where they need not be (16 segments' loads in
 // registers, 28 KB of code, took 2 us more than this).
 template <class T>
-__global__ __launch_bounds__(512) void fx_beam_join(const FxBeamArgs a) {
+__global__ __launch_bounds__(64 * kJoinWaves) void fx_beam_join(const FxBeamArgs a) {
   typedef Words<T> W;
   extern __shared__ uint4 s_join[];
   const int count = a.count, K = a.beams, lane = (int)threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), waves = (int)blockDim.x >> 6;
   uint4* loads = s_join + wave * 64;                               // [waves][64]
   double* score = (double*)(s_join + waves * 64);                  // [beams][count]
-  uint64_t* keys = (uint64_t*)score + K * count + wave * kList;    // [waves][kList]
-  uint32_t* word = (uint32_t*)((uint64_t*)score + K * count + waves * kList);   // [beams][count]
-  int* list = (int*)(word + K * count) + wave * kSegments;         // [waves][kSegments]
-  int* places = (int*)(word + K * count) + waves * kSegments + wave * 64;       // [waves][64]
+  const int room = count + kMore;
+  uint64_t* keys = (uint64_t*)score + K * count + wave * room;     // [waves][room]
+  uint32_t* word = (uint32_t*)((uint64_t*)score + K * count + waves * room);    // [beams][count]
+  int* places = (int*)(word + K * count) + wave * 64;              // [waves][64]
+  uint16_t* list = (uint16_t*)((int*)(word + K * count) + waves * 64) + wave * kSegments;   // [waves][kSegments] (2^18 words have 2 048 at most)
   const int64_t request = blockIdx.x;
   const int fours = a.parts_a_row * (FX_BEAM_SEGMENTS / 4);        // of segments of a row
   for (int k = wave; k < K; k += waves) {
@@ -289,28 +292,32 @@ __global__ __launch_bounds__(512) void fx_beam_join(const FxBeamArgs a) {
     } else if (live) {
       const float top = wave_max(fmaxf(fmaxf(group[0], group[1]), fmaxf(group[2], group[3])));
       if (top > -INFINITY) {
-        // a bound with at least `count` groups at or above it (all are at or above the least), and hopefully few more
-        float low = -wave_max(-fminf(fminf(group[0], group[1]), fminf(group[2], group[3]))), high = top;
         const auto above = [&](float b) {
           int some = 0;
 #pragma unroll
           for (int g = 0; g < 4; ++g) some += __builtin_popcountll(__ballot(group[g] >= b));
           return some;
         };
-        if (high - 64.0f > low && above(high - 64.0f) >= count) low = high - 64.0f;
-        // (quarters instead of halves, whose counts do not wait for each other; fewer segments than 12 take as long as so many)
+        // a bound with at least `count` groups at or above it and hopefully no more than `enough`; `low` is one to begin with, `high` the largest.
+        // (quarters instead of halves, whose counts do not wait for each other)
+        const auto raise = [&](float low, float high, int enough) {
+          if (high - 64.0f > low && above(high - 64.0f) >= count) low = high - 64.0f;
 #pragma unroll 1
-        for (int i = 0; i < 10; ++i) {
-          const float mid = 0.5f * low + 0.5f * high, one = 0.5f * low + 0.5f * mid, three = 0.5f * mid + 0.5f * high;
-          if (!(mid > low)) break;
-          const int at_one = above(one), at_mid = above(mid), at_three = above(three);
-          int some = at_one;
-          if (at_three >= count) low = three, some = at_three;
-          else if (at_mid >= count) low = mid, high = three, some = at_mid;
-          else if (at_one >= count) low = one, high = mid;
-          else high = one;
-          if (some >= count && some <= max(count + 2, 12)) break;
-        }
+          for (int i = 0; i < 10; ++i) {
+            const float mid = 0.5f * low + 0.5f * high, one = 0.5f * low + 0.5f * mid, three = 0.5f * mid + 0.5f * high;
+            if (!(mid > low)) break;
+            const int at_one = above(one), at_mid = above(mid), at_three = above(three);
+            int some = at_one;
+            if (at_three >= count) low = three, some = at_three;
+            else if (at_mid >= count) low = mid, high = three, some = at_mid;
+            else if (at_one >= count) low = one, high = mid;
+            else high = one;
+            if (some >= count && some <= enough) break;
+          }
+          return low;
+        };
+        // (all groups are at or above the least; of long rows, fewer segments than 12 take as long as so many)
+        const float low = raise(-wave_max(-fminf(fminf(group[0], group[1]), fminf(group[2], group[3]))), top, max(count + 2, min(12, fours)));
         float bound = fmaxf(low, kLowest);
         uint32_t last = 0xffffffffu;      // of words equal to the bound, those up to this one
         const W w = words_of<T>(a, row);
@@ -334,7 +341,8 @@ __global__ __launch_bounds__(512) void fx_beam_join(const FxBeamArgs a) {
           }
           in_wave();
           // The words of the listed segments, 32 lanes a segment, six loads under way.  Of the loads those that have a word above the bound go to LDS, 64 at most,
-          // and from there each of their words to a lane.  More than 64 (of equal words): all loads take that way, four segments at a time.
+          // and from there each of their words to a lane.  More than 64 (of rows with few segments, or many equal words): once the bound is raised by the largest
+          // words of 256 groups of the loads; if that does not help, all loads take that way, four segments at a time.
           const auto place_of = [&](int i) {   // (of none: behind the last word, where nothing is the lane's)
             if (i >= listed) return a.words;
             const int s = list[i], part = s / FX_BEAM_SEGMENTS, first = s % FX_BEAM_SEGMENTS / 4 * kPer + ((lane >> 4) & (kPer - 1));   // the load of the part
@@ -348,37 +356,59 @@ __global__ __launch_bounds__(512) void fx_beam_join(const FxBeamArgs a) {
           };
           int found = 0;
 #pragma unroll 1
-          for (int i0 = 0; i0 < listed; i0 += kUnder * 4 / kPer) {
-            Load<T> v[kUnder];
-            int place[kUnder];
-#pragma unroll
-            for (int u = 0; u < kUnder; ++u) {
-              place[u] = place_of(i0 + (4 * u + (lane >> 4)) / kPer);
-              v[u] = load(place[u]);
-            }
-            if (lse == 0.0) {   // (the first time, while they are under way)
-              double sum = part_of(first, top);
+          for (int time = 0;; ++time) {
+            found = 0;
 #pragma unroll 1
-              for (int i = lane + 64; i < a.parts_a_row; i += 64) sum += part_of(parts[i], top);
-              lse = lse_of(top, wave_sum(sum));
-              if (!(lse - lse == 0.0)) listed = 0, seen = fours;   // (a row with NaN or +infinity has no candidates)
-            }
+            for (int i0 = 0; i0 < listed; i0 += kUnder * 4 / kPer) {
+              Load<T> v[kUnder];
+              int place[kUnder];
 #pragma unroll
-            for (int u = 0; u < kUnder; ++u) {
-              float m = v[u][0];   // (of words that are other lanes', too: they are passed over below)
-#pragma unroll
-              for (int e = 1; e < W::kVec; ++e) m = fmaxf(m, v[u][e]);
-              const bool some = m >= bound && place[u] < a.words;
-              const uint64_t lanes = __ballot(some);
-              const int to = found + below(lanes);
-              if (some && to < 64) {
-                loads[to] = make_uint4(v[u].u[0], v[u].u[1], v[u].u[2], v[u].u[3]);
-                places[to] = place[u];
+              for (int u = 0; u < kUnder; ++u) {
+                place[u] = place_of(i0 + (4 * u + (lane >> 4)) / kPer);
+                v[u] = load(place[u]);
               }
-              found += __builtin_popcountll(lanes);
+              if (lse == 0.0) {   // (the first time, while they are under way)
+                double sum = part_of(first, top);
+#pragma unroll 1
+                for (int i = lane + 64; i < a.parts_a_row; i += 64) sum += part_of(parts[i], top);
+                lse = lse_of(top, wave_sum(sum));
+                if (!(lse - lse == 0.0)) listed = 0, seen = fours;   // (a row with NaN or +infinity has no candidates)
+              }
+#pragma unroll
+              for (int u = 0; u < kUnder; ++u) {
+                float m = v[u][0];   // (of words that are other lanes', too: they are passed over below)
+#pragma unroll
+                for (int e = 1; e < W::kVec; ++e) m = fmaxf(m, v[u][e]);
+                const bool some = m >= bound && place[u] < a.words;
+                const uint64_t lanes = __ballot(some);
+                const int to = found + below(lanes);
+                if (some && to < 64) {
+                  loads[to] = make_uint4(v[u].u[0], v[u].u[1], v[u].u[2], v[u].u[3]);
+                  places[to] = place[u];
+                }
+                found += __builtin_popcountll(lanes);
+              }
             }
+            if (listed == 0) found = 0;
+            if (found <= 64 || time == 1) break;
+            group[0] = group[1] = group[2] = group[3] = -INFINITY;
+#pragma unroll 1
+            for (int i0 = 0; i0 < listed; i0 += 16 / kPer) {
+#pragma unroll
+              for (int u = 0; u < 4; ++u) {
+                const int place = place_of(i0 + (4 * u + (lane >> 4)) / kPer);
+                Load<T> v = w.load(place);   // (a row of one load has not so many)
+                w.mask(v, place);
+#pragma unroll
+                for (int e = 0; e < W::kVec; ++e) group[u] = fmaxf(group[u], v[e]);
+              }
+            }
+            if (above(bound) < count) break;
+            const float raised = raise(bound, top, count + 2);
+            if (!(raised > bound)) break;
+            bound = raised;
+            last = 0xffffffffu;
           }
-          if (listed == 0) found = 0;
           const bool few = found <= 64;
           int i0 = 0;    // of the segments, where they come four at a time
 #pragma unroll 1
@@ -394,7 +424,7 @@ __global__ __launch_bounds__(512) void fx_beam_join(const FxBeamArgs a) {
             in_wave();
 #pragma unroll 1
             for (int i1 = 0; i1 < found + 64 / W::kVec; i1 += 64 / W::kVec) {   // (and once more, for what is left in the list)
-              if (n > kList - 64 || i1 >= found) {
+              if (n > room - 64 || i1 >= found) {
                 // no room for a word of each lane, or the end: the best `count`, in order; what comes has to be better than the last of them
                 uint64_t mine[kList / 64];
                 int rank[kList / 64];
@@ -440,30 +470,79 @@ __global__ __launch_bounds__(512) void fx_beam_join(const FxBeamArgs a) {
     for (int i = n + lane; i < count; i += 64) score[k * count + i] = -INFINITY;
   }
   __syncthreads();
-  // the place of a candidate: how many are better, or as good and before it; eight lanes to a candidate
-  const int all = K * count, eighth = (int)threadIdx.x & 7;
-  for (int i = (int)threadIdx.x >> 3; i < all; i += (int)blockDim.x >> 3) {
-    const double s = score[i];
-    int rank = 0;
+  const int all = K * count;
+  if (all <= kLinear) {
+    // the place of a candidate: how many are better, or as good and before it; eight lanes to a candidate
+    const int eighth = (int)threadIdx.x & 7;
+    for (int i = (int)threadIdx.x >> 3; i < all; i += (int)blockDim.x >> 3) {
+      const double s = score[i];
+      int rank = 0;
 #pragma unroll 4
-    for (int j = eighth; j < all; j += 8) {
-      const double t = score[j];
-      rank += t > s || (t == s && j < i) ? 1 : 0;
+      for (int j = eighth; j < all; j += 8) {
+        const double t = score[j];
+        rank += t > s || (t == s && j < i) ? 1 : 0;
+      }
+      rank += __shfl_xor(rank, 1, 64);
+      rank += __shfl_xor(rank, 2, 64);
+      rank += __shfl_xor(rank, 4, 64);
+      if (eighth != 0 || rank >= count || !(s > -INFINITY)) continue;
+      const int k = i / count;
+      const int64_t to = request * count + rank;
+      a.out_scores[to] = (float)s;
+      a.out_beams[to] = k;
+      a.out_words[to] = a.ended && a.ended[request * K + k] ? a.end_word : (int64_t)word[i];
     }
-    rank += __shfl_xor(rank, 1, 64);
-    rank += __shfl_xor(rank, 2, 64);
-    rank += __shfl_xor(rank, 4, 64);
-    if (eighth != 0 || rank >= count || !(s > -INFINITY)) continue;
-    const int k = i / count;
-    const int64_t to = request * count + rank;
-    a.out_scores[to] = (float)s;
-    a.out_beams[to] = k;
-    a.out_words[to] = a.ended && a.ended[request * K + k] ? a.end_word : (int64_t)word[i];
+  } else {
+    // each row's are in order: two rows' lists at a time become one, of the best `count`; a place is found by halves in the other list
+    int* from = (int*)s_join;   // [beams][count], where the loads were
+    for (int i = (int)threadIdx.x; i < all; i += (int)blockDim.x) from[i] = i;
+    for (int d = 1; d < K; d <<= 1) {
+      constexpr int kEach = 4;   // of a thread: a wave has four rows or fewer
+      __syncthreads();
+      double s[kEach];
+      int id[kEach], to[kEach];
+#pragma unroll
+      for (int e = 0; e < kEach; ++e) {
+        const int i = (int)threadIdx.x + e * (int)blockDim.x, k = i / count, at = i - k * count;
+        to[e] = -1;
+        const bool right = (k & d) != 0;
+        const int other = right ? k - d : k + d;
+        if (i >= all || (k & (d - 1)) != 0 || other >= K) continue;
+        s[e] = score[i];
+        id[e] = from[i];
+        int less = 0, more = count;   // of the other list: `less` at least go before this one, `more` at most
+        while (less < more) {
+          const int mid = (less + more) >> 1;
+          const double t = score[other * count + mid];
+          const bool before = right ? t >= s[e] : t > s[e];
+          less = before ? mid + 1 : less;
+          more = before ? more : mid;
+        }
+        if (at + less < count) to[e] = (k & ~d) * count + at + less;
+      }
+      __syncthreads();
+#pragma unroll
+      for (int e = 0; e < kEach; ++e) {
+        if (to[e] < 0) continue;
+        score[to[e]] = s[e];
+        from[to[e]] = id[e];
+      }
+    }
+    __syncthreads();
+    for (int i = (int)threadIdx.x; i < count; i += (int)blockDim.x) {
+      const double s = score[i];
+      if (!(s > -INFINITY)) continue;
+      const int k = from[i] / count;
+      const int64_t to = request * count + i;
+      a.out_scores[to] = (float)s;
+      a.out_beams[to] = k;
+      a.out_words[to] = a.ended && a.ended[request * K + k] ? a.end_word : (int64_t)word[from[i]];
+    }
   }
   // places that are left
   if (wave == 0) {
     int there = 0;
-    for (int i = lane; i < all; i += 64) there += score[i] > -INFINITY ? 1 : 0;
+    for (int i = lane; i < (all <= kLinear ? all : count); i += 64) there += score[i] > -INFINITY ? 1 : 0;
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) there += __shfl_xor(there, d, 64);
     for (int i = there + lane; i < count; i += 64) {
@@ -492,8 +571,9 @@ hipError_t fx_launch_beam_select(const FxBeamArgs& a, hipStream_t stream, int* l
   const hipError_t e = hipLaunchKernel(scans[type], dim3((unsigned)((units + kWaves - 1) / kWaves)), dim3(kThreads), kargs, 0, stream);
   if (e != hipSuccess) return e;
   *launched = 1;
-  // (64 KiB of LDS a workgroup)
-  const int a_wave = 64 * 20 + kList * 8 + kSegments * 4, waves = std::min(std::min(a.beams, kJoinWaves), (65536 - a.beams * a.count * 12) / a_wave);
+  // (64 KiB of LDS a workgroup: 32 beams of 64 candidates go in three rounds of eleven)
+  const int room = 65536 - a.beams * a.count * 12, a_wave = 64 * 20 + (a.count + kMore) * 8 + kSegments * 2;
+  const int rounds = (a.beams + std::min(kJoinWaves, room / a_wave) - 1) / std::min(kJoinWaves, room / a_wave), waves = (a.beams + rounds - 1) / rounds;
   const hipError_t f = hipLaunchKernel(joins[type], dim3((unsigned)a.requests), dim3((unsigned)waves * 64), kargs, (size_t)(a.beams * a.count * 12 + waves * a_wave), stream);
   if (f == hipSuccess) *launched = 2;
   return f;

@@ -40,16 +40,18 @@ __global__ __launch_bounds__(kPlanThreads) void fx_kv_fork_plan(const FxKvForkAr
     // of the rows that continue a partly filled page the first has it; a page that nobody continues is spare (of rows that share one: once)
     bool need = false, spare = here && tail >= 0;
     if (here) {
+#pragma unroll 4
       for (int j = 0; j < K; ++j) {
         const int w = s_want[first + j], t = s_tail[first + j];
-        need = need || (j < own && want >= 0 && w == want);
-        spare = spare && w != tail && !(j < own && t == tail);
+        need |= (j < own) & (want >= 0) & (w == want);
+        spare &= (w != tail) & !((j < own) & (t == tail));
       }
     }
     s_flags[tid] = (need ? 1 : 0) | (spare ? 2 : 0);
     __syncthreads();
     int needs = 0, spares = 0, needs_before = 0, spares_before = 0;
     if (here) {
+#pragma unroll 4
       for (int j = 0; j < K; ++j) {
         const int f = s_flags[first + j];
         needs += f & 1;
@@ -71,6 +73,7 @@ __global__ __launch_bounds__(kPlanThreads) void fx_kv_fork_plan(const FxKvForkAr
     __syncthreads();
     int64_t all = 0;
     before -= mine;
+#pragma unroll 4
     for (int w = 0; w < kPlanThreads / 64; ++w) {
       if (w < wave) before += s_sum[w];
       all += s_sum[w];
@@ -93,7 +96,8 @@ __global__ __launch_bounds__(kPlanThreads) void fx_kv_fork_plan(const FxKvForkAr
     __syncthreads();
     if (here) {
       bool alive = false;
-      for (int j = 0; j < K; ++j) alive = alive || s_from[first + j] == own;
+#pragma unroll 4
+      for (int j = 0; j < K; ++j) alive |= s_from[first + j] == own;
       FxKvForkRow row;
       row.from = granted ? parent : -1;
       row.last = last;
@@ -127,33 +131,39 @@ __global__ __launch_bounds__(kThreads) void fx_kv_fork_tables(const FxKvForkArgs
   int32_t* const table = a.table + (int64_t)group * K * a.table_stride;
   if (tid < K * (int)(sizeof(FxKvForkRow) / 4)) ((int*)s_row)[tid] = ((const int*)(a.rows + (int64_t)group * K))[tid];
   __syncthreads();
+  // (loops over rows are without branches, so that their reads do not wait for each other)
   int most = 0;
-  for (int i = 0; i < K; ++i) most = max(most, s_row[i].held);
+  uint32_t alive = 0;
+#pragma unroll 4
+  for (int i = 0; i < K; ++i) {
+    most = max(most, s_row[i].held);
+    alive |= (s_row[i].alive != 0 ? 1u : 0u) << i;
+  }
   if (((int64_t)block * kThreads << a.log_page) >= most) {   // (no row has a page here)
     if (tid == 0) a.counts[blockIdx.x] = 0;
     return;
   }
   // what the group's rows have: pages up to the one in which their tokens end (-1 behind)
   const auto has = [&](int i) { return c < (s_row[i].held >> a.log_page) + ((s_row[i].held & (page - 1)) != 0 ? 1 : 0); };
+#pragma unroll 4
   for (int i = 0; i < K; ++i) s_pages[i * kThreads + tid] = has(i) ? table[(int64_t)i * a.table_stride + c] : -1;
   // (a thread reads its own column alone, which it has written)
+#pragma unroll 4
   for (int j = 0; j < K; ++j) {
-    const FxKvForkRow& row = s_row[j];
-    if (row.from < 0) continue;
-    const int whole = row.tokens >> a.log_page;
-    if (c < whole) {
-      if (row.from != j) table[(int64_t)j * a.table_stride + c] = s_pages[row.from * kThreads + tid];
-    } else if (c == whole && (row.tokens & (page - 1)) != 0) {
-      table[(int64_t)j * a.table_stride + c] = row.last;
-    }
+    const int from = s_row[j].from, last = s_row[j].last, tokens = s_row[j].tokens, whole = tokens >> a.log_page;
+    const int moved = s_pages[max(from, 0) * kThreads + tid];
+    const bool ends = (c == whole) & ((tokens & (page - 1)) != 0);
+    if ((from >= 0) & (((c < whole) & (from != j)) | ends)) table[(int64_t)j * a.table_stride + c] = ends ? last : moved;
   }
   unsigned gone = 0;
   for (int i = 0; i < K; ++i) {
-    if (s_row[i].alive) continue;
+    if ((alive >> i & 1) != 0) continue;
     const int p = s_pages[i * kThreads + tid];
     if (p < 0 || (s_row[i].reused && c == s_row[i].held >> a.log_page)) continue;
+    const unsigned others = alive | ((1u << i) - 1);   // that keep it, or have said so (i is not among them)
     bool kept = false;
-    for (int o = 0; o < K; ++o) kept = kept || ((s_row[o].alive || o < i) && o != i && s_pages[o * kThreads + tid] == p);
+#pragma unroll 8
+    for (int o = 0; o < K; ++o) kept |= ((others >> o & 1) != 0) & (s_pages[o * kThreads + tid] == p);
     gone |= kept ? 0u : 1u << i;
   }
   // column by column

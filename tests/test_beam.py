@@ -312,3 +312,23 @@ def test_two_launches():
     beam.select(x, s)
     lib.fx_launch_stats(ctypes.byref(total), ctypes.byref(special))
     assert total.value == before + 2
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("B,K,V,count", [(5, 12, 2706, 24), (3, 11, 579, 22), (2, 17, 700, 64), (1, 16, 130, 9), (2, 9, 15000, 15), (59, 1, 978, 1), (2, 3, 700, 43), (1, 31, 4099, 5)])
+def test_rows_of_few_segments_and_many_beams(B, K, V, count, dtype):
+    x, s = logits_of(B, K, V, V + K, dtype)
+    check(x, s, count)
+    x[torch.rand(x.shape, generator=torch.Generator().manual_seed(V)).cuda() < 0.9] = -math.inf
+    check(x, s, count, spread_ended(B, K), V - 1)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("K,count", [(4, 8), (13, 26), (32, 64), (3, 64)])
+def test_beams_of_the_same_numbers_go_in_order(K, count):
+    x, _ = logits_of(1, 1, 900, 6)
+    got = beam.select(x.expand(1, K, 900).contiguous(), torch.zeros(1, K, device="cuda"), count)
+    words = torch.sort(x[0, 0], descending=True, stable=True).indices
+    assert got.beams[0].tolist() == [i % K for i in range(count)]
+    assert got.words[0].tolist() == [int(words[i // K]) for i in range(count)]
