@@ -24,7 +24,7 @@ constexpr int kSegments = 384;   // that it lists before it looks at them
 constexpr int kPer = kLoads * 4 / FX_BEAM_SEGMENTS;   // loads of 16 lanes that are a segment (1: fx_beam_scan 25.4 us instead of 24.4; 4: 22.5, but fx_beam_join 2.5 us more)
 constexpr int kUnder = 6;        // loads of a lane of fx_beam_join under way: 12 segments
 constexpr int kJoinWaves = 16;   // rows of a request at a time, at most
-constexpr int kLinear = 128;     // candidates of a request that are ranked against each other; more are joined in pairs of rows
+constexpr int kLinear = 256;     // candidates of a request that are ranked against each other; more are joined in pairs of rows (450: 17 us instead of 22; 256: 14.5, and 15 in pairs)
 constexpr float kLowest = -3.402823466e38f;   // (-infinity is none)
 
 __device__ __forceinline__ float wave_max(float m) {
@@ -341,8 +341,9 @@ __global__ __launch_bounds__(64 * kJoinWaves) void fx_beam_join(const FxBeamArgs
           }
           in_wave();
           // The words of the listed segments, 32 lanes a segment, six loads under way.  Of the loads those that have a word above the bound go to LDS, 64 at most,
-          // and from there each of their words to a lane.  More than 64 (of rows with few segments, or many equal words): once the bound is raised by the largest
-          // words of 256 groups of the loads; if that does not help, all loads take that way, four segments at a time.
+          // and from there each of their words to a lane.  If they are many (of rows with few segments, or equal words), the bound is raised once, by the largest
+          // words of 256 groups of the loads (15 beams of 247 words, 15 wanted: 17.6 us, and 21 without); if that leaves more than 64, all loads take that way, four
+          // segments at a time.
           const auto place_of = [&](int i) {   // (of none: behind the last word, where nothing is the lane's)
             if (i >= listed) return a.words;
             const int s = list[i], part = s / FX_BEAM_SEGMENTS, first = s % FX_BEAM_SEGMENTS / 4 * kPer + ((lane >> 4) & (kPer - 1));   // the load of the part
@@ -390,7 +391,7 @@ __global__ __launch_bounds__(64 * kJoinWaves) void fx_beam_join(const FxBeamArgs
               }
             }
             if (listed == 0) found = 0;
-            if (found <= 64 || time == 1) break;
+            if (found <= min(64, count + 12) || time == 1) break;
             group[0] = group[1] = group[2] = group[3] = -INFINITY;
 #pragma unroll 1
             for (int i0 = 0; i0 < listed; i0 += 16 / kPer) {
