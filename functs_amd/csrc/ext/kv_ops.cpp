@@ -172,9 +172,10 @@ Tensor kvAppend(const Tensor& q_, const Tensor& k_, const Tensor& v_, Tensor k_c
   TORCH_CHECK(positions_.dim() == 1 && positions_.size(0) == tokens, op, ": positions must be [", tokens, "], got ", positions_.sizes());
   const int dtype = dtypeOf(op, k_.scalar_type(), "k");
   c10::DeviceGuard guard(dev);
-  const Tensor positions = positions_.contiguous(), frequencies = frequencies_.contiguous();
+  const Tensor positions = positions_.contiguous(), frequencies = frequencies_.resolve_neg().contiguous();
   fx_rotary_desc d = rotaryDesc(op, positions, frequencies, magnitude, interleaved, c.depth, dev);
-  const Tensor q = q_.stride(2) == 1 ? q_ : q_.contiguous(), k = k_.stride(2) == 1 ? k_ : k_.contiguous(), v = v_.stride(2) == 1 ? v_ : v_.contiguous();
+  const auto rows = [](const Tensor& t) { return t.stride(2) == 1 ? t.resolve_neg() : t.resolve_neg().contiguous(); };
+  const Tensor q = rows(q_), k = rows(k_), v = rows(v_);
   Tensor out = at::empty(q.sizes(), q.options().memory_format(at::MemoryFormat::Contiguous));
   d.x = q.data_ptr();
   d.y = out.data_ptr();

@@ -46,7 +46,7 @@ Tensor turned(const Tensor& x_, const Tensor& positions_, const Tensor& frequenc
   const auto dev = x_.device();
   c10::DeviceGuard guard(dev);
   // (what the checks of rotaryDesc refuse is refused before anything is copied: contiguous() keeps device, type and sizes)
-  const Tensor positions = positions_.dim() == 2 && positions_.stride(1) == 1 ? positions_ : positions_.contiguous(), frequencies = frequencies_.contiguous();
+  const Tensor positions = positions_.dim() == 2 && positions_.stride(1) == 1 ? positions_ : positions_.contiguous(), frequencies = frequencies_.resolve_neg().contiguous();
   fx_rotary_desc d = rotaryDesc(kOp, positions, frequencies, magnitude, interleaved, x_.size(-1), dev);
   Tensor x = x_.resolve_neg();
   if (x.stride(-1) != 1) x = x.contiguous();

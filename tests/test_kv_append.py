@@ -215,3 +215,20 @@ def test_one_launch():
     c.append(x, x, x, n, n, f)
     lib.fx_launch_stats(ctypes.byref(total), ctypes.byref(special))
     assert total.value == before + 1
+
+
+@pytest.mark.gpu
+def test_rows_that_are_negative_lazily():
+    P, H, D = 16, 2, 32
+    f, _ = rotary.frequencies(D)
+    cache = filled(4, H, P, D, INT8, 2)
+    other = copied(cache)
+    q, k, v = (torch.view_as_complex(torch.randn(7, H, D, 2, generator=torch.Generator().manual_seed(i)).cuda()).conj().imag for i in range(3))
+    packed = [torch._neg_view(t.resolve_neg().neg().contiguous()) for t in (q, k, v)]   # the same numbers, side by side
+    assert all(t.is_neg() for t in (q, k, v, *packed))
+    p = torch.arange(7, device="cuda")
+    want = cache.append(*(t.resolve_neg().contiguous() for t in (q, k, v)), p, p, f)
+    for rows, turn in (((q, k, v), f), (packed, f), (packed, torch._neg_view(f.neg()))):
+        again = copied(other)
+        assert torch.equal(again.append(*rows, p, p, turn), want)
+        same_cache(again, cache)
