@@ -2,17 +2,25 @@
 //
 // fx_kv_fork: bound by latency (a few bytes a row and a page).  Three launches, in which nothing waits for another workgroup.  fx_kv_fork_plan,
 // one workgroup for all rows, decides who gets which page where a page is partly filled; fx_kv_fork_tables, a workgroup for 256 columns of a group's rows,
-// moves the tables and finds the pages that nobody has any more; fx_kv_fork_pack puts those side by side.
+// moves the tables and finds the pages that nobody has any more; fx_kv_fork_pack puts those side by side.  Small tables: one workgroup does all three
+// (fx_kv_fork_small).  32 groups of 4 beams, 33 columns: 9.5 us, and 13.4 in three launches; 61 of 8 beams, 938 columns: 5.3 + 5.5 + 3.2 us.
 #include <algorithm>
 
 #include "fx_kv_fork.h"
 
 namespace {
 constexpr int kPlanThreads = 1024, kThreads = 256;
+// Entries of the table that one workgroup takes, of groups of so many beams (LDS), all of them filled: 4 096 in 9.2 us, and 11.4 in three launches; 16 384 in 19 to 23, and 14
+constexpr int kSmallBeams = 8, kSmall = 6144;
 
-__global__ __launch_bounds__(kPlanThreads) void fx_kv_fork_plan(const FxKvForkArgs a) {
-  __shared__ int s_tail[kPlanThreads], s_len[kPlanThreads], s_want[kPlanThreads], s_flags[kPlanThreads], s_spare[kPlanThreads], s_from[kPlanThreads];
-  __shared__ int64_t s_sum[kPlanThreads / 64];
+// Who gets which page.  HERE: at most kPlanThreads / K * K rows; what is said of row r stays in LDS (tail: last, len: held, want: tokens, flags: 1 alive, 2 reused, from).
+struct Plan {
+  int tail[kPlanThreads], len[kPlanThreads], want[kPlanThreads], flags[kPlanThreads], spare[kPlanThreads], from[kPlanThreads];
+  int64_t sum[kPlanThreads / 64];
+  __device__ __forceinline__ FxKvForkRow row(int r) const { return {from[r], tail[r], want[r], len[r], flags[r] & 1, flags[r] >> 1, {0, 0}}; }
+};
+template <bool HERE>
+__device__ __forceinline__ void plan_rows(const FxKvForkArgs& a, Plan& s) {
   const int tid = (int)threadIdx.x, lane = tid & 63, wave = tid >> 6, K = a.beams, page = 1 << a.log_page;
   const int rows = a.groups * K, a_round = kPlanThreads / K * K;
   const int own = tid < a_round ? tid % K : 0, first = tid - own;   // place in the group, and the group's first place here
@@ -31,36 +39,36 @@ __global__ __launch_bounds__(kPlanThreads) void fx_kv_fork_plan(const FxKvForkAr
     }
     const bool has = here && parent >= 0 && parent < K;
     __syncthreads();   // (the round before has been read)
-    s_tail[tid] = tail;
-    s_len[tid] = held;
+    s.tail[tid] = tail;
+    s.len[tid] = held;
     __syncthreads();
-    const int tokens = has ? s_len[first + parent] : 0, want = has ? s_tail[first + parent] : -1;
-    s_want[tid] = want;
+    const int tokens = has ? s.len[first + parent] : 0, want = has ? s.tail[first + parent] : -1;
+    s.want[tid] = want;
     __syncthreads();
     // of the rows that continue a partly filled page the first has it; a page that nobody continues is spare (of rows that share one: once)
     bool need = false, spare = here && tail >= 0;
     if (here) {
 #pragma unroll 4
       for (int j = 0; j < K; ++j) {
-        const int w = s_want[first + j], t = s_tail[first + j];
+        const int w = s.want[first + j], t = s.tail[first + j];
         need |= (j < own) & (want >= 0) & (w == want);
         spare &= (w != tail) & !((j < own) & (t == tail));
       }
     }
-    s_flags[tid] = (need ? 1 : 0) | (spare ? 2 : 0);
+    s.flags[tid] = (need ? 1 : 0) | (spare ? 2 : 0);
     __syncthreads();
     int needs = 0, spares = 0, needs_before = 0, spares_before = 0;
     if (here) {
 #pragma unroll 4
       for (int j = 0; j < K; ++j) {
-        const int f = s_flags[first + j];
+        const int f = s.flags[first + j];
         needs += f & 1;
         spares += f >> 1;
         needs_before += j < own ? f & 1 : 0;
         spares_before += j < own ? f >> 1 : 0;
       }
     }
-    if (spare) s_spare[first + spares_before] = tail;
+    if (spare) s.spare[first + spares_before] = tail;
     // free pages of this round's groups before this one
     int64_t before = own == 0 && here ? max(needs - spares, 0) : 0;
     const int64_t mine = before;
@@ -69,44 +77,44 @@ __global__ __launch_bounds__(kPlanThreads) void fx_kv_fork_plan(const FxKvForkAr
       const int64_t o = (int64_t)__shfl_up((unsigned long long)before, (unsigned)d, 64);
       if (lane >= d) before += o;
     }
-    if (lane == 63) s_sum[wave] = before;
+    if (lane == 63) s.sum[wave] = before;
     __syncthreads();
     int64_t all = 0;
     before -= mine;
 #pragma unroll 4
     for (int w = 0; w < kPlanThreads / 64; ++w) {
-      if (w < wave) before += s_sum[w];
-      all += s_sum[w];
+      if (w < wave) before += s.sum[w];
+      all += s.sum[w];
     }
-    if (own == 0) s_len[tid] = (int)min(before, (int64_t)0x7fffffff);   // (lengths have been read)
+    if (own == 0) s.len[tid] = (int)min(before, (int64_t)0x7fffffff);   // (lengths have been read)
     __syncthreads();
-    before = s_len[first];
+    before = s.len[first];
     int last = want;
     bool granted = has;
     if (need) {
       if (needs_before < spares) {
-        last = s_spare[first + needs_before];
+        last = s.spare[first + needs_before];
       } else {
         const int64_t index = from + asked + before + (needs_before - spares);
         granted = index < a.n_free;
         last = granted ? a.free_pages[index] : -1;
       }
     }
-    s_from[tid] = granted ? parent : -1;
+    s.from[tid] = granted ? parent : -1;
     __syncthreads();
     if (here) {
       bool alive = false;
 #pragma unroll 4
-      for (int j = 0; j < K; ++j) alive |= s_from[first + j] == own;
-      FxKvForkRow row;
-      row.from = granted ? parent : -1;
-      row.last = last;
-      row.tokens = tokens;
-      row.held = held;
-      row.alive = alive ? 1 : 0;
-      row.reused = spare && spares_before < needs ? 1 : 0;
-      row.unused[0] = row.unused[1] = 0;
-      a.rows[r] = row;
+      for (int j = 0; j < K; ++j) alive |= s.from[first + j] == own;
+      const bool reused = spare && spares_before < needs;
+      if constexpr (HERE) {
+        s.tail[tid] = last;
+        s.len[tid] = held;   // (own == 0: `before` has been read)
+        s.want[tid] = tokens;
+        s.flags[tid] = (alive ? 1 : 0) | (reused ? 2 : 0);
+      } else {
+        a.rows[r] = FxKvForkRow{granted ? parent : -1, last, tokens, held, alive ? 1 : 0, reused ? 1 : 0, {0, 0}};
+      }
       a.out_lens[r] = granted ? tokens : 0;
       const bool copied = need && granted;
       a.copies[3 * (int64_t)r] = copied ? want : -1;
@@ -115,10 +123,95 @@ __global__ __launch_bounds__(kPlanThreads) void fx_kv_fork_plan(const FxKvForkAr
     }
     asked += all;
   }
-  if (tid == 0) {
-    *a.taken = (int)min(asked, (int64_t)a.n_free - from);
-    if (a.groups * a.blocks == 0) *a.n_freed = 0;   // (nothing else is launched)
+  if (tid == 0) *a.taken = (int)min(asked, (int64_t)a.n_free - from);
+}
+
+// One column of a group's rows, whose table begins at `table`: the new rows' pages.  Says which old rows' pages nobody has any more; pages: LDS of this thread alone, a row's `apart`.
+template <class Rows>
+__device__ __forceinline__ unsigned move_column(const FxKvForkArgs& a, const Rows& rows, int32_t* table, int c, int* pages, int apart) {
+  const int K = a.beams, page = 1 << a.log_page;
+  // what the group's rows have: pages up to the one in which their tokens end (-1 behind).  (Loops are without branches, so that their reads do not wait for each other.)
+  uint32_t alive = 0;
+#pragma unroll 4
+  for (int i = 0; i < K; ++i) {
+    const FxKvForkRow row = rows(i);
+    const bool has = c < (row.held + page - 1) >> a.log_page;
+    pages[i * apart] = has ? table[(int64_t)i * a.table_stride + c] : -1;
+    alive |= (row.alive != 0 ? 1u : 0u) << i;
   }
+#pragma unroll 4
+  for (int j = 0; j < K; ++j) {
+    const FxKvForkRow row = rows(j);
+    const int whole = row.tokens >> a.log_page, moved = pages[max(row.from, 0) * apart];
+    const bool ends = (c == whole) & ((row.tokens & (page - 1)) != 0);
+    if ((row.from >= 0) & (((c < whole) & (row.from != j)) | ends)) table[(int64_t)j * a.table_stride + c] = ends ? row.last : moved;
+  }
+  unsigned gone = 0;
+  for (int i = 0; i < K; ++i) {
+    if ((alive >> i & 1) != 0) continue;
+    const int p = pages[i * apart];
+    const FxKvForkRow row = rows(i);
+    if (p < 0 || (row.reused && c == row.held >> a.log_page)) continue;
+    const unsigned others = alive | ((1u << i) - 1);   // that keep it, or have said so (i is not among them)
+    bool kept = false;
+#pragma unroll 8
+    for (int o = 0; o < K; ++o) kept |= ((others >> o & 1) != 0) & (pages[o * apart] == p);
+    gone |= kept ? 0u : 1u << i;
+  }
+  return gone;
+}
+// the sum of a wave's values up to each lane's
+__device__ __forceinline__ int sum_up_to(int v, int lane) {
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int o = __shfl_up(v, (unsigned)d, 64);
+    v += lane >= d ? o : 0;
+  }
+  return v;
+}
+
+__global__ __launch_bounds__(kPlanThreads) void fx_kv_fork_plan(const FxKvForkArgs a) {
+  __shared__ Plan s;
+  plan_rows<false>(a, s);
+  if (threadIdx.x == 0 && a.groups * a.blocks == 0) *a.n_freed = 0;   // (nothing else is launched)
+}
+
+// All of it, for few rows and columns
+__global__ __launch_bounds__(kPlanThreads) void fx_kv_fork_small(const FxKvForkArgs a) {
+  extern __shared__ int s_pages[];   // [beams][kPlanThreads]
+  __shared__ Plan s;
+  __shared__ int s_upto[2][kPlanThreads / 64];
+  const int tid = (int)threadIdx.x, lane = tid & 63, wave = tid >> 6, K = a.beams;
+  plan_rows<true>(a, s);
+  __syncthreads();
+  int most = tid < a.groups * K ? s.len[tid] : 0;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) most = max(most, __shfl_xor(most, d, 64));
+  if (lane == 0) s_upto[0][wave] = most;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kPlanThreads / 64; ++w) most = max(most, s_upto[0][w]);
+  __syncthreads();
+  // (a column in which no row has a page stays as it is)
+  const int columns = (most + (1 << a.log_page) - 1) >> a.log_page, items = a.groups * columns;
+  int freed = 0;
+  for (int i0 = 0, turn = 0; i0 < items; i0 += kPlanThreads, turn ^= 1) {
+    const int i = i0 + tid, g = i / columns, c = i - g * columns;
+    unsigned gone = 0;
+    if (i < items) gone = move_column(a, [&](int j) { return s.row(g * K + j); }, a.table + (int64_t)g * K * a.table_stride, c, s_pages + tid, kPlanThreads);
+    const int mine = __builtin_popcount(gone), upto = sum_up_to(mine, lane);
+    if (lane == 63) s_upto[turn][wave] = upto;
+    __syncthreads();
+    int at = freed + upto - mine;
+#pragma unroll
+    for (int w = 0; w < kPlanThreads / 64; ++w) {
+      at += w < wave ? s_upto[turn][w] : 0;
+      freed += s_upto[turn][w];
+    }
+    for (; gone != 0; gone &= gone - 1) a.freed[at++] = s_pages[__builtin_ctz(gone) * kPlanThreads + tid];
+  }
+  for (int i = freed + tid; i < a.groups * K * a.columns; i += kPlanThreads) a.freed[i] = -1;
+  if (tid == 0) *a.n_freed = freed;
 }
 
 __global__ __launch_bounds__(kThreads) void fx_kv_fork_tables(const FxKvForkArgs a) {
@@ -126,54 +219,20 @@ __global__ __launch_bounds__(kThreads) void fx_kv_fork_tables(const FxKvForkArgs
   __shared__ FxKvForkRow s_row[FX_BEAM_MAX_BEAMS];
   __shared__ int s_sum[kThreads / 64];
   static_assert(FX_KV_FORK_COLUMNS == kThreads, "a column each");
-  const int tid = (int)threadIdx.x, lane = tid & 63, wave = tid >> 6, K = a.beams, page = 1 << a.log_page;
-  const int group = (int)(blockIdx.x / (unsigned)a.blocks), block = (int)(blockIdx.x % (unsigned)a.blocks), c = block * kThreads + tid;
-  int32_t* const table = a.table + (int64_t)group * K * a.table_stride;
+  const int tid = (int)threadIdx.x, lane = tid & 63, wave = tid >> 6, K = a.beams;
+  const int group = (int)(blockIdx.x / (unsigned)a.blocks), block = (int)(blockIdx.x % (unsigned)a.blocks);
   if (tid < K * (int)(sizeof(FxKvForkRow) / 4)) ((int*)s_row)[tid] = ((const int*)(a.rows + (int64_t)group * K))[tid];
   __syncthreads();
-  // (loops over rows are without branches, so that their reads do not wait for each other)
   int most = 0;
-  uint32_t alive = 0;
 #pragma unroll 4
-  for (int i = 0; i < K; ++i) {
-    most = max(most, s_row[i].held);
-    alive |= (s_row[i].alive != 0 ? 1u : 0u) << i;
-  }
+  for (int i = 0; i < K; ++i) most = max(most, s_row[i].held);
   if (((int64_t)block * kThreads << a.log_page) >= most) {   // (no row has a page here)
     if (tid == 0) a.counts[blockIdx.x] = 0;
     return;
   }
-  // what the group's rows have: pages up to the one in which their tokens end (-1 behind)
-  const auto has = [&](int i) { return c < (s_row[i].held >> a.log_page) + ((s_row[i].held & (page - 1)) != 0 ? 1 : 0); };
-#pragma unroll 4
-  for (int i = 0; i < K; ++i) s_pages[i * kThreads + tid] = has(i) ? table[(int64_t)i * a.table_stride + c] : -1;
-  // (a thread reads its own column alone, which it has written)
-#pragma unroll 4
-  for (int j = 0; j < K; ++j) {
-    const int from = s_row[j].from, last = s_row[j].last, tokens = s_row[j].tokens, whole = tokens >> a.log_page;
-    const int moved = s_pages[max(from, 0) * kThreads + tid];
-    const bool ends = (c == whole) & ((tokens & (page - 1)) != 0);
-    if ((from >= 0) & (((c < whole) & (from != j)) | ends)) table[(int64_t)j * a.table_stride + c] = ends ? last : moved;
-  }
-  unsigned gone = 0;
-  for (int i = 0; i < K; ++i) {
-    if ((alive >> i & 1) != 0) continue;
-    const int p = s_pages[i * kThreads + tid];
-    if (p < 0 || (s_row[i].reused && c == s_row[i].held >> a.log_page)) continue;
-    const unsigned others = alive | ((1u << i) - 1);   // that keep it, or have said so (i is not among them)
-    bool kept = false;
-#pragma unroll 8
-    for (int o = 0; o < K; ++o) kept |= ((others >> o & 1) != 0) & (s_pages[o * kThreads + tid] == p);
-    gone |= kept ? 0u : 1u << i;
-  }
+  unsigned gone = move_column(a, [&](int j) { return s_row[j]; }, a.table + (int64_t)group * K * a.table_stride, block * kThreads + tid, s_pages + tid, kThreads);
   // column by column
-  const int mine = __builtin_popcount(gone);
-  int upto = mine;
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const int o = __shfl_up(upto, (unsigned)d, 64);
-    if (lane >= d) upto += o;
-  }
+  const int mine = __builtin_popcount(gone), upto = sum_up_to(mine, lane);
   if (lane == 63) s_sum[wave] = upto;
   __syncthreads();
   int at = upto - mine, all = 0;
@@ -289,7 +348,13 @@ hipError_t fx_launch_kv_fork(const FxKvForkArgs& a, hipStream_t stream, int* lau
   FxKvForkArgs args = a;
   void* kargs[1] = {(void*)&args};
   *launched = 0;
-  hipError_t e = hipLaunchKernel((const void*)fx_kv_fork_plan, dim3(1), dim3(kPlanThreads), kargs, 0, stream);
+  hipError_t e;
+  if (a.beams <= kSmallBeams && a.groups <= kPlanThreads / a.beams && (int64_t)a.groups * a.beams * a.columns <= kSmall) {
+    e = hipLaunchKernel((const void*)fx_kv_fork_small, dim3(1), dim3(kPlanThreads), kargs, (size_t)a.beams * kPlanThreads * sizeof(int), stream);
+    *launched = e == hipSuccess ? 1 : 0;
+    return e;
+  }
+  e = hipLaunchKernel((const void*)fx_kv_fork_plan, dim3(1), dim3(kPlanThreads), kargs, 0, stream);
   if (e != hipSuccess) return e;
   const unsigned units = (unsigned)a.groups * (unsigned)a.blocks;
   *launched = 1;

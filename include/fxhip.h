@@ -661,7 +661,8 @@ int fx_kv_attention(const fx_kv_cache* cache, const fx_kv_attention_desc* desc, 
  * they are moved with the others, and neither copied nor freed.
  * The table is changed in place (rows table_stride apart, entries behind a row's tokens left as they were).  All arrays are int32 on the device: parents, lens, out_lens
  * [groups * beams], copies [groups * beams][3], freed [groups * beams * columns].  beams: 1 to 32.
- * workspace: fx_kv_fork_workspace_bytes() of device memory for each call under way, 16-byte aligned; nothing is expected in it.  Three launches. */
+ * workspace: fx_kv_fork_workspace_bytes() of device memory for each call under way, 16-byte aligned; nothing is expected in it.  One launch for few
+ * rows and columns, three otherwise. */
 typedef struct fx_kv_fork_desc {
   const int32_t* parents;
   const int32_t* lens;

@@ -171,7 +171,8 @@ def test_the_c_abi_refuses_before_it_launches():
 # ---- GPU: fork ----
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("G,K,P,M", [(1, 1, 16, 1), (1, 4, 16, 5), (3, 2, 32, 9), (32, 4, 64, 33), (70, 8, 16, 40), (5, 32, 128, 7), (2, 3, 16, 700), (300, 7, 256, 3), (1100, 1, 16, 4)])
+@pytest.mark.parametrize("G,K,P,M", [(1, 1, 16, 1), (1, 4, 16, 5), (3, 2, 32, 9), (32, 4, 64, 33), (70, 8, 16, 40), (5, 32, 128, 7), (2, 3, 16, 700), (300, 7, 256, 3), (1100, 1, 16, 4),
+                                     (128, 8, 16, 6), (146, 7, 32, 6), (1, 8, 16, 768), (5, 3, 16, 409), (1, 8, 16, 4097), (1024, 1, 64, 4)])
 @pytest.mark.parametrize("first", [False, True])
 def test_fork(G, K, P, M, first):
     rng = random.Random(G + 100 * K + M)
@@ -341,7 +342,9 @@ def test_launches():
         return total.value - before
 
     c = filled(3, 1, 16, 16, E4M3, 1)
-    assert launches(lambda: c.fork(i32([[0, 1]]), i32([3, 3]), i32([[0, 1], [2, 3]]), i32([5]))) == 3
+    assert launches(lambda: c.fork(i32([[0, 1]]), i32([3, 3]), i32([[0, 1], [2, 3]]), i32([5]))) == 1
+    for G, K, M, n in ((128, 8, 6, 1), (128, 8, 7, 3), (129, 8, 3, 3), (1, 9, 2, 3), (1, 8, 768, 1), (1, 8, 769, 3), (341, 3, 6, 1), (342, 3, 2, 3), (1024, 1, 6, 1), (1024, 1, 7, 3)):
+        assert launches(lambda: c.fork(torch.zeros(G, K, dtype=torch.int32, device="cuda"), i32([3] * (G * K)), i32([[0] * M] * (G * K)), i32([5]))) == n, (G, K, M)
     assert launches(lambda: c.fork(i32([]).view(0, 2), i32([]), i32([]).view(0, 3), i32([5]))) == 1
     assert launches(lambda: copy_pages([c] * 5, i32([[0, 1, 3]]))) == 1 and launches(lambda: copy_pages([c] * 33, i32([[0, 1, 3]]))) == 2 and launches(lambda: copy_pages([], i32([[0, 1, 3]]))) == 0
 
