@@ -8,9 +8,12 @@
 // What is compared within a row are its logits; between rows score + (logit - lse) in 64 bits.  Sums of exponentials: eight at a time in fp32, these in
 // 64 bits, so that lse is off by some 1e-8 and rows change places only where they are as near as that.
 //
-// The best `count` words: a bound is halved until at least `count` of 256 groups of segments, and hardly more, have a word at or above it; the words at or above it are a
-// few more than `count`, and are ranked by counting.  Equal numbers: lower words go first, and so as many as there may be of them never need more than a list's
-// 256 places (it is cut to the best `count` when it fills up).
+// The best `count` words: a bound is searched for, a quarter of what is left at a time, until at least `count` of 256 groups of segments, and hardly more, have a word at or
+// above it; the words at or above it are a few more than `count`, and are ranked by counting.  Equal numbers: lower words go first, and so as many as there may be of them
+// never need more than a list's places (it is cut to the best `count` when it fills up).
+//
+// 488 rows of 128 001 words, bf16, 390 of them alive: 24.4 us (4.1 TB/s; to read them and do nothing but the sum takes 18) and 10.4; 64 of 50 001: 4.8 and 8.5;
+// 4 of 32 000, fp32: 3.3 and 6.7.
 #include <algorithm>
 
 #include "fx_beam.h"

@@ -137,8 +137,8 @@ __device__ __forceinline__ int64_t lane_of(int64_t v, int lane) {   // in scalar
 // TURN: keys turn by their tokens' positions ahead of all else, and are fp32 from then on.  A lane has 8 pairs of a row (16 of its columns, or 16
 // that do not turn), forms their angles by itself and keeps the turned numbers of two iterations; where the units of a row do not fit, the last one
 // begins earlier and does some columns again.  INTER: pairs are neighbours.  Angles are formed for each head anew: 2 us of the chip's vector units for
-// 10 565 tokens, 8 heads and 32 pairs, of 69.  Slower, with queries, keys and values of that call: 8 columns a lane, angles shared by a wave in LDS and
-// numbers in registers 82 us, numbers in LDS as well 88; four waves a SIMD instead of three (registers go through memory) 76.
+// 10 565 tokens, 8 heads and 32 pairs, of 59 (fx_kv_append with its queries).  Slower there: 8 columns a lane, angles shared by a wave in LDS and
+// numbers in registers 82 us, numbers in LDS as well 88; 16 columns a lane as numbers of 16 bits, each in a register of its own, three waves a SIMD 69, four 76.
 template <int HELD, class T, bool VALUES, bool TURN = false, bool INTER = false>
 struct StoreRun {
   static_assert(!(VALUES && TURN), "values do not turn");
