@@ -4,7 +4,7 @@
 // A key is turned in fp32 and rounded once, to its code.  The first workgroups of the launch store (fx_kv_store.h), the others turn queries
 // (fx_rotary_device.h): the long runs begin first.  (Queries first: 65 us instead of 59; in turn: 57, but a step of single tokens 8.2 instead of 7.5.)
 // Bound: HBM; single tokens: latency.  Four waves a SIMD without registers in memory, which the numbers' whole words and frequencies in LDS allow: three took 69 us.
-// 10 565 tokens of 5 prompts, 32 query heads on 8 of 128 columns, fp16 to int8: 58.6 us, 4.1 TB/s; 64 single tokens, bf16 to e4m3: 7.5.
+// 10 565 tokens of 5 prompts, 32 query heads on 8 of 128 columns, fp16 to int8: 58 us, 4.1 TB/s; 64 single tokens, bf16 to e4m3: 7.4.
 #include "fx_kv_store.h"
 
 namespace {

@@ -1,9 +1,9 @@
 // Rotary positions, forward and backward (fx_rotary_device.h has the mathematics).
 //
 // Bound: HBM (each number is read and written once) from a few thousand rows on, latency below.  A workgroup takes some tokens with all their heads, so that an
-// angle is formed once, in LDS, while the first of its four units a thread are under way; what is left of the address arithmetic is multiplications.
-// 3 x 1 999 tokens of 40 heads of 128 columns, bf16, either way: 26.5 us, 4.6 TB/s (a large copy: 5.4); 30 001 of 24 heads of 64, fp16, half of their columns turning in
-// neighbouring pairs: 40 us, 4.6 TB/s; 61 single tokens: 4 us.
+// angle is formed once, in LDS, while the first of its four units a thread, two at a time, are under way; what is left of the address arithmetic is multiplications.
+// 3 x 1 999 tokens of 40 heads of 128 columns, bf16, either way: 25.6 us, 4.8 TB/s (a large copy: 5.4); 30 001 of 24 heads of 64, fp16, half of their columns turning in
+// neighbouring pairs: 35 us, 5.3 TB/s; 61 single tokens: 3.5 us.
 #include <algorithm>
 
 #include "fx_rotary_device.h"
@@ -29,7 +29,8 @@ void fx_rotary_shape(FxRotary& a) {
   a.turning = (a.turns.pairs + pv - 1) / pv;
   a.units = a.turning + (rest >= 2 * pv ? (rest + 2 * pv - 1) / (2 * pv) : rest > 0 ? 1 : 0);
   const int64_t row = (int64_t)a.units * a.heads, total = (int64_t)a.batch * a.tokens;
-  // four units a thread, and not fewer than two workgroups a CU where there are as many tokens
+  // two times two units a thread (two at once: 86 registers and 23 us become 68 and 21 for 3 x 1 999 tokens of 40 heads of 128, bf16; once, or four times: 22), and not
+  // fewer than two workgroups a CU where there are as many tokens
   int64_t per = std::min<int64_t>(std::max<int64_t>(1024 / row, 1), FX_ROTARY_ANGLES / a.turns.pairs);
   per = std::max<int64_t>(std::min(per, total / 512), 1);
   a.per = (int32_t)per;

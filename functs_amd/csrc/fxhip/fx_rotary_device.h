@@ -43,12 +43,26 @@ __device__ __forceinline__ void turn_pair(float& a, float& b, const Turn& w) {
 
 __device__ __forceinline__ unsigned divided(unsigned n, unsigned d, unsigned magic) { return magic ? __umulhi(n, magic) : n / d; }
 
-// N numbers from any address (rows of odd sizes begin anywhere)
+// N numbers from any address (rows of odd sizes begin anywhere), in whole words: halves would take a register each
 template <class T, int N>
 struct Some {
-  T e[N];
-  __device__ __forceinline__ void load(const T* p) { __builtin_memcpy(e, p, sizeof e); }
-  __device__ __forceinline__ void store(T* p) const { __builtin_memcpy(p, e, sizeof e); }
+  unsigned u[N * sizeof(T) / 4];
+  __device__ __forceinline__ void load(const T* p) { __builtin_memcpy(u, p, sizeof u); }
+  __device__ __forceinline__ void store(T* p) const { __builtin_memcpy(p, u, sizeof u); }
+  __device__ __forceinline__ float at(int i) const {
+    if constexpr (sizeof(T) == 4) return __uint_as_float(u[i]);
+    else return (float)__builtin_bit_cast(T, (unsigned short)(i % 2 ? u[i / 2] >> 16 : u[i / 2]));
+  }
+  __device__ __forceinline__ void set(int i, float a, float b) {   // numbers i and i + 1, i even
+    if constexpr (sizeof(T) == 4) u[i] = __float_as_uint(a), u[i + 1] = __float_as_uint(b);
+    else u[i / 2] = __builtin_bit_cast(unsigned short, (T)a) | (unsigned)__builtin_bit_cast(unsigned short, (T)b) << 16;
+  }
+};
+template <class T>
+struct Some<T, 1> {
+  T e;
+  __device__ __forceinline__ void load(const T* p) { e = *p; }
+  __device__ __forceinline__ void store(T* p) const { *p = e; }
 };
 
 // A workgroup's share of the rows.  A unit is PV pairs of a head, or 2 PV of the columns that do not turn: two loads and two stores of
@@ -56,18 +70,18 @@ struct Some {
 // again.  Angles are computed once for all heads and kept in LDS, behind the first loads.
 template <class T, int PV, bool INTER>
 __device__ __forceinline__ void rotary_rows(const FxRotary& a, int block, int slice, Turn* s_turn) {
-  constexpr int kThreadsHere = 256, kUnits = 4;
+  constexpr int kThreadsHere = 256, kUnits = 2;
   const int tid = (int)threadIdx.x, pairs = a.turns.pairs, rest = a.depth - 2 * pairs, total = a.batch * a.tokens;
   const int g0 = block * a.per, n = min(a.per, total - g0), row = a.units * a.heads, all = n * row;
   T* const y = (T*)a.y;
   bool first = true;
-  for (int base = slice * kThreadsHere * kUnits; base < all; base += a.slices * kThreadsHere * kUnits) {
+  for (int base = slice * kThreadsHere; base < all; base += a.slices * kThreadsHere * kUnits) {
     Some<T, PV> lo[kUnits], hi[kUnits];
     int64_t to[kUnits];              // the head's place in y
     int at[kUnits], angle[kUnits];   // at: first pair or column; angle: place of the first pair's, -1: columns that do not turn, -2: few of them, -3: nothing
 #pragma unroll
     for (int k = 0; k < kUnits; ++k) {
-      const int i = base + k * kThreadsHere + tid;
+      const int i = base + k * a.slices * kThreadsHere + tid;
       angle[k] = -3;
       if (i >= all) continue;
       const int j = (int)divided((unsigned)i, (unsigned)row, a.magic_token), in_row = i - j * row;
@@ -104,14 +118,26 @@ __device__ __forceinline__ void rotary_rows(const FxRotary& a, int block, int sl
     for (int k = 0; k < kUnits; ++k) {
       if (angle[k] < -1) continue;
       if (angle[k] >= 0) {
+        const Turn* const w = s_turn + angle[k];
+        if constexpr (PV == 1) {
+          float u = (float)lo[k].e, v = (float)hi[k].e;
+          turn_pair(u, v, w[0]);
+          lo[k].e = (T)u;
+          hi[k].e = (T)v;
+        } else {
 #pragma unroll
-        for (int i = 0; i < PV; ++i) {
-          T& ra = INTER ? (2 * i < PV ? lo[k].e[2 * i % PV] : hi[k].e[2 * i % PV]) : lo[k].e[i];
-          T& rb = INTER ? (2 * i + 1 < PV ? lo[k].e[(2 * i + 1) % PV] : hi[k].e[(2 * i + 1) % PV]) : hi[k].e[i];
-          float u = (float)ra, v = (float)rb;
-          turn_pair(u, v, s_turn[angle[k] + i]);
-          ra = (T)u;
-          rb = (T)v;
+          for (int i = 0; i < PV; i += 2) {
+            float a0 = lo[k].at(i), a1 = lo[k].at(i + 1), b0 = hi[k].at(i), b1 = hi[k].at(i + 1);
+            if constexpr (INTER) {
+              turn_pair(a0, a1, w[i / 2]);
+              turn_pair(b0, b1, w[(PV + i) / 2]);
+            } else {
+              turn_pair(a0, b0, w[i]);
+              turn_pair(a1, b1, w[i + 1]);
+            }
+            lo[k].set(i, a0, a1);
+            hi[k].set(i, b0, b1);
+          }
         }
         lo[k].store(y + to[k] + (INTER ? 2 * at[k] : at[k]));
         hi[k].store(y + to[k] + (INTER ? 2 * at[k] + PV : at[k] + pairs));
