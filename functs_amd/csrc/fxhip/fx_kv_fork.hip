@@ -279,7 +279,7 @@ __global__ __launch_bounds__(kThreads) void fx_kv_fork_pack(const FxKvForkArgs a
 // Bound: HBM, each code read and written once.  A unit is some heads of one page's keys or values in one layer: up to 16 KiB, whose filled part is
 // copied 16 bytes a lane.  Every workgroup lists the rows that copy (most have none) and takes units in turn.
 // 56 copies of 8 partly filled pages in 24 layers (8 heads of 128, 64 tokens): 32 us for 95 MB written, which the stores' way is full with (2 048 to 16 384 workgroups: 32 to
-// 34); 41 of pages of 16 tokens in 12 layers: 5.3 us, a chain of launch, list, loads.
+// 34); a step's, of 16 x 4 beams, pages of 16 tokens in 12 layers: 5.3 us, a chain of launch, list, loads.
 constexpr int kRows = 1024;   // looked at together
 typedef unsigned fx_words __attribute__((ext_vector_type(4)));
 
