@@ -344,9 +344,9 @@ __global__ __launch_bounds__(64 * kJoinWaves) void fx_beam_join(const FxBeamArgs
           }
           in_wave();
           // The words of the listed segments, 32 lanes a segment, six loads under way.  Of the loads those that have a word above the bound go to LDS, 64 at most,
-          // and from there each of their words to a lane.  If they are many (of rows with few segments, or equal words), the bound is raised once, by the largest
-          // words of 256 groups of the loads (15 beams of 247 words, 15 wanted: 17.6 us, and 21 without); if that leaves more than 64, all loads take that way, four
-          // segments at a time.
+          // and from there each of their words to a lane.  If they have more than 256 words (of rows with few segments, or equal words), the bound is raised
+          // once, by the largest words of 256 groups of the loads; if that leaves more than 64 loads, all take that way, four segments at a time.  (101 x 11 rows of
+          // 579 words, 22 wanted: 54 us without, 19 with it.)
           const auto place_of = [&](int i) {   // (of none: behind the last word, where nothing is the lane's)
             if (i >= listed) return a.words;
             const int s = list[i], part = s / FX_BEAM_SEGMENTS, first = s % FX_BEAM_SEGMENTS / 4 * kPer + ((lane >> 4) & (kPer - 1));   // the load of the part
@@ -394,7 +394,7 @@ __global__ __launch_bounds__(64 * kJoinWaves) void fx_beam_join(const FxBeamArgs
               }
             }
             if (listed == 0) found = 0;
-            if (found <= min(64, count + 12) || time == 1) break;
+            if (found <= 256 / W::kVec || time == 1) break;
             group[0] = group[1] = group[2] = group[3] = -INFINITY;
 #pragma unroll 1
             for (int i0 = 0; i0 < listed; i0 += 16 / kPer) {
@@ -426,8 +426,45 @@ __global__ __launch_bounds__(64 * kJoinWaves) void fx_beam_join(const FxBeamArgs
               found = 64;
             }
             in_wave();
+            int i1 = 0;
+            if (found * W::kVec <= 256) {
+              // few words: four to a lane, and the bound is raised by themselves if many of them are above it (15 beams of 247 words, 15 wanted: 14.4 us, by their
+              // loads 17.6, not at all 21)
+              uint32_t here[4];
+#pragma unroll
+              for (int g = 0; g < 4; ++g) {
+                const int i = (lane + 64 * g) / W::kVec, e = lane % W::kVec;
+                group[g] = -INFINITY;
+                here[g] = 0;
+                if (i >= found) continue;
+                const int place = places[i], at = tiny ? 0 : w.at(place);
+                const float z = (float)((const T*)loads)[i * W::kVec + e];
+                here[g] = (uint32_t)(at + e);
+                if (at + e >= place && place < a.words && (z > bound || (z == bound && here[g] <= last))) group[g] = z;
+              }
+              int hits = above(kLowest);
+              if (hits > count + 24) {
+                const float raised = raise(bound, top, count + 2);
+                if (raised > bound) {
+                  bound = raised;
+                  last = 0xffffffffu;
+#pragma unroll
+                  for (int g = 0; g < 4; ++g) group[g] = group[g] >= bound ? group[g] : -INFINITY;
+                  hits = above(bound);
+                }
+              }
+              if (n + hits <= room) {
+                i1 = found;   // (no others: the list is ranked)
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                  const uint64_t lanes = __ballot(group[g] >= kLowest);
+                  if (group[g] >= kLowest) keys[n + below(lanes)] = key_of(group[g], here[g]);
+                  n += __builtin_popcountll(lanes);
+                }
+              }
+            }
 #pragma unroll 1
-            for (int i1 = 0; i1 < found + 64 / W::kVec; i1 += 64 / W::kVec) {   // (and once more, for what is left in the list)
+            for (; i1 < found + 64 / W::kVec; i1 += 64 / W::kVec) {   // (and once more, for what is left in the list)
               if (n > room - 64 || i1 >= found) {
                 // no room for a word of each lane, or the end: the best `count`, in order; what comes has to be better than the last of them
                 uint64_t mine[kList / 64];
