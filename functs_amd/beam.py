@@ -3,7 +3,7 @@
     chosen = beam.select(logits, scores, ended=ended, end_word=eos)      # logits [requests, beams, words], scores [requests, beams]
     chosen.scores, chosen.beams, chosen.words                            # [requests, count], the best first
 
-Log-probabilities, sums with the beams' scores and the selection in two launches that read the logits once.  KvCache.fork moves the pages of a
+Log-probabilities, sums with the beams' scores and the selection in one or two launches that read the logits once.  KvCache.fork moves the pages of a
 cache to the beams that go on.  The selection is a TorchScript operator as well, torch.ops.functs.beam_select.  GPU tensors only, and no backward pass.
 """
 from typing import NamedTuple, Optional

@@ -1,6 +1,6 @@
 // A beam search's selection: of each request the `count` best continuations of all its beams and words, by score + logit - log sum exp(logits).
 //
-// Two launches.  fx_beam_scan reads the logits once; a wave leaves the sum of exponentials of its 2 048 (16-bit types) or 1 024 words and the largest of each
+// Two launches, or fx_beam_join alone for rows of one part.  fx_beam_scan reads the logits once; a wave leaves the sum of exponentials of its 2 048 (16-bit types) or 1 024 words and the largest of each
 // eighth of them.  fx_beam_join, a workgroup a request and a wave a row, finds from these which few segments the best words can lie in, reads those again (from the caches, as a
 // rule) and takes their best; then it ranks the rows' candidates.  (The best words of every part found by fx_beam_scan itself: 31 us for 488 rows of 128 001 words,
 // half of them instructions of that search.)
@@ -168,15 +168,10 @@ __device__ __forceinline__ int segment_max(int m) {
   return m;
 }
 
-// Bound: HBM.  A wave a part; nothing is shared between waves.
+// A wave's part of a row: its sum, and the largest word of each segment
 template <class T>
-__global__ __launch_bounds__(kThreads, 8) void fx_beam_scan(const FxBeamArgs a) {
+__device__ __forceinline__ void scan_part(const FxBeamArgs& a, int row, int part, int unit, int lane) {
   typedef Words<T> W;
-  const int lane = (int)threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-  const int unit = (int)blockIdx.x * kWaves + wave, row = unit / a.parts_a_row, part = unit - row * a.parts_a_row;
-  if (row >= a.requests * a.beams) return;
-  // (beams with no continuations of their own are not read)
-  if ((a.ended && a.ended[row]) || !(a.scores[row] > -INFINITY)) return;
   const W w = words_of<T>(a, row);
   const int begin = part * W::kPart + lane * W::kVec;   // load l: words begin + l * 64 * kVec on
   Load<T> v[kLoads];
@@ -244,9 +239,21 @@ __global__ __launch_bounds__(kThreads, 8) void fx_beam_scan(const FxBeamArgs a) 
   }
 }
 
+// Bound: HBM.  A wave a part; nothing is shared between waves.
+template <class T>
+__global__ __launch_bounds__(kThreads, 8) void fx_beam_scan(const FxBeamArgs a) {
+  const int lane = (int)threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int unit = (int)blockIdx.x * kWaves + wave, row = unit / a.parts_a_row;
+  if (row >= a.requests * a.beams) return;
+  // (beams with no continuations of their own are not read)
+  if ((a.ended && a.ended[row]) || !(a.scores[row] > -INFINITY)) return;
+  scan_part<T>(a, row, unit - row * a.parts_a_row, unit, lane);
+}
+
 // Bound: latency.  A row is a chain of some ten steps, and the code of each arrives for the first time: loops are not unrolled where they need not be (16 segments' loads in
 // registers, 28 KB of code, took 2 us more than this).
-template <class T>
+// ALONE: rows of one part, for which there was no fx_beam_scan (6 x 2 rows of 109 words: 8.2 us a call, 13.1 in two launches).
+template <class T, bool ALONE>
 __global__ __launch_bounds__(64 * kJoinWaves) void fx_beam_join(const FxBeamArgs a) {
   typedef Words<T> W;
   extern __shared__ uint4 s_join[];
@@ -265,6 +272,11 @@ __global__ __launch_bounds__(64 * kJoinWaves) void fx_beam_join(const FxBeamArgs
     // (all loads at once: what beams with no candidates of their own have there is never looked at)
     const float before = a.scores[row];
     const bool over = a.ended && a.ended[row];
+    if constexpr (ALONE) {
+      if (!over && before > -INFINITY) scan_part<T>(a, (int)row, 0, (int)row, lane);
+      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");
+      __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup");
+    }
     const int4* tops = (const int4*)a.tops + row * fours;
     const FxBeamPart* parts = a.parts + row * a.parts_a_row;
     const FxBeamPart none{-INFINITY, 0.0f, 0.0};
@@ -603,19 +615,22 @@ void fx_beam_shape(FxBeamArgs& a) {
 
 hipError_t fx_launch_beam_select(const FxBeamArgs& a, hipStream_t stream, int* launched) {
   static const void* const scans[3] = {(const void*)fx_beam_scan<float>, (const void*)fx_beam_scan<_Float16>, (const void*)fx_beam_scan<__bf16>};
-  static const void* const joins[3] = {(const void*)fx_beam_join<float>, (const void*)fx_beam_join<_Float16>, (const void*)fx_beam_join<__bf16>};
+  static const void* const joins[2][3] = {{(const void*)fx_beam_join<float, false>, (const void*)fx_beam_join<_Float16, false>, (const void*)fx_beam_join<__bf16, false>},
+                                          {(const void*)fx_beam_join<float, true>, (const void*)fx_beam_join<_Float16, true>, (const void*)fx_beam_join<__bf16, true>}};
   const int type = a.dtype == FX_DT_F32 ? 0 : a.dtype == FX_DT_F16 ? 1 : 2;
   FxBeamArgs args = a;
   void* kargs[1] = {(void*)&args};
   const int64_t units = (int64_t)a.requests * a.beams * a.parts_a_row;
   *launched = 0;
-  const hipError_t e = hipLaunchKernel(scans[type], dim3((unsigned)((units + kWaves - 1) / kWaves)), dim3(kThreads), kargs, 0, stream);
-  if (e != hipSuccess) return e;
-  *launched = 1;
+  if (a.parts_a_row > 1) {
+    const hipError_t e = hipLaunchKernel(scans[type], dim3((unsigned)((units + kWaves - 1) / kWaves)), dim3(kThreads), kargs, 0, stream);
+    if (e != hipSuccess) return e;
+    *launched = 1;
+  }
   // (64 KiB of LDS a workgroup: 32 beams of 64 candidates go in three rounds of eleven)
   const int room = 65536 - a.beams * a.count * 12, a_wave = 64 * 20 + (a.count + kMore) * 8 + kSegments * 2;
   const int rounds = (a.beams + std::min(kJoinWaves, room / a_wave) - 1) / std::min(kJoinWaves, room / a_wave), waves = (a.beams + rounds - 1) / rounds;
-  const hipError_t f = hipLaunchKernel(joins[type], dim3((unsigned)a.requests), dim3((unsigned)waves * 64), kargs, (size_t)(a.beams * a.count * 12 + waves * a_wave), stream);
-  if (f == hipSuccess) *launched = 2;
+  const hipError_t f = hipLaunchKernel(joins[a.parts_a_row > 1 ? 0 : 1][type], dim3((unsigned)a.requests), dim3((unsigned)waves * 64), kargs, (size_t)(a.beams * a.count * 12 + waves * a_wave), stream);
+  if (f == hipSuccess) ++*launched;
   return f;
 }

@@ -697,7 +697,8 @@ int fx_kv_copy(const fx_kv_cache* caches, int n_caches, const int32_t* copies, i
  * with the beam's score, whatever its logits are, which are not read.  Where there are fewer than `count`, the places behind have -infinity, beam -1 and word -1.
  * logits [requests][beams][words], a beam's words side by side, strides in elements, any alignment of its numbers; scores and ended [requests][beams], out_* [requests][count]
  * contiguous.  beams: 1 to 32, count: 1 to 64, words: 1 to 2^18.
- * workspace: fx_beam_select_workspace_bytes() of device memory for each call under way, 16-byte aligned; nothing is expected in it.  Two launches. */
+ * workspace: fx_beam_select_workspace_bytes() of device memory for each call under way, 16-byte aligned; nothing is expected in it.  Two launches,
+ * of rows of up to 4 KiB one. */
 #define FX_BEAM_MAX_BEAMS 32
 #define FX_BEAM_MAX_COUNT 64
 #define FX_BEAM_MAX_WORDS 262144

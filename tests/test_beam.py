@@ -304,14 +304,17 @@ def test_rows_beyond_two_to_the_31_numbers():
 
 
 @pytest.mark.gpu
-def test_two_launches():
+@pytest.mark.parametrize("dtype", TYPES)
+def test_two_launches(dtype):
     total, special = ctypes.c_uint64(), ctypes.c_uint64()
-    x, s = logits_of(2, 3, 10, 1)
-    lib.fx_launch_stats(ctypes.byref(total), ctypes.byref(special))
-    before = total.value
-    beam.select(x, s)
-    lib.fx_launch_stats(ctypes.byref(total), ctypes.byref(special))
-    assert total.value == before + 2
+    part = 1024 if dtype == torch.float32 else 2048
+    for V, n in ((10, 1), (part, 1), (part + 1, 2)):
+        x, s = logits_of(2, 3, V, 1, dtype)
+        lib.fx_launch_stats(ctypes.byref(total), ctypes.byref(special))
+        before = total.value
+        beam.select(x, s)
+        lib.fx_launch_stats(ctypes.byref(total), ctypes.byref(special))
+        assert total.value == before + n
 
 
 @pytest.mark.gpu
