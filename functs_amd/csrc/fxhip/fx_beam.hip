@@ -12,8 +12,8 @@
 // above it; the words at or above it are a few more than `count`, and are ranked by counting.  Equal numbers: lower words go first, and so as many as there may be of them
 // never need more than a list's places (it is cut to the best `count` when it fills up).
 //
-// 488 rows of 128 001 words, bf16, 390 of them alive: 24.4 us (4.1 TB/s; to read them and do nothing but the sum takes 18) and 10.4; 64 of 50 001: 4.8 and 8.5;
-// 4 of 32 000, fp32: 3.3 and 6.7.
+// 488 rows of 128 001 words, bf16, 390 of them alive: 24.1 us (4.1 TB/s; to read them and do nothing but the sum takes 18) and 10.6; 64 of 50 001: 4.5 and 8.6;
+// 4 of 32 000, fp32: 3.2 and 6.9.
 #include <algorithm>
 
 #include "fx_beam.h"

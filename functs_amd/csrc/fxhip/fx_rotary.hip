@@ -2,7 +2,7 @@
 //
 // Bound: HBM (each number is read and written once) from a few thousand rows on, latency below.  A workgroup takes some tokens with all their heads, so that an
 // angle is formed once, in LDS, while the first of its four units a thread, two at a time, are under way; what is left of the address arithmetic is multiplications.
-// 3 x 1 999 tokens of 40 heads of 128 columns, bf16, either way: 25.6 us, 4.8 TB/s (a large copy: 5.4); 30 001 of 24 heads of 64, fp16, half of their columns turning in
+// 3 x 1 999 tokens of 40 heads of 128 columns, bf16, either way: 26 us, 4.7 TB/s (a large copy: 5.4); 30 001 of 24 heads of 64, fp16, half of their columns turning in
 // neighbouring pairs: 35 us, 5.3 TB/s; 61 single tokens: 3.5 us.
 #include <algorithm>
 
