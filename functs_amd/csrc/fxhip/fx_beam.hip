@@ -104,22 +104,19 @@ template <> struct Load<__bf16> {
   unsigned u[4];
   __device__ __forceinline__ float operator[](int e) const { return __uint_as_float(e % 2 ? u[e / 2] & 0xffff0000u : u[e / 2] << 16); }
 };
-// Terms 2^(x c - r), r the whole number next to the largest x c: product and difference are rounded once.  c is log2 e (1 + 1.3e-8), for which the sum's
-// logarithm is put right.  Numbers whose x c may be infinite: by their difference to the largest.
+// A part's sum is of terms 2^(x c - r), r the whole number next to the largest x c: product and difference are rounded once.  c is log2 e (1 + 1.3e-8), which is 1e-8 in the terms
+// that count.  From 2^22 on fp32 has no whole number so near (a product rounded to 2^31 or more is 128 and more from itself): such parts' terms are 2^((x - largest) c), a
+// difference that is exact wherever the term is not 0, and their sum is brought to r, in 64 bits, behind.
 constexpr float kC = 1.44269504088896340736f;
-__device__ __forceinline__ bool far_from(float top) { return __builtin_fabsf(top) > 1e30f; }
-__device__ __forceinline__ float whole_of(float top) { return __builtin_rintf(top * kC); }
-// 2^(reference of a - that of b), a no more than b: exact between whole ones, and of far ones, which are the same or 2^70 apart at least, 1 or 0
-__device__ __forceinline__ double between(float a, float b) {
-  if (far_from(a) || far_from(b)) return a == b ? 1.0 : 0.0;
-  return __builtin_amdgcn_ldexp(1.0, (int)fmaxf(whole_of(a) - whole_of(b), -4000.0f));
+__device__ __forceinline__ bool far_from(float top) { return __builtin_fabsf(top) > 0x1p22f; }
+__device__ __forceinline__ double scaled(float top) { return (double)top * (double)kC; }   // (48 bits: exact)
+__device__ __forceinline__ double whole_of(float top) { return __builtin_rint(scaled(top)); }
+// a part's sum under `whole`, the r of the row's largest logit (of no words: 0, or NaN)
+__device__ __forceinline__ double part_of(const FxBeamPart& p, double whole) {
+  return p.top > -INFINITY ? p.sum * __builtin_amdgcn_ldexp(1.0, (int)fmax(whole_of(p.top) - whole, -4000.0)) : p.sum;
 }
-// a part's sum under the reference of `most`, the row's largest logit
-__device__ __forceinline__ double part_of(const FxBeamPart& p, float most) { return p.top > -INFINITY ? p.sum * between(p.top, most) : p.sum; }   // (of no words: 0, or NaN)
-__device__ __forceinline__ double lse_of(float most, double sum) {
-  const double r = far_from(most) ? (double)most * (double)kC : (double)whole_of(most);
-  return r * 0.69314718055994530942 + log(sum) - ((double)kC / 1.44269504088896340736 - 1.0) * (double)most;
-}
+// (the largest logit and what the others add to it: rounded at the logit's own size once, whatever that is)
+__device__ __forceinline__ double lse_of(float most, double whole, double sum) { return (double)most + (log(sum) + (whole - scaled(most)) * 0.69314718055994530942); }
 
 // Words of a row: load l of a part, in its lane.  Loads that would begin in a row's last words lie at its end (at), less the first ones, which are other lanes'
 template <class T>
@@ -212,7 +209,7 @@ __device__ __forceinline__ void scan_part(const FxBeamArgs& a, int row, int part
   }
   const float most = unordered(max(max(__builtin_amdgcn_readlane(all, 15), __builtin_amdgcn_readlane(all, 31)), max(__builtin_amdgcn_readlane(all, 47), __builtin_amdgcn_readlane(all, 63))));
   const bool far = far_from(most);
-  const float r = most > -INFINITY ? whole_of(most) : 0.0f;
+  const float r = most > -INFINITY ? (float)whole_of(most) : 0.0f;
   double sum = 0.0;
   if (!far) {
 #pragma unroll
@@ -233,6 +230,7 @@ __device__ __forceinline__ void scan_part(const FxBeamArgs& a, int row, int part
     }
   }
   sum = wave_sum(sum);
+  if (far && most > -INFINITY) sum *= (double)__builtin_amdgcn_exp2f((float)(scaled(most) - whole_of(most)));
   if (lane == 0) {
     a.parts[unit].top = most;
     a.parts[unit].sum = sum;
@@ -384,10 +382,11 @@ __global__ __launch_bounds__(64 * kJoinWaves) void fx_beam_join(const FxBeamArgs
                 v[u] = load(place[u]);
               }
               if (lse == 0.0) {   // (the first time, while they are under way)
-                double sum = part_of(first, top);
+                const double whole = whole_of(top);
+                double sum = part_of(first, whole);
 #pragma unroll 1
-                for (int i = lane + 64; i < a.parts_a_row; i += 64) sum += part_of(parts[i], top);
-                lse = lse_of(top, wave_sum(sum));
+                for (int i = lane + 64; i < a.parts_a_row; i += 64) sum += part_of(parts[i], whole);
+                lse = lse_of(top, whole, wave_sum(sum));
                 if (!(lse - lse == 0.0)) listed = 0, seen = fours;   // (a row with NaN or +infinity has no candidates)
               }
 #pragma unroll

@@ -691,8 +691,8 @@ int fx_kv_copy(const fx_kv_cache* caches, int n_caches, const int32_t* copies, i
 /* ---- a beam search's selection ----
  * Of each request the `count` best continuations of all its beams: candidate (beam k, word w) has the total
  *   scores[k] + (logits[k][w] - log sum_v exp(logits[k][v]))
- * formed in 64 bits (the sum's terms, exp(logit - largest), in fp32) and rounded to fp32 for out_scores.  Larger totals go first, equal ones by beam, within a
- * beam larger logits, then lower words.  No candidates have: words whose logit is -infinity (masked), rows of nothing else, rows that hold a NaN or +infinity,
+ * formed in 64 bits, of finite logits of any size (the sum's terms, relative to about the largest, in fp32), and rounded to fp32 for out_scores.  Larger totals go first,
+ * equal ones by beam, within a beam larger logits, then lower words.  No candidates have: words whose logit is -infinity (masked), rows of nothing else, rows that hold a NaN or +infinity,
  * beams whose score is -infinity or NaN (there is none yet, or none any more).  A beam that has ended (ended: one byte each, or null) has one candidate, end_word
  * with the beam's score, whatever its logits are, which are not read.  Where there are fewer than `count`, the places behind have -infinity, beam -1 and word -1.
  * logits [requests][beams][words], a beam's words side by side, strides in elements, any alignment of its numbers; scores and ended [requests][beams], out_* [requests][count]

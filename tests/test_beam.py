@@ -335,3 +335,56 @@ def test_beams_of_the_same_numbers_go_in_order(K, count):
     words = torch.sort(x[0, 0], descending=True, stable=True).indices
     assert got.beams[0].tolist() == [i % K for i in range(count)]
     assert got.words[0].tolist() == [int(words[i // K]) for i in range(count)]
+
+
+# Numbers of any size.  A total is s + (x - lse) in 64 bits: lse of 1e10 has steps of 2^-19, one of which is within OFF; lse of 1e20 and more steps of 2^14 and more, in which
+# log sum exp(x - top) <= log 262 144 < 13 is lost on either side.  (Sizes in between would need a tolerance of a step of theirs.)
+SIZES = [1e9, 2e9, 5e9, 1e10, 1e20, 1e30, 2e30, 1e38]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("V", [700, 8195])     # one part, and several, the last of which is a few words
+@pytest.mark.parametrize("size", SIZES)
+def test_finite_masks_of_any_size(size, V, dtype):
+    part = min(1024 if dtype == torch.float32 else 2048, V // 3)
+    x, s = logits_of(3, 3, V, 5, dtype)
+    x[0, 0, part:2 * part] = -size              # one whole part, or a third of a row of one part
+    x[0, 1, :] = -size                          # all but a part in the middle
+    x[0, 1, part:2 * part] = logits_of(1, 1, part, 6, dtype)[0][0, 0]
+    x[0, 2, :] = -size                          # nothing is left: all as likely
+    x[1, 0, :V - 1] = -size                     # the last word
+    x[1, 1, :] = torch.where(torch.arange(V).cuda() % 2 == 0, x[1, 1], -size)
+    x[1, 2, 3:] = -size                         # a few
+    x[2, :, :] = -size
+    for count in (4, 64):
+        got = check(x, s, count)
+        assert bool((got.beams >= 0).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("V", [700, 8195])
+@pytest.mark.parametrize("size", SIZES)
+def test_largest_words_of_any_size(size, V, dtype):
+    x, s = logits_of(3, 3, V, 7, dtype)
+    x[0, 0, V // 2] = size                      # a word above all others, of its row and of the other rows
+    x[1, :, 5] = size
+    x[2, 0, :] = size                           # a row of nothing else
+    x[2, 1, V - 100:] = size
+    for count in (1, 5):
+        got = check(x, s, count)
+        assert bool((got.beams >= 0).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("V", [700, 8195])
+@pytest.mark.parametrize("sign", [-1.0, 1.0])
+@pytest.mark.parametrize("middle", [2.0 ** 21, 2.0 ** 22, 2.0 ** 24, 2.0 ** 28])
+def test_parts_on_both_sides_of_a_size(middle, sign, V):
+    """Parts whose largest words are a little below and above a power of two, and rows of which one part alone is."""
+    x, s = logits_of(2, 3, V, 8)
+    step = torch.where(torch.arange(V).cuda() // 1024 % 2 == 0, -1.5, 1.5)
+    x[0] = sign * middle + (x[0] + step) * max(1.0, middle * 2.0 ** -23)
+    x[1, :, V // 2:] = sign * middle + x[1, :, V // 2:]
+    check(x, s, 6)
