@@ -1,9 +1,12 @@
 // functs::rotary: rotary positions (fx_rotary of include/fxhip.h), with their gradient.
 #include <c10/hip/HIPGraphsC10Utils.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/graph_task.h>
 #include <torch/library.h>
 
 #include <cmath>
+#include <unordered_set>
+#include <vector>
 
 #include "rotary_ops.h"
 
@@ -72,6 +75,37 @@ Tensor turned(const Tensor& x_, const Tensor& positions_, const Tensor& frequenc
 
 Tensor rotaryOf(const Tensor& x, const Tensor& positions, const Tensor& frequencies, double magnitude, bool interleaved, bool back);
 
+// A leaf's gradient is added up on the stream on which its first graph was made.  While that graph lives, a backward pass captured on another
+// stream would wait for this one in the middle of the capture; the default stream cannot be waited for there, and the engine ends the process.
+bool capturing(c10::Device dev) {
+  return c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(dev.index()).stream() != nullptr && c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None;
+}
+// Of a captured backward pass that is at this operator: whether anything that it runs behind, the gradients of leaves among it, is the default stream's
+bool defaultStreamBehind(c10::Device dev) {
+  const c10::Stream none = c10::hip::getDefaultHIPStreamMasqueradingAsCUDA(dev.index()).unwrap();
+  const auto* const runs = torch::autograd::get_current_graph_task_exec_info();   // (empty: all nodes run)
+  const auto here = torch::autograd::get_current_node();
+  std::vector<torch::autograd::Node*> ahead{here.get()};
+  std::unordered_set<torch::autograd::Node*> seen;
+  while (!ahead.empty()) {
+    auto* const node = ahead.back();
+    ahead.pop_back();
+    if (!node) continue;
+    for (const auto& edge : node->next_edges()) {
+      auto* const next = edge.function.get();
+      if (!next || !seen.insert(next).second) continue;
+      if (runs && !runs->empty()) {
+        const auto it = runs->find(next);
+        if (it == runs->end() || !it->second.should_execute()) continue;
+      }
+      const auto made = next->stream();
+      if (made && *made == none) return true;
+      ahead.push_back(next);
+    }
+  }
+  return false;
+}
+
 // The gradient of a rotation is the rotation back, which has a gradient of its own
 struct Rotary : public torch::autograd::Function<Rotary> {
   static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& x, const Tensor& positions, const Tensor& frequencies, double magnitude, bool interleaved,
@@ -86,6 +120,11 @@ struct Rotary : public torch::autograd::Function<Rotary> {
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
     Tensor x;
     if (grads[0].defined()) {
+      if (grads[0].is_cuda()) {
+        c10::DeviceGuard guard(grads[0].device());
+        TORCH_CHECK(!capturing(grads[0].device()) || !defaultStreamBehind(grads[0].device()), kOp,
+                    ": this captured backward pass comes to a tensor that is in a living graph of the default stream; drop its results before the capture");
+      }
       const auto saved = ctx->get_saved_variables();
       x = rotaryOf(grads[0], saved[0], saved[1], ctx->saved_data["magnitude"].toDouble(), ctx->saved_data["interleaved"].toBool(), !ctx->saved_data["back"].toBool());
     }
@@ -96,11 +135,10 @@ struct Rotary : public torch::autograd::Function<Rotary> {
 Tensor rotaryOf(const Tensor& x, const Tensor& positions, const Tensor& frequencies, double magnitude, bool interleaved, bool back) {
   TORCH_CHECK(!x._fw_grad(0).defined(), kOp, " has no forward-mode derivative: x carries a tangent");
   if (!at::GradMode::is_enabled() || !x.requires_grad()) return turned(x, positions, frequencies, magnitude, interleaved, back);
-  // A leaf's gradient is added up on the stream on which its first graph was made.  While that graph lives, a backward pass captured on another
-  // stream would wait for this one in the middle of the capture, and the engine ends the process; the call is refused here instead.
+  // (the same for a leaf that is turned itself, as soon as the call is captured and on whichever stream its graph was made)
   if (x.is_cuda() && x.is_leaf()) {
     c10::DeviceGuard guard(x.device());
-    if (c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None) {
+    if (capturing(x.device())) {
       const auto node = torch::autograd::impl::try_get_grad_accumulator(x);
       const auto made = node ? node->stream() : std::nullopt;
       const c10::Stream now = c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(x.device().index()).unwrap();

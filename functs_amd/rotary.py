@@ -61,5 +61,7 @@ def frequencies(columns: int, base: float = 10000.0, stretch: float = 1.0, how: 
 
 def rotary(x: Tensor, positions: Tensor, frequencies: Tensor, magnitude: float = 1.0, interleaved: bool = False) -> Tensor:
     """x [tokens, heads, depth] or [batch, tokens, heads, depth] (float32, float16 or bfloat16, any strides) turned; positions int32 or int64
-    [tokens], or [batch, tokens]; frequencies float64 or float32.  Has a backward pass (for x), which may be differentiated again."""
+    [tokens], or [batch, tokens]; frequencies float64 or float32.  Has a backward pass (for x), which may be differentiated again.
+    Forward and backward passes may be captured into a graph.  Refused are a captured backward pass that comes to a tensor which is in a living graph of the default
+    stream, and a captured call on a leaf that requires a gradient and is in a living graph of another stream: drop that graph's results before."""
     return torch.ops.functs.rotary(x, positions, frequencies, magnitude, interleaved)

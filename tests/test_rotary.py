@@ -338,3 +338,41 @@ def test_every_launch_is_counted():
     rotary.rotary(x, p, f)
     lib.fx_launch_stats(ctypes.byref(total), ctypes.byref(special))
     assert total.value == before + 1
+
+
+@pytest.mark.gpu
+def test_a_captured_backward_pass_to_a_leaf_of_a_living_graph_is_refused():
+    """Through views of the leaf, which are no leaves: the pass is refused where it would come to the leaf, and only there."""
+    f, _ = rotary.frequencies(16)
+    x, p, g = normal(3, 4, 16, seed=25).requires_grad_(), torch.arange(3).cuda(), normal(3, 2, 16, seed=26)
+    alive = rotary.rotary(x[:, :2], p, f)
+    graph, said = torch.cuda.CUDAGraph(), ""
+    with torch.cuda.graph(graph):
+        y = rotary.rotary(x[:, 2:], p, f)
+        try:
+            torch.autograd.grad(y, x, g)
+        except RuntimeError as e:
+            said = str(e)
+    assert "drop its results" in said
+    graph.replay()
+    check(y, x[:, 2:], p, f)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        part = x[:, 2:]
+        y = rotary.rotary(part, p, f)
+        (d,) = torch.autograd.grad(y, part, g)   # (does not come to the leaf)
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        check(y, x[:, 2:], p, f)
+        check(d, g, p, f, back=True)
+    del alive, y, part
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        (d,) = torch.autograd.grad(rotary.rotary(x[:, 2:], p, f), x, g)
+    for seed in (27, 28, 29):
+        g.copy_(normal(3, 2, 16, seed=seed))
+        graph.replay()
+        torch.cuda.synchronize()
+        check(d[:, 2:], g, p, f, back=True)
+        assert not bool(d[:, :2].any())
