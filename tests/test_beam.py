@@ -388,3 +388,18 @@ def test_parts_on_both_sides_of_a_size(middle, sign, V):
     x[0] = sign * middle + (x[0] + step) * max(1.0, middle * 2.0 ** -23)
     x[1, :, V // 2:] = sign * middle + x[1, :, V // 2:]
     check(x, s, 6)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("V,count", [(900, 4), (8197, 4), (50001, 20)])
+def test_rows_have_the_same_results_alone_and_among_many(V, count, dtype):
+    """Parts go by type and number of words, so a row's sum does not depend on the rows beside it: bit for bit."""
+    x, s = logits_of(301, 3, V, 15, dtype)
+    got = beam.select(x, s, count)
+    for some in ([0], [300], [0, 150, 299, 300]):
+        some = torch.tensor(some).cuda()
+        alone = beam.select(x[some], s[some], count)
+        assert all(torch.equal(a[some], b) for a, b in zip(got, alone))
+    order = torch.arange(300, -1, -1).cuda()
+    assert all(torch.equal(a[order], b) for a, b in zip(got, beam.select(x[order], s[order], count)))
