@@ -26,7 +26,8 @@ class Chosen(NamedTuple):
 
 def select(logits: Tensor, scores: Tensor, count: int = 0, ended: Optional[Tensor] = None, end_word: int = -1) -> Chosen:
     """The `count` (0: as many as beams) best of scores[b, k] + log_softmax(logits[b, k])[w] of each request b, best first; equal ones in the order of beams,
-    then of words.  logits float32, float16 or bfloat16 [requests, beams, words], scores float32 [requests, beams].  A masked word's logit is -infinity; a beam
+    then of words.  logits float32, float16 or bfloat16 [requests, beams, words], scores float32 [requests, beams].  A masked word's logit is -infinity
+    (a finite mask gives such words their small probability, and takes a millisecond where fewer words than `count` are left of a large vocabulary); a beam
     that does not exist yet (all but one behind a prompt) has the score -infinity.  Beams with ended[b, k] (bool) keep their score and continue with
     `end_word` alone.  Places for which there is no candidate: -infinity, -1, -1.  include/fxhip.h has every rule."""
     return Chosen(*torch.ops.functs.beam_select(logits, scores, count, ended, end_word))

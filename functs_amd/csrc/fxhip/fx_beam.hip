@@ -12,15 +12,16 @@
 // above it; the words at or above it are a few more than `count`, and are ranked by counting.  Equal numbers: lower words go first, and so as many as there may be of them
 // never need more than a list's places (it is cut to the best `count` when it fills up).
 //
-// 488 rows of 128 001 words, bf16, 390 of them alive: 24.1 us (4.1 TB/s; to read them and do nothing but the sum takes 18) and 10.6; 64 of 50 001: 4.5 and 8.6;
-// 4 of 32 000, fp32: 3.2 and 6.9.
+// 488 rows of 128 001 words, bf16, 390 of them alive: 24.5 us (4.1 TB/s; to read them and do nothing but the sum takes 18) and 10.6; 64 of 50 001: 4.6 and 8.6;
+// 4 of 32 000, fp32: 3.3 and 7.0.  Rows that are masked with one finite number but for fewer words than `count`: the bound stays at that number, every segment has words at it, and
+// fx_beam_join walks them all (4 rows of 128 001 words, 3 of them free, 8 wanted, bf16: 740 us a call, and 12 where the mask is -infinity).
 #include <algorithm>
 
 #include "fx_beam.h"
 
 namespace {
 constexpr int kThreads = 256, kWaves = kThreads / 64;
-constexpr int kLoads = 4;    // of 16 bytes that a lane of fx_beam_scan has under way (8: rows of an odd number of words took 23 us where four take 18, and little else)
+constexpr int kLoads = 4;    // of 16 bytes that a lane of fx_beam_scan has under way (read for the sum alone, without segments: 488 rows of 128 001 words 23 us with 8, 18 with 4)
 constexpr int kMore = 128;   // candidates that a wave keeps besides the best `count`: two steps' of 64
 constexpr int kList = FX_BEAM_MAX_COUNT + kMore;
 constexpr int kSegments = 384;   // that it lists before it looks at them
@@ -262,7 +263,7 @@ __global__ __launch_bounds__(64 * kJoinWaves) void fx_beam_join(const FxBeamArgs
   uint64_t* keys = (uint64_t*)score + K * count + wave * room;     // [waves][room]
   uint32_t* word = (uint32_t*)((uint64_t*)score + K * count + waves * room);    // [beams][count]
   int* places = (int*)(word + K * count) + wave * 64;              // [waves][64]
-  uint16_t* list = (uint16_t*)((int*)(word + K * count) + waves * 64) + wave * kSegments;   // [waves][kSegments] (2^18 words have 2 048 at most)
+  uint16_t* list = (uint16_t*)((int*)(word + K * count) + waves * 64) + wave * kSegments;   // [waves][kSegments]; a row of 2^18 words has 2 048 segments
   const int64_t request = blockIdx.x;
   const int fours = a.parts_a_row * (FX_BEAM_SEGMENTS / 4);        // of segments of a row
   for (int k = wave; k < K; k += waves) {

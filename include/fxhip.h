@@ -503,7 +503,8 @@ int fx_attention_steps(const float* x, const float* k, const float* v, const flo
  * The angle is formed in 64 bits (an error of about |p| frequency / 2^53), its cosine and sine are off by 2^-23 at most, products are fp32 and
  * y is rounded once.  x [batch][tokens][heads][depth], a depth contiguous, strides in elements, any alignment of its numbers; positions int32, or
  * int64 (positions_64), the tokens' side by side, position_batch_stride apart (0: all batches have the same); frequencies double, or float
- * (frequencies_32): what they hold counts as exact.  1 <= pairs <= 2048, 2 * pairs <= depth, heads * depth < 2^28, batch * tokens < 2^30. */
+ * (frequencies_32): what they hold counts as exact.  1 <= pairs <= 2048, 2 * pairs <= depth, heads * depth < 2^28, batch * tokens < 2^30, and
+ * fewer than 2^23 workgroups, which share out up to 2 048 angles and some 1 024 units of 32 bytes each (FX_E_LIMIT). */
 typedef struct fx_rotary_desc {
   const void* x;
   void* y;
@@ -660,7 +661,8 @@ int fx_kv_attention(const fx_kv_cache* cache, const fx_kv_attention_desc* desc, 
  * Pages are told apart by their numbers, column by column within a group: a page stands in one column, and in the rows of one group.  Entries below 0 are no pages:
  * they are moved with the others, and neither copied nor freed.
  * The table is changed in place (rows table_stride apart, entries behind a row's tokens left as they were).  All arrays are int32 on the device: parents, lens, out_lens
- * [groups * beams], copies [groups * beams][3], freed [groups * beams * columns].  beams: 1 to 32.
+ * [groups * beams], copies [groups * beams][3], freed [groups * beams * columns].  beams: 1 to 32; fewer than 2^26 rows, 2^24 groups times blocks of 256 columns and
+ * 2^31 entries, and rows of 2^30 tokens at most (FX_E_LIMIT).
  * workspace: fx_kv_fork_workspace_bytes() of device memory for each call under way, 16-byte aligned; nothing is expected in it.  One launch for few
  * rows and columns, three otherwise. */
 typedef struct fx_kv_fork_desc {
@@ -696,7 +698,9 @@ int fx_kv_copy(const fx_kv_cache* caches, int n_caches, const int32_t* copies, i
  * beams whose score is -infinity or NaN (there is none yet, or none any more).  A beam that has ended (ended: one byte each, or null) has one candidate, end_word
  * with the beam's score, whatever its logits are, which are not read.  Where there are fewer than `count`, the places behind have -infinity, beam -1 and word -1.
  * logits [requests][beams][words], a beam's words side by side, strides in elements, any alignment of its numbers; scores and ended [requests][beams], out_* [requests][count]
- * contiguous.  beams: 1 to 32, count: 1 to 64, words: 1 to 2^18.
+ * contiguous.  beams: 1 to 32, count: 1 to 64, words: 1 to 2^18 (up to which sums and selections are tested); requests < 2^22, and
+ * fewer than 2^26 - 4 parts of 4 KiB of all rows (FX_E_LIMIT).  Rows that are masked with a finite number but for fewer words than `count` take much longer
+ * (a millisecond for 128 001 words) than rows masked with -infinity.
  * workspace: fx_beam_select_workspace_bytes() of device memory for each call under way, 16-byte aligned; nothing is expected in it.  Two launches,
  * of rows of up to 4 KiB one. */
 #define FX_BEAM_MAX_BEAMS 32

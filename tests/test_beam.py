@@ -2,9 +2,10 @@
 
 CPU: refusals.  GPU: the operator against a plain selection in 64 bits.
 
-Words and beams have to be equal wherever the totals that decide are further apart than the kernel's are off: lse by 2^-23 for the terms (each exp is off by
-2^-22 of itself at most, from its argument, a rounded difference times a rounded log2 e, and its own rounding: |x - top| 2^-23 + 2^-23 of it, with
-x - top up to 30 where it matters: 2^-18 at most, and far less in their sum), so 2^-18 in all; a total is rounded to fp32 once."""
+Words and beams have to be equal wherever the totals that decide are further apart than the kernel's are off.  A term is 2 to the power of x c - r, c being log2 e in fp32
+(1.3e-8 too large) and r the whole number next to the largest x c: a product and a difference rounded once, by half a step of the result, which is about (x - top) c.
+From tops of 2^22 on it is (x - top) c itself, an exact difference and a rounded product.  So it is off by 2^-24 |x - top| c + 1.3e-8 |x - top| + 2^-23 (the power's own
+rounding) of itself: with x - top of 30, beyond which no term matters, 2^-18 at most, and far less in their sum.  2^-18 in all; a total is rounded to fp32 once."""
 import ctypes
 import math
 
